@@ -31,7 +31,7 @@
 extern "C" {
 #endif
 
-#define MB_ABI_VERSION 3
+#define MB_ABI_VERSION 4
 
 /* Status codes (negative = rejected by the library before any launch). */
 #define MB_OK 0
@@ -175,6 +175,125 @@ int mb_time_gemm_rotating(int dtype, const void* const* A,
                           float scale_b, void* workspace,
                           size_t workspace_bytes, int warmup, int iterations,
                           void* stream, double* elapsed_s);
+
+/*
+ * The operators of an expert layer. No counterpart in the reference, whose
+ * GEMM is one dense product (native/kernels/mfu_gemm.hip.cpp:9-21); these are
+ * the products and the data movement that a mixture of experts puts around it.
+ *
+ * A router gives each of `tokens` tokens up to top_k of `experts` experts. The
+ * assignments, sorted by expert and within an expert by token, are the "sorted
+ * rows" that the products work on. mb_route writes how they are laid out, all
+ * int32 in device memory, and the other calls take it from there:
+ *   offsets  experts + 1: expert e's sorted rows are offsets[e] .. offsets[e+1]-1
+ *   rows     tokens * top_k: the token of each sorted row, -1 past the last
+ *   slots    tokens x top_k: the sorted row of each assignment, -1 for none
+ * The host never reads them. The kernels clamp offsets to 0 .. total_rows,
+ * treat a row or slot outside its matrix as one that is not there (rows read as
+ * zeros, slots add nothing) and so stay inside the buffers whatever they hold.
+ *
+ * Leading dimensions are in elements; 0 stands for packed rows. Matrices start
+ * on any element; rows on 16 bytes (base and leading dimension) are faster in
+ * the products. Types: BFLOAT16 and FLOAT16, FLOAT32 too for logits. Products
+ * accumulate in fp32 and round once. Empty calls (no tokens, no rows) are
+ * valid. Results are the same bits from call to call: no atomics order sums.
+ */
+
+/*
+ * mb_route -- the top_k experts of each token and the sorted order of all
+ * assignments.
+ *
+ * logits (tokens x experts, FLOAT32 / BFLOAT16 / FLOAT16): a token's choices are its
+ * largest logits, ties to the lower expert. -inf and NaN are never chosen: a
+ * token with fewer than top_k other logits leaves its last choices empty
+ * (expert_ids -1, weight 0, slot -1), all of them if it has none. +inf counts as the
+ * largest finite fp32 value.
+ * weights (tokens x top_k, fp32): softmax over the chosen logits (normalize
+ * != 0) or over all of the token's logits. expert_ids: tokens x top_k.
+ * 1 <= experts <= MB_ROUTE_MAX_EXPERTS, 1 <= top_k <= min(experts, MB_ROUTE_MAX_TOP_K),
+ * tokens * top_k < 2^31. workspace: mb_route_workspace_size() bytes on 4 bytes
+ * (may be NULL when that is 0); every call writes what it reads there.
+ */
+#define MB_ROUTE_MAX_EXPERTS 1024
+#define MB_ROUTE_MAX_TOP_K 64
+int mb_route(int dtype, const void* logits, int64_t ld, int64_t tokens, int experts, int top_k, int normalize,
+             float* weights, int32_t* expert_ids, int32_t* offsets, int32_t* rows, int32_t* slots, void* workspace,
+             size_t workspace_bytes, void* stream);
+
+/* Workspace bytes mb_route needs (0 if none, or if the arguments are out of range). */
+size_t mb_route_workspace_size(int64_t tokens, int experts, int top_k);
+
+/*
+ * mb_route_grad -- the gradient of mb_route's weights with respect to the
+ * logits: grad_logits (tokens x experts, the logits' type), every element
+ * written, from grad_weights (tokens x top_k, fp32) and the call's expert_ids.
+ */
+int mb_route_grad(int dtype, const void* logits, int64_t ld, const int32_t* expert_ids, const float* grad_weights,
+                  int64_t tokens, int experts, int top_k, int normalize, void* grad_logits, int64_t ld_grad,
+                  void* stream);
+
+/*
+ * mb_gemm_grouped -- one product per expert over its sorted rows p, and the
+ * gradients of that product:
+ *
+ * op                      out                    x           y
+ * MB_GROUPED_FORWARD      C[p] = A[p] * B[e]      A           B
+ * MB_GROUPED_GRAD_ROWS    dA[p] = dC[p] * B[e]^T  dC          B
+ * MB_GROUPED_GRAD_WEIGHTS dB[e] = sum of A[p]^T * dC[p]  A   dC
+ *
+ * A and dA are total_rows x K, C and dC total_rows x N, B and dB experts
+ * matrices of K x N one after the other (K * ld apart). With `rows`, sorted
+ * row p of x is row rows[p] of its x_rows rows: A is then read in token order;
+ * without (NULL), row p of its x_rows = total_rows or more rows.
+ * FORWARD and GRAD_ROWS leave output rows at and past offsets[experts] alone.
+ * GRAD_WEIGHTS writes every matrix, zeros for an expert without rows.
+ * x, y and out must not overlap. 1 <= experts <= MB_ROUTE_MAX_EXPERTS;
+ * N, K >= 1; K * ldb below 2^31 bytes per matrix.
+ */
+#define MB_GROUPED_FORWARD 0
+#define MB_GROUPED_GRAD_ROWS 1
+#define MB_GROUPED_GRAD_WEIGHTS 2
+int mb_gemm_grouped(int op, int dtype, const void* x, int64_t ldx, int64_t x_rows, const int32_t* rows, const void* y,
+                    int64_t ldy, void* out, int64_t ldo, const int32_t* offsets, int experts, int64_t total_rows,
+                    int64_t N, int64_t K, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * mb_gemm_w4 -- products with 4-bit weights, dense (offsets NULL, experts 1)
+ * or by expert over the sorted rows of x as in mb_gemm_grouped:
+ *   out[p][n] = sum over k of x[rows[p]][k] * scales[e][n][k / group] * (q[e][n][k] - zeros[e][n][k / group])
+ *
+ * q: experts x N x ceil(K / 2) bytes, two weights a byte, the even k in the
+ * low half; a last high half past K is ignored. scales and zeros: experts x
+ * N x ceil(K / group) of x's type; zeros NULL stands for 8. `group` is a
+ * positive multiple of 32. The integers are multiplied exactly and scaled in
+ * fp32, group by group. Output rows at and past offsets[experts] are left alone.
+ * Meant for few rows per expert (decode); any number is taken.
+ */
+int mb_gemm_w4(int dtype, const void* x, int64_t ldx, int64_t x_rows, const int32_t* rows, const void* q,
+               const void* scales, const void* zeros, int group, void* out, int64_t ldo, const int32_t* offsets,
+               int experts, int64_t total_rows, int64_t N, int64_t K, void* workspace, size_t workspace_bytes,
+               void* stream);
+
+/*
+ * mb_combine -- each token's weighted sum over its sorted rows,
+ *   out[t] = sum over j of weights[t][j] * y[slots[t][j]],
+ * in order of j, fp32, rounded once. weights NULL stands for ones: the
+ * gradient of rows read through `rows`. Tokens without a slot get zeros.
+ * y: y_rows x N, out: tokens x N. 1 <= top_k <= MB_ROUTE_MAX_TOP_K.
+ */
+int mb_combine(int dtype, const void* y, int64_t ldy, int64_t y_rows, const float* weights, const int32_t* slots,
+               int64_t tokens, int top_k, int64_t N, void* out, int64_t ldo, void* stream);
+
+/*
+ * mb_combine_grad -- from grad_out (tokens x N): grad_y[slots[t][j]] =
+ * weights[t][j] * grad_out[t] and grad_weights[t][j] = the dot product of
+ * grad_out[t] and y[slots[t][j]] (fp32; 0 without a slot). Either output may
+ * be NULL; y is read for grad_weights only. Slots are distinct, as mb_route
+ * writes them; rows of grad_y that no slot names are left alone.
+ */
+int mb_combine_grad(int dtype, const void* grad_out, int64_t ldg, const void* y, int64_t ldy, int64_t y_rows,
+                    const float* weights, const int32_t* slots, int64_t tokens, int top_k, int64_t N, void* grad_y,
+                    int64_t ld_grad_y, float* grad_weights, void* stream);
 
 /*
  * mb_kernel_info -- JSON object describing the kernel configuration the

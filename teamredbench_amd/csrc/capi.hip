@@ -88,8 +88,6 @@ int current_device_props(const DeviceProps** out) {
     return MB_OK;
 }
 
-namespace {
-
 int device_for_launch(const DeviceProps** props) {
     int rc = current_device_props(props);
     if (rc != MB_OK) return rc;
@@ -99,6 +97,8 @@ int device_for_launch(const DeviceProps** props) {
     }
     return MB_OK;
 }
+
+namespace {
 
 int check_stream_args(int op, void* dst, const void* b, const void* c, uint64_t n) {
     if (n == 0) return MB_OK;

@@ -1,0 +1,166 @@
+// The way back from sorted rows to tokens, and its gradient.
+//
+//   out[t] = sum over j of w[t][j] y[slots[t][j]]            (combine)
+//   grad_y[slots[t][j]] = w[t][j] g[t]                        (gradient)
+//   grad_w[t][j] = <g[t], y[slots[t][j]]>
+//
+// Memory-bound: each row is read once and each output row written once, 16
+// bytes a lane, all of a token's rows in flight together. Sums are fp32, in
+// order of j. Rows off 16 bytes take the same loads (the hardware
+// takes 16 bytes at any address); the columns past the last whole 8 go one by one.
+#include "experts_common.hpp"
+
+namespace mb {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kBatch = 8;      // rows of a token in flight together
+
+// 8 columns from column c of a row, zeros past N.
+template <int DT>
+__device__ __forceinline__ void load_columns(const uint16_t* row, int64_t c, int64_t N, float* v) {
+    if (c + 8 <= N) {
+        const u32x4 p = *reinterpret_cast<const u32x4_any*>(row + c);
+        unpack8<DT>(p, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = c + i < N ? from_bits<DT>(row[c + i]) : 0.f;
+    }
+}
+template <int DT>
+__device__ __forceinline__ void store_columns(uint16_t* row, int64_t c, int64_t N, const float* v) {
+    if (c + 8 <= N) {
+        *reinterpret_cast<u32x4_any*>(row + c) = pack8<DT>(v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (c + i < N) row[c + i] = to_bits<DT>(v[i]);
+    }
+}
+
+// One thread per 8 columns of a token.
+template <int DT>
+__global__ void __launch_bounds__(kThreads)
+combine_kernel(const uint16_t* __restrict__ y, int64_t ldy, int64_t y_rows, const float* __restrict__ weights,
+               const int32_t* __restrict__ slots, int64_t tokens, int top_k, int64_t N, uint16_t* __restrict__ out,
+               int64_t ldo, int chunks) {
+    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    const int64_t t = i / chunks;
+    if (t >= tokens) return;
+    const int64_t c = (i - t * chunks) * 8;
+    float sum[8] = {};
+    for (int j0 = 0; j0 < top_k; j0 += kBatch) {
+        float v[kBatch][8], w[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            w[u] = 0.f;
+            const int64_t a = t * top_k + j0 + u;
+            const int64_t slot = j0 + u < top_k ? slots[a] : -1;
+            if (slot >= 0 && slot < y_rows) {
+                load_columns<DT>(y + slot * ldy, c, N, v[u]);
+                w[u] = weights ? weights[a] : 1.f;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[u][e] = 0.f;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum[e] = fmaf(w[u], v[u][e], sum[e]);
+    }
+    store_columns<DT>(out + t * ldo, c, N, sum);
+}
+
+// One block per token: its grad_y rows, and the dot products over its columns.
+template <int DT>
+__global__ void __launch_bounds__(kThreads)
+combine_grad_kernel(const uint16_t* __restrict__ g, int64_t ldg, const uint16_t* __restrict__ y, int64_t ldy,
+                    int64_t y_rows, const float* __restrict__ weights, const int32_t* __restrict__ slots, int top_k,
+                    int64_t N, uint16_t* __restrict__ grad_y, int64_t ld_grad_y, float* __restrict__ grad_weights) {
+    __shared__ float part[kThreads / 64][kBatch];
+    const int64_t t = blockIdx.x;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int j0 = 0; j0 < top_k; j0 += kBatch) {
+        int64_t slot[kBatch];
+        float w[kBatch], dot[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            const int64_t a = t * top_k + j0 + u;
+            slot[u] = j0 + u < top_k ? slots[a] : -1;
+            if (slot[u] >= y_rows) slot[u] = -1;
+            w[u] = slot[u] >= 0 && weights ? weights[a] : 1.f;
+            dot[u] = 0.f;
+        }
+        for (int64_t c = (int64_t)threadIdx.x * 8; c < N; c += kThreads * 8) {
+            float gv[8];
+            load_columns<DT>(g + t * ldg, c, N, gv);
+            if (grad_weights != nullptr) {
+#pragma unroll
+                for (int u = 0; u < kBatch; ++u) {
+                    if (slot[u] < 0) continue;
+                    float yv[8];
+                    load_columns<DT>(y + slot[u] * ldy, c, N, yv);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) dot[u] = fmaf(gv[e], yv[e], dot[u]);
+                }
+            }
+            if (grad_y != nullptr) {
+#pragma unroll
+                for (int u = 0; u < kBatch; ++u) {
+                    if (slot[u] < 0) continue;
+                    float dv[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) dv[e] = w[u] * gv[e];
+                    store_columns<DT>(grad_y + slot[u] * ld_grad_y, c, N, dv);
+                }
+            }
+        }
+        if (grad_weights != nullptr) {
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+#pragma unroll
+                for (int d = 32; d > 0; d >>= 1) dot[u] += __shfl_xor(dot[u], d);
+                if (lane == 0) part[wave][u] = dot[u];
+            }
+            __syncthreads();
+            if (threadIdx.x < kBatch && j0 + (int)threadIdx.x < top_k) {
+                float sum = 0.f;
+#pragma unroll
+                for (int v = 0; v < kThreads / 64; ++v) sum += part[v][threadIdx.x];
+                grad_weights[t * top_k + j0 + threadIdx.x] = sum;
+            }
+            __syncthreads();
+        }
+    }
+}
+
+}  // namespace
+
+int combine_launch(int dtype, const void* y, int64_t ldy, int64_t y_rows, const float* weights, const int32_t* slots,
+                   int64_t tokens, int top_k, int64_t N, void* out, int64_t ldo, hipStream_t stream) {
+    const int chunks = (int)((N + 7) / 8);
+    const int64_t blocks = (tokens * chunks + kThreads - 1) / kThreads;
+    const auto* yp = static_cast<const uint16_t*>(y);
+    auto* op = static_cast<uint16_t*>(out);
+    auto kernel = dtype == MB_DT_FLOAT16 ? combine_kernel<MB_DT_FLOAT16> : combine_kernel<MB_DT_BFLOAT16>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kThreads), 0, stream, yp, ldy, y_rows, weights, slots,
+                       tokens, top_k, N, op, ldo, chunks);
+    MB_HIP_TRY(hipGetLastError());
+    return MB_OK;
+}
+
+int combine_grad_launch(int dtype, const void* grad_out, int64_t ldg, const void* y, int64_t ldy, int64_t y_rows,
+                        const float* weights, const int32_t* slots, int64_t tokens, int top_k, int64_t N, void* grad_y,
+                        int64_t ld_grad_y, float* grad_weights, hipStream_t stream) {
+    const auto* gp = static_cast<const uint16_t*>(grad_out);
+    const auto* yp = static_cast<const uint16_t*>(y);
+    auto* gy = static_cast<uint16_t*>(grad_y);
+    auto kernel = dtype == MB_DT_FLOAT16 ? combine_grad_kernel<MB_DT_FLOAT16> : combine_grad_kernel<MB_DT_BFLOAT16>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)tokens), dim3(kThreads), 0, stream, gp, ldg, yp, ldy, y_rows, weights,
+                       slots, top_k, N, gy, ld_grad_y, grad_weights);
+    MB_HIP_TRY(hipGetLastError());
+    return MB_OK;
+}
+
+}  // namespace mb

@@ -49,6 +49,9 @@ struct DeviceProps {
 // status code (and sets the error string).
 int current_device_props(const DeviceProps** out);
 
+// The same, and MB_ERR_DEVICE unless the device is gfx950.
+int device_for_launch(const DeviceProps** out);
+
 // ---- vector types ---------------------------------------------------------
 
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));

@@ -68,6 +68,12 @@ GEMM_OUTPUT_DTYPES = {"bfloat16": "bfloat16", "float16": "float16", "float8_e4m3
 
 KIND_STREAM, KIND_GEMM = 0, 1
 
+# Expert layer (mb_route, mb_gemm_grouped, mb_gemm_w4, mb_combine)
+ROUTE_MAX_EXPERTS, ROUTE_MAX_TOP_K = 1024, 64   # MB_ROUTE_MAX_*
+ROUTE_DTYPES = ("float32", "bfloat16", "float16")
+EXPERT_DTYPES = ("bfloat16", "float16")
+GROUPED_FORWARD, GROUPED_GRAD_ROWS, GROUPED_GRAD_WEIGHTS = 0, 1, 2
+
 # Plan overrides (mb_set_tuning); names follow the "overrides" keys of mb_kernel_info.
 TUNING_KNOBS = {
     "stream_unroll": 0,
@@ -125,6 +131,42 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
             ctypes.POINTER(ctypes.c_double),
         ],
     ),
+    "mb_route": (
+        ctypes.c_int,
+        [
+            ctypes.c_int, _cvp, _i64, _i64, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, _vp, _vp, _vp, _vp, _vp,
+            ctypes.c_size_t, _vp,
+        ],
+    ),
+    "mb_route_workspace_size": (ctypes.c_size_t, [_i64, ctypes.c_int, ctypes.c_int]),
+    "mb_route_grad": (
+        ctypes.c_int,
+        [ctypes.c_int, _cvp, _i64, _cvp, _cvp, _i64, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, _i64, _vp],
+    ),
+    "mb_gemm_grouped": (
+        ctypes.c_int,
+        [
+            ctypes.c_int, ctypes.c_int, _cvp, _i64, _i64, _cvp, _cvp, _i64, _vp, _i64, _cvp, ctypes.c_int, _i64, _i64,
+            _i64, _vp, ctypes.c_size_t, _vp,
+        ],
+    ),
+    "mb_gemm_w4": (
+        ctypes.c_int,
+        [
+            ctypes.c_int, _cvp, _i64, _i64, _cvp, _cvp, _cvp, _cvp, ctypes.c_int, _vp, _i64, _cvp, ctypes.c_int, _i64,
+            _i64, _i64, _vp, ctypes.c_size_t, _vp,
+        ],
+    ),
+    "mb_combine": (
+        ctypes.c_int,
+        [ctypes.c_int, _cvp, _i64, _i64, _cvp, _cvp, _i64, ctypes.c_int, _i64, _vp, _i64, _vp],
+    ),
+    "mb_combine_grad": (
+        ctypes.c_int,
+        [
+            ctypes.c_int, _cvp, _i64, _cvp, _i64, _i64, _cvp, _cvp, _i64, ctypes.c_int, _i64, _vp, _i64, _vp, _vp,
+        ],
+    ),
     "mb_kernel_info": (
         ctypes.c_int,
         [ctypes.c_int, ctypes.c_int, ctypes.c_int, _i64, _i64, _i64, ctypes.c_char_p, ctypes.c_size_t],
@@ -139,7 +181,7 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "mb_get_tuning": (_i64, [ctypes.c_int]),
 }
 
-ABI_VERSION = 3
+ABI_VERSION = 4
 
 
 class NativeLibraryError(RuntimeError):
@@ -223,6 +265,59 @@ class NativeLibrary:
         )
         self._check(status, "mb_time_gemm_rotating")
         return out.value
+
+    # ---- expert layer --------------------------------------------------------
+    def route_workspace_size(self, tokens: int, experts: int, top_k: int) -> int:
+        return int(self.handle.mb_route_workspace_size(tokens, experts, top_k))
+
+    def route(self, dtype: int, logits: int, ld: int, tokens: int, experts: int, top_k: int, normalize: bool,
+              weights: int, expert_ids: int, offsets: int, rows: int, slots: int, workspace: int | None = None,
+              workspace_bytes: int = 0, stream: int | None = None) -> None:
+        """The top experts of each token and the sorted order of all assignments (see mb_route)."""
+        status = self.handle.mb_route(dtype, logits, ld, tokens, experts, top_k, int(normalize), weights, expert_ids,
+                                      offsets, rows, slots, workspace or None, workspace_bytes, stream or None)
+        self._check(status, "mb_route")
+
+    def route_grad(self, dtype: int, logits: int, ld: int, expert_ids: int, grad_weights: int, tokens: int,
+                   experts: int, top_k: int, normalize: bool, grad_logits: int, ld_grad: int,
+                   stream: int | None = None) -> None:
+        status = self.handle.mb_route_grad(dtype, logits, ld, expert_ids, grad_weights, tokens, experts, top_k,
+                                           int(normalize), grad_logits, ld_grad, stream or None)
+        self._check(status, "mb_route_grad")
+
+    def gemm_grouped(self, op: int, dtype: int, x: int, ldx: int, x_rows: int, rows: int | None, y: int, ldy: int,
+                     out: int, ldo: int, offsets: int, experts: int, total_rows: int, n: int, k: int,
+                     workspace: int | None = None, workspace_bytes: int = 0, stream: int | None = None) -> None:
+        """One product per expert over its sorted rows, or a gradient of it (see mb_gemm_grouped)."""
+        status = self.handle.mb_gemm_grouped(op, dtype, x, ldx, x_rows, rows or None, y, ldy, out, ldo, offsets,
+                                             experts, total_rows, n, k, workspace or None, workspace_bytes,
+                                             stream or None)
+        self._check(status, "mb_gemm_grouped")
+
+    def gemm_w4(self, dtype: int, x: int, ldx: int, x_rows: int, rows: int | None, q: int, scales: int,
+                zeros: int | None, group: int, out: int, ldo: int, offsets: int | None, experts: int, total_rows: int,
+                n: int, k: int, workspace: int | None = None, workspace_bytes: int = 0,
+                stream: int | None = None) -> None:
+        """Products with 4-bit weights, dense or by expert (see mb_gemm_w4)."""
+        status = self.handle.mb_gemm_w4(dtype, x, ldx, x_rows, rows or None, q, scales, zeros or None, group, out, ldo,
+                                        offsets or None, experts, total_rows, n, k, workspace or None,
+                                        workspace_bytes, stream or None)
+        self._check(status, "mb_gemm_w4")
+
+    def combine(self, dtype: int, y: int, ldy: int, y_rows: int, weights: int | None, slots: int, tokens: int,
+                top_k: int, n: int, out: int, ldo: int, stream: int | None = None) -> None:
+        """Each token's weighted sum over its sorted rows (see mb_combine)."""
+        status = self.handle.mb_combine(dtype, y, ldy, y_rows, weights or None, slots, tokens, top_k, n, out, ldo,
+                                        stream or None)
+        self._check(status, "mb_combine")
+
+    def combine_grad(self, dtype: int, grad_out: int, ldg: int, y: int | None, ldy: int, y_rows: int,
+                     weights: int | None, slots: int, tokens: int, top_k: int, n: int, grad_y: int | None,
+                     ld_grad_y: int, grad_weights: int | None, stream: int | None = None) -> None:
+        status = self.handle.mb_combine_grad(dtype, grad_out, ldg, y or None, ldy, y_rows, weights or None, slots,
+                                             tokens, top_k, n, grad_y or None, ld_grad_y, grad_weights or None,
+                                             stream or None)
+        self._check(status, "mb_combine_grad")
 
     # ---- metadata ----------------------------------------------------------
     def kernel_info(self, kind: int, a: int, b: int, m: int, n: int, k: int) -> dict[str, Any]:
