@@ -30,6 +30,9 @@ struct GroupedCall {
     const int32_t *rows, *offsets;
     int64_t ldx, ldy, ldo, x_rows, total_rows, N, K;
 };
+// The pipelined kernels (16-byte rows) on tile configuration `config`, one per input type.
+int gemm_grouped_tiled_bf16(const GroupedCall& c, int config, hipStream_t stream);
+int gemm_grouped_tiled_f16(const GroupedCall& c, int config, hipStream_t stream);
 int gemm_grouped_launch(const GroupedCall& c, void* workspace, size_t workspace_bytes, const DeviceProps& props,
                         hipStream_t stream);
 
@@ -83,6 +86,15 @@ struct ExpertRows {
 __device__ __forceinline__ ExpertRows expert_rows(const int32_t* offsets, int e, int total) {
     const int lo = min(max(offsets[e], 0), total), hi = min(max(offsets[e + 1], 0), total);
     return {e, lo, max(hi - lo, 0)};
+}
+
+// Tiles of BM rows that all experts' rows make. Called by whole waves.
+__device__ __forceinline__ int count_row_tiles(const int32_t* offsets, int experts, int total, int BM) {
+    int tiles = 0;
+    for (int e = __lane_id(); e < experts; e += 64) tiles += (expert_rows(offsets, e, total).count + BM - 1) / BM;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) tiles += __shfl_xor(tiles, d);
+    return __builtin_amdgcn_readfirstlane(tiles);
 }
 
 // Row tile `tile` of all experts' tiles of BM rows, in expert order: its

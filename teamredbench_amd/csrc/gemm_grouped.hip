@@ -199,10 +199,31 @@ int launch_dtype(const GroupedCall& c, hipStream_t stream) {
     return launch_any<DT, MB_GROUPED_GRAD_WEIGHTS>(c, stream);
 }
 
+// The tile configuration of the pipelined kernels, -1 for what they do not
+// take: rows off 16 bytes, or an operand (one expert's matrix, x read through
+// `rows`, a tile's rows) that passes the 2^31 bytes a buffer offset spans.
+int tiled_config(const GroupedCall& c) {
+    const uintptr_t base = reinterpret_cast<uintptr_t>(c.x) | reinterpret_cast<uintptr_t>(c.y) |
+                           reinterpret_cast<uintptr_t>(c.out);
+    if ((base & 15) != 0 || ((c.ldx | c.ldy | c.ldo | c.N | c.K) & 7) != 0 || c.total_rows == 0 || c.x_rows == 0)
+        return -1;
+    constexpr int64_t kMost = 1ll << 30;   // elements
+    const bool weights = c.op == MB_GROUPED_GRAD_WEIGHTS;
+    const int64_t x_rows = c.rows ? c.x_rows : weights ? c.total_rows : 256;
+    if (x_rows > kMost / c.ldx || (weights ? c.total_rows : c.K) > kMost / c.ldy) return -1;
+    if (weights) return 0;
+    const int64_t rows = (c.total_rows + c.experts - 1) / c.experts;
+    return rows > 256 ? 0 : rows > 64 ? 2 : 3;
+}
+
 }  // namespace
 
 int gemm_grouped_launch(const GroupedCall& c, void* workspace, size_t workspace_bytes, const DeviceProps& props,
                         hipStream_t stream) {
+    const int config = tiled_config(c);
+    if (config >= 0)
+        return c.dtype == MB_DT_FLOAT16 ? gemm_grouped_tiled_f16(c, config, stream)
+                                        : gemm_grouped_tiled_bf16(c, config, stream);
     if (c.dtype == MB_DT_FLOAT16) return launch_dtype<MB_DT_FLOAT16>(c, stream);
     return launch_dtype<MB_DT_BFLOAT16>(c, stream);
 }
