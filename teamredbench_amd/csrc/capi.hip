@@ -19,8 +19,8 @@ DeviceProps g_props[kMaxDevices];
 bool g_props_valid[kMaxDevices] = {false};
 
 // Plan overrides, -1 = the library's own choice. Process-wide, lock-free reads.
-std::atomic<int64_t> g_tuning[MB_TUNE_COUNT] = {-1, -1, -1, -1, -1, -1, -1, -1, -1, -1};
-static_assert(MB_TUNE_COUNT == 10, "initialise every knob");
+std::atomic<int64_t> g_tuning[MB_TUNE_COUNT] = {-1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1};
+static_assert(MB_TUNE_COUNT == 11, "initialise every knob");
 
 struct KnobSpec {
     const char* name;
@@ -32,15 +32,16 @@ bool is_unroll(int64_t v) { return v == 1 || v == 2 || v == 4 || v == 8; }
 bool is_threads(int64_t v) { return v >= 64 && v <= 1024 && v % 64 == 0; }
 bool is_config(int64_t v) { return v >= 0 && v <= 4; }
 bool is_splits(int64_t v) { return v >= 1 && v <= 512; }
+bool is_grouped_config(int64_t v) { return v >= 0 && v <= 5; }
 bool is_mfma(int64_t v) { return v == 16 || v == 32; }
 
 const KnobSpec kKnobs[MB_TUNE_COUNT] = {
     {"stream_unroll", is_unroll},   {"stream_nontemporal", is_bool}, {"stream_threads", is_threads},
     {"stream_schedule", is_bool},   {"gemm_force_generic", is_bool}, {"gemm_no_small_m", is_bool},
     {"gemm_tiled_config", is_config}, {"gemm_splits", is_splits},    {"gemm_fp8_mfma", is_mfma},
-    {"gemm_highp_staged", is_bool},
+    {"gemm_highp_staged", is_bool}, {"grouped_config", is_grouped_config},
 };
-constexpr int kFirstGemmKnob = MB_TUNE_GEMM_FORCE_GENERIC;
+constexpr int kFirstGemmKnob = MB_TUNE_GEMM_FORCE_GENERIC, kFirstGroupedKnob = MB_TUNE_GROUPED_CONFIG;
 
 }  // namespace
 
@@ -501,7 +502,7 @@ int mb_kernel_info(int kind, int a, int b, int64_t m, int64_t n, int64_t k, char
         j.num("workspace_bytes", (long long)plan.workspace);
         j.str("fallback", plan.fallback);
         j.str("arch", props->arch);
-        j.overrides(kFirstGemmKnob, MB_TUNE_COUNT);
+        j.overrides(kFirstGemmKnob, kFirstGroupedKnob);
         return j.emit(json, cap);
     }
     set_error("unknown kernel info kind %d", kind);

@@ -211,6 +211,7 @@ int tiled_config(const GroupedCall& c) {
     const bool weights = c.op == MB_GROUPED_GRAD_WEIGHTS;
     const int64_t x_rows = c.rows ? c.x_rows : weights ? c.total_rows : 256;
     if (x_rows > kMost / c.ldx || (weights ? c.total_rows : c.K) > kMost / c.ldy) return -1;
+    if (const int64_t forced = tuning(MB_TUNE_GROUPED_CONFIG); forced >= 0) return forced > 4 ? -1 : (int)forced;
     if (weights) return 0;
     const int64_t rows = (c.total_rows + c.experts - 1) / c.experts;
     return rows > 256 ? 0 : rows > 64 ? 2 : 3;

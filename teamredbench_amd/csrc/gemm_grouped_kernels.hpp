@@ -36,11 +36,11 @@ struct StepWaits {
 };
 
 // Loads: operand o is held in pairs (pair[o]) or stages, n[o] slots, instr[o]
-// LDS-DMA instructions per wave and slot. Step j issues, X before Y, pair
+// LDS-DMA instructions per wave and slot. Step j issues, X before Y or (y_first) after it, pair
 // (j - 1) / 2 + n of a paired operand when j is odd and stage j + n of a
 // staged one; the prologue runs the same rule over the steps before 0. Step j
 // reads stage j + 1, so its wait leaves only the loads issued after that stage's.
-constexpr StepWaits step_schedule(bool px, int nx, int ix, bool py, int ny, int iy) {
+constexpr StepWaits step_schedule(bool px, int nx, int ix, bool py, int ny, int iy, bool y_first) {
     constexpr int kSteps = 64;
     const bool pair[2] = {px, py};
     const int n[2] = {nx, ny}, instr[2] = {ix, iy};
@@ -48,7 +48,8 @@ constexpr StepWaits step_schedule(bool px, int nx, int ix, bool py, int ny, int 
     int total = 0;
     for (int v = -2 * kSteps / 4; v < kSteps; ++v) {
         if (v >= 0) before[v] = total;
-        for (int o = 0; o < 2; ++o) {
+        for (int k = 0; k < 2; ++k) {
+            const int o = y_first ? 1 - k : k;
             if (pair[o] && (v & 1) == 0) continue;
             const int i = pair[o] ? (v - 1) / 2 + n[o] : v + n[o];   // v - 1 is even
             if (i >= 0 && i < 2 * kSteps) end[o][i] = (total += instr[o]);
@@ -90,11 +91,12 @@ struct Ring {
 // Sorted row p of expert `ex` -> row of x, -1 for none.
 __device__ __forceinline__ int sorted_row(const GroupedArgs& a, const ExpertRows& ex, int p) {
     if (p >= ex.count) return -1;
-    const int r = a.rows ? a.rows[ex.first + p] : p;
+    const int r = a.rows[ex.first + p];
     return r < a.x_rows ? r : -1;
 }
 
-template <int DT, int OP, int BM, int BN, int NX, int NY, bool RAGGED_C>
+// GATHER: x is read through `rows`.
+template <int DT, int OP, int BM, int BN, int NX, int NY, bool RAGGED_C, bool GATHER>
 __global__ void __launch_bounds__(256)
 gemm_grouped_kernel(GroupedArgs args, int tiles_m_max, int tiles_n, int group_m) {
     typedef Traits<DT> Tr;
@@ -108,7 +110,9 @@ gemm_grouped_kernel(GroupedArgs args, int tiles_m_max, int tiles_n, int group_m)
     typedef Ring<YA, BN, W, NY> RY;
     constexpr int LDS_BYTES = RX::kBytes + RY::kBytes;
     static_assert(LDS_BYTES <= 160 * 1024, "LDS rings do not fit");
-    constexpr StepWaits kWaits = step_schedule(XA, NX, RX::kInstr, YA, NY, RY::kInstr);
+    // The operand with fewer slots is needed sooner after its loads: they go first.
+    constexpr bool Y_FIRST = XA == YA && NY < NX;
+    constexpr StepWaits kWaits = step_schedule(XA, NX, RX::kInstr, YA, NY, RY::kInstr, Y_FIRST);
     static_assert(kWaits.prologue >= 0 && kWaits.odd >= 0 && kWaits.even >= 0 && kWaits.prologue < 64 &&
                   kWaits.odd < 64 && kWaits.even < 64, "a needed stage is unissued, or vmcnt overflows");
     __shared__ __attribute__((aligned(1024))) unsigned char lds[LDS_BYTES];
@@ -148,12 +152,12 @@ gemm_grouped_kernel(GroupedArgs args, int tiles_m_max, int tiles_n, int group_m)
     const unsigned char* yb = args.y;
     int x_range, y_range;
     if constexpr (XA) {
-        if (args.rows == nullptr) xb += ((int64_t)ex.first + m0) * ldx;
-        x_range = ((args.rows ? args.x_rows : min(M - m0, BM)) - 1) * ldx + C * 2;
+        if constexpr (!GATHER) xb += ((int64_t)ex.first + m0) * ldx;
+        x_range = ((GATHER ? args.x_rows : min(M - m0, BM)) - 1) * ldx + C * 2;
     } else {
-        if (args.rows == nullptr) xb += (int64_t)ex.first * ldx;
+        if constexpr (!GATHER) xb += (int64_t)ex.first * ldx;
         xb += m0 * 2;
-        x_range = ((args.rows ? args.x_rows : C) - 1) * ldx + (M - m0) * 2;
+        x_range = ((GATHER ? args.x_rows : C) - 1) * ldx + (M - m0) * 2;
     }
     if constexpr (YA) {
         yb += (int64_t)ex.expert * args.K * ldy + (int64_t)n0 * ldy;
@@ -183,12 +187,12 @@ gemm_grouped_kernel(GroupedArgs args, int tiles_m_max, int tiles_n, int group_m)
         if constexpr (XA) {
             static_assert(RX::kInstr % 2 == 0 || !XA, "two swizzles serve an even number of instructions");
             const int r = lin >> 7;
-            const int row = args.rows ? sorted_row(args, ex, m0 + r) : m0 + r < M ? r : -1;
+            const int row = GATHER ? sorted_row(args, ex, m0 + r) : m0 + r < M ? r : -1;
             x_off[q] = row < 0 ? kNowhere : row * ldx + kbyte[q & 1];
         } else {
             const int r = lin / X_ROW;
             const int col = (((lin % X_ROW) >> 4) ^ b_swizzle<2, X_ROW>(r)) << 4;
-            x_off[q] = args.rows ? col : r * ldx + col;
+            x_off[q] = GATHER ? col : r * ldx + col;
         }
     }
 #pragma unroll
@@ -208,33 +212,46 @@ gemm_grouped_kernel(GroupedArgs args, int tiles_m_max, int tiles_n, int group_m)
         if constexpr (RAGGED_C) return kb + kbyte[q & 1] < C * 2 ? off : kNowhere;
         return off;
     };
-    // Gathered rows of c (matrices' gradient): the 8 of a wave's share of stage `kt`, as byte offsets.
+    // Gathered rows of c (matrices' gradient): the row numbers of a wave's 8 rows of stage `kt`, by scalar
+    // loads (lgkmcnt, so the vmcnt waits stay exact).
     constexpr int kShare = 8;
-    auto gather = [&](int kt, int (&at)[kShare]) {
-        typedef const __attribute__((address_space(4))) int32_t* ConstRows;   // scalar loads: lgkmcnt, not vmcnt
-        const ConstRows list = (ConstRows)(uintptr_t)args.rows;
+    auto gather = [&](int kt, int (&listed)[kShare]) {
+        if constexpr (WEIGHTS && GATHER) {
+            typedef int i32x8_4 __attribute__((ext_vector_type(8), aligned(4)));
+            typedef const __attribute__((address_space(4))) int32_t* ConstRows;
+            typedef const __attribute__((address_space(4))) i32x8_4* ConstRows8;
+            const ConstRows list = (ConstRows)(uintptr_t)args.rows;
+            const int first = ex.first + kt * 32 + wave * kShare;
+            if (first + kShare <= args.total) {
+                const i32x8 v = *(ConstRows8)(list + first);
 #pragma unroll
-        for (int i = 0; i < kShare; ++i) {
-            const int p = kt * 32 + wave * kShare + i;
-            const int r = list[min(ex.first + p, args.total - 1)];
-            at[i] = p < ex.count && r >= 0 && r < args.x_rows ? r * ldx : kNowhere;
+                for (int i = 0; i < kShare; ++i) listed[i] = v[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < kShare; ++i) listed[i] = list[min(first + i, args.total - 1)];
+            }
         }
     };
     // DMA instruction q of X into slot byte `at`: pair (along) or stage (across) number i.
-    auto issue_x = [&](int i, int at, auto idx, const int (&gathered)[kShare]) {
+    auto issue_x = [&](int i, int at, auto idx, const int (&listed)[kShare]) {
         constexpr int q = decltype(idx)::value;
         const unsigned to = lds_of(at) + (wave * RX::kInstr + q) * 1024;
         if constexpr (XA) {
             const int kb = i * 2 * kStageK;
             lds_dma16(rx, to, along(x_off[q], kb, q), kb);
-        } else if (args.rows != nullptr) {
+        } else if constexpr (GATHER) {
             constexpr int per = 1024 / X_ROW;   // rows of c per instruction
-            int base = gathered[q * per];
-            if constexpr (per >= 2) {
+            int base = 0;
 #pragma unroll
-                for (int s = 1; s < per; ++s) base = lane / (64 / per) == s ? gathered[q * per + s] : base;
+            for (int s = 0; s < per; ++s) {
+                const unsigned r = (unsigned)__builtin_amdgcn_readfirstlane(listed[q * per + s]);   // scalars: no indexed select
+                const int off = r < (unsigned)args.x_rows ? (int)r * ldx : kNowhere;
+                base = s == 0 || lane / (64 / per) == s ? off : base;
             }
-            lds_dma16(rx, to, base == kNowhere ? kNowhere : base + x_off[q], 0);
+            // Past the expert's rows of c: nowhere, whichever row the list names there.
+            const int p = i * 32 + wave * kShare + q * per + lane / (64 / per);
+            const int off = base + x_off[q];
+            lds_dma16(rx, to, ((base < 0) | (p >= ex.count)) ? kNowhere : off, 0);
         } else {
             lds_dma16(rx, to, x_off[q], i * 32 * ldx);
         }
@@ -309,24 +326,29 @@ gemm_grouped_kernel(GroupedArgs args, int tiles_m_max, int tiles_n, int group_m)
         ([&] {
             constexpr int v = U - V;
             constexpr int ix = XA ? (v - 1) / 2 + NX : v + NX, iy = YA ? (v - 1) / 2 + NY : v + NY;
-            if constexpr ((!XA || (v & 1) != 0) && ix >= 0) {
-                int gathered[kShare] = {};
-                if constexpr (WEIGHTS) {
-                    if (args.rows != nullptr) gather(min(ix, last), gathered);
+            auto x_loads = [&] {
+                if constexpr ((!XA || (v & 1) != 0) && ix >= 0) {
+                    const int i = min(ix, XA ? last_pair : last);
+                    int listed[kShare] = {};
+                    gather(i, listed);
+                    [&]<int... Q>(std::integer_sequence<int, Q...>) {
+                        (issue_x(i, ix * RX::kSlot, std::integral_constant<int, Q>{}, listed), ...);
+                    }(std::make_integer_sequence<int, RX::kInstr>{});
                 }
-                [&]<int... Q>(std::integer_sequence<int, Q...>) {
-                    (issue_x(min(ix, XA ? last_pair : last), ix * RX::kSlot, std::integral_constant<int, Q>{}, gathered), ...);
-                }(std::make_integer_sequence<int, RX::kInstr>{});
-            }
+            };
+            if constexpr (!Y_FIRST) x_loads();
             if constexpr ((!YA || (v & 1) != 0) && iy >= 0) {
                 [&]<int... Q>(std::integer_sequence<int, Q...>) {
                     (issue_y(min(iy, YA ? last_pair : last), Y0 + iy * RY::kSlot, std::integral_constant<int, Q>{}), ...);
                 }(std::make_integer_sequence<int, RY::kInstr>{});
             }
+            if constexpr (Y_FIRST) x_loads();
         }(), ...);
     }(std::make_integer_sequence<int, V>{});
 
     StageOps ops[2];
+    int list_sets[2][kShare] = {};   // row numbers for this step's loads and the next's
+    gather(min(NX, last), list_sets[0]);
     wait_vmcnt_and_barrier<kWaits.prologue>();
     [&]<int... R>(std::integer_sequence<int, R...>) {
         (read_op(lds, lds + Y0, std::integral_constant<int, 0>{}, std::integral_constant<int, R>{}, ops[0]), ...);
@@ -352,14 +374,12 @@ gemm_grouped_kernel(GroupedArgs args, int tiles_m_max, int tiles_n, int group_m)
         StageOps& nxt = ops[(I + 1) % 2];
         const int x_load = XA ? min((kt - 1) / 2 + NX, last_pair) : min(kt + NX, last);
         const int y_load = YA ? min((kt - 1) / 2 + NY, last_pair) : min(kt + NY, last);
-        int gathered[kShare] = {};
-        if constexpr (WEIGHTS) {
-            if (args.rows != nullptr) gather(x_load, gathered);
-        }
         [&]<int... Q>(std::integer_sequence<int, Q...>) {
             ([&] {
                 if constexpr (Q == PRE) {
                     wait_vmcnt_and_barrier<ODD ? kWaits.odd : kWaits.even>();
+                    __builtin_amdgcn_sched_barrier(0);
+                    gather(min(kt + 1 + NX, last), list_sets[(I + 1) % 2]);   // for the next step's loads
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 mfma_op(std::integral_constant<int, Q>{}, cur);
@@ -371,10 +391,11 @@ gemm_grouped_kernel(GroupedArgs args, int tiles_m_max, int tiles_n, int group_m)
                         constexpr int m = lo + R;
                         if constexpr (kIsLoad(m)) {
                             constexpr int l = (m + 1) / kStride - 1;
-                            if constexpr (l < X_LOADS)
-                                issue_x(x_load, LX * RX::kSlot, std::integral_constant<int, l>{}, gathered);
+                            constexpr int lx = Y_FIRST ? l - Y_LOADS : l, ly = Y_FIRST ? l : l - X_LOADS;
+                            if constexpr (Y_FIRST ? l >= Y_LOADS : l < X_LOADS)
+                                issue_x(x_load, LX * RX::kSlot, std::integral_constant<int, lx>{}, list_sets[I % 2]);
                             else
-                                issue_y(y_load, Y0 + LY * RY::kSlot, std::integral_constant<int, l - X_LOADS>{});
+                                issue_y(y_load, Y0 + LY * RY::kSlot, std::integral_constant<int, ly>{});
                         } else {
                             constexpr int loads_before = m / kStride < LOADS ? m / kStride : LOADS;
                             read_op(next_x, next_y, std::integral_constant<int, (I + 1) & 1>{},
@@ -447,9 +468,10 @@ struct GroupedConfig {
 
 constexpr GroupedConfig kGroupedConfigs[] = {
     {256, 256, 4, {3, 3, 5}, {4, 2, 5}},
-    {128, 256, 8, {3, 3, 6}, {6, 3, 6}},
-    {128, 128, 4, {3, 3, 6}, {6, 3, 6}},
-    {64, 128, 4, {3, 3, 6}, {6, 3, 6}},
+    {256, 128, 4, {3, 3, 5}, {6, 3, 5}},
+    {128, 128, 4, {2, 2, 5}, {6, 3, 5}},
+    {64, 128, 4, {3, 2, 5}, {6, 2, 5}},
+    {64, 64, 4, {3, 2, 5}, {6, 3, 5}},
 };
 
 template <int DT, int OP, int CFG>
@@ -465,8 +487,16 @@ int launch_grouped(const GroupedCall& c, hipStream_t stream) {
                   static_cast<unsigned char*>(c.out), c.rows, c.offsets, (int)c.ldx * 2, (int)c.ldy * 2, c.ldo * 2,
                   (int)c.x_rows, c.experts, (int)c.total_rows, (int)c.N, (int)c.K};
     const int64_t contraction = OP == MB_GROUPED_FORWARD ? c.K : c.N;
-    auto kernel = !weights && contraction % 32 != 0 ? gemm_grouped_kernel<DT, OP, cfg.bm, cfg.bn, cfg.nx[OP], cfg.ny[OP], true>
-                                                    : gemm_grouped_kernel<DT, OP, cfg.bm, cfg.bn, cfg.nx[OP], cfg.ny[OP], false>;
+    // c past the expert's rows needs no check of its own: the matrices' gradient never takes the ragged form.
+    auto pick = [&](auto gathered) {
+        constexpr bool G = decltype(gathered)::value;
+        constexpr int NX = cfg.nx[OP], NY = cfg.ny[OP];
+        if constexpr (OP != MB_GROUPED_GRAD_WEIGHTS) {
+            if (contraction % 32 != 0) return gemm_grouped_kernel<DT, OP, cfg.bm, cfg.bn, NX, NY, true, G>;
+        }
+        return gemm_grouped_kernel<DT, OP, cfg.bm, cfg.bn, NX, NY, false, G>;
+    };
+    auto kernel = c.rows ? pick(std::true_type{}) : pick(std::false_type{});
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a, (int)tiles_m, tiles_n, cfg.group_m);
     MB_HIP_TRY(hipGetLastError());
     return MB_OK;
@@ -483,7 +513,8 @@ int launch_grouped_dtype(const GroupedCall& c, int config, hipStream_t stream) {
     if (config == 0) return by_op(std::integral_constant<int, 0>{});
     if (config == 1) return by_op(std::integral_constant<int, 1>{});
     if (config == 2) return by_op(std::integral_constant<int, 2>{});
-    return by_op(std::integral_constant<int, 3>{});
+    if (config == 3) return by_op(std::integral_constant<int, 3>{});
+    return by_op(std::integral_constant<int, 4>{});
 }
 
 }  // namespace

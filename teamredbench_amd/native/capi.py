@@ -86,6 +86,7 @@ TUNING_KNOBS = {
     "gemm_splits": 7,
     "gemm_fp8_mfma": 8,
     "gemm_highp_staged": 9,
+    "grouped_config": 10,
 }
 
 # Every symbol include/mi355bench.h declares, with (restype, argtypes).
