@@ -10,6 +10,8 @@
 // takes 16 bytes at any address); the columns past the last whole 8 go one by one.
 #include "experts_common.hpp"
 
+#include <type_traits>
+
 namespace mb {
 namespace {
 
@@ -38,21 +40,23 @@ __device__ __forceinline__ void store_columns(uint16_t* row, int64_t c, int64_t 
     }
 }
 
-// One thread per 8 columns of a token.
-template <int DT>
+// One thread per 8 columns of a token: 2^lanes_log2 threads side by side on
+// one token's columns, `parts` such runs per token. K: rows in flight together.
+template <int DT, int K>
 __global__ void __launch_bounds__(kThreads)
 combine_kernel(const uint16_t* __restrict__ y, int64_t ldy, int64_t y_rows, const float* __restrict__ weights,
                const int32_t* __restrict__ slots, int64_t tokens, int top_k, int64_t N, uint16_t* __restrict__ out,
-               int64_t ldo, int chunks) {
-    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    const int64_t t = i / chunks;
-    if (t >= tokens) return;
-    const int64_t c = (i - t * chunks) * 8;
+               int64_t ldo, int lanes_log2, unsigned parts) {
+    const unsigned run = (unsigned)(((uint64_t)blockIdx.x * kThreads + threadIdx.x) >> lanes_log2);
+    const unsigned token = parts == 1 ? run : run / parts;
+    const int64_t t = token;
+    const int64_t c = ((int64_t)((run - token * parts) << lanes_log2) + (threadIdx.x & ((1u << lanes_log2) - 1))) * 8;
+    if (t >= tokens || c >= N) return;
     float sum[8] = {};
-    for (int j0 = 0; j0 < top_k; j0 += kBatch) {
-        float v[kBatch][8], w[kBatch];
+    for (int j0 = 0; j0 < top_k; j0 += K) {
+        float v[K][8], w[K];
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
+        for (int u = 0; u < K; ++u) {
             w[u] = 0.f;
             const int64_t a = t * top_k + j0 + u;
             const int64_t slot = j0 + u < top_k ? slots[a] : -1;
@@ -65,7 +69,7 @@ combine_kernel(const uint16_t* __restrict__ y, int64_t ldy, int64_t y_rows, cons
             }
         }
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u)
+        for (int u = 0; u < K; ++u)
 #pragma unroll
             for (int e = 0; e < 8; ++e) sum[e] = fmaf(w[u], v[u][e], sum[e]);
     }
@@ -139,13 +143,22 @@ combine_grad_kernel(const uint16_t* __restrict__ g, int64_t ldg, const uint16_t*
 
 int combine_launch(int dtype, const void* y, int64_t ldy, int64_t y_rows, const float* weights, const int32_t* slots,
                    int64_t tokens, int top_k, int64_t N, void* out, int64_t ldo, hipStream_t stream) {
-    const int chunks = (int)((N + 7) / 8);
-    const int64_t blocks = (tokens * chunks + kThreads - 1) / kThreads;
+    const int64_t chunks = (N + 7) / 8;
+    int lanes_log2 = 0;
+    while (lanes_log2 < 8 && (1 << lanes_log2) < chunks) ++lanes_log2;
+    const int64_t parts = (chunks + (1 << lanes_log2) - 1) >> lanes_log2;
+    const int64_t blocks = (((tokens * parts) << lanes_log2) + kThreads - 1) / kThreads;
     const auto* yp = static_cast<const uint16_t*>(y);
     auto* op = static_cast<uint16_t*>(out);
-    auto kernel = dtype == MB_DT_FLOAT16 ? combine_kernel<MB_DT_FLOAT16> : combine_kernel<MB_DT_BFLOAT16>;
+    auto pick = [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        return top_k == 1 ? combine_kernel<DT, 1> : top_k == 2 ? combine_kernel<DT, 2>
+             : top_k <= 4 ? combine_kernel<DT, 4> : combine_kernel<DT, kBatch>;
+    };
+    auto kernel = dtype == MB_DT_FLOAT16 ? pick(std::integral_constant<int, MB_DT_FLOAT16>{})
+                                         : pick(std::integral_constant<int, MB_DT_BFLOAT16>{});
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kThreads), 0, stream, yp, ldy, y_rows, weights, slots,
-                       tokens, top_k, N, op, ldo, chunks);
+                       tokens, top_k, N, op, ldo, lanes_log2, (unsigned)parts);
     MB_HIP_TRY(hipGetLastError());
     return MB_OK;
 }

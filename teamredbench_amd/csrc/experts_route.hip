@@ -1,12 +1,11 @@
 // Router: the top_k logits of each token, their softmax weights, and all
 // assignments sorted by expert (stable in token order), plus the gradient.
 //
-// Choice. One wave per token; lane l holds logits l, l + 64, ... as 64-bit keys
-// whose order is the wanted one: the logit's bits mapped so that unsigned
-// order is float order, then the complement of the expert's number, so equal logits
-// go to the lower expert and every key is distinct. -inf and NaN have key 0. Each of top_k
-// rounds takes the wave's maximum and clears it. The weights are
-// exp(l - m) / Z in fp32, m the largest logit.
+// Choice. One wave per token; lane l holds logits l PER .. l PER + PER - 1,
+// -inf for what cannot be chosen. Each of top_k rounds takes the wave's maximum
+// (six DPP steps on the vector unit, no LDS), finds the first lane that holds it and that
+// lane's first logit equal to it -- the lowest expert among equals -- and
+// clears it. The weights are exp(l - m) / Z in fp32, m the largest logit.
 //
 // Order. Within an expert, assignments stand in token order (a token has an
 // expert once), so the place of token t's assignment to expert e is the number
@@ -15,12 +14,14 @@
 // which tokens of the group chose it, its population count is the group's
 // count, and the count below bit t is t's rank. Masks are built with LDS
 // ORs, whose result does not depend on their order. At most kMaxBlocks
-// blocks, each over a run of groups, write their counts per expert;
-// a second kernel adds up the counts of earlier blocks and of lower experts and places.
-// One block (up to 64 tokens) does both in one launch.
+// blocks, each over a run of groups, write their counts per expert ([expert][block]);
+// a second kernel adds up the counts of earlier blocks and of lower experts
+// (a wave per expert, a block's count a lane) and places. One block (up to 64 tokens) does both in
+// one launch.
 #include "experts_common.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace mb {
 namespace {
@@ -39,27 +40,46 @@ __device__ __forceinline__ float load_logit(const void* p, int64_t i) {
 // Whether a logit can be chosen; +inf counts as the largest finite value.
 __device__ __forceinline__ bool usable(float v) { return v > -__builtin_inff(); }   // false for NaN
 
-// Float order as unsigned order; every usable logit maps above 0.
-__device__ __forceinline__ unsigned ordered(float v) {
-    const unsigned b = __builtin_bit_cast(unsigned, v == 0.f ? 0.f : v);   // -0 and +0 tie
-    return (b >> 31) ? ~b : b | 0x80000000u;
+// Lane 63's value of a reduction over the wave, by DPP: shifts by 1, 2, 4 and 8
+// within rows of 16 lanes, then each row's last lane to the next row(s). Lanes without a source take `none`.
+template <class Op>
+__device__ __forceinline__ float wave_reduce(float v, float none, Op op) {
+    const auto moved = [&](auto ctrl, float x) {
+        return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none),
+                                                                     __builtin_bit_cast(int, x),
+                                                                     decltype(ctrl)::value, 0xF, 0xF, false));
+    };
+    v = op(v, moved(std::integral_constant<int, 0x111>{}, v));   // row_shr:1
+    v = op(v, moved(std::integral_constant<int, 0x112>{}, v));
+    v = op(v, moved(std::integral_constant<int, 0x114>{}, v));
+    v = op(v, moved(std::integral_constant<int, 0x118>{}, v));   // row_shr:8
+    v = op(v, moved(std::integral_constant<int, 0x142>{}, v));   // row_bcast:15
+    v = op(v, moved(std::integral_constant<int, 0x143>{}, v));   // row_bcast:31
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
-__device__ __forceinline__ float unordered(unsigned u) {
-    return __builtin_bit_cast(float, (u >> 31) ? u & 0x7FFFFFFFu : ~u);
+__device__ __forceinline__ float wave_max(float v) {
+    return wave_reduce(v, -__builtin_inff(), [](float a, float b) { return fmaxf(a, b); });
 }
-
-__device__ __forceinline__ uint64_t wave_max(uint64_t v) {
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) {
-        const uint64_t o = __shfl_xor(v, d);
-        v = o > v ? o : v;
-    }
-    return v;
-}
+// The row_bcast steps add a row's total into every lane of the next row(s): in lane 63, each lane's value once.
 __device__ __forceinline__ float wave_sum(float v) {
+    return wave_reduce(v, 0.f, [](float a, float b) { return a + b; });
+}
+__device__ __forceinline__ int wave_sum(int v) {
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
     return v;
+}
+
+// Logits l PER .. of a token as this lane holds them: -inf for what cannot be chosen.
+template <int DT, int PER>
+__device__ __forceinline__ void load_logits(const void* logits, int64_t base, int experts, int lane, float* v) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int e = lane * PER + i;
+        v[i] = e < experts ? load_logit<DT>(logits, base + e) : -__builtin_inff();
+        if (v[i] > kLargest) v[i] = kLargest;
+        if (!usable(v[i])) v[i] = -__builtin_inff();
+    }
 }
 
 // One token's choices by one wave: ids and weights of its top_k, written by lane j. Returns lane
@@ -67,43 +87,42 @@ __device__ __forceinline__ float wave_sum(float v) {
 template <int DT, int PER>
 __device__ __forceinline__ int choose(const void* logits, int64_t base, int experts, int top_k, bool normalize,
                                       float* weights, int32_t* ids, int lane) {
-    uint64_t key[PER];
+    float v[PER], left[PER];
+    load_logits<DT, PER>(logits, base, experts, lane, v);
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const int e = lane + 64 * i;
-        float v = e < experts ? load_logit<DT>(logits, base + e) : -__builtin_inff();
-        if (v > kLargest) v = kLargest;
-        key[i] = usable(v) ? ((uint64_t)ordered(v) << 32) | (unsigned)~e : 0;
-    }
-    uint64_t local[PER];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) local[i] = key[i];
-    uint64_t mine = 0;   // choice `lane` of the token
-    float m = 0.f;
+    for (int i = 0; i < PER; ++i) left[i] = v[i];
+    float mine = -__builtin_inff(), m = 0.f;   // choice `lane` of the token; the largest logit
+    int id = -1;
     for (int j = 0; j < top_k; ++j) {
-        uint64_t best = local[0];
+        float best = left[0];
 #pragma unroll
-        for (int i = 1; i < PER; ++i) best = local[i] > best ? local[i] : best;
-        best = wave_max(best);
-        if (j == 0) m = unordered((unsigned)(best >> 32));
-        if (best == 0) break;   // uniform: no logit left
+        for (int i = 1; i < PER; ++i) best = fmaxf(best, left[i]);
+        const float top = wave_max(best);
+        if (!usable(top)) break;   // uniform: no logit left
+        if (j == 0) m = top;
+        const int owner = __builtin_ctzll(__ballot(best == top));
+        int at = 0;
+#pragma unroll
+        for (int i = PER - 1; i >= 0; --i) at = left[i] == top ? i : at;
+        const int e = owner * PER + __builtin_amdgcn_readlane(at, owner);
 #pragma unroll
         for (int i = 0; i < PER; ++i)
-            if (local[i] == best) local[i] = 0;
-        if (lane == j) mine = best;
+            if (lane * PER + i == e) left[i] = -__builtin_inff();
+        if (lane == j) {
+            mine = top;
+            id = e;
+        }
     }
-    const float e_mine = mine ? expf(unordered((unsigned)(mine >> 32)) - m) : 0.f;
+    const float e_mine = id >= 0 ? expf(mine - m) : 0.f;
     float z = e_mine;
     if (!normalize) {
         z = 0.f;
 #pragma unroll
-        for (int i = 0; i < PER; ++i)
-            if (key[i]) z += expf(unordered((unsigned)(key[i] >> 32)) - m);
+        for (int i = 0; i < PER; ++i) z += usable(v[i]) ? expf(v[i] - m) : 0.f;
     }
     z = wave_sum(z);
-    const int id = mine ? (int)~(unsigned)mine : -1;
     if (lane < top_k) {
-        weights[lane] = mine ? e_mine / z : 0.f;
+        weights[lane] = id >= 0 ? e_mine / z : 0.f;
         ids[lane] = id;
     }
     return id;
@@ -184,28 +203,34 @@ route_choose_kernel(const void* __restrict__ logits, int64_t ld, int64_t tokens,
         for (int p = start[experts] + threadIdx.x; p < (int)tokens * top_k; p += blockDim.x) rows[p] = -1;
         place(masks, start, 0, tokens, top_k, ids, rows, slots);
     } else {
-        for (int e = threadIdx.x; e < experts; e += blockDim.x) counts[(int64_t)blockIdx.x * experts + e] = count[e];
+        for (int e = threadIdx.x; e < experts; e += blockDim.x) counts[(int64_t)e * gridDim.x + blockIdx.x] = count[e];
     }
 }
 
 // Places every block's assignments: the counts of all blocks give offsets,
 // those of earlier blocks this block's start in each expert.
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(64 * kWaves)
 route_place_kernel(const int32_t* __restrict__ counts, int blocks, int64_t tokens, int experts, int top_k,
                    int groups_per_block, const int32_t* __restrict__ ids, int32_t* __restrict__ offsets,
                    int32_t* __restrict__ rows, int32_t* __restrict__ slots) {
     __shared__ uint64_t masks[MB_ROUTE_MAX_EXPERTS];
     __shared__ int total[MB_ROUTE_MAX_EXPERTS], start[MB_ROUTE_MAX_EXPERTS + 1], earlier[MB_ROUTE_MAX_EXPERTS];
     const int64_t groups = (tokens + kGroup - 1) / kGroup;
-    for (int e = threadIdx.x; e < experts; e += blockDim.x) {
+    const int lane = threadIdx.x & 63;
+    for (int e = threadIdx.x >> 6; e < experts; e += kWaves) {
         int before = 0, all = 0;
-        for (int b = 0; b < blocks; ++b) {
-            const int c = counts[(int64_t)b * experts + e];
-            if (b < (int)blockIdx.x) before += c;
+#pragma unroll
+        for (int b0 = 0; b0 < kMaxBlocks; b0 += 64) {
+            const int b = b0 + lane, c = b < blocks ? counts[(int64_t)e * blocks + b] : 0;
+            before += b < (int)blockIdx.x ? c : 0;
             all += c;
         }
-        earlier[e] = before;
-        total[e] = all;
+        before = wave_sum(before);
+        all = wave_sum(all);
+        if (lane == 0) {
+            earlier[e] = before;
+            total[e] = all;
+        }
     }
     __syncthreads();
     prefix(total, start, experts);
@@ -254,34 +279,30 @@ route_grad_kernel(const void* __restrict__ logits, int64_t ld, const int32_t* __
         if (id < 0 || id >= experts) id = -1;
     }
     float v[PER], gv[PER];
-    bool live[PER], chosen[PER];
-    float m = -kLargest;
+    bool chosen[PER];
+    load_logits<DT, PER>(logits, token * ld, experts, lane, v);
+    float m = -__builtin_inff();
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        const int e = lane + 64 * i;
-        v[i] = e < experts ? load_logit<DT>(logits, token * ld + e) : -__builtin_inff();
-        if (v[i] > kLargest) v[i] = kLargest;
-        live[i] = usable(v[i]);
         chosen[i] = false;
         gv[i] = 0.f;
-        if (live[i]) m = fmaxf(m, v[i]);
+        m = fmaxf(m, v[i]);
     }
     for (int j = 0; j < top_k; ++j) {
-        const int c = __shfl(id, j);
-        const float gj = __shfl(g, j);
+        const int c = __builtin_amdgcn_readlane(id, j);
+        const float gj = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, g), j));
 #pragma unroll
         for (int i = 0; i < PER; ++i)
-            if (c == lane + 64 * i) {
+            if (c == lane * PER + i) {
                 chosen[i] = true;
                 gv[i] = gj;
             }
     }
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+    m = wave_max(m);
     float p[PER], z = 0.f, dot = 0.f;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        p[i] = live[i] && (chosen[i] || !normalize) ? expf(v[i] - m) : 0.f;
+        p[i] = usable(v[i]) && (chosen[i] || !normalize) ? expf(v[i] - m) : 0.f;
         z += p[i];
         dot += p[i] * gv[i];
     }
@@ -291,7 +312,7 @@ route_grad_kernel(const void* __restrict__ logits, int64_t ld, const int32_t* __
     dot *= inv;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        const int e = lane + 64 * i;
+        const int e = lane * PER + i;
         if (e >= experts) continue;
         const float out = p[i] * inv * (gv[i] - dot);
         if constexpr (DT == MB_DT_FLOAT32) static_cast<float*>(grad_logits)[token * ld_grad + e] = out;
@@ -346,7 +367,7 @@ int route_launch(int dtype, const void* logits, int64_t ld, int64_t tokens, int 
                                logits, ld, tokens, experts, top_k, (int)normalize, per_block, weights, expert_ids,
                                counts, offsets, rows, slots);
             MB_HIP_TRY(hipGetLastError());
-            hipLaunchKernelGGL(route_place_kernel, dim3(blocks), dim3(256), 0, stream, counts, blocks, tokens, experts,
+            hipLaunchKernelGGL(route_place_kernel, dim3(blocks), dim3(64 * kWaves), 0, stream, counts, blocks, tokens, experts,
                                top_k, per_block, expert_ids, offsets, rows, slots);
             MB_HIP_TRY(hipGetLastError());
             return (int)MB_OK;
