@@ -21,10 +21,15 @@
 // groups: a 4 x 4 transpose between the four 16-lane groups, four
 // lane-swap instructions per 16 bytes.
 //
-// Waves of a block split K in units of 256 (whole 128-byte lines of a column)
-// and add their fp32 sums through LDS, in wave order. Rows that are not there
-// multiply some other row's x and are stored as zeros; units that run past K
-// take zeros for x and whatever weights lie there in bounds.
+// Up to 16 rows per expert (gemm_w4_kernel): the waves of a block share 32
+// columns and split K in units of 128, x
+// comes straight from L2 with the weights, both one unit ahead, and the waves add their fp32 sums
+// through LDS, in wave order. More rows (gemm_w4_rows_kernel): the waves
+// split 256 columns and share x through LDS, 256 k at a time, with the sums of x made on the way in.
+// Few columns: blocks split K too, into fp32 planes that a second kernel adds.
+//
+// Rows that are not there multiply some other row's x and are stored as zeros;
+// units that run past K take zeros for x and whatever weights lie there in bounds.
 #include "experts_common.hpp"
 
 #include <algorithm>
@@ -34,7 +39,6 @@ namespace mb {
 namespace {
 
 typedef u32x4 u32x4_byte __attribute__((aligned(1)));   // 16 bytes at any address
-constexpr int kUnit = 256;   // k per step of a wave
 
 template <int DT>
 __device__ __forceinline__ f32x4 mfma16(const u32x4& a, const u32x4& b, f32x4 c) {
@@ -79,86 +83,318 @@ __device__ __forceinline__ u32x4 reorder(const u32x4& v) {
                  __builtin_amdgcn_perm(v[3], v[1], 0x05040100u), __builtin_amdgcn_perm(v[3], v[1], 0x07060302u)};
 }
 
-// SPU: scales per unit and column when groups divide a unit evenly (256 / group), or 1 for groups of
-// whole units; 0 for any other group: one scale looked up per 32 k.
-template <int DT, bool ZEROS, int RT, int CT, int SPU, int W>
-__global__ void __launch_bounds__(64 * W)
-gemm_w4_kernel(const uint16_t* __restrict__ x, int64_t ldx, int64_t x_rows, const int32_t* __restrict__ rows,
-               const uint8_t* __restrict__ q, const uint16_t* __restrict__ scales, const uint16_t* __restrict__ zeros,
-               int group, uint16_t* __restrict__ out, int64_t ldo, const int32_t* __restrict__ offsets, int experts,
-               int total, int N, int K, int blocks_n) {
-    constexpr bool SUMS = DT == MB_DT_BFLOAT16 || ZEROS;     // the group's sum of x is needed
-    constexpr int STEPS = kUnit / 32;                         // MFMA steps of 32 k per unit
-    constexpr int PER = SPU > 0 ? STEPS / SPU : 1;            // steps per scale
-    constexpr int NS = STEPS / PER;
-    constexpr float kOffset = DT == MB_DT_BFLOAT16 ? 128.f : -8.f;   // the float of q is q + kOffset
-    __shared__ f32x4 red[W][RT * CT][64];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int c = lane & 15, g = lane >> 4;
-    const int tile = (int)blockIdx.x / blocks_n;
-    const int n0 = ((int)blockIdx.x - tile * blocks_n) * 16 * CT;
-    ExpertRows ex{0, 0, total};
-    int in_expert = tile;
-    if (offsets != nullptr && !find_row_tile(offsets, experts, total, tile, 16 * RT, &ex, &in_expert)) return;
-    const int p0 = ex.first + in_expert * 16 * RT, count = min(16 * RT, ex.count - in_expert * 16 * RT);
-    const int bytes = (K + 1) / 2, groups = (K + group - 1) / group;
+// sum + the two 16-bit floats of a dword, in fp32.
+template <int DT>
+__device__ __forceinline__ float add_pair(unsigned v, float sum) {
+    if constexpr (DT == MB_DT_FLOAT16) {
+        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, v), (f16x2){(_Float16)1.f, (_Float16)1.f}, sum, false);
+    } else {
+        return sum + __builtin_bit_cast(float, v << 16) + __builtin_bit_cast(float, v & 0xFFFF0000u);
+    }
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp_move(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, false));
+}
 
-    // Columns past N read the last one's weights and are not stored.
+// Bytes `at` .. + 15 of `bytes` bytes at p, zeros past their end: the last 16
+// of them shifted down, since nothing past the end may be read.
+__device__ __forceinline__ u32x4 window16(const uint8_t* p, int at, int bytes) {
+    if (bytes >= 16) {
+        const int from = min(at, bytes - 16), shift = at - from;
+        const u32x4 v = *reinterpret_cast<const u32x4_byte*>(p + from);
+        const __uint128_t wide = __builtin_bit_cast(__uint128_t, v);
+        return shift < 16 ? __builtin_bit_cast(u32x4, wide >> (8 * shift)) : u32x4{0u, 0u, 0u, 0u};
+    }
+    __uint128_t wide = 0;
+#pragma unroll 1
+    for (int b = bytes - 1; b >= at; --b) wide = (wide << 8) | p[b];
+    return __builtin_bit_cast(u32x4, wide);
+}
+
+// 8 consecutive elements of x's row from k on, zeros past K.
+__device__ __forceinline__ u32x4 load_x(const uint16_t* row, int k, int K) {
+    return window16(reinterpret_cast<const uint8_t*>(row), 2 * k, 2 * K);
+}
+
+// One operand pointer set of a block, and the loads every kernel here makes.
+// UNIT: k per step of a wave. SPU: scales per unit and column when groups divide a unit evenly (UNIT /
+// group), or 1 for groups of whole units; 0 for any other group: one scale looked up per 32 k.
+template <int DT, bool ZEROS, int CT, int UNIT, int SPU>
+struct Weights {
+    static constexpr int CHUNKS = UNIT / 128;                    // 16-byte loads per unit and column tile
+    static constexpr int STEPS = UNIT / 32;                     // MFMA steps of 32 k per unit
+    static constexpr int PER = SPU > 0 ? STEPS / SPU : 1;        // steps per scale
+    static constexpr int NS = STEPS / PER;                       // scales per unit and column
+    static constexpr bool SUMS = DT == MB_DT_BFLOAT16 || ZEROS;  // the group's sum of x is needed
+    static constexpr float kOffset = DT == MB_DT_BFLOAT16 ? 128.f : -8.f;   // the float of q is q + kOffset
+    typedef uint16_t Scales __attribute__((ext_vector_type(NS)));
+    struct Unit {
+        u32x4 q[CT][CHUNKS];
+        Scales s[CT], z[CT];
+    };
+
     const uint8_t* qp[CT];
-    int64_t sp[CT];
+    const uint16_t *sp[CT], *zp[CT];
+    int bytes, groups, group, K, g;
+
+    // Columns n0 + 16 t + c of expert `expert`; those past N read the last one's weights and are not stored.
+    __device__ __forceinline__ Weights(const uint8_t* q, const uint16_t* scales, const uint16_t* zeros, int group_,
+                                       int expert, int n0, int N, int K_, int lane)
+        : bytes((K_ + 1) / 2), groups((K_ + group_ - 1) / group_), group(group_), K(K_), g(lane >> 4) {
 #pragma unroll
-    for (int t = 0; t < CT; ++t) {
-        const int64_t column = (int64_t)ex.expert * N + min(n0 + 16 * t + c, N - 1);
-        qp[t] = q + column * bytes;
-        sp[t] = column * groups;
-    }
-    const uint16_t* xp[RT];
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-        const int r = min(16 * t + c, count - 1);
-        const int64_t row = rows ? rows[p0 + r] : p0 + r;
-        xp[t] = x + (row >= 0 && row < x_rows ? row : 0) * ldx;
+        for (int t = 0; t < CT; ++t) {
+            const int64_t column = (int64_t)expert * N + min(n0 + 16 * t + (lane & 15), N - 1);
+            qp[t] = q + column * bytes;
+            sp[t] = scales + column * groups;
+            zp[t] = ZEROS ? zeros + column * groups : nullptr;
+        }
     }
 
-    auto load_q = [&](int k0, u32x4 (&v)[CT][2]) {
+    __device__ __forceinline__ void load(int k0, Unit& u) const {
+        if (k0 + UNIT <= K) {   // uniform
+#pragma unroll
+            for (int t = 0; t < CT; ++t)
+#pragma unroll
+                for (int h = 0; h < CHUNKS; ++h)
+                    u.q[t][h] = *reinterpret_cast<const u32x4_byte*>(qp[t] + k0 / 2 + 64 * h + 16 * g);
+        } else {
+#pragma unroll
+            for (int t = 0; t < CT; ++t)
+#pragma unroll
+                for (int h = 0; h < CHUNKS; ++h) u.q[t][h] = window16(qp[t], k0 / 2 + 64 * h + 16 * g, bytes);
+        }
+#pragma unroll
+        for (int t = 0; t < CT; ++t) {
+            load_scales(sp[t], k0, u.s[t]);
+            if constexpr (ZEROS) load_scales(zp[t], k0, u.z[t]);
+        }
+    }
+    // A unit's scales: one load, on any element, where the unit has them all.
+    __device__ __forceinline__ void load_scales(const uint16_t* from, int k0, Scales& v) const {
+        if constexpr (SPU > 1) {
+            const int at = k0 / UNIT * SPU;
+            if (at + SPU <= groups) {   // uniform
+                typedef Scales Any __attribute__((aligned(2)));
+                v = *reinterpret_cast<const Any*>(from + at);
+            } else {
+#pragma unroll
+                for (int i = 0; i < NS; ++i) v[i] = from[min(at + i, groups - 1)];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NS; ++i) v[i] = from[min((k0 + i * PER * 32) / group, groups - 1)];
+        }
+    }
+};
+
+// Row of x of sorted row p; -1 for none.
+__device__ __forceinline__ int64_t x_row(const int32_t* rows, int64_t x_rows, int p) {
+    const int64_t r = rows ? rows[p] : p;
+    return r < x_rows ? r : -1;
+}
+
+struct W4Args {
+    const uint16_t* x;
+    const int32_t *rows, *offsets;
+    const uint8_t* q;
+    const uint16_t *scales, *zeros;
+    uint16_t* out;
+    float* planes;       // K splits' partial sums, [split][total][ldp]; NULL without
+    int64_t ldx, ldo, x_rows;
+    int group, experts, total, N, K, blocks_n, splits, ldp;
+};
+
+// The tile of a block: its rows, first column and units of K. False if there is none.
+struct W4Tile {
+    int expert, p0, count, n0, split, first_unit, units, turn;
+
+    // Unit number i of the block: neighbouring blocks start elsewhere in their columns (whose length is often a
+    // power of two), or all would read the same few memory channels at a time.
+    __device__ __forceinline__ int unit(int i) const {
+        const int u = i + turn;
+        return first_unit + (u < units ? u : u - units);
+    }
+};
+__device__ __forceinline__ bool w4_tile(const W4Args& a, int rows_per_tile, int columns, int unit, W4Tile* t) {
+    int b = (int)blockIdx.x;
+    t->split = b % a.splits;
+    b /= a.splits;
+    const int tile = b / a.blocks_n;
+    t->n0 = (b - tile * a.blocks_n) * columns;
+    ExpertRows ex{0, 0, a.total};
+    int in_expert = tile;
+    if (a.offsets != nullptr && !find_row_tile(a.offsets, a.experts, a.total, tile, rows_per_tile, &ex, &in_expert))
+        return false;
+    t->expert = ex.expert;
+    t->p0 = ex.first + in_expert * rows_per_tile;
+    t->count = min(rows_per_tile, ex.count - in_expert * rows_per_tile);
+    const int units = a.x_rows > 0 ? (a.K + unit - 1) / unit : 0;   // without any row of x there is nothing to add
+    t->first_unit = (int)((int64_t)units * t->split / a.splits);
+    t->units = (int)((int64_t)units * (t->split + 1) / a.splits) - t->first_unit;
+    t->turn = t->units > 0 ? b % t->units : 0;
+    return true;
+}
+
+// Rows 4 (l / 16) + r of row tile i, column 16 j + l % 16: rounded to out, or as they are to the split's plane.
+template <int DT>
+__device__ __forceinline__ void w4_store(const W4Args& a, const W4Tile& t, int i, int j, const f32x4& v, int lane) {
+    const int n = t.n0 + 16 * j + (lane & 15);
+    if (n >= a.N) return;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int p = 16 * i + 4 * (lane >> 4) + r;
+        if (p >= t.count) continue;
+        const bool there = x_row(a.rows, a.x_rows, t.p0 + p) >= 0;
+        if (a.planes != nullptr)
+            a.planes[((int64_t)t.split * a.total + t.p0 + p) * a.ldp + n] = there ? v[r] : 0.f;
+        else
+            a.out[(t.p0 + p) * a.ldo + n] = there ? to_bits<DT>(v[r]) : 0;
+    }
+}
+
+// acc += s * dot - s (offset + z) * sum for one group, 4 rows.
+template <class W, int DT, bool ZEROS>
+__device__ __forceinline__ void add_group(const typename W::Unit& u, int t, int i, const f32x4& dot, const f32x4& sum,
+                                          f32x4& acc) {
+    const float s = from_bits<DT>(u.s[t][i]);
+    const float z = ZEROS ? from_bits<DT>(u.z[t][i]) : 8.f;
+    const float off = -s * (W::kOffset + z);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        acc[r] = fmaf(s, dot[r], acc[r]);
+        if constexpr (W::SUMS) acc[r] = fmaf(off, sum[r], acc[r]);
+    }
+}
+
+template <int DT, bool ZEROS, int CT, int UNIT, int SPU, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES)
+gemm_w4_kernel(W4Args a) {
+    typedef Weights<DT, ZEROS, CT, UNIT, SPU> W;
+    __shared__ f32x4 red[WAVES][CT][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    W4Tile tile;
+    if (!w4_tile(a, 16, 16 * CT, UNIT, &tile)) return;
+    const W weights(a.q, a.scales, a.zeros, a.group, tile.expert, tile.n0, a.N, a.K, lane);
+    const int64_t row = x_row(a.rows, a.x_rows, tile.p0 + min(lane & 15, tile.count - 1));
+    const uint16_t* xp = a.x + max(row, (int64_t)0) * a.ldx + 8 * (lane >> 4);
+    const u32x4 ones = DT == MB_DT_FLOAT16 ? u32x4{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u}
+                                           : u32x4{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
+    auto fetch = [&](int u, u32x4 (&v)[W::STEPS]) {
+        const int k0 = u * UNIT;
+        if (k0 + UNIT <= a.K) {
+#pragma unroll
+            for (int s = 0; s < W::STEPS; ++s) v[s] = *reinterpret_cast<const u32x4_any*>(xp + k0 + 32 * s);
+        } else {
+#pragma unroll
+            for (int s = 0; s < W::STEPS; ++s)
+                v[s] = load_x(xp - 8 * (lane >> 4), k0 + 32 * s + 8 * (lane >> 4), a.K);
+        }
+    };
+    f32x4 acc[CT];
+#pragma unroll
+    for (int t = 0; t < CT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto compute = [&](typename W::Unit& w, const u32x4 (&xv)[W::STEPS]) {
 #pragma unroll
         for (int t = 0; t < CT; ++t)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int at = k0 / 2 + 64 * h + 16 * g;
-                if (at + 16 <= bytes) {
-                    v[t][h] = *reinterpret_cast<const u32x4_byte*>(qp[t] + at);
-                } else {
-                    u32x4 p = {0u, 0u, 0u, 0u};
+            for (int h = 0; h < W::CHUNKS; ++h) w.q[t][h] = transpose_groups(w.q[t][h]);
+        f32x4 dot[CT], sum;
 #pragma unroll
-                    for (int b = 0; b < 15; ++b)
-                        if (at + b < bytes) p[b >> 2] |= (unsigned)qp[t][at + b] << (8 * (b & 3));
-                    v[t][h] = p;
-                }
+        for (int s = 0; s < W::STEPS; ++s) {
+            if (s % W::PER == 0) {
+                sum = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int t = 0; t < CT; ++t) dot[t] = f32x4{0.f, 0.f, 0.f, 0.f};
             }
-    };
-    auto load_x = [&](int t, int k, auto whole) -> u32x4 {   // k .. k + 7 of row tile t's row
-        if (decltype(whole)::value || k + 8 <= K) return *reinterpret_cast<const u32x4_any*>(xp[t] + k);
-        u32x4 p = {0u, 0u, 0u, 0u};
+            const u32x4 x = reorder(xv[s]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (k + e < K) p[e >> 1] |= (unsigned)xp[t][k + e] << (16 * (e & 1));
-        return p;
-    };
-    // Scale (zero point) number i of a unit and column tile t.
-    auto load_scales = [&](const uint16_t* from, int t, int k0, auto whole, uint16_t (&v)[NS]) {
-        if constexpr (SPU > 1) {
-            if (decltype(whole)::value) {
-                typedef uint16_t vec __attribute__((ext_vector_type(SPU)));
-                typedef vec vec_any __attribute__((aligned(2)));
-                const vec s = *reinterpret_cast<const vec_any*>(from + sp[t] + k0 / kUnit * SPU);
+            for (int t = 0; t < CT; ++t) dot[t] = mfma16<DT>(x, widen<DT>(w.q[t][s >> 2][s & 3]), dot[t]);
+            if constexpr (W::SUMS) sum = mfma16<DT>(x, ones, sum);
+            if (s % W::PER == W::PER - 1) {
 #pragma unroll
-                for (int i = 0; i < NS; ++i) v[i] = s[i];
-                return;
+                for (int t = 0; t < CT; ++t) add_group<W, DT, ZEROS>(w, t, s / W::PER, dot[t], sum, acc[t]);
             }
         }
+    };
+    // A unit's weights go out before the one ahead of it is computed.
+    typename W::Unit now, next;
+    if (wave < tile.units) weights.load(tile.unit(wave) * UNIT, next);
+#pragma unroll 1
+    for (int u = wave; u < tile.units; u += WAVES) {
+        u32x4 xv[W::STEPS];
+        now = next;
+        fetch(tile.unit(u), xv);
+        if (u + WAVES < tile.units) weights.load(tile.unit(u + WAVES) * UNIT, next);
+        compute(now, xv);
+    }
 #pragma unroll
-        for (int i = 0; i < NS; ++i) v[i] = from[sp[t] + min((k0 + i * PER * 32) / group, groups - 1)];
+    for (int t = 0; t < CT; ++t) red[wave][t][lane] = acc[t];
+    __syncthreads();
+    if (wave < CT) {
+        f32x4 v = red[0][wave][lane];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) v += red[w][wave][lane];
+        w4_store<DT>(a, tile, 0, wave, v, lane);
+    }
+}
+
+// 16 RT rows; WAVES waves of CT x 16 columns each.
+template <int DT, bool ZEROS, int RT, int CT, int UNIT, int SPU, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES)
+gemm_w4_rows_kernel(W4Args a) {
+    typedef Weights<DT, ZEROS, CT, UNIT, SPU> W;
+    constexpr int ROWS = 16 * RT;
+    constexpr int PITCH = UNIT * 2 + 16;              // bytes per row: 16 rows' 16-byte reads hit all banks once
+    constexpr int PIECES = UNIT / 8;                  // 16-byte pieces per row and unit
+    constexpr int STRIDE = 64 * WAVES / PIECES;       // rows staged at once
+    constexpr int LOADS = ROWS / STRIDE;
+    static_assert(ROWS % STRIDE == 0, "rows must split over the threads");
+    __shared__ __attribute__((aligned(16))) unsigned char xs[2][ROWS * PITCH];
+    __shared__ __attribute__((aligned(16))) float sums[2][W::NS][ROWS];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    W4Tile tile;
+    if (!w4_tile(a, ROWS, 16 * CT * WAVES, UNIT, &tile)) return;
+    tile.n0 += 16 * CT * wave;
+    const W weights(a.q, a.scales, a.zeros, a.group, tile.expert, tile.n0, a.N, a.K, lane);
+
+    // Staging: thread t brings piece t % PIECES of rows t / PIECES + STRIDE i.
+    const int piece = tid % PIECES, first_row = tid / PIECES;
+    const uint16_t* xp[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+        const int64_t row = x_row(a.rows, a.x_rows, tile.p0 + min(first_row + STRIDE * i, tile.count - 1));
+        xp[i] = a.x + max(row, (int64_t)0) * a.ldx;
+    }
+    auto fetch = [&](int u, u32x4 (&v)[LOADS]) {
+        const int k = u * UNIT + 8 * piece;
+        if ((u + 1) * UNIT <= a.K) {
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) v[i] = *reinterpret_cast<const u32x4_any*>(xp[i] + k);
+        } else {
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) v[i] = load_x(xp[i], k, a.K);
+        }
+    };
+    auto stage = [&](int slot, const u32x4 (&v)[LOADS]) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int row = first_row + STRIDE * i;
+            *reinterpret_cast<u32x4*>(xs[slot] + row * PITCH + 16 * piece) = reorder(v[i]);
+            if constexpr (W::SUMS) {
+                float sum = 0.f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum = add_pair<DT>(v[i][e], sum);
+                // A group's 4 PER pieces lie in neighbouring lanes: rotations within them add up in each.
+                sum += dpp_move<0xB1>(sum);                          // quad_perm 1 0 3 2
+                sum += dpp_move<0x4E>(sum);                          // quad_perm 2 3 0 1
+                if constexpr (W::PER >= 2) sum += dpp_move<0x141>(sum);   // row_half_mirror
+                if constexpr (W::PER >= 4) sum += dpp_move<0x140>(sum);   // row_mirror
+                if constexpr (W::PER >= 8) sum += __shfl_xor(sum, 16);
+                if (piece % (4 * W::PER) == 0) sums[slot][piece / (4 * W::PER)][row] = sum;
+            }
+        }
     };
 
     f32x4 acc[RT][CT];
@@ -166,136 +402,155 @@ gemm_w4_kernel(const uint16_t* __restrict__ x, int64_t ldx, int64_t x_rows, cons
     for (int i = 0; i < RT; ++i)
 #pragma unroll
         for (int j = 0; j < CT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const u32x4 ones = DT == MB_DT_FLOAT16 ? u32x4{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u}
-                                           : u32x4{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
-
-    auto unit = [&](int k0, u32x4 (&w)[CT][2], auto whole) {
-        uint16_t sv[CT][NS], zv[CT][NS];
-#pragma unroll
-        for (int t = 0; t < CT; ++t) {
-            load_scales(scales, t, k0, whole, sv[t]);
-            if constexpr (ZEROS) load_scales(zeros, t, k0, whole, zv[t]);
-        }
+    const int c = lane & 15, g = lane >> 4;
+    auto compute = [&](int slot, typename W::Unit& w) {
 #pragma unroll
         for (int t = 0; t < CT; ++t)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) w[t][h] = transpose_groups(w[t][h]);
-        f32x4 dot[RT][CT], sum[RT];
+            for (int h = 0; h < W::CHUNKS; ++h) w.q[t][h] = transpose_groups(w.q[t][h]);
+        f32x4 dot[RT][CT];
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s) {
-            if (s % PER == 0) {
+        for (int s = 0; s < W::STEPS; ++s) {
+            if (s % W::PER == 0) {
 #pragma unroll
-                for (int i = 0; i < RT; ++i) {
-                    sum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int i = 0; i < RT; ++i)
 #pragma unroll
                     for (int j = 0; j < CT; ++j) dot[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-                }
             }
-            u32x4 xv[RT];
+            u32x4 x[RT];
 #pragma unroll
-            for (int i = 0; i < RT; ++i) xv[i] = reorder(load_x(i, k0 + 32 * s + 8 * g, whole));
+            for (int i = 0; i < RT; ++i)
+                x[i] = *reinterpret_cast<const u32x4*>(xs[slot] + (16 * i + c) * PITCH + 64 * s + 16 * g);
 #pragma unroll
             for (int j = 0; j < CT; ++j) {
-                const u32x4 wv = widen<DT>(w[j][s >> 2][s & 3]);
+                const u32x4 wv = widen<DT>(w.q[j][s >> 2][s & 3]);
 #pragma unroll
-                for (int i = 0; i < RT; ++i) dot[i][j] = mfma16<DT>(xv[i], wv, dot[i][j]);
+                for (int i = 0; i < RT; ++i) dot[i][j] = mfma16<DT>(x[i], wv, dot[i][j]);
             }
-            if constexpr (SUMS) {
+            if (s % W::PER == W::PER - 1) {
 #pragma unroll
-                for (int i = 0; i < RT; ++i) sum[i] = mfma16<DT>(xv[i], ones, sum[i]);
-            }
-            if (s % PER == PER - 1) {
+                for (int i = 0; i < RT; ++i) {
+                    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+                    if constexpr (W::SUMS) sum = *reinterpret_cast<const f32x4*>(&sums[slot][s / W::PER][16 * i + 4 * g]);
 #pragma unroll
-                for (int j = 0; j < CT; ++j) {
-                    const float sc = from_bits<DT>(sv[j][s / PER]);
-                    const float z = ZEROS ? from_bits<DT>(zv[j][s / PER]) : 8.f;
-                    const float off = -sc * (kOffset + z);
-#pragma unroll
-                    for (int i = 0; i < RT; ++i)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            acc[i][j][r] = fmaf(sc, dot[i][j][r], acc[i][j][r]);
-                            if constexpr (SUMS) acc[i][j][r] = fmaf(off, sum[i][r], acc[i][j][r]);
-                        }
+                    for (int j = 0; j < CT; ++j) add_group<W, DT, ZEROS>(w, j, s / W::PER, dot[i][j], sum, acc[i][j]);
                 }
             }
         }
     };
 
-    const int units = x_rows > 0 ? (K + kUnit - 1) / kUnit : 0;
-    u32x4 w[CT][2];
-    if (wave < units) load_q(wave * kUnit, w);
-    for (int u = wave; u < units; u += W) {
-        u32x4 next[CT][2];
-        if (u + W < units) load_q((u + W) * kUnit, next);
-        if ((u + 1) * kUnit <= K) unit(u * kUnit, w, std::true_type{});
-        else unit(u * kUnit, w, std::false_type{});
-#pragma unroll
-        for (int t = 0; t < CT; ++t)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) w[t][h] = next[t][h];
+    // Round u loads unit u and computes unit u - 1; one barrier a round. x of unit u goes into the slot that
+    // every wave left before this round's barrier.
+    typename W::Unit now, next;
+    u32x4 xv[LOADS];
+#pragma unroll 1
+    for (int u = 0; u <= tile.units; ++u) {
+        __syncthreads();
+        now = next;
+        if (u < tile.units) {
+            fetch(tile.unit(u), xv);
+            weights.load(tile.unit(u) * UNIT, next);
+        }
+        if (u > 0) compute((u - 1) & 1, now);
+        if (u < tile.units) stage(u & 1, xv);
     }
-
-    // Register r of lane l holds row 4 (l / 16) + r, column l % 16.
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
-        for (int j = 0; j < CT; ++j) red[wave][i * CT + j][lane] = acc[i][j];
-    __syncthreads();
-    for (int t = wave; t < RT * CT; t += W) {
-        f32x4 v = red[0][t][lane];
-#pragma unroll
-        for (int u = 1; u < W; ++u) v += red[u][t][lane];
-        const int n = n0 + 16 * (t % CT) + c;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int p = 16 * (t / CT) + 4 * g + r;
-            if (p >= count || n >= N) continue;
-            const int64_t row = rows ? rows[p0 + p] : p0 + p;
-            out[(p0 + p) * ldo + n] = row >= 0 && row < x_rows ? to_bits<DT>(v[r]) : 0;
-        }
-    }
+        for (int j = 0; j < CT; ++j) w4_store<DT>(a, tile, i, j, acc[i][j], lane);
 }
 
-template <int DT, bool ZEROS, int RT, int CT, int SPU, int W>
-int launch_w4(const W4Call& c, hipStream_t stream) {
-    const int blocks_n = (int)((c.N + 16 * CT - 1) / (16 * CT));
-    const int64_t tiles = c.offsets ? c.total_rows / (16 * RT) + std::min<int64_t>(c.experts, c.total_rows)
-                                    : (c.total_rows + 16 * RT - 1) / (16 * RT);
-    hipLaunchKernelGGL((gemm_w4_kernel<DT, ZEROS, RT, CT, SPU, W>), dim3((unsigned)(tiles * blocks_n)), dim3(64 * W), 0,
-                       stream, static_cast<const uint16_t*>(c.x), c.ldx, c.x_rows, c.rows,
-                       static_cast<const uint8_t*>(c.q), static_cast<const uint16_t*>(c.scales),
-                       static_cast<const uint16_t*>(c.zeros), c.group, static_cast<uint16_t*>(c.out), c.ldo, c.offsets,
-                       c.experts, (int)c.total_rows, (int)c.N, (int)c.K, blocks_n);
+// out = the sum of the K splits' planes, in split order, for the rows of any expert.
+template <int DT>
+__global__ void __launch_bounds__(256)
+gemm_w4_sum_kernel(W4Args a) {
+    const int quads = a.ldp / 4;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t p = i / quads;
+    if (p >= a.total) return;
+    if (a.offsets != nullptr && (p < a.offsets[0] || p >= a.offsets[a.experts])) return;
+    const int n = 4 * (int)(i - p * quads);
+    const float* from = a.planes + p * a.ldp + n;
+    f32x4 v = *reinterpret_cast<const f32x4*>(from);
+    for (int s = 1; s < a.splits; ++s) v += *reinterpret_cast<const f32x4*>(from + (int64_t)s * a.total * a.ldp);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (n + e < a.N) a.out[p * a.ldo + n + e] = to_bits<DT>(v[e]);
+}
+
+// K splits: as many as give every CU `want` blocks, keep `least` units of K in each, and fit the workspace.
+int w4_splits(const W4Call& c, int64_t blocks, int64_t want, int unit, int least, size_t workspace_bytes,
+              const DeviceProps& props) {
+    const int64_t units = (c.K + unit - 1) / unit;
+    const int64_t plane = c.total_rows * ((c.N + 3) / 4 * 4) * (int64_t)sizeof(float);
+    int64_t splits = std::min(want * props.cu_count / blocks, units / least);
+    splits = std::min(splits, (int64_t)(workspace_bytes / plane));
+    return (int)std::max<int64_t>(1, splits);
+}
+
+template <int RT>
+constexpr int w4_unit() { return 256; }
+
+template <int DT, bool ZEROS, int RT, int SPU>
+int launch_w4(const W4Call& c, void* workspace, size_t workspace_bytes, const DeviceProps& props, hipStream_t stream) {
+    constexpr int CT = 2, WAVES = 8, UNIT = w4_unit<RT>(), ROWS = RT == 0 ? 16 : 16 * RT;
+    constexpr int COLUMNS = RT == 0 ? 16 * CT : 16 * CT * WAVES;
+    const int blocks_n = (int)((c.N + COLUMNS - 1) / COLUMNS);
+    const int64_t tiles = c.offsets ? c.total_rows / ROWS + std::min<int64_t>(c.experts, c.total_rows)
+                                    : (c.total_rows + ROWS - 1) / ROWS;
+    // Tiles there will be if the rows are spread over the experts.
+    const int64_t likely = std::max<int64_t>(std::min<int64_t>(c.experts, c.total_rows), c.total_rows / ROWS);
+    const int splits = w4_splits(c, likely * blocks_n, RT == 0 ? 2 : 1, UNIT, RT == 0 ? 2 * WAVES : 4, workspace_bytes, props);
+    W4Args a{static_cast<const uint16_t*>(c.x), c.rows, c.offsets, static_cast<const uint8_t*>(c.q),
+             static_cast<const uint16_t*>(c.scales), static_cast<const uint16_t*>(c.zeros),
+             static_cast<uint16_t*>(c.out), splits > 1 ? static_cast<float*>(workspace) : nullptr, c.ldx, c.ldo,
+             c.x_rows, c.group, c.experts, (int)c.total_rows, (int)c.N, (int)c.K, blocks_n, splits,
+             (int)((c.N + 3) / 4 * 4)};
+    const dim3 grid((unsigned)(tiles * blocks_n * splits));
+    if constexpr (RT == 0)
+        hipLaunchKernelGGL((gemm_w4_kernel<DT, ZEROS, CT, UNIT, SPU, WAVES>), grid, dim3(64 * WAVES), 0, stream, a);
+    else
+        hipLaunchKernelGGL((gemm_w4_rows_kernel<DT, ZEROS, RT, CT, UNIT, SPU, WAVES>), grid, dim3(64 * WAVES), 0, stream, a);
     MB_HIP_TRY(hipGetLastError());
+    if (splits > 1) {
+        const int64_t quads = c.total_rows * (a.ldp / 4);
+        hipLaunchKernelGGL((gemm_w4_sum_kernel<DT>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, stream, a);
+        MB_HIP_TRY(hipGetLastError());
+    }
     return MB_OK;
 }
 
-template <int DT, bool ZEROS, int RT, int CT, int W>
-int launch_group(const W4Call& c, hipStream_t stream) {
-    if (c.group == 32) return launch_w4<DT, ZEROS, RT, CT, 8, W>(c, stream);
-    if (c.group == 64) return launch_w4<DT, ZEROS, RT, CT, 4, W>(c, stream);
-    if (c.group == 128) return launch_w4<DT, ZEROS, RT, CT, 2, W>(c, stream);
-    if (c.group % kUnit == 0) return launch_w4<DT, ZEROS, RT, CT, 1, W>(c, stream);
-    return launch_w4<DT, ZEROS, RT, CT, 0, W>(c, stream);
+template <int DT, bool ZEROS, int RT>
+int launch_group(const W4Call& c, void* workspace, size_t bytes, const DeviceProps& props, hipStream_t stream) {
+    constexpr int UNIT = w4_unit<RT>();
+    if (c.group == 32) return launch_w4<DT, ZEROS, RT, UNIT / 32>(c, workspace, bytes, props, stream);
+    if (c.group == 64) return launch_w4<DT, ZEROS, RT, UNIT / 64>(c, workspace, bytes, props, stream);
+    if (UNIT > 128 && c.group == 128) return launch_w4<DT, ZEROS, RT, UNIT / 128>(c, workspace, bytes, props, stream);
+    if (c.group % UNIT == 0) return launch_w4<DT, ZEROS, RT, 1>(c, workspace, bytes, props, stream);
+    return launch_w4<DT, ZEROS, RT, 0>(c, workspace, bytes, props, stream);
 }
 
 template <int DT, bool ZEROS>
-int launch_rows(const W4Call& c, hipStream_t stream) {
+int launch_rows(const W4Call& c, void* workspace, size_t bytes, const DeviceProps& props, hipStream_t stream) {
     // Rows of an expert, were they even: tiles of 16, 32 or 64 of them share one pass over the weights.
     const int64_t rows = (c.total_rows + c.experts - 1) / c.experts;
-    if (rows <= 16) return launch_group<DT, ZEROS, 1, 2, 8>(c, stream);
-    if (rows <= 32) return launch_group<DT, ZEROS, 2, 2, 8>(c, stream);
-    return launch_group<DT, ZEROS, 4, 2, 4>(c, stream);
+    if (rows <= 16 && c.experts < 8) return launch_group<DT, ZEROS, 0>(c, workspace, bytes, props, stream);
+    if (rows <= 16) return launch_group<DT, ZEROS, 1>(c, workspace, bytes, props, stream);
+    if (rows <= 32) return launch_group<DT, ZEROS, 2>(c, workspace, bytes, props, stream);
+    return launch_group<DT, ZEROS, 4>(c, workspace, bytes, props, stream);
 }
 
 }  // namespace
 
 int gemm_w4_launch(const W4Call& c, void* workspace, size_t workspace_bytes, const DeviceProps& props,
                    hipStream_t stream) {
+    // The workspace only makes small calls faster: one off 16 bytes is left alone.
+    if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0) workspace_bytes = 0;
     if (c.dtype == MB_DT_FLOAT16)
-        return c.zeros ? launch_rows<MB_DT_FLOAT16, true>(c, stream) : launch_rows<MB_DT_FLOAT16, false>(c, stream);
-    return c.zeros ? launch_rows<MB_DT_BFLOAT16, true>(c, stream) : launch_rows<MB_DT_BFLOAT16, false>(c, stream);
+        return c.zeros ? launch_rows<MB_DT_FLOAT16, true>(c, workspace, workspace_bytes, props, stream)
+                       : launch_rows<MB_DT_FLOAT16, false>(c, workspace, workspace_bytes, props, stream);
+    return c.zeros ? launch_rows<MB_DT_BFLOAT16, true>(c, workspace, workspace_bytes, props, stream)
+                   : launch_rows<MB_DT_BFLOAT16, false>(c, workspace, workspace_bytes, props, stream);
 }
 
 }  // namespace mb
