@@ -347,8 +347,8 @@ int mb_kernel_info(int kind, int a, int b, int64_t m, int64_t n, int64_t k,
                                           the stage depth rounds every split up to whole stages) */
 #define MB_TUNE_GEMM_FP8_MFMA 8        /* 16 or 32: the fp8 MFMA shape on the tiled kernel */
 #define MB_TUNE_GEMM_HIGHP_STAGED 9    /* 1: fp32 / fp64 on the register-staged kernel */
-#define MB_TUNE_GROUPED_CONFIG 10       /* mb_gemm_grouped, rows on 16 bytes: 0: 256x256, 1: 256x128, 2: 128x128,
-                                           3: 64x128, 4: 64x64 tiles; 5: the bounds-checked kernel */
+#define MB_TUNE_GROUPED_CONFIG 10       /* mb_gemm_grouped, rows on 16 bytes: 0: 256x256, 1: 128x128, 2: 64x64 tiles;
+                                           3: the kernel for any rows */
 #define MB_TUNE_COUNT 11
 
 /* Force `knob` to `value`, or restore the library's choice with value -1.

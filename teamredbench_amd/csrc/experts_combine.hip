@@ -18,21 +18,26 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kBatch = 8;      // rows of a token in flight together
 
-// 8 columns from column c of a row, zeros past N.
-template <int DT>
+// 8 columns from column c of a row, zeros past N. STREAM: nontemporal, for
+// rows read or written once that together pass the caches (8192 tokens of
+// 4 x 4096: 66 us with it, 85 without; the gradient, 114 without and 122 with).
+template <int DT, bool STREAM>
 __device__ __forceinline__ void load_columns(const uint16_t* row, int64_t c, int64_t N, float* v) {
     if (c + 8 <= N) {
-        const u32x4 p = *reinterpret_cast<const u32x4_any*>(row + c);
+        const auto* from = reinterpret_cast<const u32x4_any*>(row + c);
+        const u32x4 p = STREAM ? __builtin_nontemporal_load(from) : *from;
         unpack8<DT>(p, v);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = c + i < N ? from_bits<DT>(row[c + i]) : 0.f;
     }
 }
-template <int DT>
+template <int DT, bool STREAM>
 __device__ __forceinline__ void store_columns(uint16_t* row, int64_t c, int64_t N, const float* v) {
     if (c + 8 <= N) {
-        *reinterpret_cast<u32x4_any*>(row + c) = pack8<DT>(v);
+        auto* to = reinterpret_cast<u32x4_any*>(row + c);
+        if constexpr (STREAM) __builtin_nontemporal_store(pack8<DT>(v), to);
+        else *to = pack8<DT>(v);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -61,7 +66,7 @@ combine_kernel(const uint16_t* __restrict__ y, int64_t ldy, int64_t y_rows, cons
             const int64_t a = t * top_k + j0 + u;
             const int64_t slot = j0 + u < top_k ? slots[a] : -1;
             if (slot >= 0 && slot < y_rows) {
-                load_columns<DT>(y + slot * ldy, c, N, v[u]);
+                load_columns<DT, true>(y + slot * ldy, c, N, v[u]);
                 w[u] = weights ? weights[a] : 1.f;
             } else {
 #pragma unroll
@@ -73,7 +78,7 @@ combine_kernel(const uint16_t* __restrict__ y, int64_t ldy, int64_t y_rows, cons
 #pragma unroll
             for (int e = 0; e < 8; ++e) sum[e] = fmaf(w[u], v[u][e], sum[e]);
     }
-    store_columns<DT>(out + t * ldo, c, N, sum);
+    store_columns<DT, true>(out + t * ldo, c, N, sum);
 }
 
 // One block per token: its grad_y rows, and the dot products over its columns.
@@ -98,13 +103,13 @@ combine_grad_kernel(const uint16_t* __restrict__ g, int64_t ldg, const uint16_t*
         }
         for (int64_t c = (int64_t)threadIdx.x * 8; c < N; c += kThreads * 8) {
             float gv[8];
-            load_columns<DT>(g + t * ldg, c, N, gv);
+            load_columns<DT, false>(g + t * ldg, c, N, gv);
             if (grad_weights != nullptr) {
 #pragma unroll
                 for (int u = 0; u < kBatch; ++u) {
                     if (slot[u] < 0) continue;
                     float yv[8];
-                    load_columns<DT>(y + slot[u] * ldy, c, N, yv);
+                    load_columns<DT, false>(y + slot[u] * ldy, c, N, yv);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) dot[u] = fmaf(gv[e], yv[e], dot[u]);
                 }
@@ -116,7 +121,7 @@ combine_grad_kernel(const uint16_t* __restrict__ g, int64_t ldg, const uint16_t*
                     float dv[8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) dv[e] = w[u] * gv[e];
-                    store_columns<DT>(grad_y + slot[u] * ld_grad_y, c, N, dv);
+                    store_columns<DT, false>(grad_y + slot[u] * ld_grad_y, c, N, dv);
                 }
             }
         }

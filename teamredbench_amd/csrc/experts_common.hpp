@@ -30,7 +30,10 @@ struct GroupedCall {
     const int32_t *rows, *offsets;
     int64_t ldx, ldy, ldo, x_rows, total_rows, N, K;
 };
-// The pipelined kernels (16-byte rows) on tile configuration `config`, one per input type.
+// Tile heights and widths of the pipelined grouped kernels.
+constexpr int kGroupedTileCount = 3;
+constexpr int kGroupedTiles[kGroupedTileCount] = {256, 128, 64};
+// The pipelined kernels (rows on 16 bytes) on tiles of kGroupedTiles[config], one per input type.
 int gemm_grouped_tiled_bf16(const GroupedCall& c, int config, hipStream_t stream);
 int gemm_grouped_tiled_f16(const GroupedCall& c, int config, hipStream_t stream);
 int gemm_grouped_launch(const GroupedCall& c, void* workspace, size_t workspace_bytes, const DeviceProps& props,

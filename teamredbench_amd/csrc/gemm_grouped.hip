@@ -7,30 +7,41 @@
 //   GRAD_ROWS     sorted row N          K     dC, c in a row   B, c in a row
 //   GRAD_WEIGHTS  K          sorted row N     A, m in a row    dC, n in a row
 //
+// Rows on 16 bytes go to the LDS-DMA pipelines of gemm_grouped_kernels.hpp.
 // gemm_grouped_any_kernel takes any size, stride and alignment: 128 x 128
-// tiles, 4 waves of 64 x 64 on v_mfma_f32_32x32x16, a stage of 32 c. Both
-// operands go through registers into LDS as [m or n][32 c] (rows padded to 80
-// bytes), every element checked against its expert's bounds and zero outside, so rows
-// of neighbouring experts and whatever lies past K or N never enter a sum.
-#include "experts_common.hpp"
+// tiles, 4 waves of 64 x 64 on v_mfma_f32_32x32x16, a stage of 32 c, through
+// registers into one of two LDS buffers while the other is computed. Global
+// loads are 16 bytes at any element (the hardware takes them); an operand whose rows run along c is kept as
+// [m or n][32 c] in rows of 80 bytes, one whose rows run across it as [32 c][m or n], swizzled, and read with the
+// transposing LDS reads. Rows of c past the
+// expert's and c past the end load as zeros; columns past the matrix hold
+// whatever the row's window holds there and are not stored; nothing past a
+// row's last element is read.
+#include "gemm_grouped_kernels.hpp"
 
 #include <algorithm>
+#include <cmath>
 
 namespace mb {
 namespace {
 
 constexpr int kTile = 128;
-constexpr int kStage = 32;                 // c per stage
-constexpr int kPitch = kStage * 2 + 16;    // LDS row pitch, bytes
+constexpr int kStage = 32;                      // c per stage
+constexpr int kPitch = kStage * 2 + 16;         // bytes per LDS row along c
+constexpr int kAnyBuffer = kTile * kPitch;      // bytes per operand and buffer (an operand across c takes less)
 
-template <int DT>
-__device__ __forceinline__ f32x16 mfma32(const u32x4& a, const u32x4& b, f32x16 c) {
-    if constexpr (DT == MB_DT_FLOAT16)
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
-                                                       0, 0);
-    else
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
-                                                        0, 0, 0);
+// Elements c .. c + 7 of a row of `n`; zeros past its end, none of which is read.
+__device__ __forceinline__ u32x4 row_window(const uint16_t* row, int c, int n) {
+    if (c + 8 <= n) return *reinterpret_cast<const u32x4_any*>(row + c);
+    if (c >= n) return u32x4{0u, 0u, 0u, 0u};
+    if (n >= 8) {   // the row's last 8, shifted down
+        const __uint128_t wide = __builtin_bit_cast(__uint128_t, (u32x4)*reinterpret_cast<const u32x4_any*>(row + n - 8));
+        return __builtin_bit_cast(u32x4, wide >> (16 * (c + 8 - n)));
+    }
+    __uint128_t wide = 0;
+#pragma unroll 1
+    for (int i = n - 1; i >= c; --i) wide = (wide << 16) | row[i];
+    return __builtin_bit_cast(u32x4, wide);
 }
 
 template <int DT, int OP>
@@ -38,9 +49,9 @@ __global__ void __launch_bounds__(256)
 gemm_grouped_any_kernel(const uint16_t* __restrict__ x, int64_t ldx, int64_t x_rows, const int32_t* __restrict__ rows,
                         const uint16_t* __restrict__ y, int64_t ldy, uint16_t* __restrict__ out, int64_t ldo,
                         const int32_t* __restrict__ offsets, int experts, int total, int N, int K, int tiles_n) {
-    constexpr bool XC = OP != MB_GROUPED_GRAD_WEIGHTS;   // X's rows run along c (else along m)
-    constexpr bool YC = OP == MB_GROUPED_GRAD_ROWS;      // Y's rows run along c (else along n)
-    __shared__ __attribute__((aligned(16))) unsigned char lds_x[kTile * kPitch], lds_y[kTile * kPitch];
+    constexpr bool XC = OP != MB_GROUPED_GRAD_WEIGHTS;   // X's rows run along c
+    constexpr bool YC = OP == MB_GROUPED_GRAD_ROWS;      // Y's rows run along c
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[2][2][kAnyBuffer];   // buffer, operand
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int wm = wave >> 1, wn = wave & 1;
     const int tile = (int)blockIdx.x / tiles_n, n0 = ((int)blockIdx.x - tile * tiles_n) * kTile;
@@ -67,56 +78,61 @@ gemm_grouped_any_kernel(const uint16_t* __restrict__ x, int64_t ldx, int64_t x_r
     };
     const uint16_t* yb = OP == MB_GROUPED_GRAD_WEIGHTS ? y + ex.first * ldy : y + (int64_t)ex.expert * K * ldy;
 
-    // This thread's 16 elements of a stage: row (column) of the tile and half of the stage when c runs in a
-    // row, else a column of the tile and 16 of the stage's c.
-    auto load_c = [&](const uint16_t* row, int c, u32x4* v) {   // 16 elements of a row from c on
-        if (row != nullptr && c + 16 <= C) {
-            v[0] = *reinterpret_cast<const u32x4_any*>(row + c);
-            v[1] = *reinterpret_cast<const u32x4_any*>(row + c + 8);
-            return;
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const unsigned lo = row != nullptr && c + 2 * i < C ? row[c + 2 * i] : 0u;
-            const unsigned hi = row != nullptr && c + 2 * i + 1 < C ? row[c + 2 * i + 1] : 0u;
-            v[i >> 2][i & 3] = lo | (hi << 16);
-        }
-    };
-    const int cr = tid >> 1, ch = (tid & 1) * 16;       // c runs in a row
-    const int mr = tid & 127, mh = (tid >> 7) * 16;     // it does not
-    const uint16_t* x_ptr = nullptr;
+    // A thread brings two 16-byte pieces of each operand's stage. Along c: 16 c of tile row tid / 2.
+    // Across: 8 columns from 8 (tid % 16) on, of c tid / 16 and + 16.
+    const int along_row = tid >> 1, along_c = (tid & 1) * 16;
+    const int across_c = tid >> 4, across_col = (tid & 15) * 8;
+    const uint16_t *x_along = nullptr, *y_along = nullptr;
     if constexpr (XC) {
-        const int64_t r = m0 + cr < M ? x_row(m0 + cr) : -1;
-        if (r >= 0) x_ptr = x + r * ldx;
+        const int64_t r = m0 + along_row < M ? x_row(m0 + along_row) : -1;
+        if (r >= 0) x_along = x + r * ldx;
     }
-    const uint16_t* y_ptr = nullptr;
     if constexpr (YC) {
-        if (n0 + cr < NN) y_ptr = yb + (int64_t)(n0 + cr) * ldy;
+        if (n0 + along_row < NN) y_along = yb + (int64_t)(n0 + along_row) * ldy;
     }
-    auto load_x = [&](int c, u32x4* v) {
+    auto load_along = [&](const uint16_t* row, int c, u32x4 (&v)[2]) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            v[h] = row != nullptr ? row_window(row, c + along_c + 8 * h, C) : u32x4{0u, 0u, 0u, 0u};
+    };
+    auto load_x = [&](int c, u32x4 (&v)[2]) {
         if constexpr (XC) {
-            load_c(x_ptr, c + ch, v);
+            load_along(x_along, c, v);
         } else {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int p = c + mh + i;
+            for (int h = 0; h < 2; ++h) {
+                const int p = c + across_c + 16 * h;
                 const int64_t r = p < C ? x_row(p) : -1;
-                const unsigned e = r >= 0 && m0 + mr < M ? x[r * ldx + m0 + mr] : 0u;
-                v[i >> 3][(i >> 1) & 3] = (i & 1) ? v[i >> 3][(i >> 1) & 3] | (e << 16) : e;
+                v[h] = r >= 0 ? row_window(x + r * ldx, m0 + across_col, M) : u32x4{0u, 0u, 0u, 0u};
             }
         }
     };
-    auto load_y = [&](int c, u32x4* v) {
+    auto load_y = [&](int c, u32x4 (&v)[2]) {
         if constexpr (YC) {
-            load_c(y_ptr, c + ch, v);
+            load_along(y_along, c, v);
         } else {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int p = c + mh + i;
-                const unsigned e = p < C && n0 + mr < NN ? yb[p * ldy + n0 + mr] : 0u;
-                v[i >> 3][(i >> 1) & 3] = (i & 1) ? v[i >> 3][(i >> 1) & 3] | (e << 16) : e;
+            for (int h = 0; h < 2; ++h) {
+                const int p = c + across_c + 16 * h;
+                v[h] = p < C ? row_window(yb + p * ldy, n0 + across_col, NN) : u32x4{0u, 0u, 0u, 0u};
             }
         }
+    };
+    auto store = [&](unsigned char* to, bool along, const u32x4 (&v)[2]) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int c = across_c + 16 * h;
+            const int at = along ? along_row * kPitch + along_c * 2 + 16 * h
+                                 : c * kTile * 2 + (((across_col >> 3) ^ b_swizzle<2, kTile * 2>(c)) << 4);
+            *reinterpret_cast<u32x4*>(to + at) = v[h];
+        }
+    };
+    // Fragment of 32 rows (columns) from `base` on, substep s.
+    auto fragment = [&](const unsigned char* from, bool along, int base, int s) {
+        if (along)
+            return *reinterpret_cast<const u32x4*>(from + (base + (lane & 31)) * kPitch + 32 * s + 16 * (lane >> 5));
+        const u32x2 lo = read_b_piece<DT, kTile>(from, base, s, 0, lane), hi = read_b_piece<DT, kTile>(from, base, s, 1, lane);
+        return u32x4{lo[0], lo[1], hi[0], hi[1]};
     };
 
     f32x16 acc[2][2];
@@ -131,14 +147,11 @@ gemm_grouped_any_kernel(const uint16_t* __restrict__ x, int64_t ldx, int64_t x_r
         load_x(0, xv);
         load_y(0, yv);
     }
-    for (int c = 0; c < C; c += kStage) {
-        unsigned char* px = XC ? lds_x + cr * kPitch + ch * 2 : lds_x + mr * kPitch + mh * 2;
-        unsigned char* py = YC ? lds_y + cr * kPitch + ch * 2 : lds_y + mr * kPitch + mh * 2;
-        *reinterpret_cast<u32x4*>(px) = xv[0];
-        *reinterpret_cast<u32x4*>(px + 16) = xv[1];
-        *reinterpret_cast<u32x4*>(py) = yv[0];
-        *reinterpret_cast<u32x4*>(py + 16) = yv[1];
-        __syncthreads();
+    int buf = 0;
+    for (int c = 0; c < C; c += kStage, buf ^= 1) {
+        store(lds[buf][0], XC, xv);
+        store(lds[buf][1], YC, yv);
+        __syncthreads();   // the other buffer was left by every wave before this barrier
         if (c + kStage < C) {
             load_x(c + kStage, xv);
             load_y(c + kStage, yv);
@@ -148,16 +161,14 @@ gemm_grouped_any_kernel(const uint16_t* __restrict__ x, int64_t ldx, int64_t x_r
             u32x4 xf[2], yf[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const int at = 32 * s + 16 * (lane >> 5);
-                xf[i] = *reinterpret_cast<const u32x4*>(lds_x + (64 * wm + 32 * i + (lane & 31)) * kPitch + at);
-                yf[i] = *reinterpret_cast<const u32x4*>(lds_y + (64 * wn + 32 * i + (lane & 31)) * kPitch + at);
+                xf[i] = fragment(lds[buf][0], XC, 64 * wm + 32 * i, s);
+                yf[i] = fragment(lds[buf][1], YC, 64 * wn + 32 * i, s);
             }
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) acc[i][j] = mfma32<DT>(yf[j], xf[i], acc[i][j]);
+                for (int j = 0; j < 2; ++j) acc[i][j] = Traits<DT>::mfma(yf[j], xf[i], acc[i][j]);
         }
-        __syncthreads();
     }
 
     // Register 4g + q of lane l holds out(32i + l % 32, 32j + 8g + 4 (l / 32) + q).
@@ -170,9 +181,17 @@ gemm_grouped_any_kernel(const uint16_t* __restrict__ x, int64_t ldx, int64_t x_r
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int n = n0 + 64 * wn + 32 * j + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
-                if (n < NN) row[n] = to_bits<DT>(acc[i][j][r]);
+            for (int g = 0; g < 4; ++g) {
+                typedef u32x2 u32x2_any __attribute__((aligned(2)));
+                const int n = n0 + 64 * wn + 32 * j + 8 * g + 4 * (lane >> 5);
+                const f32x16& v = acc[i][j];
+                if (n + 4 <= NN) {
+                    *reinterpret_cast<u32x2_any*>(row + n) = pack4<DT>(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 3; ++r)
+                        if (n + r < NN) row[n + r] = to_bits<DT>(v[4 * g + r]);
+                }
             }
     }
 }
@@ -193,7 +212,7 @@ int launch_any(const GroupedCall& c, hipStream_t stream) {
 }
 
 template <int DT>
-int launch_dtype(const GroupedCall& c, hipStream_t stream) {
+int launch_any_op(const GroupedCall& c, hipStream_t stream) {
     if (c.op == MB_GROUPED_FORWARD) return launch_any<DT, MB_GROUPED_FORWARD>(c, stream);
     if (c.op == MB_GROUPED_GRAD_ROWS) return launch_any<DT, MB_GROUPED_GRAD_ROWS>(c, stream);
     return launch_any<DT, MB_GROUPED_GRAD_WEIGHTS>(c, stream);
@@ -202,31 +221,68 @@ int launch_dtype(const GroupedCall& c, hipStream_t stream) {
 // The tile configuration of the pipelined kernels, -1 for what they do not
 // take: rows off 16 bytes, or an operand (one expert's matrix, x read through
 // `rows`, a tile's rows) that passes the 2^31 bytes a buffer offset spans.
-int tiled_config(const GroupedCall& c) {
+int tiled_config(const GroupedCall& c, const DeviceProps& props) {
     const uintptr_t base = reinterpret_cast<uintptr_t>(c.x) | reinterpret_cast<uintptr_t>(c.y) |
                            reinterpret_cast<uintptr_t>(c.out);
     if ((base & 15) != 0 || ((c.ldx | c.ldy | c.ldo | c.N | c.K) & 7) != 0 || c.total_rows == 0 || c.x_rows == 0)
         return -1;
-    constexpr int64_t kMost = 1ll << 30;   // elements
+    // Every row a tile can address, those past its operand's end too, stays below 2^30 elements.
+    constexpr int64_t kMost = (1ll << 30) - 1, kTileRows = 256;
     const bool weights = c.op == MB_GROUPED_GRAD_WEIGHTS;
-    const int64_t x_rows = c.rows ? c.x_rows : weights ? c.total_rows : 256;
-    if (x_rows > kMost / c.ldx || (weights ? c.total_rows : c.K) > kMost / c.ldy) return -1;
-    if (const int64_t forced = tuning(MB_TUNE_GROUPED_CONFIG); forced >= 0) return forced > 4 ? -1 : (int)forced;
-    if (weights) return 0;
-    const int64_t rows = (c.total_rows + c.experts - 1) / c.experts;
-    return rows > 256 ? 0 : rows > 64 ? 2 : 3;
+    const int64_t x_rows = c.rows ? c.x_rows : weights ? c.total_rows : 0;
+    const int64_t y_rows = weights ? c.total_rows : c.K;
+    if (std::max(x_rows, kTileRows) > kMost / c.ldx - kTileRows || std::max(y_rows, kTileRows) > kMost / c.ldy - kTileRows)
+        return -1;
+    if (const int64_t forced = tuning(MB_TUNE_GROUPED_CONFIG); forced >= 0)
+        return forced < kGroupedTileCount ? (int)forced : -1;
+
+    // The tile whose predicted time is least; a smaller one has to gain 3%. A
+    // block takes an overhead (its first loads and its stores) and a time per
+    // 32 of the contraction, measured at 16384 rows x 4096 x 14336 over 8
+    // experts with every CU full: 0.75 us on 256 x 256 tiles (one a CU), 0.535
+    // on 128 x 128 (two) and 0.386 on 64 x 64 (three). Nothing beats the bytes, at 5.2 TB/s. An expert's row tiles: its
+    // rows, were they even, and half a tile; with fewer rows than a tile one, and a share of experts that pass it.
+    constexpr double kStageUs[kGroupedTileCount] = {0.75, 0.535, 0.386};
+    constexpr double kBlockUs[kGroupedTileCount] = {8, 4, 4};
+    constexpr int kPerCu[kGroupedTileCount] = {1, 2, 3};
+    const int64_t hit = std::min<int64_t>(c.experts, c.total_rows);   // experts with rows, at most
+    const double per_expert = (double)c.total_rows / c.experts;
+    const int64_t NN = c.op == MB_GROUPED_GRAD_ROWS ? c.K : c.N, C = c.op == MB_GROUPED_GRAD_ROWS ? c.N : c.K;
+    const double bytes_us = 2.0 * ((double)hit * c.K * c.N + (double)c.total_rows * (c.K + c.N)) / 5.2e6;
+    int best = 0;
+    double best_us = 0;
+    for (int i = 0; i < kGroupedTileCount; ++i) {
+        const int tile = kGroupedTiles[i];
+        const double wide = (double)((NN + tile - 1) / tile);
+        double blocks, stages;
+        if (weights) {
+            blocks = (double)c.experts * ((c.K + tile - 1) / tile) * wide;
+            stages = std::max(1.0, per_expert / 32);
+        } else {
+            const double tiles = per_expert / tile;
+            blocks = hit * wide * std::max(1.0 + 0.55 * std::max(0.0, tiles - 0.35), tiles + 0.45);
+            stages = (double)((C + 31) / 32);
+        }
+        const double rounds = std::ceil(blocks / props.cu_count) / kPerCu[i];
+        const double us = std::max(bytes_us, rounds * (kBlockUs[i] + stages * kStageUs[i]));
+        if (i == 0 || us < 0.97 * best_us) {
+            best = i;
+            best_us = us;
+        }
+    }
+    return best;
 }
 
 }  // namespace
 
 int gemm_grouped_launch(const GroupedCall& c, void* workspace, size_t workspace_bytes, const DeviceProps& props,
                         hipStream_t stream) {
-    const int config = tiled_config(c);
+    const int config = tiled_config(c, props);
     if (config >= 0)
         return c.dtype == MB_DT_FLOAT16 ? gemm_grouped_tiled_f16(c, config, stream)
                                         : gemm_grouped_tiled_bf16(c, config, stream);
-    if (c.dtype == MB_DT_FLOAT16) return launch_dtype<MB_DT_FLOAT16>(c, stream);
-    return launch_dtype<MB_DT_BFLOAT16>(c, stream);
+    if (c.dtype == MB_DT_FLOAT16) return launch_any_op<MB_DT_FLOAT16>(c, stream);
+    return launch_any_op<MB_DT_BFLOAT16>(c, stream);
 }
 
 }  // namespace mb

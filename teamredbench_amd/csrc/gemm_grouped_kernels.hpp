@@ -462,26 +462,26 @@ gemm_grouped_kernel(GroupedArgs args, int tiles_m_max, int tiles_n, int group_m)
 }
 
 struct GroupedConfig {
-    int bm, bn, group_m;
+    int group_m;
     int nx[3], ny[3];   // ring slots by op
 };
 
-constexpr GroupedConfig kGroupedConfigs[] = {
-    {256, 256, 4, {3, 3, 5}, {4, 2, 5}},
-    {256, 128, 4, {3, 3, 5}, {6, 3, 5}},
-    {128, 128, 4, {2, 2, 5}, {6, 3, 5}},
-    {64, 128, 4, {3, 2, 5}, {6, 2, 5}},
-    {64, 64, 4, {3, 2, 5}, {6, 3, 5}},
+// Tiles of kGroupedTiles; 256 x 256 fills the LDS of a CU, 128 x 128 half of it, 64 x 64 a third.
+constexpr GroupedConfig kGroupedConfigs[kGroupedTileCount] = {
+    {4, {3, 3, 5}, {4, 2, 5}},
+    {4, {2, 2, 5}, {6, 3, 5}},
+    {4, {3, 2, 5}, {6, 3, 5}},
 };
 
 template <int DT, int OP, int CFG>
 int launch_grouped(const GroupedCall& c, hipStream_t stream) {
     constexpr GroupedConfig cfg = kGroupedConfigs[CFG];
+    constexpr int TILE = kGroupedTiles[CFG];
     const int64_t NN = OP == MB_GROUPED_GRAD_ROWS ? c.K : c.N;
-    const int tiles_n = (int)((NN + cfg.bn - 1) / cfg.bn);
+    const int tiles_n = (int)((NN + TILE - 1) / TILE);
     const bool weights = OP == MB_GROUPED_GRAD_WEIGHTS;
-    const int64_t tiles_m = weights ? (c.K + cfg.bm - 1) / cfg.bm
-                                    : c.total_rows / cfg.bm + std::min<int64_t>(c.experts, c.total_rows);
+    const int64_t tiles_m = weights ? (c.K + TILE - 1) / TILE
+                                    : c.total_rows / TILE + std::min<int64_t>(c.experts, c.total_rows);
     const int64_t blocks = tiles_m * tiles_n * (weights ? c.experts : 1);
     GroupedArgs a{static_cast<const unsigned char*>(c.x), static_cast<const unsigned char*>(c.y),
                   static_cast<unsigned char*>(c.out), c.rows, c.offsets, (int)c.ldx * 2, (int)c.ldy * 2, c.ldo * 2,
@@ -492,9 +492,9 @@ int launch_grouped(const GroupedCall& c, hipStream_t stream) {
         constexpr bool G = decltype(gathered)::value;
         constexpr int NX = cfg.nx[OP], NY = cfg.ny[OP];
         if constexpr (OP != MB_GROUPED_GRAD_WEIGHTS) {
-            if (contraction % 32 != 0) return gemm_grouped_kernel<DT, OP, cfg.bm, cfg.bn, NX, NY, true, G>;
+            if (contraction % 32 != 0) return gemm_grouped_kernel<DT, OP, TILE, TILE, NX, NY, true, G>;
         }
-        return gemm_grouped_kernel<DT, OP, cfg.bm, cfg.bn, NX, NY, false, G>;
+        return gemm_grouped_kernel<DT, OP, TILE, TILE, NX, NY, false, G>;
     };
     auto kernel = c.rows ? pick(std::true_type{}) : pick(std::false_type{});
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a, (int)tiles_m, tiles_n, cfg.group_m);
@@ -512,9 +512,7 @@ int launch_grouped_dtype(const GroupedCall& c, int config, hipStream_t stream) {
     };
     if (config == 0) return by_op(std::integral_constant<int, 0>{});
     if (config == 1) return by_op(std::integral_constant<int, 1>{});
-    if (config == 2) return by_op(std::integral_constant<int, 2>{});
-    if (config == 3) return by_op(std::integral_constant<int, 3>{});
-    return by_op(std::integral_constant<int, 4>{});
+    return by_op(std::integral_constant<int, 2>{});
 }
 
 }  // namespace
