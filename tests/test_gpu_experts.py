@@ -293,6 +293,16 @@ def test_grouped_large_tiles(lib, op):
         _grouped(lib, op, "bfloat16", counts, n, k, tokens=None if op == capi.GROUPED_GRAD_ROWS else 1500)
 
 
+@pytest.mark.parametrize("config", [0, 1, 2, 3])
+@pytest.mark.parametrize("op", OPS)
+def test_grouped_on_every_tile(lib, tune, op, config):
+    # every ring from one stage of the contraction to several turns of it, and a contraction off the stage
+    tune(grouped_config=config)
+    for k in (8, 32, 40, 64, 96, 128, 160, 256, 456, 800):
+        _grouped(lib, op, "bfloat16", [70, 0, 1, 300], 264, k, tokens=None if op == capi.GROUPED_GRAD_ROWS else 200)
+        _grouped(lib, op, "float16", [k, 3, 33], k, 136)
+
+
 def test_grouped_many_experts(lib):
     counts = [(7 * e) % 11 if e % 5 else 0 for e in range(capi.ROUTE_MAX_EXPERTS)]
     for op in OPS:
@@ -436,6 +446,23 @@ def test_w4_dense(lib, dtype, rows, n, k, group, zeros):
 def test_w4_experts(lib, dtype, counts, n, k, group):
     _w4(lib, dtype, counts, n, k, group, True, tokens=20)
     _w4(lib, dtype, counts, n, k, group, False, extra=19, seed=1)
+
+
+@pytest.mark.parametrize("rows, n", [(3, 96), (16, 64), (30, 200), (64, 100)])
+def test_w4_k_splits(lib, rows, n, monkeypatch):
+    # few columns and a long K: blocks split K over the workspace; without one, or with one off 16 bytes, they do not
+    outs = [_w4(lib, "float16", [rows], n, 16384, 128, True, dense=True, seed=4)]
+    real = lib.handle.mb_gemm_w4
+    for pointer, size in ((None, 0), (1, 1 << 20), (0, 1 << 12)):
+
+        def call(*args, pointer=pointer, size=size):
+            args = list(args)
+            args[-3], args[-2] = (None if pointer is None else args[-3] + pointer), size
+            return real(*args)
+
+        monkeypatch.setattr(lib, "gemm_w4", lambda *a: lib._check(call(*a), "mb_gemm_w4"))
+        outs.append(_w4(lib, "float16", [rows], n, 16384, 128, True, dense=True, seed=4))
+    assert all(torch.equal(outs[1], out) for out in outs[2:])   # one and the same order of sums
 
 
 def test_w4_offsets_past_32_bits(lib):
