@@ -249,6 +249,9 @@ int mb_route_grad(int dtype, const void* logits, int64_t ld, const int32_t* expe
  * GRAD_WEIGHTS writes every matrix, zeros for an expert without rows.
  * x, y and out must not overlap. 1 <= experts <= MB_ROUTE_MAX_EXPERTS;
  * N, K >= 1; K * ldb below 2^31 bytes per matrix.
+ * workspace: any size, NULL included. Calls of few tiles run faster with one
+ * on 16 bytes that holds 2 to 16 fp32 copies of out (they split the
+ * contraction); what it holds before the call does not matter.
  */
 #define MB_GROUPED_FORWARD 0
 #define MB_GROUPED_GRAD_ROWS 1
@@ -267,7 +270,8 @@ int mb_gemm_grouped(int op, int dtype, const void* x, int64_t ldx, int64_t x_row
  * N x ceil(K / group) of x's type; zeros NULL stands for 8. `group` is a
  * positive multiple of 32. The integers are multiplied exactly and scaled in
  * fp32, group by group. Output rows at and past offsets[experts] are left alone.
- * Meant for few rows per expert (decode); any number is taken.
+ * Meant for few rows per expert (decode); any number is taken. workspace: as
+ * in mb_gemm_grouped.
  */
 int mb_gemm_w4(int dtype, const void* x, int64_t ldx, int64_t x_rows, const int32_t* rows, const void* q,
                const void* scales, const void* zeros, int group, void* out, int64_t ldo, const int32_t* offsets,

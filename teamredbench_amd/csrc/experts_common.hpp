@@ -33,9 +33,13 @@ struct GroupedCall {
 // Tile heights and widths of the pipelined grouped kernels.
 constexpr int kGroupedTileCount = 3;
 constexpr int kGroupedTiles[kGroupedTileCount] = {256, 128, 64};
-// The pipelined kernels (rows on 16 bytes) on tiles of kGroupedTiles[config], one per input type.
-int gemm_grouped_tiled_bf16(const GroupedCall& c, int config, hipStream_t stream);
-int gemm_grouped_tiled_f16(const GroupedCall& c, int config, hipStream_t stream);
+struct GroupedPlan {
+    int config;   // tiles of kGroupedTiles[config] on the pipelined kernels; -1: the kernel for any rows
+    int splits;   // of the contraction, over fp32 planes in the workspace (tiles of 128 and 64)
+};
+// The pipelined kernels (rows on 16 bytes), one per input type.
+int gemm_grouped_tiled_bf16(const GroupedCall& c, const GroupedPlan& plan, void* workspace, hipStream_t stream);
+int gemm_grouped_tiled_f16(const GroupedCall& c, const GroupedPlan& plan, void* workspace, hipStream_t stream);
 int gemm_grouped_launch(const GroupedCall& c, void* workspace, size_t workspace_bytes, const DeviceProps& props,
                         hipStream_t stream);
 

@@ -218,40 +218,47 @@ int launch_any_op(const GroupedCall& c, hipStream_t stream) {
     return launch_any<DT, MB_GROUPED_GRAD_WEIGHTS>(c, stream);
 }
 
-// The tile configuration of the pipelined kernels, -1 for what they do not
-// take: rows off 16 bytes, or an operand (one expert's matrix, x read through
-// `rows`, a tile's rows) that passes the 2^31 bytes a buffer offset spans.
-int tiled_config(const GroupedCall& c, const DeviceProps& props) {
+// How a call runs. The pipelined kernels do not take rows off 16 bytes, nor an
+// operand (one expert's matrix, x read through `rows`, a tile's rows) that
+// passes the 2^31 bytes a buffer offset spans.
+GroupedPlan grouped_plan(const GroupedCall& c, size_t workspace_bytes, const DeviceProps& props) {
+    constexpr GroupedPlan kAny{-1, 1};
     const uintptr_t base = reinterpret_cast<uintptr_t>(c.x) | reinterpret_cast<uintptr_t>(c.y) |
                            reinterpret_cast<uintptr_t>(c.out);
     if ((base & 15) != 0 || ((c.ldx | c.ldy | c.ldo | c.N | c.K) & 7) != 0 || c.total_rows == 0 || c.x_rows == 0)
-        return -1;
+        return kAny;
     // Every row a tile can address, those past its operand's end too, stays below 2^30 elements.
     constexpr int64_t kMost = (1ll << 30) - 1, kTileRows = 256;
     const bool weights = c.op == MB_GROUPED_GRAD_WEIGHTS;
     const int64_t x_rows = c.rows ? c.x_rows : weights ? c.total_rows : 0;
     const int64_t y_rows = weights ? c.total_rows : c.K;
     if (std::max(x_rows, kTileRows) > kMost / c.ldx - kTileRows || std::max(y_rows, kTileRows) > kMost / c.ldy - kTileRows)
-        return -1;
-    if (const int64_t forced = tuning(MB_TUNE_GROUPED_CONFIG); forced >= 0)
-        return forced < kGroupedTileCount ? (int)forced : -1;
+        return kAny;
+    const int64_t forced = tuning(MB_TUNE_GROUPED_CONFIG);
+    if (forced >= kGroupedTileCount) return kAny;
 
-    // The tile whose predicted time is least; a smaller one has to gain 3%. A
-    // block takes an overhead (its first loads and its stores) and a time per
-    // 32 of the contraction, measured at 16384 rows x 4096 x 14336 over 8
-    // experts with every CU full: 0.75 us on 256 x 256 tiles (one a CU), 0.535
-    // on 128 x 128 (two) and 0.386 on 64 x 64 (three). Nothing beats the bytes, at 5.2 TB/s. An expert's row tiles: its
-    // rows, were they even, and half a tile; with fewer rows than a tile one, and a share of experts that pass it.
+    // The tile and split count whose predicted time is least; each smaller
+    // tile or further split has to gain 3%. A block takes an overhead (its
+    // first loads and its stores) and a time per 32 of the contraction,
+    // measured at 16384 rows x 4096 x 14336 over 8 experts with every CU full:
+    // 0.75 us on 256 x 256 tiles (one a CU), 0.535 on 128 x 128 (two) and
+    // 0.386 on 64 x 64 (three). Nothing beats the bytes, at 5.2 TB/s. An
+    // expert's row tiles: its rows, were they even, and half a tile; with
+    // fewer rows than a tile one, and a share of experts that pass it. Splits cost a second
+    // launch and their planes, written and read.
     constexpr double kStageUs[kGroupedTileCount] = {0.75, 0.535, 0.386};
     constexpr double kBlockUs[kGroupedTileCount] = {8, 4, 4};
     constexpr int kPerCu[kGroupedTileCount] = {1, 2, 3};
+    constexpr double kSumUs = 5, kBytesPerUs = 5.2e6;
     const int64_t hit = std::min<int64_t>(c.experts, c.total_rows);   // experts with rows, at most
     const double per_expert = (double)c.total_rows / c.experts;
     const int64_t NN = c.op == MB_GROUPED_GRAD_ROWS ? c.K : c.N, C = c.op == MB_GROUPED_GRAD_ROWS ? c.N : c.K;
-    const double bytes_us = 2.0 * ((double)hit * c.K * c.N + (double)c.total_rows * (c.K + c.N)) / 5.2e6;
-    int best = 0;
+    const double plane = 4.0 * (double)(weights ? c.experts * c.K : c.total_rows) * (double)NN;
+    const double bytes_us = 2.0 * ((double)hit * c.K * c.N + (double)c.total_rows * (c.K + c.N)) / kBytesPerUs;
+    GroupedPlan best = kAny;
     double best_us = 0;
     for (int i = 0; i < kGroupedTileCount; ++i) {
+        if (forced >= 0 && forced != i) continue;
         const int tile = kGroupedTiles[i];
         const double wide = (double)((NN + tile - 1) / tile);
         double blocks, stages;
@@ -263,11 +270,15 @@ int tiled_config(const GroupedCall& c, const DeviceProps& props) {
             blocks = hit * wide * std::max(1.0 + 0.55 * std::max(0.0, tiles - 0.35), tiles + 0.45);
             stages = (double)((C + 31) / 32);
         }
-        const double rounds = std::ceil(blocks / props.cu_count) / kPerCu[i];
-        const double us = std::max(bytes_us, rounds * (kBlockUs[i] + stages * kStageUs[i]));
-        if (i == 0 || us < 0.97 * best_us) {
-            best = i;
-            best_us = us;
+        for (int splits = 1; splits <= 16; splits *= 2) {
+            if (splits > 1 && (i == 0 || stages < 4.0 * splits || plane * splits > (double)workspace_bytes)) break;
+            const double rounds = std::ceil(blocks * splits / props.cu_count) / kPerCu[i];
+            double us = std::max(bytes_us, rounds * (kBlockUs[i] + stages / splits * kStageUs[i]));
+            if (splits > 1) us += kSumUs + 2 * splits * plane / kBytesPerUs;
+            if (best.config < 0 || us < 0.97 * best_us) {
+                best = {i, splits};
+                best_us = us;
+            }
         }
     }
     return best;
@@ -277,10 +288,12 @@ int tiled_config(const GroupedCall& c, const DeviceProps& props) {
 
 int gemm_grouped_launch(const GroupedCall& c, void* workspace, size_t workspace_bytes, const DeviceProps& props,
                         hipStream_t stream) {
-    const int config = tiled_config(c, props);
-    if (config >= 0)
-        return c.dtype == MB_DT_FLOAT16 ? gemm_grouped_tiled_f16(c, config, stream)
-                                        : gemm_grouped_tiled_bf16(c, config, stream);
+    // The workspace only makes small calls faster: one off 16 bytes is left alone.
+    if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0) workspace_bytes = 0;
+    const GroupedPlan plan = grouped_plan(c, workspace_bytes, props);
+    if (plan.config >= 0)
+        return c.dtype == MB_DT_FLOAT16 ? gemm_grouped_tiled_f16(c, plan, workspace, stream)
+                                        : gemm_grouped_tiled_bf16(c, plan, workspace, stream);
     if (c.dtype == MB_DT_FLOAT16) return launch_any_op<MB_DT_FLOAT16>(c, stream);
     return launch_any_op<MB_DT_BFLOAT16>(c, stream);
 }

@@ -3,8 +3,8 @@
 
 namespace mb {
 
-int gemm_grouped_tiled_bf16(const GroupedCall& c, int config, hipStream_t stream) {
-    return launch_grouped_dtype<MB_DT_BFLOAT16>(c, config, stream);
+int gemm_grouped_tiled_bf16(const GroupedCall& c, const GroupedPlan& plan, void* workspace, hipStream_t stream) {
+    return launch_grouped_dtype<MB_DT_BFLOAT16>(c, plan, workspace, stream);
 }
 
 }  // namespace mb

@@ -77,6 +77,10 @@ struct GroupedArgs {
     int ldx, ldy;          // bytes per row
     int64_t ldo;           // bytes per row
     int x_rows, experts, total, N, K;
+    // Splits of the contraction: split s of a tile writes its fp32 sums to plane s of `planes` ([rows of out][ldp]).
+    // c_len: c per split (forward, rows' gradient), whole pairs of stages.
+    float* planes;
+    int splits, c_len, ldp;
 };
 
 // One operand of one tile: its LDS ring, DMA offsets and operand reads. ALONG: rows along c.
@@ -129,15 +133,21 @@ gemm_grouped_kernel(GroupedArgs args, int tiles_m_max, int tiles_n, int group_m)
     if constexpr (WEIGHTS) {
         // An expert's tiles are dealt to the 8 XCDs (block b runs on XCD b % 8) in runs, so every XCD gets its share of every
         // expert, however uneven the experts' rows; within it, a compact patch.
-        const int tiles = tiles_m_max * tiles_n, e = (int)blockIdx.x / tiles;
-        block_coords((int)blockIdx.x - e * tiles, tiles_m_max, tiles_n, 1, group_m, &tm, &tn, &split);
+        const int tiles = tiles_m_max * tiles_n * args.splits, e = (int)blockIdx.x / tiles;
+        block_coords((int)blockIdx.x - e * tiles, tiles_m_max, tiles_n, args.splits, group_m, &tm, &tn, &split);
         ex = expert_rows(args.offsets, e, args.total);
+        if (args.splits > 1) {   // this split's share of the expert's rows; none for the last splits of a short one
+            const int share = (ex.count + 32 * args.splits - 1) / (32 * args.splits) * 32;
+            const int from = min(split * share, ex.count);
+            ex.first += from;
+            ex.count = min(share, ex.count - from);
+        }
         ex.first = __builtin_amdgcn_readfirstlane(ex.first);
         ex.count = __builtin_amdgcn_readfirstlane(ex.count);
     } else {
         const int tiles_m = count_row_tiles(args.offsets, args.experts, args.total, BM);
-        if ((int)blockIdx.x >= tiles_m * tiles_n) return;
-        block_coords((int)blockIdx.x, tiles_m, tiles_n, 1, group_m, &tm, &tn, &split);
+        if ((int)blockIdx.x >= tiles_m * tiles_n * args.splits) return;
+        block_coords((int)blockIdx.x, tiles_m, tiles_n, args.splits, group_m, &tm, &tn, &split);
         if (!find_row_tile(args.offsets, args.experts, args.total, tm, BM, &ex, &tm)) return;
     }
     const int M = WEIGHTS ? args.K : ex.count;
@@ -145,6 +155,7 @@ gemm_grouped_kernel(GroupedArgs args, int tiles_m_max, int tiles_n, int group_m)
     const int C = WEIGHTS ? ex.count : YA ? args.N : args.K;
     const int m0 = tm * BM, n0 = tn * BN;
     const int ldx = args.ldx, ldy = args.ldy;
+    const int c0 = WEIGHTS ? 0 : split * args.c_len;   // first c of this block
 
     // Buffer resources. Along c: the tile's rows (gathered: all of x). Across c: the expert's rows from the
     // tile's first column on.
@@ -237,7 +248,7 @@ gemm_grouped_kernel(GroupedArgs args, int tiles_m_max, int tiles_n, int group_m)
         constexpr int q = decltype(idx)::value;
         const unsigned to = lds_of(at) + (wave * RX::kInstr + q) * 1024;
         if constexpr (XA) {
-            const int kb = i * 2 * kStageK;
+            const int kb = c0 * 2 + i * 2 * kStageK;
             lds_dma16(rx, to, along(x_off[q], kb, q), kb);
         } else if constexpr (GATHER) {
             constexpr int per = 1024 / X_ROW;   // rows of c per instruction
@@ -260,10 +271,10 @@ gemm_grouped_kernel(GroupedArgs args, int tiles_m_max, int tiles_n, int group_m)
         constexpr int q = decltype(idx)::value;
         const unsigned to = lds_of(at) + (wave * RY::kInstr + q) * 1024;
         if constexpr (YA) {
-            const int kb = i * 2 * kStageK;
+            const int kb = c0 * 2 + i * 2 * kStageK;
             lds_dma16(ry, to, along(y_off[q], kb, q), kb);
         } else {
-            lds_dma16(ry, to, y_off[q], i * 32 * ldy);
+            lds_dma16(ry, to, y_off[q], (c0 + i * 32) * ldy);
         }
     };
     constexpr int Y0 = RX::kBytes;   // the Y ring follows the X ring
@@ -317,7 +328,7 @@ gemm_grouped_kernel(GroupedArgs args, int tiles_m_max, int tiles_n, int group_m)
         acc[i][j] = Tr::mfma(o.b[s][j], o.a[s][i], acc[i][j]);
     };
 
-    const int ksteps = max((C + 31) >> 5, 1);
+    const int ksteps = max(((WEIGHTS ? C : min(C - c0, args.c_len)) + 31) >> 5, 1);
     const int last = ksteps - 1, last_pair = last / 2;
     // Every load of one operand's pair or stage that step v issues, as N_SLOTS of them exist.
     constexpr int VX = XA ? 2 * NX - 1 : NX, VY = YA ? 2 * NY - 1 : NY;
@@ -415,6 +426,29 @@ gemm_grouped_kernel(GroupedArgs args, int tiles_m_max, int tiles_n, int group_m)
     }
     wait_vmcnt_and_barrier<0>();
 
+    if constexpr (BM < 256) {
+        if (args.planes != nullptr) {
+            const int64_t rows = WEIGHTS ? (int64_t)args.experts * args.K : args.total;
+            float* part = args.planes + (split * rows + (WEIGHTS ? (int64_t)ex.expert * args.K : ex.first)) * args.ldp;
+#pragma unroll
+            for (int i = 0; i < FM; ++i) {
+                const int m = m0 + wm * WTM + 32 * i + (lane & 31);
+                if (m >= M) continue;
+#pragma unroll
+                for (int j = 0; j < FN; ++j)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const int n = n0 + wn * WTN + 32 * j + 8 * g + 4 * half;   // ldp is a multiple of 8
+                        const f32x16& v = acc[i][j];
+                        if (n < args.ldp)
+                            *reinterpret_cast<f32x4*>(part + m * (int64_t)args.ldp + n) =
+                                f32x4{v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]};
+                    }
+            }
+            return;
+        }
+    }
+
     // Epilogue: 16-bit rows through LDS, stored as whole row segments; register 4g + q of lane l holds
     // out(32i + l % 32, 32j + 8g + 4 (l / 32) + q).
     unsigned char* ob = args.out + (WEIGHTS ? (int64_t)ex.expert * args.K : (int64_t)ex.first) * args.ldo;
@@ -461,6 +495,22 @@ gemm_grouped_kernel(GroupedArgs args, int tiles_m_max, int tiles_n, int group_m)
     }
 }
 
+// out = the sum of the splits' planes, in split order; rows of no expert are left alone.
+template <int DT>
+__global__ void __launch_bounds__(256)
+gemm_grouped_sum_kernel(GroupedArgs a, int64_t rows, int columns, bool sorted) {
+    const int quads = a.ldp / 4;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t m = i / quads;
+    if (m >= rows) return;
+    if (sorted && (m < a.offsets[0] || m >= a.offsets[a.experts])) return;
+    const int n = 4 * (int)(i - m * quads);
+    const float* from = a.planes + m * a.ldp + n;
+    f32x4 v = *reinterpret_cast<const f32x4*>(from);
+    for (int s = 1; s < a.splits; ++s) v += *reinterpret_cast<const f32x4*>(from + s * rows * a.ldp);
+    if (n < columns) *reinterpret_cast<u32x2*>(a.out + m * a.ldo + n * 2) = pack4<DT>(v[0], v[1], v[2], v[3]);
+}
+
 struct GroupedConfig {
     int group_m;
     int nx[3], ny[3];   // ring slots by op
@@ -474,7 +524,7 @@ constexpr GroupedConfig kGroupedConfigs[kGroupedTileCount] = {
 };
 
 template <int DT, int OP, int CFG>
-int launch_grouped(const GroupedCall& c, hipStream_t stream) {
+int launch_grouped(const GroupedCall& c, int splits, float* planes, hipStream_t stream) {
     constexpr GroupedConfig cfg = kGroupedConfigs[CFG];
     constexpr int TILE = kGroupedTiles[CFG];
     const int64_t NN = OP == MB_GROUPED_GRAD_ROWS ? c.K : c.N;
@@ -482,11 +532,14 @@ int launch_grouped(const GroupedCall& c, hipStream_t stream) {
     const bool weights = OP == MB_GROUPED_GRAD_WEIGHTS;
     const int64_t tiles_m = weights ? (c.K + TILE - 1) / TILE
                                     : c.total_rows / TILE + std::min<int64_t>(c.experts, c.total_rows);
-    const int64_t blocks = tiles_m * tiles_n * (weights ? c.experts : 1);
+    const int64_t contraction = OP == MB_GROUPED_FORWARD ? c.K : c.N;
+    const int c_len = (int)((contraction + 64 * splits - 1) / (64 * splits) * 64);
+    if (!weights) splits = (int)((contraction + c_len - 1) / c_len);   // none is empty
+    if (splits == 1) planes = nullptr;
+    const int64_t blocks = tiles_m * tiles_n * (weights ? c.experts : 1) * splits;
     GroupedArgs a{static_cast<const unsigned char*>(c.x), static_cast<const unsigned char*>(c.y),
                   static_cast<unsigned char*>(c.out), c.rows, c.offsets, (int)c.ldx * 2, (int)c.ldy * 2, c.ldo * 2,
-                  (int)c.x_rows, c.experts, (int)c.total_rows, (int)c.N, (int)c.K};
-    const int64_t contraction = OP == MB_GROUPED_FORWARD ? c.K : c.N;
+                  (int)c.x_rows, c.experts, (int)c.total_rows, (int)c.N, (int)c.K, planes, splits, c_len, (int)NN};
     // c past the expert's rows needs no check of its own: the matrices' gradient never takes the ragged form.
     auto pick = [&](auto gathered) {
         constexpr bool G = decltype(gathered)::value;
@@ -499,16 +552,24 @@ int launch_grouped(const GroupedCall& c, hipStream_t stream) {
     auto kernel = c.rows ? pick(std::true_type{}) : pick(std::false_type{});
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a, (int)tiles_m, tiles_n, cfg.group_m);
     MB_HIP_TRY(hipGetLastError());
+    if (splits > 1) {
+        const int64_t rows = weights ? c.experts * c.K : c.total_rows;
+        hipLaunchKernelGGL((gemm_grouped_sum_kernel<DT>), dim3((unsigned)((rows * (NN / 4) + 255) / 256)), dim3(256), 0,
+                           stream, a, rows, (int)NN, !weights);
+        MB_HIP_TRY(hipGetLastError());
+    }
     return MB_OK;
 }
 
 template <int DT>
-int launch_grouped_dtype(const GroupedCall& c, int config, hipStream_t stream) {
+int launch_grouped_dtype(const GroupedCall& c, const GroupedPlan& plan, void* workspace, hipStream_t stream) {
+    const int config = plan.config;
+    auto* planes = static_cast<float*>(workspace);
     auto by_op = [&](auto cfg) {
         constexpr int CFG = decltype(cfg)::value;
-        if (c.op == MB_GROUPED_FORWARD) return launch_grouped<DT, MB_GROUPED_FORWARD, CFG>(c, stream);
-        if (c.op == MB_GROUPED_GRAD_ROWS) return launch_grouped<DT, MB_GROUPED_GRAD_ROWS, CFG>(c, stream);
-        return launch_grouped<DT, MB_GROUPED_GRAD_WEIGHTS, CFG>(c, stream);
+        if (c.op == MB_GROUPED_FORWARD) return launch_grouped<DT, MB_GROUPED_FORWARD, CFG>(c, plan.splits, planes, stream);
+        if (c.op == MB_GROUPED_GRAD_ROWS) return launch_grouped<DT, MB_GROUPED_GRAD_ROWS, CFG>(c, plan.splits, planes, stream);
+        return launch_grouped<DT, MB_GROUPED_GRAD_WEIGHTS, CFG>(c, plan.splits, planes, stream);
     };
     if (config == 0) return by_op(std::integral_constant<int, 0>{});
     if (config == 1) return by_op(std::integral_constant<int, 1>{});

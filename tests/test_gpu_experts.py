@@ -195,7 +195,8 @@ def _offsets(counts: list[int]) -> torch.Tensor:
     return torch.tensor([0] + list(np.cumsum(counts)), dtype=torch.int32)
 
 
-def _grouped(lib, op, dtype, counts, n, k, *, tokens=None, extra=0, pad=(0, 0, 0), shift=0, seed=0):
+def _grouped(lib, op, dtype, counts, n, k, *, tokens=None, extra=0, pad=(0, 0, 0), shift=0, seed=0,
+             workspace=1 << 20):
     """One call and its check. tokens: x is read through `rows` of that many tokens (forward, weights).
     extra: sorted rows past the last expert's. pad: columns between rows of x, y, out. shift: elements the
     matrices start past an allocation."""
@@ -228,7 +229,7 @@ def _grouped(lib, op, dtype, counts, n, k, *, tokens=None, extra=0, pad=(0, 0, 0
     y = _strided(right, right.shape[1] + pad[1], shift)
     out = _strided(torch.full((out_rows, out_cols), CANARY, dtype=t), out_cols + pad[2], shift, CANARY)
     doff, drows = offsets.cuda(), None if rows is None else rows.cuda()
-    workspace = torch.full((1 << 20,), 255, dtype=torch.uint8, device="cuda")
+    workspace = torch.full((max(workspace, 1),), 255, dtype=torch.uint8, device="cuda")
     print(f"[grouped] op {op} {dtype} counts {counts if experts < 9 else experts} n {n} k {k} tokens {tokens} "
           f"extra {extra} pad {pad} shift {shift}", flush=True)
     lib.gemm_grouped(op, capi.DTYPES[dtype], x.data_ptr(), x.stride(0), left.shape[0],
@@ -301,6 +302,16 @@ def test_grouped_on_every_tile(lib, tune, op, config):
     for k in (8, 32, 40, 64, 96, 128, 160, 256, 456, 800):
         _grouped(lib, op, "bfloat16", [70, 0, 1, 300], 264, k, tokens=None if op == capi.GROUPED_GRAD_ROWS else 200)
         _grouped(lib, op, "float16", [k, 3, 33], k, 136)
+
+
+@pytest.mark.parametrize("op", OPS)
+def test_grouped_splits(lib, op):
+    # few tiles and a long contraction: blocks split it over the workspace; a smaller workspace, fewer splits
+    for counts, n, k in [([16, 0, 5], 1024, 512), ([3, 130], 512, 2048), ([700, 0, 1500], 64, 96), ([2000], 136, 72),
+                         ([40], 4104, 136), ([1, 0, 2, 33], 1000, 1096)]:
+        for workspace in (64 << 20, 300_000, 0):
+            _grouped(lib, op, "bfloat16", counts, n, k, workspace=workspace, extra=9,
+                     tokens=None if op == capi.GROUPED_GRAD_ROWS else 60)
 
 
 def test_grouped_many_experts(lib):
