@@ -269,7 +269,7 @@ int mb_gemm_grouped(int op, int dtype, const void* x, int64_t ldx, int64_t x_row
  * low half; a last high half past K is ignored. scales and zeros: experts x
  * N x ceil(K / group) of x's type; zeros NULL stands for 8. `group` is a
  * positive multiple of 32. The integers are multiplied exactly and scaled in
- * fp32, group by group. Output rows at and past offsets[experts] are left alone.
+ * fp32, group by group; a row of x with an infinity comes out as NaN. Output rows at and past offsets[experts] are left alone.
  * Meant for few rows per expert (decode); any number is taken. workspace: as
  * in mb_gemm_grouped.
  */

@@ -46,7 +46,8 @@ int check_route(const char* what, int dtype, int64_t tokens, int experts, int to
                       "%s: needs tokens >= 0, 1 <= experts <= %d, 1 <= top_k <= min(experts, %d) (got %lld, %d, %d)",
                       what, MB_ROUTE_MAX_EXPERTS, MB_ROUTE_MAX_TOP_K, (long long)tokens, experts, top_k);
     if (tokens >= kMostRows / top_k)
-        return refuse(MB_ERR_SHAPE, "%s: tokens * top_k must be below 2^31 (%lld * %d)", what, (long long)tokens, top_k);
+        return refuse(MB_ERR_SHAPE, "%s: tokens * top_k must be below 2^31 (%lld * %d)", what, (long long)tokens,
+                      top_k);
     return MB_OK;
 }
 

@@ -3,10 +3,11 @@
 //
 // Choice. 16 lanes per token (64 past 256 experts or 16 choices); lane l of
 // them holds logits l PER .. l PER + PER - 1, -inf for what cannot be chosen.
-// Each of top_k rounds takes the token's maximum and then the lowest expert that has it, by
-// rotations within the 16 lanes (DPP: no LDS), and clears it. The weights are
-// exp(l - m) / Z in fp32, m the largest logit. The vector unit's issue bounds this, and four tokens share each
-// instruction: 8.8 us at 16384 x 128 top 8, against 17.5 us with a whole wave per token.
+// Each of top_k rounds takes the token's maximum and then the lowest expert
+// that has it, by rotations within the 16 lanes (DPP: no LDS), and clears it.
+// The weights are exp(l - m) / Z in fp32, m the largest logit. The vector
+// unit's issue bounds this, and four tokens share each instruction: 8.8 us at
+// 16384 x 128 top 8, against 17.5 us with a whole wave per token.
 //
 // Order. Within an expert, assignments stand in token order (a token has an
 // expert once), so the place of token t's assignment to expert e is the number
@@ -14,11 +15,11 @@
 // chose e. Tokens go in groups of 64: one 64-bit mask per expert in LDS says
 // which tokens of the group chose it, its population count is the group's
 // count, and the count below bit t is t's rank. Masks are built with LDS
-// ORs, whose result does not depend on their order. At most kMaxBlocks
-// blocks, each over a run of groups, write their counts per expert ([expert][block]);
-// a second kernel adds up the counts of earlier blocks and of lower experts
-// (a wave per expert, a block's count a lane) and places. One block (up to 64 tokens) does both in
-// one launch.
+// ORs, whose result does not depend on their order. At most kMaxBlocks blocks,
+// each over a run of groups, write their counts per expert ([expert][block]); a
+// second kernel adds up the counts of earlier blocks and of lower experts (a
+// wave per expert, a block's count a lane: 8 us where a thread per expert took
+// 64) and places. One block (up to 64 tokens) does both in one launch, 3.5 us.
 #include "experts_common.hpp"
 
 #include <algorithm>
@@ -398,8 +399,8 @@ int route_launch(int dtype, const void* logits, int64_t ld, int64_t tokens, int 
         return with_lanes(experts, top_k, [&](auto lanes, auto per) {
             constexpr int DT = decltype(dt)::value, LANES = decltype(lanes)::value, PER = decltype(per)::value;
             if (blocks == 1) {
-                hipLaunchKernelGGL((route_choose_kernel<DT, LANES, PER, true>), dim3(1), dim3(64 * kWaves), 0, stream, logits,
-                                   ld, tokens, experts, top_k, (int)normalize, per_block, weights, expert_ids, counts,
+                hipLaunchKernelGGL((route_choose_kernel<DT, LANES, PER, true>), dim3(1), dim3(64 * kWaves), 0, stream,
+                                   logits, ld, tokens, experts, top_k, (int)normalize, per_block, weights, expert_ids, counts,
                                    offsets, rows, slots);
                 MB_HIP_TRY(hipGetLastError());
                 return (int)MB_OK;
@@ -408,8 +409,8 @@ int route_launch(int dtype, const void* logits, int64_t ld, int64_t tokens, int 
                                logits, ld, tokens, experts, top_k, (int)normalize, per_block, weights, expert_ids,
                                counts, offsets, rows, slots);
             MB_HIP_TRY(hipGetLastError());
-            hipLaunchKernelGGL(route_place_kernel, dim3(blocks), dim3(64 * kWaves), 0, stream, counts, blocks, tokens, experts,
-                               top_k, per_block, expert_ids, offsets, rows, slots);
+            hipLaunchKernelGGL(route_place_kernel, dim3(blocks), dim3(64 * kWaves), 0, stream, counts, blocks, tokens,
+                               experts, top_k, per_block, expert_ids, offsets, rows, slots);
             MB_HIP_TRY(hipGetLastError());
             return (int)MB_OK;
         });
@@ -424,7 +425,8 @@ int route_grad_launch(int dtype, const void* logits, int64_t ld, const int32_t* 
             constexpr int DT = decltype(dt)::value, LANES = decltype(lanes)::value, PER = decltype(per)::value;
             constexpr int kTokens = 256 / LANES;   // per block
             hipLaunchKernelGGL((route_grad_kernel<DT, LANES, PER>), dim3((unsigned)((tokens + kTokens - 1) / kTokens)),
-                               dim3(256), 0, stream, logits, ld, expert_ids, grad_weights, tokens, experts, top_k, (int)normalize,
+                               dim3(256), 0, stream, logits, ld, expert_ids, grad_weights, tokens, experts, top_k,
+                               (int)normalize,
                                grad_logits, ld_grad);
             MB_HIP_TRY(hipGetLastError());
             return (int)MB_OK;

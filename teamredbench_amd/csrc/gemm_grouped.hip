@@ -11,12 +11,13 @@
 // gemm_grouped_any_kernel takes any size, stride and alignment: 128 x 128
 // tiles, 4 waves of 64 x 64 on v_mfma_f32_32x32x16, a stage of 32 c, through
 // registers into one of two LDS buffers while the other is computed. Global
-// loads are 16 bytes at any element (the hardware takes them); an operand whose rows run along c is kept as
-// [m or n][32 c] in rows of 80 bytes, one whose rows run across it as [32 c][m or n], swizzled, and read with the
-// transposing LDS reads. Rows of c past the
-// expert's and c past the end load as zeros; columns past the matrix hold
-// whatever the row's window holds there and are not stored; nothing past a
-// row's last element is read.
+// loads are 16 bytes at any element (the hardware takes them; element by
+// element it took twice as long, 645 against 317 us for 12004 rows over 60
+// experts, 2057 -> 1411). An operand whose rows run along c is kept as [m or
+// n][32 c] in rows of 80 bytes, one whose rows run across it as [32 c][m or n],
+// swizzled, and read with the transposing LDS reads. Rows of c past the
+// expert's and c past the end load as zeros; nothing past a row's last element
+// is read. Bound by the loads' latency: one stage ahead, two blocks a CU.
 #include "gemm_grouped_kernels.hpp"
 
 #include <algorithm>
@@ -35,8 +36,8 @@ __device__ __forceinline__ u32x4 row_window(const uint16_t* row, int c, int n) {
     if (c + 8 <= n) return *reinterpret_cast<const u32x4_any*>(row + c);
     if (c >= n) return u32x4{0u, 0u, 0u, 0u};
     if (n >= 8) {   // the row's last 8, shifted down
-        const __uint128_t wide = __builtin_bit_cast(__uint128_t, (u32x4)*reinterpret_cast<const u32x4_any*>(row + n - 8));
-        return __builtin_bit_cast(u32x4, wide >> (16 * (c + 8 - n)));
+        const u32x4 v = *reinterpret_cast<const u32x4_any*>(row + n - 8);
+        return __builtin_bit_cast(u32x4, __builtin_bit_cast(__uint128_t, v) >> (16 * (c + 8 - n)));
     }
     __uint128_t wide = 0;
 #pragma unroll 1
@@ -131,7 +132,8 @@ gemm_grouped_any_kernel(const uint16_t* __restrict__ x, int64_t ldx, int64_t x_r
     auto fragment = [&](const unsigned char* from, bool along, int base, int s) {
         if (along)
             return *reinterpret_cast<const u32x4*>(from + (base + (lane & 31)) * kPitch + 32 * s + 16 * (lane >> 5));
-        const u32x2 lo = read_b_piece<DT, kTile>(from, base, s, 0, lane), hi = read_b_piece<DT, kTile>(from, base, s, 1, lane);
+        const u32x2 lo = read_b_piece<DT, kTile>(from, base, s, 0, lane);
+        const u32x2 hi = read_b_piece<DT, kTile>(from, base, s, 1, lane);
         return u32x4{lo[0], lo[1], hi[0], hi[1]};
     };
 
@@ -186,7 +188,8 @@ gemm_grouped_any_kernel(const uint16_t* __restrict__ x, int64_t ldx, int64_t x_r
                 const int n = n0 + 64 * wn + 32 * j + 8 * g + 4 * (lane >> 5);
                 const f32x16& v = acc[i][j];
                 if (n + 4 <= NN) {
-                    *reinterpret_cast<u32x2_any*>(row + n) = pack4<DT>(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
+                    *reinterpret_cast<u32x2_any*>(row + n) =
+                        pack4<DT>(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
                 } else {
 #pragma unroll
                     for (int r = 0; r < 3; ++r)
@@ -232,7 +235,8 @@ GroupedPlan grouped_plan(const GroupedCall& c, size_t workspace_bytes, const Dev
     const bool weights = c.op == MB_GROUPED_GRAD_WEIGHTS;
     const int64_t x_rows = c.rows ? c.x_rows : weights ? c.total_rows : 0;
     const int64_t y_rows = weights ? c.total_rows : c.K;
-    if (std::max(x_rows, kTileRows) > kMost / c.ldx - kTileRows || std::max(y_rows, kTileRows) > kMost / c.ldy - kTileRows)
+    if (std::max(x_rows, kTileRows) > kMost / c.ldx - kTileRows ||
+        std::max(y_rows, kTileRows) > kMost / c.ldy - kTileRows)
         return kAny;
     const int64_t forced = tuning(MB_TUNE_GROUPED_CONFIG);
     if (forced >= kGroupedTileCount) return kAny;

@@ -21,6 +21,11 @@
 // reads as zeros; c past the expert's rows (matrices' gradient) lies past the
 // operand's range. Columns past the matrix read whatever follows in range and
 // are not stored.
+//
+// Many rows per expert are bound by the MFMAs at the clock the power limit
+// leaves, as the dense kernel is (16384 rows over 8 experts, 4096 -> 14336:
+// 1574 us, 1.22 PFLOP/s); few rows by the matrices' bytes, which the deep rings
+// keep in flight (128 rows over 32 experts, 4096 -> 2048: 88 us, 6.1 TB/s).
 #pragma once
 
 #include "experts_common.hpp"
@@ -36,11 +41,12 @@ struct StepWaits {
 };
 
 // Loads: operand o is held in pairs (pair[o]) or stages, n[o] slots, instr[o]
-// LDS-DMA instructions per wave and slot. Step j issues, X before Y or (y_first) after it, pair
+// LDS-DMA instructions per wave and slot. Step j issues, X before Y, pair
 // (j - 1) / 2 + n of a paired operand when j is odd and stage j + n of a
 // staged one; the prologue runs the same rule over the steps before 0. Step j
-// reads stage j + 1, so its wait leaves only the loads issued after that stage's.
-constexpr StepWaits step_schedule(bool px, int nx, int ix, bool py, int ny, int iy, bool y_first) {
+// reads stage j + 1, so its wait leaves only the loads issued after that
+// stage's. (Y first where it has fewer slots: no faster.)
+constexpr StepWaits step_schedule(bool px, int nx, int ix, bool py, int ny, int iy) {
     constexpr int kSteps = 64;
     const bool pair[2] = {px, py};
     const int n[2] = {nx, ny}, instr[2] = {ix, iy};
@@ -48,8 +54,7 @@ constexpr StepWaits step_schedule(bool px, int nx, int ix, bool py, int ny, int 
     int total = 0;
     for (int v = -2 * kSteps / 4; v < kSteps; ++v) {
         if (v >= 0) before[v] = total;
-        for (int k = 0; k < 2; ++k) {
-            const int o = y_first ? 1 - k : k;
+        for (int o = 0; o < 2; ++o) {
             if (pair[o] && (v & 1) == 0) continue;
             const int i = pair[o] ? (v - 1) / 2 + n[o] : v + n[o];   // v - 1 is even
             if (i >= 0 && i < 2 * kSteps) end[o][i] = (total += instr[o]);
@@ -114,9 +119,7 @@ gemm_grouped_kernel(GroupedArgs args, int tiles_m_max, int tiles_n, int group_m)
     typedef Ring<YA, BN, W, NY> RY;
     constexpr int LDS_BYTES = RX::kBytes + RY::kBytes;
     static_assert(LDS_BYTES <= 160 * 1024, "LDS rings do not fit");
-    // The operand with fewer slots is needed sooner after its loads: they go first.
-    constexpr bool Y_FIRST = XA == YA && NY < NX;
-    constexpr StepWaits kWaits = step_schedule(XA, NX, RX::kInstr, YA, NY, RY::kInstr, Y_FIRST);
+    constexpr StepWaits kWaits = step_schedule(XA, NX, RX::kInstr, YA, NY, RY::kInstr);
     static_assert(kWaits.prologue >= 0 && kWaits.odd >= 0 && kWaits.even >= 0 && kWaits.prologue < 64 &&
                   kWaits.odd < 64 && kWaits.even < 64, "a needed stage is unissued, or vmcnt overflows");
     __shared__ __attribute__((aligned(1024))) unsigned char lds[LDS_BYTES];
@@ -131,8 +134,9 @@ gemm_grouped_kernel(GroupedArgs args, int tiles_m_max, int tiles_n, int group_m)
     ExpertRows ex;
     int tm, tn, split;
     if constexpr (WEIGHTS) {
-        // An expert's tiles are dealt to the 8 XCDs (block b runs on XCD b % 8) in runs, so every XCD gets its share of every
-        // expert, however uneven the experts' rows; within it, a compact patch.
+        // An expert's tiles are dealt to the 8 XCDs (block b runs on XCD b % 8)
+        // in runs, so every XCD gets its share of every expert, however uneven
+        // the experts' rows; within it, a compact patch.
         const int tiles = tiles_m_max * tiles_n * args.splits, e = (int)blockIdx.x / tiles;
         block_coords((int)blockIdx.x - e * tiles, tiles_m_max, tiles_n, args.splits, group_m, &tm, &tn, &split);
         ex = expert_rows(args.offsets, e, args.total);
@@ -255,7 +259,8 @@ gemm_grouped_kernel(GroupedArgs args, int tiles_m_max, int tiles_n, int group_m)
             int base = 0;
 #pragma unroll
             for (int s = 0; s < per; ++s) {
-                const unsigned r = (unsigned)__builtin_amdgcn_readfirstlane(listed[q * per + s]);   // scalars: no indexed select
+                // Scalars: a select among array elements would become an indexed load.
+                const unsigned r = (unsigned)__builtin_amdgcn_readfirstlane(listed[q * per + s]);
                 const int off = r < (unsigned)args.x_rows ? (int)r * ldx : kNowhere;
                 base = s == 0 || lane / (64 / per) == s ? off : base;
             }
@@ -337,23 +342,20 @@ gemm_grouped_kernel(GroupedArgs args, int tiles_m_max, int tiles_n, int group_m)
         ([&] {
             constexpr int v = U - V;
             constexpr int ix = XA ? (v - 1) / 2 + NX : v + NX, iy = YA ? (v - 1) / 2 + NY : v + NY;
-            auto x_loads = [&] {
-                if constexpr ((!XA || (v & 1) != 0) && ix >= 0) {
-                    const int i = min(ix, XA ? last_pair : last);
-                    int listed[kShare] = {};
-                    gather(i, listed);
-                    [&]<int... Q>(std::integer_sequence<int, Q...>) {
-                        (issue_x(i, ix * RX::kSlot, std::integral_constant<int, Q>{}, listed), ...);
-                    }(std::make_integer_sequence<int, RX::kInstr>{});
-                }
-            };
-            if constexpr (!Y_FIRST) x_loads();
-            if constexpr ((!YA || (v & 1) != 0) && iy >= 0) {
+            if constexpr ((!XA || (v & 1) != 0) && ix >= 0) {
+                const int i = min(ix, XA ? last_pair : last);
+                int listed[kShare] = {};
+                gather(i, listed);
                 [&]<int... Q>(std::integer_sequence<int, Q...>) {
-                    (issue_y(min(iy, YA ? last_pair : last), Y0 + iy * RY::kSlot, std::integral_constant<int, Q>{}), ...);
+                    (issue_x(i, ix * RX::kSlot, std::integral_constant<int, Q>{}, listed), ...);
+                }(std::make_integer_sequence<int, RX::kInstr>{});
+            }
+            if constexpr ((!YA || (v & 1) != 0) && iy >= 0) {
+                const int i = min(iy, YA ? last_pair : last);
+                [&]<int... Q>(std::integer_sequence<int, Q...>) {
+                    (issue_y(i, Y0 + iy * RY::kSlot, std::integral_constant<int, Q>{}), ...);
                 }(std::make_integer_sequence<int, RY::kInstr>{});
             }
-            if constexpr (Y_FIRST) x_loads();
         }(), ...);
     }(std::make_integer_sequence<int, V>{});
 
@@ -402,11 +404,10 @@ gemm_grouped_kernel(GroupedArgs args, int tiles_m_max, int tiles_n, int group_m)
                         constexpr int m = lo + R;
                         if constexpr (kIsLoad(m)) {
                             constexpr int l = (m + 1) / kStride - 1;
-                            constexpr int lx = Y_FIRST ? l - Y_LOADS : l, ly = Y_FIRST ? l : l - X_LOADS;
-                            if constexpr (Y_FIRST ? l >= Y_LOADS : l < X_LOADS)
-                                issue_x(x_load, LX * RX::kSlot, std::integral_constant<int, lx>{}, list_sets[I % 2]);
+                            if constexpr (l < X_LOADS)
+                                issue_x(x_load, LX * RX::kSlot, std::integral_constant<int, l>{}, list_sets[I % 2]);
                             else
-                                issue_y(y_load, Y0 + LY * RY::kSlot, std::integral_constant<int, ly>{});
+                                issue_y(y_load, Y0 + LY * RY::kSlot, std::integral_constant<int, l - X_LOADS>{});
                         } else {
                             constexpr int loads_before = m / kStride < LOADS ? m / kStride : LOADS;
                             read_op(next_x, next_y, std::integral_constant<int, (I + 1) & 1>{},
@@ -567,8 +568,10 @@ int launch_grouped_dtype(const GroupedCall& c, const GroupedPlan& plan, void* wo
     auto* planes = static_cast<float*>(workspace);
     auto by_op = [&](auto cfg) {
         constexpr int CFG = decltype(cfg)::value;
-        if (c.op == MB_GROUPED_FORWARD) return launch_grouped<DT, MB_GROUPED_FORWARD, CFG>(c, plan.splits, planes, stream);
-        if (c.op == MB_GROUPED_GRAD_ROWS) return launch_grouped<DT, MB_GROUPED_GRAD_ROWS, CFG>(c, plan.splits, planes, stream);
+        if (c.op == MB_GROUPED_FORWARD)
+            return launch_grouped<DT, MB_GROUPED_FORWARD, CFG>(c, plan.splits, planes, stream);
+        if (c.op == MB_GROUPED_GRAD_ROWS)
+            return launch_grouped<DT, MB_GROUPED_GRAD_ROWS, CFG>(c, plan.splits, planes, stream);
         return launch_grouped<DT, MB_GROUPED_GRAD_WEIGHTS, CFG>(c, plan.splits, planes, stream);
     };
     if (config == 0) return by_op(std::integral_constant<int, 0>{});

@@ -12,8 +12,8 @@
 // byte permutes). bf16 multiplies 128 + q and an MFMA against ones gives the
 // group's sum of x, so group by group, in fp32,
 //   out += s * (sum x (128 + q)) - s (128 + z) * (sum x);
-// the offset costs 5 of fp32's 24 bits beside a bf16 result's 8. fp16, which keeps 11, subtracts 1032
-// first (exact), and needs the sum of x only for z - 8.
+// the offset costs 5 of fp32's 24 bits beside a bf16 result's 8. fp16, which
+// keeps 11, subtracts 1032 first (exact), and needs the sum of x only for z - 8.
 //
 // Lanes. Lane l reads column l % 16; its 16 bytes are k 32 (l / 16) .. + 31 of a
 // chunk of 128, so a column's reads are 64 contiguous bytes. The MFMA wants k
@@ -22,11 +22,14 @@
 // lane-swap instructions per 16 bytes.
 //
 // Up to 16 rows per expert (gemm_w4_kernel): the waves of a block share 32
-// columns and split K in units of 256, x
-// comes straight from L2 with the weights, both one unit ahead, and the waves add their fp32 sums
-// through LDS, in wave order. More rows (gemm_w4_rows_kernel): the waves
-// split 256 columns and share x through LDS, 256 k at a time, with the sums of x made on the way in.
-// Few columns: blocks split K too, into fp32 planes that a second kernel adds.
+// columns and split K in units of 256; weights come one unit ahead, x straight
+// from L2, and the waves add their fp32 sums through LDS, in wave order: 10.8 us
+// at 1 x 14336 x 4096, of which the bytes are 5.9. More rows, or columns
+// enough without (gemm_w4_rows_kernel): the waves split 256 columns and share x
+// through LDS, 256 k at a time, with the sums of x made on the way in: 57 us
+// (4.9 TB/s) for 256 rows over 64 experts, 4096 -> 2048, and 61 us at 64 x
+// 50257 x 4096, where widening and scaling bound it. Few columns: blocks split
+// K too, into fp32 planes that a second kernel adds.
 //
 // Rows that are not there multiply some other row's x and are stored as zeros;
 // units that run past K take zeros for x and whatever weights lie there in bounds.
@@ -642,7 +645,8 @@ int launch_rows(const W4Call& c, void* workspace, size_t bytes, const DeviceProp
         // 4096: 66 against 91 us).
         const int64_t blocks = likely_tiles(c, 16) * ((c.N + 31) / 32);
         if (blocks < props.cu_count) return launch_group<DT, ZEROS, 0, 1, 8>(c, workspace, bytes, props, stream);
-        if (2 * blocks < 3 * props.cu_count) return launch_group<DT, ZEROS, 0, 2, 8>(c, workspace, bytes, props, stream);
+        if (2 * blocks < 3 * props.cu_count)
+            return launch_group<DT, ZEROS, 0, 2, 8>(c, workspace, bytes, props, stream);
         if (blocks < 8 * props.cu_count) return launch_group<DT, ZEROS, 0, 2, 4>(c, workspace, bytes, props, stream);
         return launch_group<DT, ZEROS, 1, 2, 8>(c, workspace, bytes, props, stream);
     }

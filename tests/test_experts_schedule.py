@@ -21,17 +21,15 @@ STEPS = 60
 def rings(tmp_path_factory):
     hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
     exe = tmp_path_factory.mktemp("schedule") / "experts_schedule_host"
-    subprocess.run([hipcc, "--offload-host-only", "-O1", "-std=c++20", "-w", str(TESTS / "experts_schedule_host.cpp"), "-o",
-                    str(exe)], check=True)
+    subprocess.run([hipcc, "--offload-host-only", "-O1", "-std=c++20", "-w", str(TESTS / "experts_schedule_host.cpp"),
+                    "-o", str(exe)], check=True)
     out = subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout
     return [tuple(int(v) for v in line.split()) for line in out.splitlines()]
 
 
-def _replay(px, nx, ix, py, ny, iy, y_first, odd, even, prologue) -> str | None:
+def _replay(px, nx, ix, py, ny, iy, odd, even, prologue) -> str | None:
     """What goes wrong, or None."""
     operands = [("x", px, nx, ix), ("y", py, ny, iy)]
-    if y_first:
-        operands.reverse()
     issued: list[tuple[str, int]] = []   # (operand, pair or stage) of every load, in order
 
     def issue(step):

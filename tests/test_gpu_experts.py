@@ -452,8 +452,8 @@ def test_w4_dense(lib, dtype, rows, n, k, group, zeros):
 
 
 @pytest.mark.parametrize("dtype", HALF)
-@pytest.mark.parametrize("counts, n, k, group", [([1, 0, 5, 17, 0], 72, 256, 64), ([0, 0], 16, 64, 32), ([3] * 40, 40, 512, 128),
-                                                 ([70, 1, 33], 100, 200, 32), ([16, 15, 1, 64], 130, 1184, 96)])
+@pytest.mark.parametrize("counts, n, k, group", [([1, 0, 5, 17, 0], 72, 256, 64), ([0, 0], 16, 64, 32),
+                                                 ([3] * 40, 40, 512, 128), ([70, 1, 33], 100, 200, 32), ([16, 15, 1, 64], 130, 1184, 96)])
 def test_w4_experts(lib, dtype, counts, n, k, group):
     _w4(lib, dtype, counts, n, k, group, True, tokens=20)
     _w4(lib, dtype, counts, n, k, group, False, extra=19, seed=1)
