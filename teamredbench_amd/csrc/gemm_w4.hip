@@ -25,7 +25,7 @@
 // columns and split K in units of 256; weights come one unit ahead, x straight
 // from L2, and the waves add their fp32 sums through LDS, in wave order: 10.8 us
 // at 1 x 14336 x 4096, of which the bytes are 5.9. More rows, or columns
-// enough without (gemm_w4_rows_kernel): the waves split 256 columns and share x
+// enough without (gemm_w4_rows_kernel): the waves split the block's columns and share x
 // through LDS, 256 k at a time, with the sums of x made on the way in: 57 us
 // (4.9 TB/s) for 256 rows over 64 experts, 4096 -> 2048, and 61 us at 64 x
 // 50257 x 4096, where widening and scaling bound it. Few columns: blocks split
@@ -596,7 +596,7 @@ int launch_w4(const W4Call& c, void* workspace, size_t workspace_bytes, const De
     const int blocks_n = (int)((c.N + COLUMNS - 1) / COLUMNS);
     const int64_t tiles = c.offsets ? c.total_rows / ROWS + std::min<int64_t>(c.experts, c.total_rows)
                                     : (c.total_rows + ROWS - 1) / ROWS;
-    const int splits = w4_splits(c, likely_tiles(c, ROWS) * blocks_n, RT == 0 ? 2 * WAVES : 4, workspace_bytes, props);
+    const int splits = w4_splits(c, likely_tiles(c, ROWS) * blocks_n, RT == 0 ? 2 * WAVES : 2, workspace_bytes, props);
     W4Args a{static_cast<const uint16_t*>(c.x), c.rows, c.offsets, static_cast<const uint8_t*>(c.q),
              static_cast<const uint16_t*>(c.scales), static_cast<const uint16_t*>(c.zeros),
              static_cast<uint16_t*>(c.out), splits > 1 ? static_cast<float*>(workspace) : nullptr, c.ldx, c.ldo,
@@ -626,12 +626,20 @@ int launch_group(const W4Call& c, void* workspace, size_t bytes, const DevicePro
     return launch_w4<DT, ZEROS, RT, CT, WAVES, 0>(c, workspace, bytes, props, stream);
 }
 
-// Row tiles of RT x 16 rows on 256-column blocks, or on 64-column ones where those leave CUs without work.
+// Row tiles of RT x 16 rows, 16 columns a wave. 64 rows: blocks of 256 columns
+// (16 waves share a stage of x) while there are enough of them for 2 in 5 CUs
+// (64 x 28672 x 8192: 67 us, 72 on 128 columns). Else 128 columns, which leave more to split K
+// over (64 x 8192 x 8192: 27 us, 39 on 64 columns; 32 rows of 50257 x 4096: 41, 44 on 256), and 64 for a handful.
+// Two column tiles a wave gained nothing: half the waves, twice the registers.
 template <int DT, bool ZEROS, int RT>
 int launch_columns(const W4Call& c, void* workspace, size_t bytes, const DeviceProps& props, hipStream_t stream) {
-    if (likely_tiles(c, 16 * RT) * ((c.N + 255) / 256) * 4 < 3 * props.cu_count)
-        return launch_group<DT, ZEROS, RT, 1, 4>(c, workspace, bytes, props, stream);
-    return launch_group<DT, ZEROS, RT, 2, 8>(c, workspace, bytes, props, stream);
+    const int64_t tiles = likely_tiles(c, 16 * RT);
+    if constexpr (RT == 4) {
+        if (tiles * ((c.N + 255) / 256) * 5 >= 2 * props.cu_count)
+            return launch_group<DT, ZEROS, RT, 1, 16>(c, workspace, bytes, props, stream);
+    }
+    if (tiles * ((c.N + 127) / 128) >= 16) return launch_group<DT, ZEROS, RT, 1, 8>(c, workspace, bytes, props, stream);
+    return launch_group<DT, ZEROS, RT, 1, 4>(c, workspace, bytes, props, stream);
 }
 
 template <int DT, bool ZEROS>
