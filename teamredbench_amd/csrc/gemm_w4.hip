@@ -25,9 +25,9 @@
 // columns and split K in units of 256; weights come one unit ahead, x straight
 // from L2, and the waves add their fp32 sums through LDS, in wave order: 10.8 us
 // at 1 x 14336 x 4096, of which the bytes are 5.9. More rows, or columns
-// enough without (gemm_w4_rows_kernel): the waves split the block's columns and share x
-// through LDS, 256 k at a time, with the sums of x made on the way in: 57 us
-// (4.9 TB/s) for 256 rows over 64 experts, 4096 -> 2048, and 61 us at 64 x
+// enough without (gemm_w4_rows_kernel): the waves split the block's columns and
+// share x through LDS, 256 k at a time, with the sums of x made on the way in:
+// 57 us (4.9 TB/s) for 256 rows over 64 experts, 4096 -> 2048, and 58 us at 64 x
 // 50257 x 4096, where widening and scaling bound it. Few columns: blocks split
 // K too, into fp32 planes that a second kernel adds.
 //
@@ -628,9 +628,10 @@ int launch_group(const W4Call& c, void* workspace, size_t bytes, const DevicePro
 
 // Row tiles of RT x 16 rows, 16 columns a wave. 64 rows: blocks of 256 columns
 // (16 waves share a stage of x) while there are enough of them for 2 in 5 CUs
-// (64 x 28672 x 8192: 67 us, 72 on 128 columns). Else 128 columns, which leave more to split K
-// over (64 x 8192 x 8192: 27 us, 39 on 64 columns; 32 rows of 50257 x 4096: 41, 44 on 256), and 64 for a handful.
-// Two column tiles a wave gained nothing: half the waves, twice the registers.
+// (64 x 28672 x 8192: 67 us, 72 on 128 columns). Else 128 columns, which leave
+// more to split K over (64 x 8192 x 8192: 27 us, 39 on 64 columns; 32 rows of
+// 50257 x 4096: 41, 44 on 256), and 64 for a handful. Two column tiles a wave
+// lost: half the waves, twice the registers (64 x 50257 x 4096: 61 for 58 us).
 template <int DT, bool ZEROS, int RT>
 int launch_columns(const W4Call& c, void* workspace, size_t bytes, const DeviceProps& props, hipStream_t stream) {
     const int64_t tiles = likely_tiles(c, 16 * RT);
