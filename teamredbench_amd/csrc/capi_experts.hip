@@ -8,7 +8,7 @@ using namespace mb;
 namespace {
 
 constexpr int64_t kMostRows = 1ll << 31;      // rows and slots are int32
-constexpr int64_t kMostBlocks = 1ll << 31;    // of a launch
+constexpr int64_t kMostBlocks = 1ll << 30;    // of a launch, in tiles of the smallest size
 
 bool is_half(int dtype) { return dtype == MB_DT_BFLOAT16 || dtype == MB_DT_FLOAT16; }
 
@@ -179,7 +179,7 @@ int mb_gemm_w4(int dtype, const void* x, int64_t ldx, int64_t x_rows, const int3
     if (!leading(&ldx, K, x_rows) || !leading(&ldo, N, total_rows))
         return refuse(MB_ERR_INVALID_ARG, "mb_gemm_w4: a leading dimension (%lld, %lld) is below its rows",
                       (long long)ldx, (long long)ldo);
-    if (total_rows + experts >= kMostBlocks / N)
+    if (total_rows / 16 + experts >= kMostBlocks / ((N + 15) / 16))
         return refuse(MB_ERR_SHAPE, "mb_gemm_w4: too many tiles for one launch");
     const DeviceProps* props = nullptr;
     if (total_rows == 0) return device_for_launch(&props);
@@ -200,7 +200,7 @@ int check_combine(const char* what, int dtype, int64_t y_rows, int64_t tokens, i
         return refuse(MB_ERR_INVALID_ARG,
                       "%s: needs tokens >= 0, 0 <= y_rows < 2^31, 1 <= top_k <= %d, N >= 1 (got %lld, %lld, %d, %lld)",
                       what, MB_ROUTE_MAX_TOP_K, (long long)tokens, (long long)y_rows, top_k, (long long)N);
-    if (tokens >= kMostBlocks / ((N + 2047) / 2048))
+    if (tokens >= kMostRows / ((N + 2047) / 2048))   // runs of 2048 columns are int32
         return refuse(MB_ERR_SHAPE, "%s: too many tokens for one launch (%lld)", what, (long long)tokens);
     return MB_OK;
 }

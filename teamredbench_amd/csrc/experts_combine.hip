@@ -52,7 +52,7 @@ __global__ void __launch_bounds__(kThreads)
 combine_kernel(const uint16_t* __restrict__ y, int64_t ldy, int64_t y_rows, const float* __restrict__ weights,
                const int32_t* __restrict__ slots, int64_t tokens, int top_k, int64_t N, uint16_t* __restrict__ out,
                int64_t ldo, int lanes_log2, unsigned parts) {
-    const unsigned run = (unsigned)(((uint64_t)blockIdx.x * kThreads + threadIdx.x) >> lanes_log2);
+    const unsigned run = (unsigned)(((uint64_t)block_number() * kThreads + threadIdx.x) >> lanes_log2);
     const unsigned token = parts == 1 ? run : run / parts;
     const int64_t t = token;
     const int64_t c = ((int64_t)((run - token * parts) << lanes_log2) + (threadIdx.x & ((1u << lanes_log2) - 1))) * 8;
@@ -85,10 +85,12 @@ combine_kernel(const uint16_t* __restrict__ y, int64_t ldy, int64_t y_rows, cons
 template <int DT>
 __global__ void __launch_bounds__(kThreads)
 combine_grad_kernel(const uint16_t* __restrict__ g, int64_t ldg, const uint16_t* __restrict__ y, int64_t ldy,
-                    int64_t y_rows, const float* __restrict__ weights, const int32_t* __restrict__ slots, int top_k,
-                    int64_t N, uint16_t* __restrict__ grad_y, int64_t ld_grad_y, float* __restrict__ grad_weights) {
+                    int64_t y_rows, const float* __restrict__ weights, const int32_t* __restrict__ slots,
+                    int64_t tokens, int top_k, int64_t N, uint16_t* __restrict__ grad_y, int64_t ld_grad_y,
+                    float* __restrict__ grad_weights) {
     __shared__ float part[kThreads / 64][kBatch];
-    const int64_t t = blockIdx.x;
+    const int64_t t = block_number();
+    if (t >= tokens) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (int j0 = 0; j0 < top_k; j0 += kBatch) {
         int64_t slot[kBatch];
@@ -162,7 +164,7 @@ int combine_launch(int dtype, const void* y, int64_t ldy, int64_t y_rows, const 
     };
     auto kernel = dtype == MB_DT_FLOAT16 ? pick(std::integral_constant<int, MB_DT_FLOAT16>{})
                                          : pick(std::integral_constant<int, MB_DT_BFLOAT16>{});
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kThreads), 0, stream, yp, ldy, y_rows, weights, slots,
+    hipLaunchKernelGGL(kernel, launch_grid(blocks), dim3(kThreads), 0, stream, yp, ldy, y_rows, weights, slots,
                        tokens, top_k, N, op, ldo, lanes_log2, (unsigned)parts);
     MB_HIP_TRY(hipGetLastError());
     return MB_OK;
@@ -175,8 +177,8 @@ int combine_grad_launch(int dtype, const void* grad_out, int64_t ldg, const void
     const auto* yp = static_cast<const uint16_t*>(y);
     auto* gy = static_cast<uint16_t*>(grad_y);
     auto kernel = dtype == MB_DT_FLOAT16 ? combine_grad_kernel<MB_DT_FLOAT16> : combine_grad_kernel<MB_DT_BFLOAT16>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)tokens), dim3(kThreads), 0, stream, gp, ldg, yp, ldy, y_rows, weights,
-                       slots, top_k, N, gy, ld_grad_y, grad_weights);
+    hipLaunchKernelGGL(kernel, launch_grid(tokens), dim3(kThreads), 0, stream, gp, ldg, yp, ldy, y_rows, weights,
+                       slots, tokens, top_k, N, gy, ld_grad_y, grad_weights);
     MB_HIP_TRY(hipGetLastError());
     return MB_OK;
 }

@@ -4,6 +4,8 @@
 
 #include "mb_common.hpp"
 
+#include <algorithm>
+
 namespace mb {
 
 typedef u32x4 u32x4_any __attribute__((aligned(2)));   // 16 bytes on any 16-bit element
@@ -56,6 +58,15 @@ int gemm_w4_launch(const W4Call& c, void* workspace, size_t workspace_bytes, con
 
 
 namespace {
+
+// A grid of at least `blocks` blocks. One dimension of a grid spans below 2^32
+// threads and more are not refused but lost: blocks past kGridX go along y, and
+// those past the last (fewer than kGridX) return at once.
+constexpr int kGridX = 1 << 21;   // 2^31 threads in blocks of 1024
+inline dim3 launch_grid(int64_t blocks) {
+    return dim3((unsigned)std::min<int64_t>(blocks, kGridX), (unsigned)((blocks + kGridX - 1) / kGridX));
+}
+__device__ __forceinline__ unsigned block_number() { return blockIdx.y * (unsigned)kGridX + blockIdx.x; }
 
 // 16-bit element <-> fp32.
 template <int DT>

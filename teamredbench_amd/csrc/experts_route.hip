@@ -294,7 +294,7 @@ route_grad_kernel(const void* __restrict__ logits, int64_t ld, const int32_t* __
                   const float* __restrict__ grad_weights, int64_t tokens, int experts, int top_k, int normalize,
                   void* __restrict__ grad_logits, int64_t ld_grad) {
     const int lane = threadIdx.x & (LANES - 1);
-    const int64_t token = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+    const int64_t token = (int64_t)block_number() * (256 / LANES) + threadIdx.x / LANES;
     if (token >= tokens) return;   // all of a token's lanes: no reduction misses any
     int id = -1;
     float g = 0.f;
@@ -424,7 +424,7 @@ int route_grad_launch(int dtype, const void* logits, int64_t ld, const int32_t* 
         return with_lanes(experts, top_k, [&](auto lanes, auto per) {
             constexpr int DT = decltype(dt)::value, LANES = decltype(lanes)::value, PER = decltype(per)::value;
             constexpr int kTokens = 256 / LANES;   // per block
-            hipLaunchKernelGGL((route_grad_kernel<DT, LANES, PER>), dim3((unsigned)((tokens + kTokens - 1) / kTokens)),
+            hipLaunchKernelGGL((route_grad_kernel<DT, LANES, PER>), launch_grid((tokens + kTokens - 1) / kTokens),
                                dim3(256), 0, stream, logits, ld, expert_ids, grad_weights, tokens, experts, top_k,
                                (int)normalize,
                                grad_logits, ld_grad);

@@ -55,12 +55,13 @@ gemm_grouped_any_kernel(const uint16_t* __restrict__ x, int64_t ldx, int64_t x_r
     __shared__ __attribute__((aligned(1024))) unsigned char lds[2][2][kAnyBuffer];   // buffer, operand
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int wm = wave >> 1, wn = wave & 1;
-    const int tile = (int)blockIdx.x / tiles_n, n0 = ((int)blockIdx.x - tile * tiles_n) * kTile;
+    const int block = (int)block_number(), tile = block / tiles_n, n0 = (block - tile * tiles_n) * kTile;
     ExpertRows ex;
     int m0;
     if constexpr (OP == MB_GROUPED_GRAD_WEIGHTS) {
         const int tiles_m = (K + kTile - 1) / kTile;
         const int e = tile / tiles_m;
+        if (e >= experts) return;
         ex = expert_rows(offsets, e, total);
         m0 = (tile - e * tiles_m) * kTile;
     } else {
@@ -206,7 +207,7 @@ int launch_any(const GroupedCall& c, hipStream_t stream) {
     const int64_t tiles_m = OP == MB_GROUPED_GRAD_WEIGHTS
                                 ? c.experts * ((c.K + kTile - 1) / kTile)
                                 : c.total_rows / kTile + std::min<int64_t>(c.experts, c.total_rows);
-    hipLaunchKernelGGL((gemm_grouped_any_kernel<DT, OP>), dim3((unsigned)(tiles_m * tiles_n)), dim3(256), 0, stream,
+    hipLaunchKernelGGL((gemm_grouped_any_kernel<DT, OP>), launch_grid(tiles_m * tiles_n), dim3(256), 0, stream,
                        static_cast<const uint16_t*>(c.x), c.ldx, c.x_rows, c.rows, static_cast<const uint16_t*>(c.y),
                        c.ldy, static_cast<uint16_t*>(c.out), c.ldo, c.offsets, c.experts, (int)c.total_rows, (int)c.N,
                        (int)c.K, tiles_n);

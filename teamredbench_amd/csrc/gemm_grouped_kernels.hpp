@@ -132,13 +132,15 @@ gemm_grouped_kernel(GroupedArgs args, int tiles_m_max, int tiles_n, int group_m)
 
     // Tile of this block.
     ExpertRows ex;
+    const int block = (int)block_number();
     int tm, tn, split;
     if constexpr (WEIGHTS) {
         // An expert's tiles are dealt to the 8 XCDs (block b runs on XCD b % 8)
         // in runs, so every XCD gets its share of every expert, however uneven
         // the experts' rows; within it, a compact patch.
-        const int tiles = tiles_m_max * tiles_n * args.splits, e = (int)blockIdx.x / tiles;
-        block_coords((int)blockIdx.x - e * tiles, tiles_m_max, tiles_n, args.splits, group_m, &tm, &tn, &split);
+        const int tiles = tiles_m_max * tiles_n * args.splits, e = block / tiles;
+        if (e >= args.experts) return;
+        block_coords(block - e * tiles, tiles_m_max, tiles_n, args.splits, group_m, &tm, &tn, &split);
         ex = expert_rows(args.offsets, e, args.total);
         if (args.splits > 1) {   // this split's share of the expert's rows; none for the last splits of a short one
             const int share = (ex.count + 32 * args.splits - 1) / (32 * args.splits) * 32;
@@ -150,8 +152,8 @@ gemm_grouped_kernel(GroupedArgs args, int tiles_m_max, int tiles_n, int group_m)
         ex.count = __builtin_amdgcn_readfirstlane(ex.count);
     } else {
         const int tiles_m = count_row_tiles(args.offsets, args.experts, args.total, BM);
-        if ((int)blockIdx.x >= tiles_m * tiles_n * args.splits) return;
-        block_coords((int)blockIdx.x, tiles_m, tiles_n, args.splits, group_m, &tm, &tn, &split);
+        if (block >= tiles_m * tiles_n * args.splits) return;
+        block_coords(block, tiles_m, tiles_n, args.splits, group_m, &tm, &tn, &split);
         if (!find_row_tile(args.offsets, args.experts, args.total, tm, BM, &ex, &tm)) return;
     }
     const int M = WEIGHTS ? args.K : ex.count;
@@ -551,7 +553,7 @@ int launch_grouped(const GroupedCall& c, int splits, float* planes, hipStream_t 
         return gemm_grouped_kernel<DT, OP, TILE, TILE, NX, NY, false, G>;
     };
     auto kernel = c.rows ? pick(std::true_type{}) : pick(std::false_type{});
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a, (int)tiles_m, tiles_n, cfg.group_m);
+    hipLaunchKernelGGL(kernel, launch_grid(blocks), dim3(256), 0, stream, a, (int)tiles_m, tiles_n, cfg.group_m);
     MB_HIP_TRY(hipGetLastError());
     if (splits > 1) {
         const int64_t rows = weights ? c.experts * c.K : c.total_rows;

@@ -236,14 +236,15 @@ struct W4Tile {
     }
 };
 __device__ __forceinline__ bool w4_tile(const W4Args& a, int rows_per_tile, int columns, W4Tile* t) {
-    int b = (int)blockIdx.x;
+    int b = (int)block_number();
     t->split = b % a.splits;
     b /= a.splits;
     const int tile = b / a.blocks_n;
     t->n0 = (b - tile * a.blocks_n) * columns;
     ExpertRows ex{0, 0, a.total};
     int in_expert = tile;
-    if (a.offsets != nullptr && !find_row_tile(a.offsets, a.experts, a.total, tile, rows_per_tile, &ex, &in_expert))
+    if (a.offsets == nullptr ? tile > (a.total - 1) / rows_per_tile
+                             : !find_row_tile(a.offsets, a.experts, a.total, tile, rows_per_tile, &ex, &in_expert))
         return false;
     t->expert = ex.expert;
     t->p0 = ex.first + in_expert * rows_per_tile;
@@ -602,7 +603,7 @@ int launch_w4(const W4Call& c, void* workspace, size_t workspace_bytes, const De
              static_cast<uint16_t*>(c.out), splits > 1 ? static_cast<float*>(workspace) : nullptr, c.ldx, c.ldo,
              c.x_rows, c.group, c.experts, (int)c.total_rows, (int)c.N, (int)c.K, blocks_n, splits,
              (int)((c.N + 3) / 4 * 4)};
-    const dim3 grid((unsigned)(tiles * blocks_n * splits));
+    const dim3 grid = launch_grid(tiles * blocks_n * splits);
     if constexpr (RT == 0)
         hipLaunchKernelGGL((gemm_w4_kernel<DT, ZEROS, CT, SPU, WAVES>), grid, dim3(64 * WAVES), 0, stream, a);
     else
