@@ -285,28 +285,22 @@ gemm_w4_kernel(W4Args a) {
     const Cols columns(a.q, tile.expert, tile.n0, a.N, a.K, lane);
     const G groups{a.group, (a.K + a.group - 1) / a.group};
     const Widen<DT> widened;
-    const uint16_t *sp[CT], *zp[CT];
-#pragma unroll
-    for (int t = 0; t < CT; ++t) {
-        const int64_t column = (int64_t)tile.expert * a.N + min(tile.n0 + 16 * t + (lane & 15), a.N - 1);
-        sp[t] = a.scales + column * groups.groups;
-        zp[t] = ZEROS ? a.zeros + column * groups.groups : nullptr;
-    }
+    // Scales: lane group 0 brings those of column tile 0, group 1 of tile 1, groups 2 and 3 the zero points.
+    const int held = lane >> 4;
+    const uint16_t* sp = (ZEROS && held >= 2 ? a.zeros : a.scales) +
+                         ((int64_t)tile.expert * a.N +
+                          min(tile.n0 + 16 * (CT == 1 ? 0 : held & 1) + (lane & 15), a.N - 1)) * groups.groups;
     const int64_t row = x_row(a.rows, a.x_rows, tile.p0 + min(lane & 15, tile.count - 1));
     const uint16_t* xp = a.x + max(row, (int64_t)0) * a.ldx;
     const u32x4 ones = DT == MB_DT_FLOAT16 ? u32x4{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u}
                                            : u32x4{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
     struct Unit {
         u32x4 q[CT][Cols::CHUNKS];
-        typename G::Scales s[CT], z[CT];
+        typename G::Scales s;
     };
     auto load = [&](int k0, Unit& u) {
         columns.load(k0, u.q);
-#pragma unroll
-        for (int t = 0; t < CT; ++t) {
-            u.s[t] = groups.load(sp[t], k0);
-            if constexpr (ZEROS) u.z[t] = groups.load(zp[t], k0);
-        }
+        u.s = groups.load(sp, k0);
     };
     f32x4 acc[CT];
 #pragma unroll
@@ -316,6 +310,12 @@ gemm_w4_kernel(W4Args a) {
         for (int t = 0; t < CT; ++t)
 #pragma unroll
             for (int h = 0; h < Cols::CHUNKS; ++h) w.q[t][h] = transpose_groups(w.q[t][h]);
+        u32x4 held_by[(G::NS + 1) / 2];   // two scales of each lane group, in every lane
+#pragma unroll
+        for (int i = 0; i < (G::NS + 1) / 2; ++i) {
+            const unsigned pair = w.s[2 * i] | (unsigned)w.s[G::NS > 1 ? 2 * i + 1 : 0] << 16;
+            held_by[i] = transpose_groups(u32x4{pair, pair, pair, pair});
+        }
         f32x4 dot[CT], sum;
 #pragma unroll
         for (int s = 0; s < G::STEPS; ++s) {
@@ -331,8 +331,9 @@ gemm_w4_kernel(W4Args a) {
             if (s % G::PER == G::PER - 1) {
 #pragma unroll
                 for (int t = 0; t < CT; ++t) {
-                    const float scale = from_bits<DT>(w.s[t][s / G::PER]);
-                    const float off = -scale * (G::kOffset + (ZEROS ? from_bits<DT>(w.z[t][s / G::PER]) : 8.f));
+                    const int n = s / G::PER;
+                    auto of = [&](int group) { return from_bits<DT>((uint16_t)(held_by[n / 2][group] >> (n % 2 * 16))); };
+                    const float scale = of(t), off = -scale * (G::kOffset + (ZEROS ? of(2 + t) : 8.f));
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         acc[t][r] = fmaf(scale, dot[t][r], acc[t][r]);
