@@ -19,17 +19,24 @@
 // chunk of 128, so a column's reads are 64 contiguous bytes. The MFMA wants k
 // 8 (l / 16) .. + 7 of 32 consecutive ones, so that one MFMA never mixes two
 // groups: a 4 x 4 transpose between the four 16-lane groups, four
-// lane-swap instructions per 16 bytes.
+// lane-swap instructions per 16 bytes. (Few rows: lane l reads column l / 4, and
+// a second transpose follows within each four lanes; see Columns.)
 //
 // Up to 16 rows per expert (gemm_w4_kernel): the waves of a block share 32
 // columns and split K in units of 256; weights come one unit ahead, x straight
-// from L2, and the waves add their fp32 sums through LDS, in wave order: 10.8 us
-// at 1 x 14336 x 4096, of which the bytes are 5.9. More rows, or columns
-// enough without (gemm_w4_rows_kernel): the waves split the block's columns and
-// share x through LDS, 256 k at a time, with the sums of x made on the way in:
-// 57 us (4.9 TB/s) for 256 rows over 64 experts, 4096 -> 2048, and 58 us at 64 x
-// 50257 x 4096, where widening and scaling bound it. Few columns: blocks split
-// K too, into fp32 planes that a second kernel adds.
+// from L2, and the waves add their fp32 sums through LDS, in wave order. L1
+// bounds it: a 16-byte load takes it 16 cycles if each four lanes read 64
+// contiguous bytes and 64 if a quarter wave's 16 lanes read as many lines. So
+// weights come in the first way and a unit's scales by one load (16 x 8192 x
+// 8192, groups of 32 with zero points: 18.8 -> 16.0 us; weights alone 8); x, in
+// rows as the MFMA takes them, is what is left. 10.1 us at 1 x 14336 x 4096, of which
+// the bytes are 5.9.
+//
+// More rows, or columns enough without (gemm_w4_rows_kernel): the waves split
+// the block's columns and share x through LDS, 256 k at a time, with the sums of
+// x made on the way in: 57 us (4.9 TB/s) for 256 rows over 64 experts, 4096 ->
+// 2048, and 58 us at 64 x 50257 x 4096, where widening and scaling bound it. Few
+// columns: blocks split K too, into fp32 planes that a second kernel adds.
 //
 // Rows that are not there multiply some other row's x and are stored as zeros;
 // units that run past K take zeros for x and whatever weights lie there in bounds.
@@ -61,6 +68,17 @@ __device__ __forceinline__ u32x4 transpose_groups(u32x4 v) {
     const auto lo = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
     const auto hi = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
     return u32x4{lo[0], lo[1], hi[0], hi[1]};
+}
+
+// Dword j of lane l <-> dword l % 4 of lane j, among each four lanes.
+__device__ __forceinline__ u32x4 transpose_quads(u32x4 v) {
+    const bool odd = __lane_id() & 1, high = __lane_id() & 2;
+    auto lane1 = [](unsigned x) { return (unsigned)__builtin_amdgcn_mov_dpp((int)x, 0xB1, 0xF, 0xF, true); };   // l ^ 1
+    auto lane2 = [](unsigned x) { return (unsigned)__builtin_amdgcn_mov_dpp((int)x, 0x4E, 0xF, 0xF, true); };   // l ^ 2
+    const u32x4 from1{lane1(v[1]), lane1(v[0]), lane1(v[3]), lane1(v[2])};
+    const u32x4 a{odd ? from1[0] : v[0], odd ? v[1] : from1[1], odd ? from1[2] : v[2], odd ? v[3] : from1[3]};
+    const u32x4 from2{lane2(a[2]), lane2(a[3]), lane2(a[0]), lane2(a[1])};
+    return u32x4{high ? from2[0] : a[0], high ? from2[1] : a[1], high ? a[2] : from2[2], high ? a[3] : from2[3]};
 }
 
 // 8 weights of a dword as floats, in k order 0 4 1 5 2 6 3 7: 128 + q (bf16), q - 8 (fp16). `mask` and
@@ -172,17 +190,21 @@ struct Groups {
 };
 
 // The columns n0 + 16 t + c of an expert; those past N read the last one's weights and are not stored.
-template <int CT>
+// QUADS: lane l reads 16-byte piece l % 4 of column l / 4's 64 bytes, which costs L1 a quarter of the time, and
+// transpose_quads() after transpose_groups() leaves it the k of column_of(l). Where the vector unit bounds, not L1
+// (gemm_w4_rows_kernel: 1 to 4% slower with it), piece l / 16 of column l % 16.
+__device__ __forceinline__ int column_of(int lane) { return 4 * (lane & 3) + ((lane >> 2) & 3); }
+template <int CT, bool QUADS>
 struct Columns {
     static constexpr int CHUNKS = kUnit / 128;   // 16-byte loads per unit and column tile
     const uint8_t* qp[CT];
     int bytes, K, g;
 
     __device__ __forceinline__ Columns(const uint8_t* q, int expert, int n0, int N, int K_, int lane)
-        : bytes((K_ + 1) / 2), K(K_), g(lane >> 4) {
+        : bytes((K_ + 1) / 2), K(K_), g(QUADS ? lane & 3 : lane >> 4) {
 #pragma unroll
         for (int t = 0; t < CT; ++t)
-            qp[t] = q + ((int64_t)expert * N + min(n0 + 16 * t + (lane & 15), N - 1)) * bytes;
+            qp[t] = q + ((int64_t)expert * N + min(n0 + 16 * t + (QUADS ? lane >> 2 : lane & 15), N - 1)) * bytes;
     }
     __device__ __forceinline__ void load(int k0, u32x4 (&q)[CT][CHUNKS]) const {
         const bool whole = k0 + kUnit <= K;   // uniform
@@ -256,10 +278,11 @@ __device__ __forceinline__ bool w4_tile(const W4Args& a, int rows_per_tile, int 
     return true;
 }
 
-// Rows 4 (l / 16) + r of row tile i, column 16 j + l % 16: rounded to out, or as they are to the split's plane.
+// Rows 4 (l / 16) + r of row tile i, column 16 j + c: rounded to out, or as they are to the split's plane.
 template <int DT>
-__device__ __forceinline__ void w4_store(const W4Args& a, const W4Tile& t, int i, int j, const f32x4& v, int lane) {
-    const int n = t.n0 + 16 * j + (lane & 15);
+__device__ __forceinline__ void w4_store(const W4Args& a, const W4Tile& t, int i, int j, int c, const f32x4& v,
+                                         int lane) {
+    const int n = t.n0 + 16 * j + c;
     if (n >= a.N) return;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -277,7 +300,7 @@ template <int DT, bool ZEROS, int CT, int SPU, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES)
 gemm_w4_kernel(W4Args a) {
     typedef Groups<DT, ZEROS, SPU> G;
-    typedef Columns<CT> Cols;
+    typedef Columns<CT, true> Cols;
     __shared__ f32x4 red[WAVES][CT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     W4Tile tile;
@@ -289,7 +312,7 @@ gemm_w4_kernel(W4Args a) {
     const int held = lane >> 4;
     const uint16_t* sp = (ZEROS && held >= 2 ? a.zeros : a.scales) +
                          ((int64_t)tile.expert * a.N +
-                          min(tile.n0 + 16 * (CT == 1 ? 0 : held & 1) + (lane & 15), a.N - 1)) * groups.groups;
+                          min(tile.n0 + 16 * (CT == 1 ? 0 : held & 1) + column_of(lane), a.N - 1)) * groups.groups;
     const int64_t row = x_row(a.rows, a.x_rows, tile.p0 + min(lane & 15, tile.count - 1));
     const uint16_t* xp = a.x + max(row, (int64_t)0) * a.ldx;
     const u32x4 ones = DT == MB_DT_FLOAT16 ? u32x4{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u}
@@ -309,7 +332,7 @@ gemm_w4_kernel(W4Args a) {
 #pragma unroll
         for (int t = 0; t < CT; ++t)
 #pragma unroll
-            for (int h = 0; h < Cols::CHUNKS; ++h) w.q[t][h] = transpose_groups(w.q[t][h]);
+            for (int h = 0; h < Cols::CHUNKS; ++h) w.q[t][h] = transpose_quads(transpose_groups(w.q[t][h]));
         u32x4 held_by[(G::NS + 1) / 2];   // two scales of each lane group, in every lane
 #pragma unroll
         for (int i = 0; i < (G::NS + 1) / 2; ++i) {
@@ -368,7 +391,7 @@ gemm_w4_kernel(W4Args a) {
         f32x4 v = red[0][wave][lane];
 #pragma unroll
         for (int w = 1; w < WAVES; ++w) v += red[w][wave][lane];
-        w4_store<DT>(a, tile, 0, wave, v, lane);
+        w4_store<DT>(a, tile, 0, wave, column_of(lane), v, lane);
     }
 }
 
@@ -381,7 +404,7 @@ template <int DT, bool ZEROS, int RT, int CT, int SPU, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES)
 gemm_w4_rows_kernel(W4Args a) {
     typedef Groups<DT, ZEROS, SPU> G;
-    typedef Columns<CT> Cols;
+    typedef Columns<CT, false> Cols;
     constexpr int ROWS = 16 * RT, COLUMNS = 16 * CT * WAVES;
     constexpr int PITCH = kUnit * 2 + 16;             // bytes per row: 16 rows' 16-byte reads hit all banks once
     constexpr int PIECES = kUnit / 8;                 // 16-byte pieces per row and unit
@@ -554,7 +577,7 @@ gemm_w4_rows_kernel(W4Args a) {
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
-        for (int j = 0; j < CT; ++j) w4_store<DT>(a, tile, i, j, acc[i][j], lane);
+        for (int j = 0; j < CT; ++j) w4_store<DT>(a, tile, i, j, c, acc[i][j], lane);
 }
 
 // out = the sum of the K splits' planes, in split order, for the rows of any expert.
