@@ -674,9 +674,9 @@ int launch_rows(const W4Call& c, void* workspace, size_t bytes, const DeviceProp
     const int64_t rows = (c.total_rows + c.experts - 1) / c.experts;
     if (rows <= 16) {
         // Blocks of 32 columns whose waves split K; with more of them than CUs, fewer waves a block (more blocks at
-        // once: 4 x 28672 x 8192 46.5 against 51.4 us, 16 x 8192 x 8192, one block a CU, 20.8 against 18.8). Once
-        // there are enough columns for a wave to take whole ones, that is faster (64 experts of 2048 x
-        // 4096: 66 against 91 us).
+        // once: 128 rows over 16 experts of 2048 x 4096 20.5 against 23.3 us; 16 x 8192 x 8192, one block a CU,
+        // 18.7 against 16.0). Once there are enough columns for a wave to take whole ones, that is faster (256 rows
+        // over 64 experts of 2048 x 4096: 58 against 68 us).
         const int64_t blocks = likely_tiles(c, 16) * ((c.N + 31) / 32);
         if (blocks < props.cu_count) return launch_group<DT, ZEROS, 0, 1, 8>(c, workspace, bytes, props, stream);
         if (2 * blocks < 3 * props.cu_count)
