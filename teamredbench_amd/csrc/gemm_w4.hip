@@ -5,15 +5,17 @@
 // they go from HBM into registers once, 16 bytes a lane, and straight to the
 // matrix cores (v_mfma_f32_16x16x32: 16 rows x 16 columns x 32 k).
 //
-// Integers to 16-bit floats. A dword holds k .. k + 7 of one column. (w >> 4i)
-// & 0x000F000F leaves nibbles i and i + 4 in its halves; with the exponent of
-// 128 (bf16) or 1024 (fp16) ORed in, each half is the float 128 + q or 1024 + q.
-// That puts k in the order 0 4 1 5 2 6 3 7, which x's operand takes too (four
-// byte permutes). bf16 multiplies 128 + q and an MFMA against ones gives the
-// group's sum of x, so group by group, in fp32,
-//   out += s * (sum x (128 + q)) - s (128 + z) * (sum x);
-// the offset costs 5 of fp32's 24 bits beside a bf16 result's 8. fp16, which
-// keeps 11, subtracts 1032 first (exact), and needs the sum of x only for z - 8.
+// Integers to 16-bit floats. A dword holds k .. k + 7 of one column. Shifted and
+// masked, it leaves nibbles i and i + 4 in its halves; with an exponent ORed in,
+// each half is a float: 16 + q (bf16: the nibble on bits 3 .. 6, the exponent of
+// 16) or 1024 + q (fp16: on the lowest). That puts k in the order 0 4 1 5 2 6 3
+// 7, which x's operand takes too (four byte permutes). bf16 multiplies 16 + q
+// and an MFMA against ones gives the group's sum of x, so group by group, in fp32,
+//   out += s * (sum x (16 + q) - (16 + z) * (sum x));
+// 16 is the least offset under which four bits fit bf16's seven (the nibble on
+// the lowest bits makes it 128: one shift in eight instructions less, but a
+// group's sums some 30 times the result, where these are 5). fp16
+// subtracts 1032 first (exact), and needs the sum of x only for z - 8.
 //
 // Lanes. Lane l reads column l % 16; its 16 bytes are k 32 (l / 16) .. + 31 of a
 // chunk of 128, so a column's reads are 64 contiguous bytes. The MFMA wants k
@@ -81,15 +83,17 @@ __device__ __forceinline__ u32x4 transpose_quads(u32x4 v) {
     return u32x4{high ? from2[0] : a[0], high ? from2[1] : a[1], high ? a[2] : from2[2], high ? a[3] : from2[3]};
 }
 
-// 8 weights of a dword as floats, in k order 0 4 1 5 2 6 3 7: 128 + q (bf16), q - 8 (fp16). `mask` and
-// `exponent` are 0x000F000F and the exponent's bits in registers the compiler cannot see through: it then ANDs
+// 8 weights of a dword as floats, in k order 0 4 1 5 2 6 3 7: 16 + q (bf16), q - 8 (fp16). `mask` and
+// `exponent` are the nibbles' and the exponent's bits in registers the compiler cannot see through: it then ANDs
 // and ORs in one instruction, where literals take two.
 template <int DT>
 __device__ __forceinline__ u32x4 widen(unsigned w, unsigned mask, unsigned exponent) {
     u32x4 v;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const unsigned pair = ((w >> (4 * i)) & mask) | exponent;
+        constexpr int kLowest = DT == MB_DT_FLOAT16 ? 0 : 3;   // bit of the float that the nibble's lowest takes
+        const unsigned nibbles = 4 * i < kLowest ? w << kLowest : w >> (4 * i - kLowest);
+        const unsigned pair = (nibbles & mask) | exponent;
         if constexpr (DT == MB_DT_FLOAT16) {
             typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
             const f16x2 f = __builtin_bit_cast(f16x2, pair) - (f16x2){(_Float16)1032.f, (_Float16)1032.f};
@@ -153,7 +157,7 @@ struct Groups {
     static constexpr int PER = SPU > 0 ? STEPS / SPU : 1;        // steps per scale
     static constexpr int NS = STEPS / PER;                       // scales per unit and column
     static constexpr bool SUMS = DT == MB_DT_BFLOAT16 || ZEROS;  // the group's sum of x is needed
-    static constexpr float kOffset = DT == MB_DT_BFLOAT16 ? 128.f : -8.f;   // the float of q is q + kOffset
+    static constexpr float kOffset = DT == MB_DT_BFLOAT16 ? 16.f : -8.f;   // the float of q is q + kOffset
     typedef uint16_t Scales __attribute__((ext_vector_type(NS)));
 
     int group, groups;
@@ -221,7 +225,8 @@ struct Columns {
 // The mask and exponent of widen().
 template <int DT>
 struct Widen {
-    unsigned mask = 0x000F000Fu, exponent = DT == MB_DT_FLOAT16 ? 0x64006400u : 0x43004300u;
+    unsigned mask = DT == MB_DT_FLOAT16 ? 0x000F000Fu : 0x00780078u;
+    unsigned exponent = DT == MB_DT_FLOAT16 ? 0x64006400u : 0x41804180u;
     __device__ __forceinline__ Widen() {
         asm("" : "+s"(mask));
         asm("" : "+v"(exponent));
@@ -356,12 +361,10 @@ gemm_w4_kernel(W4Args a) {
                 for (int t = 0; t < CT; ++t) {
                     const int n = s / G::PER;
                     auto of = [&](int group) { return from_bits<DT>((uint16_t)(held_by[n / 2][group] >> (n % 2 * 16))); };
-                    const float scale = of(t), off = -scale * (G::kOffset + (ZEROS ? of(2 + t) : 8.f));
+                    const float scale = of(t), off = -(G::kOffset + (ZEROS ? of(2 + t) : 8.f));
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        acc[t][r] = fmaf(scale, dot[t][r], acc[t][r]);
-                        if constexpr (G::SUMS) acc[t][r] = fmaf(off, sum[r], acc[t][r]);
-                    }
+                    for (int r = 0; r < 4; ++r)   // the offset comes off the group's sum before its scale
+                        acc[t][r] = fmaf(scale, G::SUMS ? fmaf(off, sum[r], dot[t][r]) : dot[t][r], acc[t][r]);
                 }
             }
         }
@@ -477,25 +480,23 @@ gemm_w4_rows_kernel(W4Args a) {
 #pragma unroll
         for (int j = 0; j < CT; ++j)
             s[j] = *reinterpret_cast<const typename G::Scales*>(&scales[held][0][16 * (CT * wave + j) + c][at]);
-        if constexpr (G::SUMS) {
+        // The offset's terms of groups 4 m .. + 3.
+        auto offsets = [&](int m) {
+            float off[CT];
 #pragma unroll
-            for (int m = 0; m < QUADS; ++m) {
-                float off[CT];
-#pragma unroll
-                for (int j = 0; j < CT; ++j) {
-                    const int col = 16 * (CT * wave + j) + c, n = min(at + 4 * m + g, 7);
-                    const float z = ZEROS ? from_bits<DT>(scales[held][ZEROS][col][n]) : 8.f;
-                    off[j] = 4 * m + g < G::NS ? -from_bits<DT>(scales[held][0][col][n]) * (G::kOffset + z) : 0.f;
-                }
-#pragma unroll
-                for (int i = 0; i < RT; ++i) {
-                    const float sum = sums[slot][4 * m + g][16 * i + c];
-#pragma unroll
-                    for (int j = 0; j < CT; ++j)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(sum, off[j], acc[i][j], 0, 0, 0);
-                }
+            for (int j = 0; j < CT; ++j) {
+                const int col = 16 * (CT * wave + j) + c, n = min(at + 4 * m + g, 7);
+                const float z = ZEROS ? from_bits<DT>(scales[held][ZEROS][col][n]) : 8.f;
+                off[j] = 4 * m + g < G::NS ? -from_bits<DT>(scales[held][0][col][n]) * (G::kOffset + z) : 0.f;
             }
-        }
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+                const float sum = sums[slot][4 * m + g][16 * i + c];
+#pragma unroll
+                for (int j = 0; j < CT; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(sum, off[j], acc[i][j], 0, 0, 0);
+            }
+        };
 #pragma unroll
         for (int t = 0; t < CT; ++t)
 #pragma unroll
@@ -503,6 +504,8 @@ gemm_w4_rows_kernel(W4Args a) {
         f32x4 dot[RT][CT];
 #pragma unroll
         for (int st = 0; st < G::STEPS; ++st) {
+            // Just before the groups that take them off again: acc stays near the result.
+            if (G::SUMS && st % (4 * G::PER) == 0) offsets(st / (4 * G::PER));
             if (st % G::PER == 0) {
 #pragma unroll
                 for (int i = 0; i < RT; ++i)

@@ -1,0 +1,54 @@
+"""Products with 4-bit weights, bit for bit (-m gpu): inputs whose sums are exact in fp32 (w4_inputs.py),
+so that the result is the formula's in 64 bits, rounded once."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import w4_inputs
+from teamredbench_amd.native import capi
+
+pytestmark = pytest.mark.gpu
+
+HALF = ["bfloat16", "float16"]
+CANARY = 7.0
+
+
+def _run(lib, c: dict, *, workspace: int = 1 << 20, dense: bool | None = None) -> torch.Tensor:
+    """One call on the case's inputs. dense: without offsets (default: where there is one expert)."""
+    dense = len(c["counts"]) == 1 if dense is None else dense
+    offsets = torch.tensor([sum(c["counts"][:e]) for e in range(len(c["counts"]) + 1)], dtype=torch.int32)
+    dev = {name: None if c[name] is None else c[name].cuda() for name in ("x", "rows", "q", "s", "z")}
+    dev["offsets"] = None if dense else offsets.cuda()
+    p = {name: None if v is None else v.data_ptr() for name, v in dev.items()}
+    out = torch.full((c["total"], c["n"]), CANARY, dtype=dev["x"].dtype, device="cuda")
+    scratch = torch.full((max(workspace, 1),), 255, dtype=torch.uint8, device="cuda")
+    print(f"[w4] {c['dtype']} counts {c['counts']} n {c['n']} k {c['k']} group {c['group']} zeros {c['z'] is not None} "
+          f"tokens {None if c['rows'] is None else len(c['x'])} workspace {workspace}", flush=True)
+    lib.gemm_w4(capi.DTYPES[c["dtype"]], p["x"], 0, len(c["x"]), p["rows"], p["q"], p["s"], p["z"], c["group"],
+                out.data_ptr(), 0, p["offsets"], len(c["counts"]), c["total"], c["n"], c["k"],
+                scratch.data_ptr() if workspace else None, workspace, torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    return out.cpu()
+
+
+def _same(got: torch.Tensor, exact: torch.Tensor) -> None:
+    want = exact.to(got.dtype)
+    assert torch.equal(got, want), (f"{int((got != want).sum())} of {got.numel()} differ, the largest by "
+                                    f"{float((got.double() - want.double()).abs().max())}")
+
+
+# ---- sums beside which the result is small --------------------------------------
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("rows, n", [(1, 96), (16, 1000), (3, 8300), (20, 200), (64, 2100)])
+def test_weights_near_their_zero_point(lib, dtype, rows, n, zeros):
+    # Up to 16 rows are scaled group by group: a group's sum of x (16 + q) stays below 256 * 63 * 31 < 2^24 at any
+    # scale. More rows add the offset's terms of 128 k (groups of 32; 256 k of larger ones) to the scaled sums:
+    # 64 * 128 * 63 * 31 and 32 * 256 * 63 * 31 leave 2^24 room for the result.
+    for group, k in ((32, 2048), (128, 2000), (96, 1056), (256, 1300)):
+        powers = 8 if rows <= 16 else 6 if group % 64 else 5
+        c = w4_inputs.near_zero_point(dtype, rows, n, k, group, zeros, powers, seed=rows + group)
+        _same(_run(lib, c), w4_inputs.product(c))
