@@ -268,8 +268,10 @@ int mb_gemm_grouped(int op, int dtype, const void* x, int64_t ldx, int64_t x_row
  * q: experts x N x ceil(K / 2) bytes, two weights a byte, the even k in the
  * low half; a last high half past K is ignored. scales and zeros: experts x
  * N x ceil(K / group) of x's type; zeros NULL stands for 8. `group` is a
- * positive multiple of 32. The integers are multiplied exactly and scaled in
- * fp32, group by group; a row of x with an infinity comes out as NaN. Output rows at and past offsets[experts] are left alone.
+ * positive multiple of 32. Sums are fp32 and rounded once. With BFLOAT16 the weights are
+ * held with an offset of 16: rounding errors go with |scales| (31 + |zeros|) |x|, and
+ * any finite x is taken while |scales| times the sum of |x| over 256 k stays below
+ * 2^136. A row of x with an infinity comes out as NaN. Output rows at and past offsets[experts] are left alone.
  * Meant for few rows per expert (decode); any number is taken. workspace: as
  * in mb_gemm_grouped.
  */

@@ -7,14 +7,16 @@
 //
 // Integers to 16-bit floats. A dword holds k .. k + 7 of one column. Shifted and
 // masked, it leaves nibbles i and i + 4 in its halves; with an exponent ORed in,
-// each half is a float: 16 + q (bf16: the nibble on bits 3 .. 6, the exponent of
-// 16) or 1024 + q (fp16: on the lowest). That puts k in the order 0 4 1 5 2 6 3
-// 7, which x's operand takes too (four byte permutes). bf16 multiplies 16 + q
-// and an MFMA against ones gives the group's sum of x, so group by group, in fp32,
-//   out += s * (sum x (16 + q) - (16 + z) * (sum x));
-// 16 is the least offset under which four bits fit bf16's seven (the nibble on
+// each half is a float: 1 + q / 16 (bf16: the nibble on bits 3 .. 6) or 1024 + q
+// (fp16: on the lowest). That puts k in the order 0 4 1 5 2 6 3 7, which x's
+// operand takes too (four byte permutes). bf16 multiplies 1 + q / 16 and an MFMA
+// against ones gives the group's sum of x, so group by group, in fp32,
+//   out / 16 += s * (sum x (1 + q / 16) - (1 + z / 16) * (sum x)).
+// An offset of 16 q's is the least under which four bits fit bf16's seven (the nibble on
 // the lowest bits makes it 128: one shift in eight instructions less, but a
-// group's sums some 30 times the result, where these are 5). fp16
+// group's sums some 30 times the result, where these are 5). bf16's x may be as
+// large as fp32's range: both operands against it carry 2^-9, so that no sum
+// over a unit of 256 k leaves it, and the stores take 2^13 back. fp16
 // subtracts 1032 first (exact), and needs the sum of x only for z - 8.
 //
 // Lanes. Lane l reads column l % 16; its 16 bytes are k 32 (l / 16) .. + 31 of a
@@ -53,6 +55,21 @@ namespace {
 typedef u32x4 u32x4_byte __attribute__((aligned(1)));   // 16 bytes at any address
 constexpr int kUnit = 256;   // k per step of a wave: whole 128-byte lines of a column
 
+// How weights are held: a float h (q + kOffset), h = kStep times the operand that stands for 1 in the sums of x
+// (kOnes, two of them). Sums are h times what they stand for, and the stores take kBack = 1 / h.
+template <int DT>
+struct Held {
+    static constexpr float kOffset = 16.f, kStep = 1.f / 16, kBack = 8192.f;
+    static constexpr unsigned kOnes = 0x3B003B00u;                                   // 2^-9
+    static constexpr unsigned kMask = 0x00780078u, kExponent = 0x3B003B00u;          // 2^-9 (1 + q / 16)
+};
+template <>
+struct Held<MB_DT_FLOAT16> {
+    static constexpr float kOffset = -8.f, kStep = 1.f, kBack = 1.f;
+    static constexpr unsigned kOnes = 0x3C003C00u;
+    static constexpr unsigned kMask = 0x000F000Fu, kExponent = 0x64006400u;          // 1024 + q, less 1032
+};
+
 template <int DT>
 __device__ __forceinline__ f32x4 mfma16(const u32x4& a, const u32x4& b, f32x4 c) {
     if constexpr (DT == MB_DT_FLOAT16)
@@ -83,9 +100,8 @@ __device__ __forceinline__ u32x4 transpose_quads(u32x4 v) {
     return u32x4{high ? from2[0] : a[0], high ? from2[1] : a[1], high ? a[2] : from2[2], high ? a[3] : from2[3]};
 }
 
-// 8 weights of a dword as floats, in k order 0 4 1 5 2 6 3 7: 16 + q (bf16), q - 8 (fp16). `mask` and
-// `exponent` are the nibbles' and the exponent's bits in registers the compiler cannot see through: it then ANDs
-// and ORs in one instruction, where literals take two.
+// 8 weights of a dword as floats (see Held), in k order 0 4 1 5 2 6 3 7. `mask` and `exponent` are Held's in
+// registers the compiler cannot see through: it then ANDs and ORs in one instruction, where literals take two.
 template <int DT>
 __device__ __forceinline__ u32x4 widen(unsigned w, unsigned mask, unsigned exponent) {
     u32x4 v;
@@ -111,16 +127,17 @@ __device__ __forceinline__ u32x4 reorder(const u32x4& v) {
                  __builtin_amdgcn_perm(v[3], v[1], 0x05040100u), __builtin_amdgcn_perm(v[3], v[1], 0x07060302u)};
 }
 
-// sum + the two 16-bit floats of a dword, in fp32.
+// sum + the two 16-bit floats of a dword, each times the ones of Held, in fp32.
 template <int DT>
 __device__ __forceinline__ float add_pair(unsigned v, float sum) {
     if constexpr (DT == MB_DT_FLOAT16) {
         typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-        return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, v), (f16x2){(_Float16)1.f, (_Float16)1.f}, sum, false);
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, v), __builtin_bit_cast(f16x2, Held<DT>::kOnes), sum,
+                                      false);
     } else {
         typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, v), __builtin_bit_cast(bf16x2, 0x3F803F80u),
-                                               sum, false);
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, v),
+                                               __builtin_bit_cast(bf16x2, Held<DT>::kOnes), sum, false);
     }
 }
 template <int CTRL>
@@ -157,7 +174,6 @@ struct Groups {
     static constexpr int PER = SPU > 0 ? STEPS / SPU : 1;        // steps per scale
     static constexpr int NS = STEPS / PER;                       // scales per unit and column
     static constexpr bool SUMS = DT == MB_DT_BFLOAT16 || ZEROS;  // the group's sum of x is needed
-    static constexpr float kOffset = DT == MB_DT_BFLOAT16 ? 16.f : -8.f;   // the float of q is q + kOffset
     typedef uint16_t Scales __attribute__((ext_vector_type(NS)));
 
     int group, groups;
@@ -225,8 +241,7 @@ struct Columns {
 // The mask and exponent of widen().
 template <int DT>
 struct Widen {
-    unsigned mask = DT == MB_DT_FLOAT16 ? 0x000F000Fu : 0x00780078u;
-    unsigned exponent = DT == MB_DT_FLOAT16 ? 0x64006400u : 0x41804180u;
+    unsigned mask = Held<DT>::kMask, exponent = Held<DT>::kExponent;
     __device__ __forceinline__ Widen() {
         asm("" : "+s"(mask));
         asm("" : "+v"(exponent));
@@ -283,7 +298,7 @@ __device__ __forceinline__ bool w4_tile(const W4Args& a, int rows_per_tile, int 
     return true;
 }
 
-// Rows 4 (l / 16) + r of row tile i, column 16 j + c: rounded to out, or as they are to the split's plane.
+// Rows 4 (l / 16) + r of row tile i, column 16 j + c: rounded to out, or in fp32 to the split's plane.
 template <int DT>
 __device__ __forceinline__ void w4_store(const W4Args& a, const W4Tile& t, int i, int j, int c, const f32x4& v,
                                          int lane) {
@@ -293,11 +308,11 @@ __device__ __forceinline__ void w4_store(const W4Args& a, const W4Tile& t, int i
     for (int r = 0; r < 4; ++r) {
         const int p = 16 * i + 4 * (lane >> 4) + r;
         if (p >= t.count) continue;
-        const bool there = x_row(a.rows, a.x_rows, t.p0 + p) >= 0;
+        const float sum = x_row(a.rows, a.x_rows, t.p0 + p) >= 0 ? v[r] * Held<DT>::kBack : 0.f;
         if (a.planes != nullptr)
-            a.planes[((int64_t)t.split * a.total + t.p0 + p) * a.ldp + n] = there ? v[r] : 0.f;
+            a.planes[((int64_t)t.split * a.total + t.p0 + p) * a.ldp + n] = sum;
         else
-            a.out[(t.p0 + p) * a.ldo + n] = there ? to_bits<DT>(v[r]) : 0;
+            a.out[(t.p0 + p) * a.ldo + n] = to_bits<DT>(sum);
     }
 }
 
@@ -320,8 +335,7 @@ gemm_w4_kernel(W4Args a) {
                           min(tile.n0 + 16 * (CT == 1 ? 0 : held & 1) + column_of(lane), a.N - 1)) * groups.groups;
     const int64_t row = x_row(a.rows, a.x_rows, tile.p0 + min(lane & 15, tile.count - 1));
     const uint16_t* xp = a.x + max(row, (int64_t)0) * a.ldx;
-    const u32x4 ones = DT == MB_DT_FLOAT16 ? u32x4{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u}
-                                           : u32x4{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
+    const u32x4 ones{Held<DT>::kOnes, Held<DT>::kOnes, Held<DT>::kOnes, Held<DT>::kOnes};
     struct Unit {
         u32x4 q[CT][Cols::CHUNKS];
         typename G::Scales s;
@@ -361,7 +375,8 @@ gemm_w4_kernel(W4Args a) {
                 for (int t = 0; t < CT; ++t) {
                     const int n = s / G::PER;
                     auto of = [&](int group) { return from_bits<DT>((uint16_t)(held_by[n / 2][group] >> (n % 2 * 16))); };
-                    const float scale = of(t), off = -(G::kOffset + (ZEROS ? of(2 + t) : 8.f));
+                    const float scale = of(t);
+                    const float off = -Held<DT>::kStep * (Held<DT>::kOffset + (ZEROS ? of(2 + t) : 8.f));
 #pragma unroll
                     for (int r = 0; r < 4; ++r)   // the offset comes off the group's sum before its scale
                         acc[t][r] = fmaf(scale, G::SUMS ? fmaf(off, sum[r], dot[t][r]) : dot[t][r], acc[t][r]);
@@ -487,7 +502,9 @@ gemm_w4_rows_kernel(W4Args a) {
             for (int j = 0; j < CT; ++j) {
                 const int col = 16 * (CT * wave + j) + c, n = min(at + 4 * m + g, 7);
                 const float z = ZEROS ? from_bits<DT>(scales[held][ZEROS][col][n]) : 8.f;
-                off[j] = 4 * m + g < G::NS ? -from_bits<DT>(scales[held][0][col][n]) * (G::kOffset + z) : 0.f;
+                off[j] = 4 * m + g < G::NS ? -from_bits<DT>(scales[held][0][col][n]) *
+                                                 (Held<DT>::kStep * (Held<DT>::kOffset + z))
+                                           : 0.f;
             }
 #pragma unroll
             for (int i = 0; i < RT; ++i) {

@@ -52,3 +52,28 @@ def test_weights_near_their_zero_point(lib, dtype, rows, n, zeros):
         powers = 8 if rows <= 16 else 6 if group % 64 else 5
         c = w4_inputs.near_zero_point(dtype, rows, n, k, group, zeros, powers, seed=rows + group)
         _same(_run(lib, c), w4_inputs.product(c))
+
+
+# ---- the ends of the range ---------------------------------------------------------
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("rows, n", [(1, 96), (16, 1000), (3, 8300), (20, 200), (64, 2100)])
+@pytest.mark.parametrize("x_power, s_power", [(118, -30), (125, -40), (-100, 20), (-80, -20)])
+def test_bf16_range(lib, rows, n, x_power, s_power, zeros):
+    # results are finite and normal in bf16: no step on the way may pass the range of fp32
+    for group, k in ((32, 530), (64, 800), (128, 1000), (512, 700)):
+        c = w4_inputs.case("bfloat16", [rows], n, k, group, zeros, seed=group)
+        exact = w4_inputs.product(c) * 2.0 ** (x_power + s_power)
+        c["x"], c["s"] = c["x"] * 2.0**x_power, c["s"] * 2.0**s_power
+        _same(_run(lib, c), exact)
+
+
+@pytest.mark.parametrize("rows, n", [(1, 96), (16, 1000), (20, 200), (64, 2100)])
+def test_bf16_largest_x(lib, rows, n):
+    # every x is 2^127 or its negative, and all weights but two of a column are zero: sums of x alone pass the range
+    for group, k in ((32, 530), (128, 1000), (512, 700)):
+        c = w4_inputs.near_zero_point("bfloat16", rows, n, k, group, False, 0, seed=group)
+        c["x"] = torch.full_like(c["x"], 2.0**127)
+        c["x"][1::2] *= -1.0
+        _same(_run(lib, c), w4_inputs.product(c))
