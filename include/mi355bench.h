@@ -271,7 +271,9 @@ int mb_gemm_grouped(int op, int dtype, const void* x, int64_t ldx, int64_t x_row
  * positive multiple of 32. Sums are fp32 and rounded once. With BFLOAT16 the weights are
  * held with an offset of 16: rounding errors go with |scales| (31 + |zeros|) |x|, and
  * any finite x is taken while |scales| times the sum of |x| over 256 k stays below
- * 2^136. A row of x with an infinity comes out as NaN. Output rows at and past offsets[experts] are left alone.
+ * 2^136. A row of x with an infinity or a NaN has no finite output, and the others
+ * are not touched by it: with FLOAT16 and zeros NULL it is the formula's, else NaN may
+ * stand where the formula has an infinity. Output rows at and past offsets[experts] are left alone.
  * Meant for few rows per expert (decode); any number is taken. workspace: as
  * in mb_gemm_grouped.
  */

@@ -77,3 +77,33 @@ def test_bf16_largest_x(lib, rows, n):
         c["x"] = torch.full_like(c["x"], 2.0**127)
         c["x"][1::2] *= -1.0
         _same(_run(lib, c), w4_inputs.product(c))
+
+
+# ---- infinities and NaN --------------------------------------------------------------
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("rows, n", [(9, 96), (16, 1000), (20, 200), (64, 2100)])
+def test_rows_that_are_not_finite(lib, dtype, rows, n, zeros):
+    for group, k in ((32, 530), (128, 1001), (96, 700)):
+        c = w4_inputs.case(dtype, [rows], n, k, group, zeros, seed=group)
+        exact = w4_inputs.product(c)
+        for row, value, at in ((0, torch.inf, 3), (2, -torch.inf, k - 1), (5, torch.nan, k // 2)):
+            c["x"][row, at] = value
+        got = _run(lib, c)
+        finite = torch.isfinite(c["x"]).all(1)
+        _same(got[finite], exact[finite])                  # the other rows of the tile are not touched
+        assert not torch.isfinite(got[~finite]).any()
+        assert torch.isnan(got[5]).all()
+        if dtype == "float16" and not zeros:               # the formula's: NaN where a weight is zero
+            want = w4_inputs.product(c)[~finite].half()
+            assert torch.equal(got[~finite].isnan(), want.isnan())
+            assert torch.equal(got[~finite].nan_to_num(0.0), want.nan_to_num(0.0))
+        # a row that is not there is zeros, whatever the rows of x that are there hold
+        c["rows"] = torch.arange(rows, dtype=torch.int32)
+        c["rows"][1], c["rows"][4] = -1, rows
+        got = _run(lib, c)
+        assert (got[1] == 0).all() and (got[4] == 0).all()
+        finite[1] = finite[4] = False
+        _same(got[finite], exact[finite])
