@@ -357,7 +357,10 @@ int mb_kernel_info(int kind, int a, int b, int64_t m, int64_t n, int64_t k,
 #define MB_TUNE_GEMM_HIGHP_STAGED 9    /* 1: fp32 / fp64 on the register-staged kernel */
 #define MB_TUNE_GROUPED_CONFIG 10       /* mb_gemm_grouped, rows on 16 bytes: 0: 256x256, 1: 128x128, 2: 64x64 tiles;
                                            3: the kernel for any rows */
-#define MB_TUNE_COUNT 11
+#define MB_TUNE_W4_CONFIG 11            /* mb_gemm_w4, tiles of rows x columns: 0 and 1: 16 x 16 and 16 x 32, 8 waves
+                                           split K; 2: 16 x 32, 4 waves do; 3: 16 x 256; 4: 32 x 128; 5: 32 x 64;
+                                           6: 64 x 256; 7: 64 x 128; 8: 64 x 64 */
+#define MB_TUNE_COUNT 12
 
 /* Force `knob` to `value`, or restore the library's choice with value -1.
  * Returns MB_ERR_INVALID_ARG for an unknown knob or a value outside the

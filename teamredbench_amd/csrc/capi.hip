@@ -1,6 +1,7 @@
 // C ABI of libmi355bench.so (declared in include/mi355bench.h): argument
 // validation, per-device property cache, dispatch into the stream and GEMM
 // kernel families, event-timed loops and kernel metadata.
+#include "gemm_w4_plan.hpp"
 #include "mb_common.hpp"
 
 #include <atomic>
@@ -19,8 +20,8 @@ DeviceProps g_props[kMaxDevices];
 bool g_props_valid[kMaxDevices] = {false};
 
 // Plan overrides, -1 = the library's own choice. Process-wide, lock-free reads.
-std::atomic<int64_t> g_tuning[MB_TUNE_COUNT] = {-1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1};
-static_assert(MB_TUNE_COUNT == 11, "initialise every knob");
+std::atomic<int64_t> g_tuning[MB_TUNE_COUNT] = {-1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1};
+static_assert(MB_TUNE_COUNT == 12, "initialise every knob");
 
 struct KnobSpec {
     const char* name;
@@ -33,6 +34,7 @@ bool is_threads(int64_t v) { return v >= 64 && v <= 1024 && v % 64 == 0; }
 bool is_config(int64_t v) { return v >= 0 && v <= 4; }
 bool is_splits(int64_t v) { return v >= 1 && v <= 512; }
 bool is_grouped_config(int64_t v) { return v >= 0 && v <= 3; }
+bool is_w4_config(int64_t v) { return v >= 0 && v < kW4ConfigCount; }
 bool is_mfma(int64_t v) { return v == 16 || v == 32; }
 
 const KnobSpec kKnobs[MB_TUNE_COUNT] = {
@@ -40,6 +42,7 @@ const KnobSpec kKnobs[MB_TUNE_COUNT] = {
     {"stream_schedule", is_bool},   {"gemm_force_generic", is_bool}, {"gemm_no_small_m", is_bool},
     {"gemm_tiled_config", is_config}, {"gemm_splits", is_splits},    {"gemm_fp8_mfma", is_mfma},
     {"gemm_highp_staged", is_bool}, {"grouped_config", is_grouped_config},
+    {"w4_config", is_w4_config},
 };
 constexpr int kFirstGemmKnob = MB_TUNE_GEMM_FORCE_GENERIC, kFirstGroupedKnob = MB_TUNE_GROUPED_CONFIG;
 

@@ -45,6 +45,7 @@
 // Rows that are not there multiply some other row's x and are stored as zeros;
 // units that run past K take zeros for x and whatever weights lie there in bounds.
 #include "experts_common.hpp"
+#include "gemm_w4_plan.hpp"
 
 #include <algorithm>
 #include <type_traits>
@@ -618,11 +619,6 @@ gemm_w4_sum_kernel(W4Args a) {
         if (n + e < a.N) a.out[p * a.ldo + n + e] = to_bits<DT>(v[e]);
 }
 
-// Row tiles there are if the rows are spread over the experts.
-int64_t likely_tiles(const W4Call& c, int rows) {
-    return std::max<int64_t>(std::min<int64_t>(c.experts, c.total_rows), (c.total_rows + rows - 1) / rows);
-}
-
 // K splits: as many as give every CU one of the `blocks`, keep `least` units
 // of K in each, and fit the workspace. Two blocks a CU cost more than they gave (16 x 8192 x
 // 8192: 25 against 19 us: the planes and their sum).
@@ -641,7 +637,7 @@ int launch_w4(const W4Call& c, void* workspace, size_t workspace_bytes, const De
     const int blocks_n = (int)((c.N + COLUMNS - 1) / COLUMNS);
     const int64_t tiles = c.offsets ? c.total_rows / ROWS + std::min<int64_t>(c.experts, c.total_rows)
                                     : (c.total_rows + ROWS - 1) / ROWS;
-    const int splits = w4_splits(c, likely_tiles(c, ROWS) * blocks_n, RT == 0 ? 2 * WAVES : 2, workspace_bytes, props);
+    const int splits = w4_splits(c, w4_likely_tiles(c.total_rows, c.experts, ROWS) * blocks_n, RT == 0 ? 2 * WAVES : 2, workspace_bytes, props);
     W4Args a{static_cast<const uint16_t*>(c.x), c.rows, c.offsets, static_cast<const uint8_t*>(c.q),
              static_cast<const uint16_t*>(c.scales), static_cast<const uint16_t*>(c.zeros),
              static_cast<uint16_t*>(c.out), splits > 1 ? static_cast<float*>(workspace) : nullptr, c.ldx, c.ldo,
@@ -671,41 +667,18 @@ int launch_group(const W4Call& c, void* workspace, size_t bytes, const DevicePro
     return launch_w4<DT, ZEROS, RT, CT, WAVES, 0>(c, workspace, bytes, props, stream);
 }
 
-// Row tiles of RT x 16 rows, 16 columns a wave. 64 rows: blocks of 256 columns
-// (16 waves share a stage of x) while there are enough of them for 2 in 5 CUs
-// (64 x 28672 x 8192: 67 us, 72 on 128 columns). Else 128 columns, which leave
-// more to split K over (64 x 8192 x 8192: 27 us, 39 on 64 columns; 32 rows of
-// 50257 x 4096: 41, 44 on 256), and 64 for a handful. Two column tiles a wave
-// lost: half the waves, twice the registers (64 x 50257 x 4096: 61 for 58 us).
-template <int DT, bool ZEROS, int RT>
-int launch_columns(const W4Call& c, void* workspace, size_t bytes, const DeviceProps& props, hipStream_t stream) {
-    const int64_t tiles = likely_tiles(c, 16 * RT);
-    if constexpr (RT == 4) {
-        if (tiles * ((c.N + 255) / 256) * 5 >= 2 * props.cu_count)
-            return launch_group<DT, ZEROS, RT, 1, 16>(c, workspace, bytes, props, stream);
-    }
-    if (tiles * ((c.N + 127) / 128) >= 16) return launch_group<DT, ZEROS, RT, 1, 8>(c, workspace, bytes, props, stream);
-    return launch_group<DT, ZEROS, RT, 1, 4>(c, workspace, bytes, props, stream);
-}
-
 template <int DT, bool ZEROS>
-int launch_rows(const W4Call& c, void* workspace, size_t bytes, const DeviceProps& props, hipStream_t stream) {
-    // Rows of an expert, were they even: tiles of 16, 32 or 64 of them share one pass over the weights.
-    const int64_t rows = (c.total_rows + c.experts - 1) / c.experts;
-    if (rows <= 16) {
-        // Blocks of 32 columns whose waves split K; with more of them than CUs, fewer waves a block (more blocks at
-        // once: 128 rows over 16 experts of 2048 x 4096 20.5 against 23.3 us; 16 x 8192 x 8192, one block a CU,
-        // 18.7 against 16.0). Once there are enough columns for a wave to take whole ones, that is faster (256 rows
-        // over 64 experts of 2048 x 4096: 58 against 68 us).
-        const int64_t blocks = likely_tiles(c, 16) * ((c.N + 31) / 32);
-        if (blocks < props.cu_count) return launch_group<DT, ZEROS, 0, 1, 8>(c, workspace, bytes, props, stream);
-        if (2 * blocks < 3 * props.cu_count)
-            return launch_group<DT, ZEROS, 0, 2, 8>(c, workspace, bytes, props, stream);
-        if (blocks < 8 * props.cu_count) return launch_group<DT, ZEROS, 0, 2, 4>(c, workspace, bytes, props, stream);
-        return launch_group<DT, ZEROS, 1, 2, 8>(c, workspace, bytes, props, stream);
-    }
-    if (rows <= 32) return launch_columns<DT, ZEROS, 2>(c, workspace, bytes, props, stream);
-    return launch_columns<DT, ZEROS, 4>(c, workspace, bytes, props, stream);
+int launch_config(const W4Call& c, void* workspace, size_t bytes, const DeviceProps& props, hipStream_t stream) {
+    const int64_t forced = tuning(MB_TUNE_W4_CONFIG);
+    const int config = forced >= 0 ? (int)forced : w4_config(c.total_rows, c.experts, c.N, props.cu_count);
+    int rc = MB_ERR_INVALID_ARG;   // every config below kW4ConfigCount is taken
+    [&]<int... I>(std::integer_sequence<int, I...>) {
+        ([&] {
+            constexpr W4Config w = kW4Configs[I];
+            if (config == I) rc = launch_group<DT, ZEROS, w.rt, w.ct, w.waves>(c, workspace, bytes, props, stream);
+        }(), ...);
+    }(std::make_integer_sequence<int, kW4ConfigCount>{});
+    return rc;
 }
 
 }  // namespace
@@ -715,10 +688,10 @@ int gemm_w4_launch(const W4Call& c, void* workspace, size_t workspace_bytes, con
     // The workspace only makes small calls faster: one off 16 bytes is left alone.
     if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0) workspace_bytes = 0;
     if (c.dtype == MB_DT_FLOAT16)
-        return c.zeros ? launch_rows<MB_DT_FLOAT16, true>(c, workspace, workspace_bytes, props, stream)
-                       : launch_rows<MB_DT_FLOAT16, false>(c, workspace, workspace_bytes, props, stream);
-    return c.zeros ? launch_rows<MB_DT_BFLOAT16, true>(c, workspace, workspace_bytes, props, stream)
-                   : launch_rows<MB_DT_BFLOAT16, false>(c, workspace, workspace_bytes, props, stream);
+        return c.zeros ? launch_config<MB_DT_FLOAT16, true>(c, workspace, workspace_bytes, props, stream)
+                       : launch_config<MB_DT_FLOAT16, false>(c, workspace, workspace_bytes, props, stream);
+    return c.zeros ? launch_config<MB_DT_BFLOAT16, true>(c, workspace, workspace_bytes, props, stream)
+                   : launch_config<MB_DT_BFLOAT16, false>(c, workspace, workspace_bytes, props, stream);
 }
 
 }  // namespace mb

@@ -87,6 +87,7 @@ TUNING_KNOBS = {
     "gemm_fp8_mfma": 8,
     "gemm_highp_staged": 9,
     "grouped_config": 10,
+    "w4_config": 11,
 }
 
 # Every symbol include/mi355bench.h declares, with (restype, argtypes).

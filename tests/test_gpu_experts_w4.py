@@ -107,3 +107,44 @@ def test_rows_that_are_not_finite(lib, dtype, rows, n, zeros):
         assert (got[1] == 0).all() and (got[4] == 0).all()
         finite[1] = finite[4] = False
         _same(got[finite], exact[finite])
+
+
+# ---- every kernel -----------------------------------------------------------------------
+
+CONFIGS = range(9)
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("config", CONFIGS)
+def test_every_kernel(lib, tune, config, dtype, zeros):
+    # each way to find a unit's scales, K of several units with a ragged end, columns off every tile
+    tune(w4_config=config)
+    for group, k in ((32, 838), (64, 1000), (128, 2049), (96, 1120), (256, 512), (512, 1300)):
+        for counts, tokens in (([70], None), ([16], 5), ([5, 0, 70, 17, 1], 40)):
+            c = w4_inputs.case(dtype, counts, 300, k, group, zeros, tokens=tokens, seed=group + len(counts))
+            _same(_run(lib, c), w4_inputs.product(c))
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("config", CONFIGS)
+def test_k_splits_of_every_kernel(lib, tune, config, dtype):
+    # few columns and a long K: blocks split it over the workspace, as many as fit there
+    tune(w4_config=config)
+    for counts, n in (([16], 40), ([3, 0, 20], 72)):
+        c = w4_inputs.case(dtype, counts, n, 16461, 128, True, seed=n)
+        exact = w4_inputs.product(c)
+        for workspace in (1 << 20, 3 * 4 * n * c["total"], 0):
+            _same(_run(lib, c, workspace=workspace), exact)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("rows, experts, n, k", [(16, 1, 4000, 1500), (16, 1, 8200, 1500), (16, 1, 12300, 1500),
+                                                 (256, 64, 1056, 700), (32, 1, 2100, 1500), (32, 1, 100, 1500),
+                                                 (64, 1, 26500, 1500), (64, 1, 8192, 1500), (64, 1, 100, 1500)])
+def test_kernels_as_picked(lib, dtype, rows, experts, n, k):
+    # just inside each range of the plan
+    counts = [rows // experts] * experts
+    for zeros, group in ((True, 64), (False, 128)):
+        c = w4_inputs.case(dtype, counts, n, k, group, zeros, seed=n)
+        _same(_run(lib, c), w4_inputs.product(c))
