@@ -37,15 +37,20 @@ int check_half(const char* what, int dtype) {
     return refuse(MB_ERR_UNSUPPORTED, "%s takes bfloat16 and float16, not %s", what, dtype_name(dtype));
 }
 
+bool route_counts(int64_t tokens, int experts, int top_k) {
+    return tokens >= 0 && experts >= 1 && experts <= MB_ROUTE_MAX_EXPERTS && top_k >= 1 &&
+           top_k <= MB_ROUTE_MAX_TOP_K && top_k <= experts;
+}
+bool route_slots_fit(int64_t tokens, int top_k) { return tokens <= (kMostRows - 1) / top_k; }
+
 int check_route(const char* what, int dtype, int64_t tokens, int experts, int top_k) {
     if (dtype != MB_DT_FLOAT32 && !is_half(dtype))
         return refuse(MB_ERR_UNSUPPORTED, "%s takes float32, bfloat16 and float16, not %s", what, dtype_name(dtype));
-    if (tokens < 0 || experts < 1 || experts > MB_ROUTE_MAX_EXPERTS || top_k < 1 || top_k > MB_ROUTE_MAX_TOP_K ||
-        top_k > experts)
+    if (!route_counts(tokens, experts, top_k))
         return refuse(MB_ERR_INVALID_ARG,
                       "%s: needs tokens >= 0, 1 <= experts <= %d, 1 <= top_k <= min(experts, %d) (got %lld, %d, %d)",
                       what, MB_ROUTE_MAX_EXPERTS, MB_ROUTE_MAX_TOP_K, (long long)tokens, experts, top_k);
-    if (tokens >= kMostRows / top_k)
+    if (!route_slots_fit(tokens, top_k))
         return refuse(MB_ERR_SHAPE, "%s: tokens * top_k must be below 2^31 (%lld * %d)", what, (long long)tokens,
                       top_k);
     return MB_OK;
@@ -79,7 +84,7 @@ int check_rows(const char* what, const int32_t* rows, const int32_t* offsets, in
 extern "C" {
 
 size_t mb_route_workspace_size(int64_t tokens, int experts, int top_k) {
-    if (tokens < 0 || experts < 1 || experts > MB_ROUTE_MAX_EXPERTS || top_k < 1 || top_k > experts) return 0;
+    if (!route_counts(tokens, experts, top_k) || !route_slots_fit(tokens, top_k)) return 0;
     return route_workspace(tokens, experts);
 }
 

@@ -1,0 +1,38 @@
+"""The last sizes that the expert layer's entry points take and the first that they refuse (no GPU)."""
+from __future__ import annotations
+
+import pytest
+
+from teamredbench_amd.native import capi
+
+P = 1 << 20   # an address that is never read
+
+
+@pytest.fixture(autouse=True)
+def _no_error_left():
+    yield
+    capi.load_library().set_tuning("gemm_splits", None)   # a call that succeeds clears the thread's last error
+
+
+def _route_status(tokens: int, top_k: int) -> int:
+    """The refusal of a call that has every buffer but the workspace."""
+    with pytest.raises(capi.NativeLibraryError) as err:
+        capi.load_library().route(capi.DT_FLOAT32, P, 0, tokens, 128, top_k, True, P, P, P, P, P)
+    return err.value.status
+
+
+@pytest.mark.parametrize("top_k", [1, 2, 3, 7, 64])
+def test_route_takes_up_to_2_31_assignments(top_k):
+    last = ((1 << 31) - 1) // top_k          # tokens * top_k < 2^31
+    assert _route_status(last, top_k) == capi.MB_ERR_WORKSPACE        # sizes taken, the workspace is missing
+    assert _route_status(last + 1, top_k) == capi.MB_ERR_SHAPE
+
+
+def test_route_workspace_size_of_what_route_refuses():
+    lib = capi.load_library()
+    last = ((1 << 31) - 1) // 3
+    assert lib.route_workspace_size(last, 128, 3) > 0
+    assert lib.route_workspace_size(last + 1, 128, 3) == 0
+    assert lib.route_workspace_size(1000, 128, 64) > 0
+    assert lib.route_workspace_size(1000, 128, 65) == 0
+    assert lib.route_workspace_size(1000, 1025, 2) == lib.route_workspace_size(1000, 128, 0) == 0
