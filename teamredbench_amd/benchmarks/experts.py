@@ -14,8 +14,12 @@ metrics are the ones of its GEMM benchmark (src/teamredbench/benchmarks/mfu.py:3
   records, one per operator of a layer: case "experts_<operator>_t<tokens>e<experts>k<top_k>_<k>x<n>"
           with raw_metrics elapsed_s, achieved_ops / peak_tops and gemm_bytes for the products,
           moved_bytes / peak_bandwidth_gbps for the rest; operator "layer" is the whole forward
-          pass, and its metadata holds the in-run parity check of the layer's
-          output against torch's fp32 products on the same inputs.
+          pass. The backward operators are the gradients of the weighted sum, of the hidden rows, of
+          W_up and of the logits (those of W_down and x are the same calls on other matrices).
+          metadata["parity"] holds the in-run check after the timed calls, against torch on the same inputs: of
+          the layer's output (records of the forward operators), of each gradient (its own record), for up to
+          verify_max_tokens tokens, and for W_up's gradient the experts with most and fewest rows.
+          A record whose check fails is failed.
 
 The calls go through libmi355bench.so (mb_route, mb_gemm_grouped, mb_gemm_w4,
 mb_combine and their gradients) on torch's current stream; torch owns the memory.
@@ -31,6 +35,7 @@ from teamredbench_amd.parity import gemm_parity
 from teamredbench_amd.registry import register_benchmark
 from teamredbench_amd.utils import timed_iterations
 
+GRADIENTS = ("combine_grad", "rows_grad", "up_grad", "route_grad")
 DEFAULT_LAYERS = [{"tokens": 4096, "experts": 16, "top_k": 4, "k": 4096, "n": 2048}]
 
 
@@ -38,7 +43,7 @@ class ExpertLayer:
     """The buffers of one layer and its operators' calls, forward and backward."""
 
     def __init__(self, torch: Any, lib: capi.NativeLibrary, dtype: str, layer: dict[str, int], device: Any, seed: int):
-        self.torch, self.lib, self.dtype = torch, lib, capi.DTYPES[dtype]
+        self.torch, self.lib, self.dtype, self.dtype_name = torch, lib, capi.DTYPES[dtype], dtype
         self.tokens, self.experts, self.top_k, self.k, self.n = (
             int(layer[name]) for name in ("tokens", "experts", "top_k", "k", "n"))
         self.group = int(layer.get("group", 0))
@@ -148,6 +153,61 @@ class ExpertLayer:
         return out
 
 
+    # ---- checks: each gradient from the buffers its call read, in 64 bits (fp32 for a whole matrix) -------------
+    def _sample(self, tokens: int) -> tuple[Any, Any, Any]:
+        """The first tokens' assignments: token, choice and sorted row of each."""
+        token, choice = self.torch.nonzero(self.slots[:tokens] >= 0, as_tuple=True)
+        return token, choice, self.slots[token, choice].long()
+
+    def check_forward(self, tokens: int) -> dict[str, tuple[str, Any, Any]]:
+        """Output name -> (dtype, what was computed, what it should be)."""
+        return {"out": (self.dtype_name, self.out[:tokens].float(), self.expected(tokens))}
+
+    def check_combine_grad(self, tokens: int) -> dict[str, tuple[str, Any, Any]]:
+        token, choice, row = self._sample(tokens)
+        grad = self.grad_out[token].double()
+        return {"grad_y": (self.dtype_name, self.grad_y[row], self.weights[token, choice, None].double() * grad),
+                "grad_weights": ("float32", self.grad_weights[token, choice], (grad * self.y[row].double()).sum(1))}
+
+    def check_rows_grad(self, tokens: int) -> dict[str, tuple[str, Any, Any]]:
+        token, choice, row = self._sample(tokens)
+        expert = self.ids[token, choice]
+        wanted = self.torch.empty(row.numel(), self.n, device=row.device)
+        for e in expert.unique().tolist():
+            at = expert == e
+            wanted[at] = self.grad_y[row[at]].float() @ self.down[e].float().t().contiguous()
+        return {"grad_hidden": (self.dtype_name, self.grad_hidden[row], wanted)}
+
+    def check_up_grad(self, tokens: int) -> dict[str, tuple[str, Any, Any]]:
+        counts = self.offsets.diff()
+        checked = {}
+        for name, e in (("most", int(counts.argmax())), ("fewest", int(counts.argmin()))):
+            lo, hi = int(self.offsets[e]), int(self.offsets[e + 1])
+            x = self.x[self.rows[lo:hi].long()].float()
+            checked[f"grad_up of the expert with {name} rows"] = (
+                self.dtype_name, self.grad_up[e], x.t().contiguous() @ self.grad_hidden[lo:hi].float())
+        return checked
+
+    def check_route_grad(self, tokens: int) -> dict[str, tuple[str, Any, Any]]:
+        ids = self.ids[:tokens].long()
+        chosen = self.torch.softmax(self.logits[:tokens].double().gather(1, ids), dim=1)
+        g = self.grad_weights[:tokens].double()
+        part = chosen * (g - (chosen * g).sum(1, keepdim=True))
+        wanted = self.torch.zeros(tokens, self.experts, dtype=part.dtype, device=part.device).scatter_(1, ids, part)
+        return {"grad_logits": ("float32", self.grad_logits[:tokens], wanted)}
+
+
+def parity_of(torch: Any, checked: dict[str, tuple[str, Any, Any]]) -> dict[str, Any]:
+    """The parity of the output that is nearest to its bound, or furthest over it, and every output's distance."""
+    each = {name: gemm_parity(torch, dtype, got, want) if torch.count_nonzero(want) else
+            {"rel_frobenius": 0.0, "bound": 0.0, "passed": not torch.count_nonzero(got)}
+            for name, (dtype, got, want) in checked.items()}
+    worst = max(each.values(), key=lambda p: (not p["passed"], p["rel_frobenius"] / p["bound"] if p["bound"] else 0.0))
+    return {"vs": "torch", **{key: worst[key] for key in ("rel_frobenius", "bound")},
+            "passed": all(p["passed"] for p in each.values()),
+            "outputs": {name: p["rel_frobenius"] for name, p in each.items()}}
+
+
 @register_benchmark("experts")
 class ExpertsBenchmark(Benchmark):
     default_metrics = ["latency_us", "achieved_tops", "mfu_pct", "hbm_bandwidth_gbps"]
@@ -186,16 +246,23 @@ class ExpertsBenchmark(Benchmark):
         if backward:
             layer.prepare_backward()
         suffix = f"t{layer.tokens}e{layer.experts}k{layer.top_k}_{layer.k}x{layer.n}"
+        operators = self._operators(layer, spec.bytes_per_element, backward)
+        times = {name: timed_iterations(call, torch_module=torch, warmup=warmup, iterations=iterations)
+                 for name, call, _ in operators}
+        rows = min(layer.tokens, int(self.params.get("verify_max_tokens", 64)))
+        parity: dict[str, dict[str, Any]] = {}
+        if bool(self.params.get("verify", True)):
+            for name in ("forward", *(GRADIENTS if backward else ())):
+                checked = getattr(layer, f"check_{name}")(rows)
+                parity[name] = {**parity_of(torch, checked), "rows_checked": rows}
         records = []
-        for name, call, work in self._operators(layer, spec.bytes_per_element, backward):
-            elapsed = timed_iterations(call, torch_module=torch, warmup=warmup, iterations=iterations)
+        for name, _, work in operators:
             metadata = {"backend": "native", "kernel": "experts_gfx950", "operator": name, "timing": "wall_clock",
                         **{key: int(value) for key, value in shape.items()}}
-            if name == "layer" and bool(self.params.get("verify", True)):
-                rows = min(layer.tokens, int(self.params.get("verify_max_tokens", 64)))
-                metadata["parity"] = gemm_parity(torch, spec.name, layer.out[:rows].float(), layer.expected(rows))
-                metadata["parity"]["rows_checked"] = rows
-            raw = {"elapsed_s": elapsed, **work}
+            check = name if name in GRADIENTS else "forward"
+            if check in parity:
+                metadata["parity"] = parity[check]
+            raw = {"elapsed_s": times[name], **work}
             if "achieved_ops" in work:
                 raw["peak_tops"] = peak_tops
             if "moved_bytes" in work:
