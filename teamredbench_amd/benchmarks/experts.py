@@ -10,30 +10,37 @@ metrics are the ones of its GEMM benchmark (src/teamredbench/benchmarks/mfu.py:3
           {tokens, experts, top_k, k, n, group} (k: width of a token, n: width
           of the hidden row; group: with it W_down is 4-bit, one scale per group of n), warmup (10),
           iterations (50), seed (0), backward (default true where no layer is 4-bit), verify (default true),
-          verify_max_tokens (default 64)
+          verify_max_tokens (default 64), operand_sets ("auto", or a count: the timed calls cycle through that
+          many copies of the layer's buffers; "auto" takes enough that the smallest product bound by memory, by
+          its arithmetic intensity, spans three times the 256 MB Infinity Cache, at most 1024 and half of the
+          free memory)
   records, one per operator of a layer: case "experts_<operator>_t<tokens>e<experts>k<top_k>_<k>x<n>"
           with raw_metrics elapsed_s, achieved_ops / peak_tops and gemm_bytes for the products,
-          moved_bytes / peak_bandwidth_gbps for the rest; operator "layer" is the whole forward
-          pass. The backward operators are the gradients of the weighted sum, of the hidden rows, of
-          W_up and of the logits (those of W_down and x are the same calls on other matrices).
-          metadata["parity"] holds the in-run check after the timed calls, against torch on the same inputs: of
-          the layer's output (records of the forward operators), of each gradient (its own record), for up to
-          verify_max_tokens tokens, and for W_up's gradient the experts with most and fewest rows.
-          A record whose check fails is failed.
+          moved_bytes / peak_bandwidth_gbps for the rest; operator "layer" is the whole forward pass. The
+          backward operators are the gradients of the weighted sum, of the hidden rows, of W_up and of the
+          logits (those of W_down and x are the same calls on other matrices).
+          metadata: operand_sets, operand_footprint_bytes of the operator over all sets, cache_resident (they
+          fit the Infinity Cache: the rate is the cache's, not HBM's) and parity, the in-run check after the timed
+          calls, against torch on the same inputs: of the layer's output (records of the forward operators) or
+          of the gradient itself, for up to verify_max_tokens tokens, and for W_up's gradient the experts
+          with most and fewest rows. A record whose check fails is failed.
 
 The calls go through libmi355bench.so (mb_route, mb_gemm_grouped, mb_gemm_w4,
 mb_combine and their gradients) on torch's current stream; torch owns the memory.
 """
 from __future__ import annotations
 
-from typing import Any, Callable
+import copy
+import itertools
+from typing import Any
 
 from teamredbench_amd.benchmarks.base import Benchmark, BenchmarkRecord
+from teamredbench_amd.benchmarks.mfu import INFINITY_CACHE_BYTES, MAX_OPERAND_SETS, OPERAND_FOOTPRINT_TARGET
 from teamredbench_amd.device import rocm_device_available
 from teamredbench_amd.native import capi
 from teamredbench_amd.parity import gemm_parity
 from teamredbench_amd.registry import register_benchmark
-from teamredbench_amd.utils import timed_iterations
+from teamredbench_amd.utils import tensor_nbytes, timed_iterations
 
 GRADIENTS = ("combine_grad", "rows_grad", "up_grad", "route_grad")
 DEFAULT_LAYERS = [{"tokens": 4096, "experts": 16, "top_k": 4, "k": 4096, "n": 2048}]
@@ -81,6 +88,22 @@ class ExpertLayer:
         self.grad_y, self.grad_weights = torch.empty_like(self.y), torch.empty_like(self.weights)
         self.grad_hidden, self.grad_up = torch.empty_like(self.hidden), torch.empty_like(self.up)
         self.grad_logits = torch.empty_like(self.logits)
+
+    def buffers(self) -> dict[str, Any]:
+        """Every tensor of the layer but the workspace, by attribute."""
+        return {name: value for name, value in vars(self).items()
+                if isinstance(value, self.torch.Tensor) and name != "workspace"}
+
+    def clone(self) -> "ExpertLayer":
+        """The same layer on buffers of its own. The workspace, which no call leaves anything in, is shared."""
+        other = copy.copy(self)
+        for name, value in self.buffers().items():
+            setattr(other, name, value.clone())
+        return other
+
+    def backward(self) -> None:
+        for name in GRADIENTS:
+            getattr(self, name)()
 
     def _workspace(self) -> tuple[int, int, int]:
         return self.workspace.data_ptr(), self.workspace.numel(), self.stream
@@ -197,6 +220,10 @@ class ExpertLayer:
         return {"grad_logits": ("float32", self.grad_logits[:tokens], wanted)}
 
 
+def _bytes(work: dict[str, int]) -> int:
+    return work.get("gemm_bytes", 0) or work.get("moved_bytes", 0)
+
+
 def parity_of(torch: Any, checked: dict[str, tuple[str, Any, Any]]) -> dict[str, Any]:
     """The parity of the output that is nearest to its bound, or furthest over it, and every output's distance."""
     each = {name: gemm_parity(torch, dtype, got, want) if torch.count_nonzero(want) else
@@ -210,32 +237,51 @@ def parity_of(torch: Any, checked: dict[str, tuple[str, Any, Any]]) -> dict[str,
 
 @register_benchmark("experts")
 class ExpertsBenchmark(Benchmark):
-    default_metrics = ["latency_us", "achieved_tops", "mfu_pct", "hbm_bandwidth_gbps"]
+    default_metrics = ["latency_us", "achieved_tops", "mfu_pct", "hbm_bandwidth_gbps", "gemm_bandwidth_gbps"]
 
-    def _operators(self, layer: ExpertLayer, size: int, backward: bool) -> list[tuple[str, Callable[[], None], dict]]:
-        """(name, call, what it computes and moves) of each operator, inputs read once and outputs written once."""
+    def _operators(self, layer: ExpertLayer, size: int, backward: bool) -> list[tuple[str, str, dict]]:
+        """(name, the layer's method, what it computes and moves) of each operator, inputs read once and outputs
+        written once."""
         tokens, experts, total, k, n = layer.tokens, layer.experts, layer.total, layer.k, layer.n
         hit = min(experts, total)
         product = {"achieved_ops": 2 * total * k * n}
         matrix = hit * k * n * size
-        down = hit * k * (n // 2 + -(-n // layer.group) * size) if layer.group else matrix
+        down = hit * k * ((n + 1) // 2 + -(-n // layer.group) * size) if layer.group else matrix
         assignments = total * 16 + (experts + 1) * 4
         operators = [
-            ("route", layer.route, {"moved_bytes": tokens * experts * 4 + assignments}),
-            ("up", layer.up_product, {**product, "gemm_bytes": matrix + (tokens * k + total * n) * size}),
-            ("down", layer.down_product, {**product, "gemm_bytes": down + total * (n + k) * size}),
-            ("combine", layer.combine, {"moved_bytes": (total + tokens) * k * size + total * 8}),
-            ("layer", layer.forward, {"achieved_ops": 4 * total * k * n}),
+            ("route", "route", {"moved_bytes": tokens * experts * 4 + assignments}),
+            ("up", "up_product", {**product, "gemm_bytes": matrix + (tokens * k + total * n) * size}),
+            ("down", "down_product", {**product, "gemm_bytes": down + total * (n + k) * size}),
+            ("combine", "combine", {"moved_bytes": (total + tokens) * k * size + total * 8}),
         ]
+        moved = sum(_bytes(work) for _, _, work in operators)
+        operators.append(("layer", "forward", {"achieved_ops": 4 * total * k * n, "gemm_bytes": moved}))
         if backward:
             operators += [
-                ("combine_grad", layer.combine_grad, {"moved_bytes": (2 * total + tokens) * k * size + total * 12}),
-                ("rows_grad", layer.rows_grad, {**product, "gemm_bytes": matrix + total * (n + k) * size}),
-                ("up_grad", layer.up_grad,
+                ("combine_grad", "combine_grad", {"moved_bytes": (2 * total + tokens) * k * size + total * 12}),
+                ("rows_grad", "rows_grad", {**product, "gemm_bytes": matrix + total * (n + k) * size}),
+                ("up_grad", "up_grad",
                  {**product, "gemm_bytes": experts * k * n * size + (tokens * k + total * n) * size}),
-                ("route_grad", layer.route_grad, {"moved_bytes": 2 * tokens * experts * 4 + total * 8}),
+                ("route_grad", "route_grad", {"moved_bytes": 2 * tokens * experts * 4 + total * 8}),
             ]
         return operators
+
+    def _operand_sets(self, operators: list[tuple[str, str, dict]], peak_tops: float | None, set_bytes: int,
+                      free_bytes: int) -> int:
+        """Copies of the layer to cycle through (see the module's operand_sets)."""
+        requested = self.params.get("operand_sets", "auto")
+        if requested != "auto":
+            return max(1, int(requested))
+        hbm = self.context.hardware_profile.peak_hbm_bandwidth_gbps
+        if not peak_tops or not hbm:
+            return 1
+        ridge = peak_tops * 1e12 / (hbm * 1e9)
+        bound = [work["gemm_bytes"] for name, _, work in operators
+                 if name != "layer" and "gemm_bytes" in work and work["achieved_ops"] < ridge * work["gemm_bytes"]]
+        if not bound:
+            return 1
+        sets = -(-OPERAND_FOOTPRINT_TARGET // min(bound))
+        return max(1, min(sets, MAX_OPERAND_SETS, free_bytes // 2 // set_bytes))
 
     def _cases(self, lib, torch, spec, shape: dict[str, int], peak_tops) -> list[BenchmarkRecord]:
         peak_hbm = self.context.hardware_profile.peak_hbm_bandwidth_gbps
@@ -245,10 +291,18 @@ class ExpertsBenchmark(Benchmark):
         layer.forward()
         if backward:
             layer.prepare_backward()
+            layer.backward()
         suffix = f"t{layer.tokens}e{layer.experts}k{layer.top_k}_{layer.k}x{layer.n}"
         operators = self._operators(layer, spec.bytes_per_element, backward)
-        times = {name: timed_iterations(call, torch_module=torch, warmup=warmup, iterations=iterations)
-                 for name, call, _ in operators}
+        set_bytes = sum(tensor_nbytes(value) for value in layer.buffers().values())
+        sets = self._operand_sets(operators, peak_tops, set_bytes, torch.cuda.mem_get_info(self.device)[0])
+        layers = [layer, *(layer.clone() for _ in range(sets - 1))]
+        times = {}
+        for name, method, _ in operators:
+            calls = itertools.cycle([getattr(one, method) for one in layers])
+            times[name] = timed_iterations(lambda: next(calls)(), torch_module=torch, warmup=warmup,
+                                           iterations=iterations)
+        del layers, calls
         rows = min(layer.tokens, int(self.params.get("verify_max_tokens", 64)))
         parity: dict[str, dict[str, Any]] = {}
         if bool(self.params.get("verify", True)):
@@ -258,6 +312,8 @@ class ExpertsBenchmark(Benchmark):
         records = []
         for name, _, work in operators:
             metadata = {"backend": "native", "kernel": "experts_gfx950", "operator": name, "timing": "wall_clock",
+                        "operand_sets": sets, "operand_footprint_bytes": sets * _bytes(work),
+                        "cache_resident": sets * _bytes(work) <= INFINITY_CACHE_BYTES,
                         **{key: int(value) for key, value in shape.items()}}
             check = name if name in GRADIENTS else "forward"
             if check in parity:
