@@ -12,7 +12,7 @@
 namespace mb {
 
 namespace {
-thread_local std::string g_last_error;
+thread_local char g_last_error[1024];   // in place: a refusal allocates nothing, so it throws nothing
 
 constexpr int kMaxDevices = 64;
 std::mutex g_props_mutex;
@@ -54,15 +54,15 @@ int64_t tuning(int knob) {
 }
 
 void set_error(const char* fmt, ...) {
-    char buf[1024];
+    char buf[sizeof(g_last_error)];   // an argument may be the last error's own text
     va_list ap;
     va_start(ap, fmt);
     vsnprintf(buf, sizeof(buf), fmt, ap);
     va_end(ap);
-    g_last_error = buf;
+    std::strcpy(g_last_error, buf);
 }
 
-void clear_error() { g_last_error.clear(); }
+void clear_error() { g_last_error[0] = 0; }
 
 int hip_fail(hipError_t err, const char* what) {
     set_error("%s failed: %s (hipError_t %d)", what, hipGetErrorString(err), (int)err);
@@ -284,7 +284,7 @@ int mb_set_tuning(int knob, int64_t value) {
 int64_t mb_get_tuning(int knob) { return tuning(knob); }
 
 
-const char* mb_last_error(void) { return g_last_error.c_str(); }
+const char* mb_last_error(void) { return g_last_error; }
 
 namespace {
 

@@ -56,7 +56,6 @@ struct W4Call {
 int gemm_w4_launch(const W4Call& c, void* workspace, size_t workspace_bytes, const DeviceProps& props,
                    hipStream_t stream);
 
-
 namespace {
 
 // A grid of at least `blocks` blocks. One dimension of a grid spans below 2^32

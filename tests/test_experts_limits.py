@@ -36,3 +36,26 @@ def test_route_workspace_size_of_what_route_refuses():
     assert lib.route_workspace_size(1000, 128, 64) > 0
     assert lib.route_workspace_size(1000, 128, 65) == 0
     assert lib.route_workspace_size(1000, 1025, 2) == lib.route_workspace_size(1000, 128, 0) == 0
+
+
+def test_error_text_is_held_in_place():
+    # per thread, at one address, replaced by each refusal and empty again after a call that is taken
+    import ctypes
+    import threading
+
+    handle = capi.load_library().handle
+    text = ctypes.CFUNCTYPE(ctypes.c_void_p)(("mb_last_error", handle))
+    refusals = [lambda: _route_status(-1, 1), lambda: _route_status(1 << 31, 7), lambda: _route_status(1000, 1)]
+    at = set()
+    for refuse in refusals:
+        refuse()
+        at.add(text())
+        assert handle.mb_last_error().startswith(b"mb_route: ")
+    assert len(at) == 1
+    other = []
+    thread = threading.Thread(target=lambda: other.append(handle.mb_last_error()))
+    thread.start()
+    thread.join()
+    assert other == [b""]
+    capi.load_library().set_tuning("gemm_splits", None)
+    assert handle.mb_last_error() == b"" and text() in at
