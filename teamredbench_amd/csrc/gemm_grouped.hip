@@ -12,7 +12,7 @@
 // tiles, 4 waves of 64 x 64 on v_mfma_f32_32x32x16, a stage of 32 c, through
 // registers into one of two LDS buffers while the other is computed. Global
 // loads are 16 bytes at any element (the hardware takes them; element by
-// element it took twice as long, 645 against 317 us for 12004 rows over 60
+// element it took twice as long, 645 against 324 us for 12004 rows over 60
 // experts, 2057 -> 1411). An operand whose rows run along c is kept as [m or
 // n][32 c] in rows of 80 bytes, one whose rows run across it as [32 c][m or n],
 // swizzled, and read with the transposing LDS reads. Rows of c past the

@@ -24,8 +24,8 @@
 //
 // Many rows per expert are bound by the MFMAs at the clock the power limit
 // leaves, as the dense kernel is (16384 rows over 8 experts, 4096 -> 14336:
-// 1574 us, 1.22 PFLOP/s); few rows by the matrices' bytes, which the deep rings
-// keep in flight (128 rows over 32 experts, 4096 -> 2048: 88 us, 6.1 TB/s).
+// 1574 to 1654 us on two GPUs, 1.16 to 1.22 PFLOP/s); few rows by the matrices' bytes, which the deep
+// rings keep in flight (128 rows over 32 experts, 4096 -> 2048: 88 to 92 us, 5.9 to 6.1 TB/s).
 #pragma once
 
 #include "experts_common.hpp"

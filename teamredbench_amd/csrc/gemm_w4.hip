@@ -33,14 +33,14 @@
 // contiguous bytes and 64 if a quarter wave's 16 lanes read as many lines. So
 // weights come in the first way and a unit's scales by one load (16 x 8192 x
 // 8192, groups of 32 with zero points: 18.8 -> 16.0 us; weights alone 8); x, in
-// rows as the MFMA takes them, is what is left. 10.1 us at 1 x 14336 x 4096, of which
+// rows as the MFMA takes them, is what is left. 10.2 us at 1 x 14336 x 4096, of which
 // the bytes are 5.9.
 //
 // More rows, or columns enough without (gemm_w4_rows_kernel): the waves split
 // the block's columns and share x through LDS, 256 k at a time, with the sums of
-// x made on the way in: 57 us (4.9 TB/s) for 256 rows over 64 experts, 4096 ->
-// 2048, and 58 us at 64 x 50257 x 4096, where widening and scaling bound it. Few
-// columns: blocks split K too, into fp32 planes that a second kernel adds.
+// x made on the way in: 59 us (4.7 TB/s) for 256 rows over 64 experts, 4096 ->
+// 2048, and 58.7 us at 64 x 50257 x 4096, where widening and scaling take 34 on
+// the 197 CUs that have a block. Few columns: blocks split K too, into fp32 planes that a second kernel adds.
 //
 // Rows that are not there multiply some other row's x and are stored as zeros;
 // units that run past K take zeros for x and whatever weights lie there in bounds.
