@@ -31,7 +31,7 @@
 extern "C" {
 #endif
 
-#define MB_ABI_VERSION 4
+#define MB_ABI_VERSION 5
 
 /* Status codes (negative = rejected by the library before any launch). */
 #define MB_OK 0
@@ -302,6 +302,65 @@ int mb_combine(int dtype, const void* y, int64_t ldy, int64_t y_rows, const floa
 int mb_combine_grad(int dtype, const void* grad_out, int64_t ldg, const void* y, int64_t ldy, int64_t y_rows,
                     const float* weights, const int32_t* slots, int64_t tokens, int top_k, int64_t N, void* grad_y,
                     int64_t ld_grad_y, float* grad_weights, void* stream);
+
+/*
+ * Microscaled 4-bit floating point (MX4): quantisation, and products on the
+ * matrix cores, which take it at twice fp8's rate. No counterpart in the
+ * reference, whose narrowest type is fp8 (src/teamredbench/dtypes.py:23-24).
+ *
+ * MX4 holds a row in blocks of 32 elements: e2m1 floats (codes 0 .. 7: 0, 0.5, 1,
+ * 1.5, 2, 3, 4, 6; 8 added: negative) times the block's scale, 2^(byte - 127), 255
+ * for NaN (e8m0). A matrix of R rows and C columns is
+ *   q       R rows of MB_MX4_ROW_BYTES(C) bytes, two elements a byte, the even column in the low half
+ *   scales  R rows of MB_MX4_ROW_SCALES(C) bytes, one per 32 columns
+ * packed, q on 16 bytes and scales on 4. A row's last unit of 128 columns is whole: what lies
+ * past C is zeros, which mb_mx4_quantize writes and the products add up as they are.
+ */
+#define MB_MX4_ROW_BYTES(columns) (((columns) + 127) / 128 * 64)
+#define MB_MX4_ROW_SCALES(columns) (((columns) + 127) / 128 * 4)
+
+/*
+ * mb_mx4_quantize -- x (rows x columns, FLOAT32 / BFLOAT16 / FLOAT16) as MX4
+ * along its rows (q, scales) and along its columns, i.e. the transposed matrix of
+ * `columns` rows (qt, scales_t), in one pass over x. Either pair may be NULL.
+ *
+ * A block's scale goes by its largest magnitude m 2^e, 1 <= m < 2:
+ *   MB_MX4_SCALE_FLOOR  2^(e - 2), the rule of the OCP MX specification 1.0: what lies above 6 scales becomes 6
+ *   MB_MX4_SCALE_FIT    2^(e - 1) where m > 1.5, else 2^(e - 2): nothing saturates
+ * and 2^-127 where that is less. Elements are x / scale rounded to the nearest
+ * value, ties to the even code. A block that holds an infinity or a NaN becomes
+ * NaN as a whole (scale 255, codes 0). A linear layer's gradients are products of such forms:
+ * with y = x w^T, dx = dy w contracts over y's columns (dy along its rows, w along its columns), dw = dy^T x over
+ * its rows (dy and x along their columns). The gradient of the quantisation itself is passed straight through.
+ */
+#define MB_MX4_SCALE_FLOOR 0
+#define MB_MX4_SCALE_FIT 1
+int mb_mx4_quantize(int dtype, const void* x, int64_t ldx, int64_t rows, int64_t columns, int scale_rule, void* q,
+                    void* scales, void* qt, void* scales_t, void* stream);
+
+/*
+ * mb_mx4_dequantize -- the values of an MX4 matrix, out (rows x columns,
+ * FLOAT32 / BFLOAT16 / FLOAT16), rounded once (BFLOAT16 holds every value below 2^128 exactly).
+ */
+int mb_mx4_dequantize(int dtype, const void* q, const void* scales, int64_t rows, int64_t columns, void* out,
+                      int64_t ldo, void* stream);
+
+/*
+ * mb_gemm_mx4 -- products of MX4 matrices, dense (offsets NULL, experts 1) or
+ * by expert over the sorted rows of x as in mb_gemm_grouped:
+ *   out[p][n] = sum over k of x[rows[p]][k] * w[e][n][k]
+ *
+ * x: x_rows rows, w: experts x N rows, both along K and MX4; out: BFLOAT16 or FLOAT16.
+ * Sums are fp32, rounded once. NaN blocks make their rows' (columns') outputs NaN. Output rows
+ * at and past offsets[experts] are left alone; rows that are not there give zeros.
+ * 1 <= K <= MB_MX4_MAX_K, 1 <= N < 2^30. x, w and out must not overlap.
+ * workspace: any size, NULL included; calls of few tiles run faster with one on
+ * 16 bytes that holds 2 to 16 fp32 copies of out (they split K).
+ */
+#define MB_MX4_MAX_K 8388608
+int mb_gemm_mx4(int dtype, const void* x, const void* x_scales, int64_t x_rows, const int32_t* rows, const void* w,
+                const void* w_scales, void* out, int64_t ldo, const int32_t* offsets, int experts, int64_t total_rows,
+                int64_t N, int64_t K, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * mb_kernel_info -- JSON object describing the kernel configuration the

@@ -74,6 +74,22 @@ ROUTE_DTYPES = ("float32", "bfloat16", "float16")
 EXPERT_DTYPES = ("bfloat16", "float16")
 GROUPED_FORWARD, GROUPED_GRAD_ROWS, GROUPED_GRAD_WEIGHTS = 0, 1, 2
 
+# Microscaled 4-bit floating point (mb_mx4_*, mb_gemm_mx4)
+MX4_SCALE_FLOOR, MX4_SCALE_FIT = 0, 1   # MB_MX4_SCALE_*
+MX4_MAX_K = 8388608                     # MB_MX4_MAX_K
+MX4_VALUE_DTYPES = ("float32", "bfloat16", "float16")
+MX4_OUTPUT_DTYPES = ("bfloat16", "float16")
+
+
+def mx4_row_bytes(columns: int) -> int:
+    """Bytes of elements in an MX4 row (MB_MX4_ROW_BYTES)."""
+    return (columns + 127) // 128 * 64
+
+
+def mx4_row_scales(columns: int) -> int:
+    """Bytes of scales in an MX4 row (MB_MX4_ROW_SCALES)."""
+    return (columns + 127) // 128 * 4
+
 # Plan overrides (mb_set_tuning); names follow the "overrides" keys of mb_kernel_info.
 TUNING_KNOBS = {
     "stream_unroll": 0,
@@ -169,6 +185,18 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
             ctypes.c_int, _cvp, _i64, _cvp, _i64, _i64, _cvp, _cvp, _i64, ctypes.c_int, _i64, _vp, _i64, _vp, _vp,
         ],
     ),
+    "mb_mx4_quantize": (
+        ctypes.c_int,
+        [ctypes.c_int, _cvp, _i64, _i64, _i64, ctypes.c_int, _vp, _vp, _vp, _vp, _vp],
+    ),
+    "mb_mx4_dequantize": (ctypes.c_int, [ctypes.c_int, _cvp, _cvp, _i64, _i64, _vp, _i64, _vp]),
+    "mb_gemm_mx4": (
+        ctypes.c_int,
+        [
+            ctypes.c_int, _cvp, _cvp, _i64, _cvp, _cvp, _cvp, _vp, _i64, _cvp, ctypes.c_int, _i64, _i64, _i64, _vp,
+            ctypes.c_size_t, _vp,
+        ],
+    ),
     "mb_kernel_info": (
         ctypes.c_int,
         [ctypes.c_int, ctypes.c_int, ctypes.c_int, _i64, _i64, _i64, ctypes.c_char_p, ctypes.c_size_t],
@@ -183,7 +211,7 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "mb_get_tuning": (_i64, [ctypes.c_int]),
 }
 
-ABI_VERSION = 4
+ABI_VERSION = 5
 
 
 class NativeLibraryError(RuntimeError):
@@ -320,6 +348,31 @@ class NativeLibrary:
                                              tokens, top_k, n, grad_y or None, ld_grad_y, grad_weights or None,
                                              stream or None)
         self._check(status, "mb_combine_grad")
+
+    # ---- microscaled 4-bit floating point --------------------------------------
+    def mx4_quantize(self, dtype: int, x: int, ldx: int, rows: int, columns: int, scale_rule: int, q: int | None,
+                     scales: int | None, qt: int | None = None, scales_t: int | None = None,
+                     stream: int | None = None) -> None:
+        """MX4 along x's rows (q, scales) and along its columns (qt, scales_t); either pair may be None
+        (see mb_mx4_quantize)."""
+        status = self.handle.mb_mx4_quantize(dtype, x, ldx, rows, columns, scale_rule, q or None, scales or None,
+                                             qt or None, scales_t or None, stream or None)
+        self._check(status, "mb_mx4_quantize")
+
+    def mx4_dequantize(self, dtype: int, q: int, scales: int, rows: int, columns: int, out: int, ldo: int,
+                       stream: int | None = None) -> None:
+        """The values of an MX4 matrix (see mb_mx4_dequantize)."""
+        status = self.handle.mb_mx4_dequantize(dtype, q, scales, rows, columns, out, ldo, stream or None)
+        self._check(status, "mb_mx4_dequantize")
+
+    def gemm_mx4(self, dtype: int, x: int, x_scales: int, x_rows: int, rows: int | None, w: int, w_scales: int,
+                 out: int, ldo: int, offsets: int | None, experts: int, total_rows: int, n: int, k: int,
+                 workspace: int | None = None, workspace_bytes: int = 0, stream: int | None = None) -> None:
+        """Products of MX4 matrices, dense or by expert (see mb_gemm_mx4)."""
+        status = self.handle.mb_gemm_mx4(dtype, x, x_scales, x_rows, rows or None, w, w_scales, out, ldo,
+                                         offsets or None, experts, total_rows, n, k, workspace or None,
+                                         workspace_bytes, stream or None)
+        self._check(status, "mb_gemm_mx4")
 
     # ---- metadata ----------------------------------------------------------
     def kernel_info(self, kind: int, a: int, b: int, m: int, n: int, k: int) -> dict[str, Any]:
