@@ -20,8 +20,8 @@ DeviceProps g_props[kMaxDevices];
 bool g_props_valid[kMaxDevices] = {false};
 
 // Plan overrides, -1 = the library's own choice. Process-wide, lock-free reads.
-std::atomic<int64_t> g_tuning[MB_TUNE_COUNT] = {-1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1};
-static_assert(MB_TUNE_COUNT == 12, "initialise every knob");
+std::atomic<int64_t> g_tuning[MB_TUNE_COUNT] = {-1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1};
+static_assert(MB_TUNE_COUNT == 14, "initialise every knob");
 
 struct KnobSpec {
     const char* name;
@@ -35,6 +35,8 @@ bool is_config(int64_t v) { return v >= 0 && v <= 4; }
 bool is_splits(int64_t v) { return v >= 1 && v <= 512; }
 bool is_grouped_config(int64_t v) { return v >= 0 && v <= 3; }
 bool is_w4_config(int64_t v) { return v >= 0 && v < kW4ConfigCount; }
+bool is_mx4_config(int64_t v) { return v >= 0 && v <= 3; }
+bool is_mx4_splits(int64_t v) { return v >= 1 && v <= 16; }
 bool is_mfma(int64_t v) { return v == 16 || v == 32; }
 
 const KnobSpec kKnobs[MB_TUNE_COUNT] = {
@@ -42,7 +44,7 @@ const KnobSpec kKnobs[MB_TUNE_COUNT] = {
     {"stream_schedule", is_bool},   {"gemm_force_generic", is_bool}, {"gemm_no_small_m", is_bool},
     {"gemm_tiled_config", is_config}, {"gemm_splits", is_splits},    {"gemm_fp8_mfma", is_mfma},
     {"gemm_highp_staged", is_bool}, {"grouped_config", is_grouped_config},
-    {"w4_config", is_w4_config},
+    {"w4_config", is_w4_config},      {"mx4_config", is_mx4_config},  {"mx4_splits", is_mx4_splits},
 };
 constexpr int kFirstGemmKnob = MB_TUNE_GEMM_FORCE_GENERIC, kFirstGroupedKnob = MB_TUNE_GROUPED_CONFIG;
 

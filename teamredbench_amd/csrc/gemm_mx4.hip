@@ -3,7 +3,7 @@
 //
 // gemm_mx4_any_kernel: a wave makes 32 rows x 32 columns from operands that go
 // from global memory straight into the matrix cores' registers. 64-bit addresses, any size.
-#include "mx4_common.hpp"
+#include "gemm_mx4_kernels.hpp"
 
 namespace mb {
 namespace {
@@ -57,16 +57,40 @@ gemm_mx4_any_kernel(Mx4Call c, int tiles_n) {
     }
 }
 
-}  // namespace
-
-int gemm_mx4_launch(const Mx4Call& c, void* workspace, size_t workspace_bytes, const DeviceProps& props,
-                    hipStream_t stream) {
+int launch_any(const Mx4Call& c, hipStream_t stream) {
     const int64_t tiles_m = c.offsets ? c.total_rows / kTile + std::min<int64_t>(c.experts, c.total_rows)
                                       : (c.total_rows + kTile - 1) / kTile;
     const int64_t tiles_n = (c.N + kTile - 1) / kTile;
     hipLaunchKernelGGL(gemm_mx4_any_kernel, launch_grid(tiles_m * tiles_n), dim3(64), 0, stream, c, (int)tiles_n);
     MB_HIP_TRY(hipGetLastError());
     return MB_OK;
+}
+
+Mx4Plan mx4_plan(const Mx4Call& c, size_t workspace_bytes, const DeviceProps& props) {
+    // Rows read through a list lie within the 2^31 bytes that a buffer offset spans.
+    if (c.rows != nullptr && c.x_rows > ((1ll << 31) - 1) / (c.units * kMx4UnitBytes)) return {-1, 1};
+    const int64_t forced = tuning(MB_TUNE_MX4_CONFIG);
+    int config = forced >= 0 ? (forced == 3 ? -1 : (int)forced) : c.total_rows <= 32 ? -1 : c.total_rows > 512 ? 0 : 1;
+    int splits = 1;
+    if (config > 0) {
+        const int64_t want = tuning(MB_TUNE_MX4_SPLITS);
+        const size_t plane = (size_t)c.total_rows * ((c.N + 3) / 4 * 4) * 4;
+        splits = want > 0 ? (int)want : 1;
+        while (splits > 1 && plane * splits > workspace_bytes) --splits;
+    }
+    return {config, splits};
+}
+
+}  // namespace
+
+int gemm_mx4_launch(const Mx4Call& c, void* workspace, size_t workspace_bytes, const DeviceProps& props,
+                    hipStream_t stream) {
+    // The workspace only makes small calls faster: one off 16 bytes is left alone.
+    if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0) workspace_bytes = 0;
+    const Mx4Plan plan = mx4_plan(c, workspace_bytes, props);
+    if (plan.config < 0) return launch_any(c, stream);
+    return c.dtype == MB_DT_FLOAT16 ? gemm_mx4_tiled_f16(c, plan, workspace, stream)
+                                    : gemm_mx4_tiled_bf16(c, plan, workspace, stream);
 }
 
 }  // namespace mb

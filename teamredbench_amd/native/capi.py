@@ -104,6 +104,8 @@ TUNING_KNOBS = {
     "gemm_highp_staged": 9,
     "grouped_config": 10,
     "w4_config": 11,
+    "mx4_config": 12,
+    "mx4_splits": 13,
 }
 
 # Every symbol include/mi355bench.h declares, with (restype, argtypes).

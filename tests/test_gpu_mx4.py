@@ -325,6 +325,36 @@ def test_results_repeat_bit_for_bit(lib):
         assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
 
 
+CONFIGS = [(0, None), (1, 1), (1, 2), (1, 5), (2, 1), (2, 3), (2, 16), (3, None)]
+
+
+@pytest.mark.parametrize("config, splits", CONFIGS)
+def test_every_kernel(lib, tune, config, splits):
+    """Each kernel and split count on the shapes, whatever the plan would pick."""
+    tune(mx4_config=config, mx4_splits=splits)
+    for m, n, k in [*DENSE, (70, 130, 6000)]:
+        print(f"[kernel] {config} splits {splits} {m}x{n}x{k}", flush=True)
+        a, b = mx4.random(m, k, m + k), mx4.random(n, k, n * 3 + k)
+        wanted = _rounded(_exact_product(a, b), "bfloat16")
+        x, w = mx4.on_gpu(*a), mx4.on_gpu(*b)
+        out = _strided(torch.full((m + 1, n), CANARY, dtype=wanted.dtype), n + 5, 0, CANARY)
+        _product(lib, "bfloat16", x, w, out, total=m, n=n, k=k)
+        assert torch.equal(out[:m].cpu(), wanted)
+        assert (out[m:] == CANARY).all()
+        assert (torch.as_strided(out, (m, 5), (n + 5, 1), n) == CANARY).all()
+
+
+@pytest.mark.parametrize("config, splits", CONFIGS)
+def test_every_kernel_by_expert(lib, tune, config, splits):
+    tune(mx4_config=config, mx4_splits=splits)
+    for counts, x_rows in EXPERTS:
+        for n, k in ((70, 300), (264, 1500)):
+            test_product_by_expert(lib, counts, x_rows, n, k)
+    test_rows_before_the_first_expert_are_left_alone(lib)
+    for offsets in ([-5, 10, 30], [0, 100, 30], [20, 10, 0]):
+        test_broken_offsets_stay_in_bounds(lib, offsets)
+
+
 # ---- together ---------------------------------------------------------------
 
 
