@@ -16,17 +16,7 @@ int gemm_mx4_tiled_bf16(const Mx4Call& c, const Mx4Plan& plan, void* workspace, 
 int gemm_mx4_tiled_f16(const Mx4Call& c, const Mx4Plan& plan, void* workspace, hipStream_t stream);
 
 constexpr int kMx4TileCount = 3;
-struct Mx4Tile {
-    int bm, bn;
-    bool x_pairs;   // a ring slot holds a pair of units (whole 128-byte lines of every row), or one
-    int nx;
-    bool w_pairs;
-    int nw;
-};
-#ifndef MX4_BIG
-#define MX4_BIG {256, 256, true, 3, false, 3}
-#endif
-constexpr Mx4Tile kMx4Tiles[kMx4TileCount] = {MX4_BIG, {128, 128, true, 2, true, 2}, {64, 64, true, 2, true, 2}};
+constexpr int kMx4Tiles[kMx4TileCount] = {256, 128, 64};
 
 namespace {
 
@@ -42,42 +32,59 @@ struct Mx4Args {
     bool out_16;                          // out's rows start on 16 bytes
 };
 
-// One operand's LDS ring: slots of T rows, one unit (64 bytes) or a pair (128) each, then their scales.
-template <bool PAIR, int T, int N_SLOTS>
-struct Mx4Ring {
-    static constexpr int kRow = PAIR ? 128 : 64;
-    static constexpr int kScaleRow = PAIR ? 8 : 4;
-    static constexpr int kData = T * kRow;
-    static constexpr int kDwords = T * kScaleRow / 4 / 4;              // scale dwords per wave and slot
-    static constexpr int kScaleInstr = (kDwords + 63) / 64;
-    // A wave with half an instruction's dwords loads its neighbour's too; the last wave's go to the slack behind.
-    static constexpr int kSlot = kData + T * kScaleRow + (kScaleInstr * 64 - kDwords) * 4;
-    static constexpr int kDataInstr = kData / 1024 / 4;
-    static constexpr int kInstr = kDataInstr + kScaleInstr;
-    static constexpr int kBytes = N_SLOTS * kSlot;
-    static_assert(kData % 4096 == 0 && kSlot % 16 == 0, "a slot must split over the waves");
-};
+// Ring slots: elements two slots of a pair of units (whole 128-byte lines of every row), scales two slots of 8
+// units (32 bytes of every row).
+constexpr int kPairBytes = 128, kChunkUnits = 8, kChunkBytes = 32;
 
-template <bool PAIR>
-__device__ __forceinline__ int mx4_swizzle(int row) {
-    return PAIR ? swz_a2(row) : swz_a(row);
+// Loads of step j: pair (j - 1) / 2 + 2 of x and w on odd j, then scale chunk (j - 7) / 8 + 2 where j % 8 == 7,
+// `pair` and `chunk` instructions per wave; the prologue runs the same rule over the steps before 0. Step j reads
+// unit j + 1, so its wait leaves only the loads issued after that unit's. By j % 8, the least of all steps.
+struct Mx4Waits {
+    int step[kChunkUnits], prologue;
+};
+constexpr Mx4Waits mx4_schedule(int pair, int chunk) {
+    constexpr int kSteps = 64, kFirst = -(kChunkUnits + 1);
+    int pair_end[kSteps] = {}, chunk_end[kSteps] = {}, before[kSteps] = {};
+    int total = 0;
+    for (int v = kFirst; v < kSteps; ++v) {
+        if (v >= 0) before[v] = total;
+        if ((v & 1) != 0 && (v - 1) / 2 + 2 >= 0 && (v - 1) / 2 + 2 < kSteps) pair_end[(v - 1) / 2 + 2] = (total += pair);
+        if ((v & 7) == 7) chunk_end[(v + 1) / kChunkUnits + 1] = (total += chunk);
+    }
+    Mx4Waits r{};
+    r.prologue = before[0] - (pair_end[0] > chunk_end[0] ? pair_end[0] : chunk_end[0]);
+    for (int i = 0; i < kChunkUnits; ++i) r.step[i] = 63;
+    for (int j = 0; j + 1 < kSteps; ++j) {
+        const int p = pair_end[(j + 1) / 2], c = chunk_end[(j + 1) / kChunkUnits];
+        const int wait = before[j] - (p > c ? p : c);
+        if (wait < r.step[j % kChunkUnits]) r.step[j % kChunkUnits] = wait;
+    }
+    return r;
 }
 
-template <int DT, int CFG>
+#ifndef MX4_STRIDE
+#define MX4_STRIDE 2
+#endif
+
+template <int DT, int TILE>
 __global__ void __launch_bounds__(256)
 gemm_mx4_kernel(Mx4Args args, int tiles_n, int group_m) {
-    constexpr Mx4Tile kTile = kMx4Tiles[CFG];
-    constexpr int BM = kTile.bm, BN = kTile.bn, NX = kTile.nx, NW = kTile.nw;
-    constexpr bool XP = kTile.x_pairs, WP = kTile.w_pairs;
+    constexpr int BM = TILE, BN = TILE;
     constexpr int WTM = BM / 2, WTN = BN / 2;
     constexpr int FM = WTM / 32, FN = WTN / 32;
-    typedef Mx4Ring<XP, BM, NX> RX;
-    typedef Mx4Ring<WP, BN, NW> RW;
-    constexpr int LDS_BYTES = RX::kBytes + RW::kBytes;
-    static_assert(LDS_BYTES <= 160 * 1024, "LDS rings do not fit");
-    constexpr StepWaits kWaits = step_schedule(XP, NX, RX::kInstr, WP, NW, RW::kInstr);
-    static_assert(kWaits.prologue >= 0 && kWaits.odd >= 0 && kWaits.even >= 0 && kWaits.prologue < 64 &&
-                  kWaits.odd < 64 && kWaits.even < 64, "a needed stage is unissued, or vmcnt overflows");
+    constexpr int SLOT = TILE * kPairBytes, SCALE_SLOT = TILE * kChunkBytes;   // one operand's
+    constexpr int W0 = 2 * SLOT;                          // x's elements, w's, x's scales, w's: two slots each
+    constexpr int XS0 = 4 * SLOT, WS0 = XS0 + 2 * SCALE_SLOT;
+    constexpr int LDS_BYTES = WS0 + 2 * SCALE_SLOT;
+    constexpr int INSTR = SLOT / 1024 / 4;                // DMA instructions per wave, operand and pair
+    constexpr int SCALE_INSTR = 2 * SCALE_SLOT / 1024 / 4;   // ... per wave and chunk, both operands
+    static_assert(LDS_BYTES <= 160 * 1024 && SLOT % 4096 == 0 && SCALE_INSTR >= 1, "LDS rings");
+    constexpr Mx4Waits kWaits = mx4_schedule(2 * INSTR, SCALE_INSTR);
+    static_assert([&] {
+        for (int w : kWaits.step)
+            if (w < 0) return false;
+        return kWaits.prologue >= 0 && kWaits.prologue < 64;
+    }(), "a needed unit is unissued, or vmcnt overflows");
     __shared__ __attribute__((aligned(1024))) unsigned char lds[LDS_BYTES];
 
     const int tid = threadIdx.x;
@@ -109,55 +116,51 @@ gemm_mx4_kernel(Mx4Args args, int tiles_n, int group_m) {
     };
     const __amdgpu_buffer_rsrc_t rx = resource(args.x, x_first, args.ld, x_count);
     const __amdgpu_buffer_rsrc_t rw = resource(args.w, w_first, args.ld, w_count);
-    const __amdgpu_buffer_rsrc_t rxs = resource(args.xs, x_first, args.lds, x_count);
-    const __amdgpu_buffer_rsrc_t rws = resource(args.ws, w_first, args.lds, w_count);
 
-    // This lane's byte offsets of its pieces in slot 0: 16 bytes of elements (an instruction fills 8 rows of a
-    // pair, or 16 of a unit) and scale dwords.
-    int x_off[RX::kDataInstr], xs_off[RX::kScaleInstr], w_off[RW::kDataInstr], ws_off[RW::kScaleInstr];
-    auto offsets = [&](auto ring, auto pair, auto row_of, int (&off)[decltype(ring)::kDataInstr],
-                       int (&s_off)[decltype(ring)::kScaleInstr], int rows) {
-        typedef decltype(ring) R;
-        constexpr int kChunks = R::kRow / 16, kScales = R::kScaleRow / 4;
-#pragma unroll
-        for (int q = 0; q < R::kDataInstr; ++q) {
-            const int lin = (wave * R::kDataInstr + q) * 64 + lane;
-            const int row = row_of(lin / kChunks);
-            const int chunk = (lin % kChunks) ^ mx4_swizzle<decltype(pair)::value>(lin / kChunks);
-            off[q] = row < 0 ? kNowhere : row * args.ld + 16 * chunk;
-        }
-#pragma unroll
-        for (int q = 0; q < R::kScaleInstr; ++q) {
-            const int lin = wave * R::kDwords + q * 64 + lane;
-            const int row = lin / kScales < rows ? row_of(lin / kScales) : -1;
-            s_off[q] = row < 0 ? kNowhere : row * args.lds + 4 * (lin % kScales);
-        }
-    };
-    offsets(RX{}, std::bool_constant<XP>{}, [&](int r) {
+    auto x_row = [&](int r) {
         if (m0 + r >= M) return -1;
         if (!gather) return r;
         const int listed = args.rows[ex.first + m0 + r];
         return listed < args.x_rows ? listed : -1;
-    }, x_off, xs_off, BM);
-    offsets(RW{}, std::bool_constant<WP>{}, [&](int r) { return n0 + r < args.N ? r : -1; }, w_off, ws_off, BN);
-
-    auto lds_of = [&](int at) { return (unsigned)(uintptr_t)(MB_LDS unsigned char*)(lds + at); };
-    // DMA instruction q of unit (pair) i into the slot at byte `at`.
-    auto issue = [&](auto ring, const __amdgpu_buffer_rsrc_t& r, const __amdgpu_buffer_rsrc_t& rs, const int* off,
-                     const int* s_off, int i, int at, auto idx) {
-        typedef decltype(ring) R;
-        constexpr int q = decltype(idx)::value;
-        if constexpr (q < R::kDataInstr) {
-            lds_dma16(r, lds_of(at) + (wave * R::kDataInstr + q) * 1024, off[q], u0 * 64 + i * R::kRow);
-        } else {
-            constexpr int s = q - R::kDataInstr;
-            lds_dma4(rs, lds_of(at + R::kData) + (wave * R::kDwords + s * 64) * 4, s_off[s],
-                     u0 * 4 + i * R::kScaleRow);
-        }
     };
-    auto issue_x = [&](int i, int at, auto idx) { issue(RX{}, rx, rxs, x_off, xs_off, i, at, idx); };
-    auto issue_w = [&](int i, int at, auto idx) { issue(RW{}, rw, rws, w_off, ws_off, i, at, idx); };
-    constexpr int W0 = RX::kBytes;   // w's ring follows x's
+    auto w_row = [&](int r) { return n0 + r < args.N ? r : -1; };
+
+    // This lane's byte offsets of its 16-byte pieces: an instruction fills 8 rows of a pair, or the scales of 32
+    // rows. Waves 0 and 1 load x's scales, 2 and 3 w's.
+    int x_off[INSTR], w_off[INSTR], s_off[SCALE_INSTR];
+#pragma unroll
+    for (int q = 0; q < INSTR; ++q) {
+        const int r = (wave * INSTR + q) * 8 + (lane >> 3);
+        const int byte = ((lane & 7) ^ swz_a2(r)) << 4;
+        const int xr = x_row(r), wr = w_row(r);
+        x_off[q] = xr < 0 ? kNowhere : xr * args.ld + byte;
+        w_off[q] = wr < 0 ? kNowhere : wr * args.ld + byte;
+    }
+    const bool scales_of_x = wave < 2;
+#pragma unroll
+    for (int q = 0; q < SCALE_INSTR; ++q) {
+        const int r = ((wave & 1) * SCALE_INSTR + q) * 32 + (lane >> 1);
+        const int row = scales_of_x ? x_row(r) : w_row(r);
+        s_off[q] = row < 0 ? kNowhere : row * args.lds + (((lane & 1) ^ ((r >> 3) & 1)) << 4);
+    }
+    const __amdgpu_buffer_rsrc_t rs = scales_of_x ? resource(args.xs, x_first, args.lds, x_count)
+                                                  : resource(args.ws, w_first, args.lds, w_count);
+
+    const unsigned lds0 = (unsigned)(uintptr_t)(MB_LDS unsigned char*)lds;
+    auto issue_x = [&](int pair, int at, auto idx) {
+        constexpr int q = decltype(idx)::value;
+        lds_dma16(rx, lds0 + at + (wave * INSTR + q) * 1024, x_off[q], u0 * kMx4UnitBytes + pair * kPairBytes);
+    };
+    auto issue_w = [&](int pair, int at, auto idx) {
+        constexpr int q = decltype(idx)::value;
+        lds_dma16(rw, lds0 + W0 + at + (wave * INSTR + q) * 1024, w_off[q], u0 * kMx4UnitBytes + pair * kPairBytes);
+    };
+    auto issue_scales = [&](int chunk, auto idx) {
+        constexpr int q = decltype(idx)::value;
+        const unsigned to = lds0 + (scales_of_x ? XS0 : WS0) + (chunk & 1) * SCALE_SLOT;
+        lds_dma16(rs, to + ((wave & 1) * SCALE_INSTR + q) * 1024, s_off[q],
+                  u0 * kMx4UnitScales + chunk * kChunkBytes);
+    };
 
     f32x16 acc[FM][FN];
 #pragma unroll
@@ -175,34 +178,36 @@ gemm_mx4_kernel(Mx4Args args, int tiles_n, int group_m) {
     };
     constexpr int N_READS = 3 * (FM + FN);
     constexpr int N_MFMA = 2 * FM * FN;
-    auto read_piece = [&](auto ring, auto pair, const unsigned char* slot, int row, auto par, int t) {
-        typedef decltype(ring) R;
-        constexpr int first = R::kRow == 128 ? 4 * decltype(par)::value : 0;
-        const int chunk = (first + 2 * half + t) ^ mx4_swizzle<decltype(pair)::value>(row);
-        return *reinterpret_cast<const u32x4*>(slot + row * R::kRow + 16 * chunk);
+    // Byte offsets of this lane's reads from a slot's start: its row of fragment 0, chunk 4 P + 2 half + t.
+    const int x_lane = wm * WTM + r32, w_lane = wn * WTN + r32;
+    auto piece_at = [&](int row, int chunk) { return row * kPairBytes + ((chunk ^ swz_a2(row)) << 4); };
+    // Scales: 16 bytes hold 4 units; `xs_at` and `ws_at` move to the other slot every 8 units.
+    auto scales_at = [&](int row, int unit) {
+        return row * kChunkBytes + (((unit >> 2) ^ ((row >> 3) & 1)) << 4) + 4 * (unit & 3) + 2 * half;
     };
-    auto read_scales = [&](auto ring, const unsigned char* slot, int row, auto par) -> unsigned {
-        typedef decltype(ring) R;
-        constexpr int first = R::kRow == 128 ? 4 * decltype(par)::value : 0;
-        return *reinterpret_cast<const uint16_t*>(slot + R::kData + row * R::kScaleRow + first + 2 * half);
-    };
+    int slot_flip = 0;   // SCALE_SLOT while the current chunk's number is odd
     // Read number r of a unit, in the order the MFMAs consume operands: x fragment 0, w's, x's others; with substep
     // 0's elements their scales.
-    auto read_op = [&](const unsigned char* xslot, const unsigned char* wslot, auto par, auto idx, UnitOps& o) {
-        constexpr int r = decltype(idx)::value;
+    auto read_op = [&](auto unit, auto idx, UnitOps& o) {   // unit: its number modulo 8, 8 for the next chunk's first
+        constexpr int u = decltype(unit)::value, r = decltype(idx)::value;
         constexpr int t = r < 2 * (FM + FN) ? 0 : 1;
         constexpr int f = t == 0 ? r / 2 : r - 2 * (FM + FN);
         constexpr bool scales = t == 0 && r % 2 == 1;
-        if constexpr (f >= 1 && f <= FN) {
-            constexpr int j = f - 1;
-            const int row = wn * WTN + 32 * j + r32;
-            if constexpr (scales) o.sb[j] = read_scales(RW{}, wslot, row, par);
-            else o.b[t][j] = read_piece(RW{}, std::bool_constant<WP>{}, wslot, row, par, t);
+        constexpr int at = (u / 2) % 2 * SLOT, chunk = 4 * (u % 2) + t;
+        constexpr bool is_w = f >= 1 && f <= FN;
+        constexpr int frag = is_w ? f - 1 : f == 0 ? 0 : f - FN;
+        const int row = (is_w ? w_lane : x_lane) + 32 * frag;
+        if constexpr (scales) {
+            const int flip = u == kChunkUnits ? slot_flip ^ SCALE_SLOT : slot_flip;
+            const unsigned v =
+                *reinterpret_cast<const uint16_t*>(lds + (is_w ? WS0 : XS0) + flip + scales_at(row, u % kChunkUnits));
+            if constexpr (is_w) o.sb[frag] = v;
+            else o.sa[frag] = v;
         } else {
-            constexpr int i = f == 0 ? 0 : f - FN;
-            const int row = wm * WTM + 32 * i + r32;
-            if constexpr (scales) o.sa[i] = read_scales(RX{}, xslot, row, par);
-            else o.a[t][i] = read_piece(RX{}, std::bool_constant<XP>{}, xslot, row, par, t);
+            const u32x4 v =
+                *reinterpret_cast<const u32x4*>(lds + (is_w ? W0 : 0) + at + piece_at(row, chunk + 2 * half));
+            if constexpr (is_w) o.b[t][frag] = v;
+            else o.a[t][frag] = v;
         }
     };
     auto mfma_op = [&](auto idx, const UnitOps& o) {
@@ -212,56 +217,43 @@ gemm_mx4_kernel(Mx4Args args, int tiles_n, int group_m) {
     };
 
     const int ksteps = min(args.units - u0, args.split_units);
-    const int last = ksteps - 1, last_pair = last / 2;
-    constexpr int VX = XP ? 2 * NX - 1 : NX, VW = WP ? 2 * NW - 1 : NW;
-    constexpr int V = VX > VW ? VX : VW;
-    [&]<int... U>(std::integer_sequence<int, U...>) {
-        ([&] {
-            constexpr int v = U - V;
-            constexpr int ix = XP ? (v - 1) / 2 + NX : v + NX, iw = WP ? (v - 1) / 2 + NW : v + NW;
-            if constexpr ((!XP || (v & 1) != 0) && ix >= 0) {
-                [&]<int... Q>(std::integer_sequence<int, Q...>) {
-                    (issue_x(min(ix, XP ? last_pair : last), ix * RX::kSlot, std::integral_constant<int, Q>{}), ...);
-                }(std::make_integer_sequence<int, RX::kInstr>{});
-            }
-            if constexpr ((!WP || (v & 1) != 0) && iw >= 0) {
-                [&]<int... Q>(std::integer_sequence<int, Q...>) {
-                    (issue_w(min(iw, WP ? last_pair : last), W0 + iw * RW::kSlot, std::integral_constant<int, Q>{}),
-                     ...);
-                }(std::make_integer_sequence<int, RW::kInstr>{});
-            }
-        }(), ...);
-    }(std::make_integer_sequence<int, V>{});
+    const int last_pair = (ksteps - 1) / 2, last_chunk = (ksteps - 1) / kChunkUnits;
+    auto all = [&](auto count, auto&& f) {
+        [&]<int... Q>(std::integer_sequence<int, Q...>) {
+            (f(std::integral_constant<int, Q>{}), ...);
+        }(std::make_integer_sequence<int, decltype(count)::value>{});
+    };
+    constexpr std::integral_constant<int, INSTR> kPieces{};
+    constexpr std::integral_constant<int, SCALE_INSTR> kScalePieces{};
+    all(kScalePieces, [&](auto q) { issue_scales(0, q); });
+    all(kPieces, [&](auto q) { issue_x(0, 0, q); });
+    all(kPieces, [&](auto q) { issue_w(0, 0, q); });
+    all(kPieces, [&](auto q) { issue_x(min(1, last_pair), SLOT, q); });
+    all(kPieces, [&](auto q) { issue_w(min(1, last_pair), SLOT, q); });
+    all(kScalePieces, [&](auto q) { issue_scales(1, q); });   // past the row's end: zeros or other scales, unused
 
     UnitOps ops[2];
     wait_vmcnt_and_barrier<kWaits.prologue>();
-    [&]<int... R>(std::integer_sequence<int, R...>) {
-        (read_op(lds, lds + W0, std::integral_constant<int, 0>{}, std::integral_constant<int, R>{}, ops[0]), ...);
-    }(std::make_integer_sequence<int, N_READS>{});
+    all(std::integral_constant<int, N_READS>{},
+        [&](auto r) { read_op(std::integral_constant<int, 0>{}, r, ops[0]); });
 
-    auto slot = [](bool pairs, int n, int unit) constexpr { return pairs ? (unit / 2) % n : unit % n; };
     auto step = [&](auto idx, int kt) {
-        constexpr int I = decltype(idx)::value;
-        constexpr bool ODD = (I & 1) != 0;
-        constexpr int X_LOADS = !XP || ODD ? RX::kInstr : 0, W_LOADS = !WP || ODD ? RW::kInstr : 0;
-        constexpr int LOADS = X_LOADS + W_LOADS;
+        constexpr int I = decltype(idx)::value;               // kt % 8
+        constexpr int DATA_LOADS = I % 2 ? 2 * INSTR : 0, LOADS = DATA_LOADS + (I == 7 ? SCALE_INSTR : 0);
         constexpr int N_MEM = N_READS + LOADS;
         constexpr int PRE = N_MFMA >= 16 ? kPreBarrierMfma : 0;
         constexpr int PER = (N_MEM + N_MFMA - PRE - 1) / (N_MFMA - PRE);
-        constexpr int kStride = LOADS > 0 ? N_MEM / LOADS : N_MEM + 1;   // loads sit evenly among the reads
+        // Loads sit among the reads, as early as every MX4_STRIDE-th memory instruction.
+        constexpr int kStride = LOADS == 0 ? N_MEM + 1 : N_MEM / LOADS < MX4_STRIDE ? N_MEM / LOADS : MX4_STRIDE;
         constexpr auto kIsLoad = [](int m) { return (m + 1) % kStride == 0 && (m + 1) / kStride <= LOADS; };
-        const unsigned char* next_x = lds + slot(XP, NX, I + 1) * RX::kSlot;
-        const unsigned char* next_w = lds + W0 + slot(WP, NW, I + 1) * RW::kSlot;
-        constexpr int LX = XP ? ((I + 2 * NX - 1) / 2) % NX : I % NX;    // the slot this step's load fills
-        constexpr int LW = WP ? ((I + 2 * NW - 1) / 2) % NW : I % NW;
         const UnitOps& cur = ops[I % 2];
         UnitOps& nxt = ops[(I + 1) % 2];
-        const int x_load = XP ? min((kt - 1) / 2 + NX, last_pair) : min(kt + NX, last);
-        const int w_load = WP ? min((kt - 1) / 2 + NW, last_pair) : min(kt + NW, last);
+        const int pair = min((kt - 1) / 2 + 2, last_pair);    // into the slot of the pair that unit kt ends
+        const int chunk = min((kt - 7) / kChunkUnits + 2, last_chunk + 1);
         [&]<int... Q>(std::integer_sequence<int, Q...>) {
             ([&] {
                 if constexpr (Q == PRE) {
-                    wait_vmcnt_and_barrier<ODD ? kWaits.odd : kWaits.even>();
+                    wait_vmcnt_and_barrier<kWaits.step[I]>();
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 mfma_op(std::integral_constant<int, Q>{}, cur);
@@ -272,14 +264,17 @@ gemm_mx4_kernel(Mx4Args args, int tiles_n, int group_m) {
                     ([&] {
                         constexpr int m = lo + R;
                         if constexpr (kIsLoad(m)) {
-                            constexpr int l = (m + 1) / kStride - 1;
-                            if constexpr (l < X_LOADS)
-                                issue_x(x_load, LX * RX::kSlot, std::integral_constant<int, l>{});
-                            else
-                                issue_w(w_load, W0 + LW * RW::kSlot, std::integral_constant<int, l - X_LOADS>{});
+                            constexpr int l = (m + 1) / kStride - 1, at = (I / 2) % 2 * SLOT;
+                            if constexpr (l >= DATA_LOADS) {
+                                issue_scales(chunk, std::integral_constant<int, l - DATA_LOADS>{});
+                            } else if constexpr (l < INSTR) {
+                                issue_x(pair, at, std::integral_constant<int, l>{});
+                            } else {
+                                issue_w(pair, at, std::integral_constant<int, l - INSTR>{});
+                            }
                         } else {
                             constexpr int loads_before = m / kStride < LOADS ? m / kStride : LOADS;
-                            read_op(next_x, next_w, std::integral_constant<int, (I + 1) & 1>{},
+                            read_op(std::integral_constant<int, I + 1>{},
                                     std::integral_constant<int, m - loads_before>{}, nxt);
                         }
                     }(), ...);
@@ -288,11 +283,11 @@ gemm_mx4_kernel(Mx4Args args, int tiles_n, int group_m) {
             }(), ...);
         }(std::make_integer_sequence<int, N_MFMA>{});
     };
-    constexpr int UNROLL = std::lcm(2, std::lcm(XP ? 2 * NX : NX, WP ? 2 * NW : NW));
-    for (int kt = 0; kt < ksteps; kt += UNROLL) {
+    for (int kt = 0; kt < ksteps; kt += kChunkUnits) {
         [&]<int... I>(std::integer_sequence<int, I...>) {
             ((kt + I < ksteps ? step(std::integral_constant<int, I>{}, kt + I) : void()), ...);
-        }(std::make_integer_sequence<int, UNROLL>{});
+        }(std::make_integer_sequence<int, kChunkUnits>{});
+        slot_flip ^= SCALE_SLOT;
     }
     wait_vmcnt_and_barrier<0>();
 
@@ -400,10 +395,10 @@ gemm_mx4_sum_kernel(Mx4Args a) {
 
 template <int DT, int CFG>
 int launch_mx4(const Mx4Call& c, int splits, void* workspace, hipStream_t stream) {
-    constexpr Mx4Tile kTile = kMx4Tiles[CFG];
-    const int tiles_n = (int)((c.N + kTile.bn - 1) / kTile.bn);
-    const int64_t tiles_m = c.offsets ? c.total_rows / kTile.bm + std::min<int64_t>(c.experts, c.total_rows)
-                                      : (c.total_rows + kTile.bm - 1) / kTile.bm;
+    constexpr int TILE = kMx4Tiles[CFG];
+    const int tiles_n = (int)((c.N + TILE - 1) / TILE);
+    const int64_t tiles_m = c.offsets ? c.total_rows / TILE + std::min<int64_t>(c.experts, c.total_rows)
+                                      : (c.total_rows + TILE - 1) / TILE;
     const int split_units = (int)((c.units + 2 * splits - 1) / (2 * splits) * 2);   // whole pairs
     splits = (int)((c.units + split_units - 1) / split_units);                      // none is empty
     const bool out_16 = ((reinterpret_cast<uintptr_t>(c.out) | (uintptr_t)(c.ldo * 2)) & 15) == 0;
@@ -413,7 +408,7 @@ int launch_mx4(const Mx4Call& c, int splits, void* workspace, hipStream_t stream
                     (int)c.units * kMx4UnitScales, (int)c.units, (int)c.x_rows, c.experts, (int)c.total_rows, (int)c.N,
                     splits > 1 ? static_cast<float*>(workspace) : nullptr, splits, split_units,
                     (int)((c.N + 3) / 4 * 4), out_16};
-    hipLaunchKernelGGL((gemm_mx4_kernel<DT, CFG>), launch_grid(tiles_m * tiles_n * splits), dim3(256), 0, stream, a,
+    hipLaunchKernelGGL((gemm_mx4_kernel<DT, TILE>), launch_grid(tiles_m * tiles_n * splits), dim3(256), 0, stream, a,
                        tiles_n, 4);
     MB_HIP_TRY(hipGetLastError());
     if (splits > 1) {
