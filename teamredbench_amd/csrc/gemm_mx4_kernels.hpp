@@ -103,7 +103,9 @@ gemm_mx4_kernel(Mx4Args args, int tiles_n, int group_m) {
     block_coords(block, tiles_m, tiles_n, args.splits, group_m, &tm, &tn, &split);
     if (by_expert && !find_row_tile(args.offsets, args.experts, args.total, tm, BM, &ex, &tm)) return;
     const int M = ex.count, m0 = tm * BM, n0 = tn * BN;
-    const int u0 = split * args.split_units;
+    // Units of K of this block, in whole pairs: the second unit of a last pair that has but one is zeros.
+    const int u0 = split * args.split_units, k_units = min(args.units - u0, args.split_units);
+    const int ksteps = (k_units + 1) & ~1, half_pair = k_units & 1 ? k_units / 2 : -1;
 
     // Buffer resources over the tile's rows (gathered: all of x): rows and units past them read as zeros.
     const bool gather = args.rows != nullptr;
@@ -128,11 +130,13 @@ gemm_mx4_kernel(Mx4Args args, int tiles_n, int group_m) {
     // This lane's byte offsets of its 16-byte pieces: an instruction fills 8 rows of a pair, or the scales of 32
     // rows. Waves 0 and 1 load x's scales, 2 and 3 w's.
     int x_off[INSTR], w_off[INSTR], s_off[SCALE_INSTR];
+    bool x_second[2];   // the piece lies in its pair's second unit (the swizzle repeats every 16 rows)
 #pragma unroll
     for (int q = 0; q < INSTR; ++q) {
         const int r = (wave * INSTR + q) * 8 + (lane >> 3);
         const int byte = ((lane & 7) ^ swz_a2(r)) << 4;
         const int xr = x_row(r), wr = w_row(r);
+        if (q < 2) x_second[q] = byte >= kMx4UnitBytes;
         x_off[q] = xr < 0 ? kNowhere : xr * args.ld + byte;
         w_off[q] = wr < 0 ? kNowhere : wr * args.ld + byte;
     }
@@ -149,7 +153,8 @@ gemm_mx4_kernel(Mx4Args args, int tiles_n, int group_m) {
     const unsigned lds0 = (unsigned)(uintptr_t)(MB_LDS unsigned char*)lds;
     auto issue_x = [&](int pair, int at, auto idx) {
         constexpr int q = decltype(idx)::value;
-        lds_dma16(rx, lds0 + at + (wave * INSTR + q) * 1024, x_off[q], u0 * kMx4UnitBytes + pair * kPairBytes);
+        const int off = pair == half_pair && x_second[q & 1] ? kNowhere : x_off[q];
+        lds_dma16(rx, lds0 + at + (wave * INSTR + q) * 1024, off, u0 * kMx4UnitBytes + pair * kPairBytes);
     };
     auto issue_w = [&](int pair, int at, auto idx) {
         constexpr int q = decltype(idx)::value;
@@ -170,53 +175,54 @@ gemm_mx4_kernel(Mx4Args args, int tiles_n, int group_m) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
-    // Operands of a unit: two substeps of 64 k. Lane half h takes blocks 2h and 2h + 1 of a row's four, so one
-    // 16-bit read brings both of its scales, the first MFMA takes byte 0 and the second byte 1.
+    // Operands of a unit: two substeps of 64 k. Of the 8 blocks of a pair, lane half h takes 4h .. 4h + 3, two a
+    // unit, so one dword brings its scales of a pair, a byte for each MFMA.
     struct UnitOps {
         u32x4 a[2][FM], b[2][FN];
-        unsigned sa[FM], sb[FN];
     };
-    constexpr int N_READS = 3 * (FM + FN);
+    struct PairScales {
+        unsigned a[FM], b[FN];
+    };
     constexpr int N_MFMA = 2 * FM * FN;
-    // Byte offsets of this lane's reads from a slot's start: its row of fragment 0, chunk 4 P + 2 half + t.
+    // Byte offsets of this lane's reads from a slot's start.
     const int x_lane = wm * WTM + r32, w_lane = wn * WTN + r32;
     auto piece_at = [&](int row, int chunk) { return row * kPairBytes + ((chunk ^ swz_a2(row)) << 4); };
-    // Scales: 16 bytes hold 4 units; `xs_at` and `ws_at` move to the other slot every 8 units.
-    auto scales_at = [&](int row, int unit) {
-        return row * kChunkBytes + (((unit >> 2) ^ ((row >> 3) & 1)) << 4) + 4 * (unit & 3) + 2 * half;
+    auto scales_at = [&](int row, int unit) {   // 16 bytes hold 4 units; unit: the even one of the pair, modulo 8
+        return row * kChunkBytes + (((unit >> 2) ^ ((row >> 3) & 1)) << 4) + 4 * (unit & 2) + 4 * half;
     };
     int slot_flip = 0;   // SCALE_SLOT while the current chunk's number is odd
-    // Read number r of a unit, in the order the MFMAs consume operands: x fragment 0, w's, x's others; with substep
-    // 0's elements their scales.
-    auto read_op = [&](auto unit, auto idx, UnitOps& o) {   // unit: its number modulo 8, 8 for the next chunk's first
+    // Read number r of unit u (its number modulo 8, 8 for the next chunk's first), in the order the MFMAs consume
+    // operands: x fragment 0, w's, x's others; a pair's first unit brings the pair's scales too.
+    auto read_op = [&](auto unit, auto idx, UnitOps& o, PairScales& s) {
         constexpr int u = decltype(unit)::value, r = decltype(idx)::value;
-        constexpr int t = r < 2 * (FM + FN) ? 0 : 1;
-        constexpr int f = t == 0 ? r / 2 : r - 2 * (FM + FN);
-        constexpr bool scales = t == 0 && r % 2 == 1;
-        constexpr int at = (u / 2) % 2 * SLOT, chunk = 4 * (u % 2) + t;
+        constexpr int FIRST = (u % 2 ? 1 : 2) * (FM + FN);   // reads of substep 0
+        constexpr int t = r < FIRST ? 0 : 1;
+        constexpr int f = t == 1 ? r - FIRST : u % 2 ? r : r / 2;
+        constexpr bool scales = u % 2 == 0 && t == 0 && r % 2 == 1;
+        constexpr int at = (u / 2) % 2 * SLOT, chunk = 2 * (u % 2) + t;
         constexpr bool is_w = f >= 1 && f <= FN;
         constexpr int frag = is_w ? f - 1 : f == 0 ? 0 : f - FN;
         const int row = (is_w ? w_lane : x_lane) + 32 * frag;
         if constexpr (scales) {
             const int flip = u == kChunkUnits ? slot_flip ^ SCALE_SLOT : slot_flip;
             const unsigned v =
-                *reinterpret_cast<const uint16_t*>(lds + (is_w ? WS0 : XS0) + flip + scales_at(row, u % kChunkUnits));
-            if constexpr (is_w) o.sb[frag] = v;
-            else o.sa[frag] = v;
+                *reinterpret_cast<const unsigned*>(lds + (is_w ? WS0 : XS0) + flip + scales_at(row, u % kChunkUnits));
+            if constexpr (is_w) s.b[frag] = v;
+            else s.a[frag] = v;
         } else {
             const u32x4 v =
-                *reinterpret_cast<const u32x4*>(lds + (is_w ? W0 : 0) + at + piece_at(row, chunk + 2 * half));
+                *reinterpret_cast<const u32x4*>(lds + (is_w ? W0 : 0) + at + piece_at(row, chunk + 4 * half));
             if constexpr (is_w) o.b[t][frag] = v;
             else o.a[t][frag] = v;
         }
     };
-    auto mfma_op = [&](auto idx, const UnitOps& o) {
+    auto mfma_op = [&](auto parity, auto idx, const UnitOps& o, const PairScales& s) {
         constexpr int q = decltype(idx)::value;
         constexpr int t = q / (FM * FN), i = (q / FN) % FM, j = q % FN;
-        acc[i][j] = mfma_mx4<t, t>(o.b[t][j], o.sb[j], o.a[t][i], o.sa[i], acc[i][j]);
+        constexpr int byte = 2 * decltype(parity)::value + t;
+        acc[i][j] = mfma_mx4<byte, byte>(o.b[t][j], s.b[j], o.a[t][i], s.a[i], acc[i][j]);
     };
 
-    const int ksteps = min(args.units - u0, args.split_units);
     const int last_pair = (ksteps - 1) / 2, last_chunk = (ksteps - 1) / kChunkUnits;
     auto all = [&](auto count, auto&& f) {
         [&]<int... Q>(std::integer_sequence<int, Q...>) {
@@ -234,13 +240,14 @@ gemm_mx4_kernel(Mx4Args args, int tiles_n, int group_m) {
 
     UnitOps ops[2];
     wait_vmcnt_and_barrier<kWaits.prologue>();
-    all(std::integral_constant<int, N_READS>{},
-        [&](auto r) { read_op(std::integral_constant<int, 0>{}, r, ops[0]); });
+    PairScales scales[2];
+    all(std::integral_constant<int, 3 * (FM + FN)>{},
+        [&](auto r) { read_op(std::integral_constant<int, 0>{}, r, ops[0], scales[0]); });
 
     auto step = [&](auto idx, int kt) {
         constexpr int I = decltype(idx)::value;               // kt % 8
         constexpr int DATA_LOADS = I % 2 ? 2 * INSTR : 0, LOADS = DATA_LOADS + (I == 7 ? SCALE_INSTR : 0);
-        constexpr int N_MEM = N_READS + LOADS;
+        constexpr int N_READS = (I % 2 ? 3 : 2) * (FM + FN), N_MEM = N_READS + LOADS;
         constexpr int PRE = N_MFMA >= 16 ? kPreBarrierMfma : 0;
         constexpr int PER = (N_MEM + N_MFMA - PRE - 1) / (N_MFMA - PRE);
         // Loads sit among the reads, as early as every MX4_STRIDE-th memory instruction.
@@ -248,15 +255,25 @@ gemm_mx4_kernel(Mx4Args args, int tiles_n, int group_m) {
         constexpr auto kIsLoad = [](int m) { return (m + 1) % kStride == 0 && (m + 1) / kStride <= LOADS; };
         const UnitOps& cur = ops[I % 2];
         UnitOps& nxt = ops[(I + 1) % 2];
+        PairScales& cur_scales = scales[I / 2 % 2];
+        PairScales& nxt_scales = scales[(I + 1) / 2 % 2];
         const int pair = min((kt - 1) / 2 + 2, last_pair);    // into the slot of the pair that unit kt ends
         const int chunk = min((kt - 7) / kChunkUnits + 2, last_chunk + 1);
+        if constexpr (I % 2 == 0) {
+            if (kt / 2 == half_pair) {   // no unit there: 2^-127 for whatever lies behind the row's scales
+#pragma unroll
+                for (int i = 0; i < FM; ++i) cur_scales.a[i] = half ? 0u : cur_scales.a[i];
+#pragma unroll
+                for (int j = 0; j < FN; ++j) cur_scales.b[j] = half ? 0u : cur_scales.b[j];
+            }
+        }
         [&]<int... Q>(std::integer_sequence<int, Q...>) {
             ([&] {
                 if constexpr (Q == PRE) {
                     wait_vmcnt_and_barrier<kWaits.step[I]>();
                     __builtin_amdgcn_sched_barrier(0);
                 }
-                mfma_op(std::integral_constant<int, Q>{}, cur);
+                mfma_op(std::integral_constant<int, I % 2>{}, std::integral_constant<int, Q>{}, cur, cur_scales);
                 constexpr int S = Q < PRE ? 0 : (Q - PRE) * PER;
                 constexpr int lo = Q < PRE ? 0 : S < N_MEM ? S : N_MEM;
                 constexpr int hi = Q < PRE ? 0 : S + PER < N_MEM ? S + PER : N_MEM;
@@ -275,7 +292,7 @@ gemm_mx4_kernel(Mx4Args args, int tiles_n, int group_m) {
                         } else {
                             constexpr int loads_before = m / kStride < LOADS ? m / kStride : LOADS;
                             read_op(std::integral_constant<int, I + 1>{},
-                                    std::integral_constant<int, m - loads_before>{}, nxt);
+                                    std::integral_constant<int, m - loads_before>{}, nxt, nxt_scales);
                         }
                     }(), ...);
                 }(std::make_integer_sequence<int, hi - lo>{});
