@@ -62,10 +62,6 @@ constexpr Mx4Waits mx4_schedule(int pair, int chunk) {
     return r;
 }
 
-#ifndef MX4_STRIDE
-#define MX4_STRIDE 2
-#endif
-
 template <int DT, int TILE>
 __global__ void __launch_bounds__(256)
 gemm_mx4_kernel(Mx4Args args, int tiles_n, int group_m) {
@@ -249,10 +245,11 @@ gemm_mx4_kernel(Mx4Args args, int tiles_n, int group_m) {
         constexpr int DATA_LOADS = I % 2 ? 2 * INSTR : 0, LOADS = DATA_LOADS + (I == 7 ? SCALE_INSTR : 0);
         constexpr int N_READS = (I % 2 ? 3 : 2) * (FM + FN), N_MEM = N_READS + LOADS;
         constexpr int PRE = N_MFMA >= 16 ? kPreBarrierMfma : 0;
-        constexpr int PER = (N_MEM + N_MFMA - PRE - 1) / (N_MFMA - PRE);
-        // Loads sit among the reads, as early as every MX4_STRIDE-th memory instruction.
-        constexpr int kStride = LOADS == 0 ? N_MEM + 1 : N_MEM / LOADS < MX4_STRIDE ? N_MEM / LOADS : MX4_STRIDE;
-        constexpr auto kIsLoad = [](int m) { return (m + 1) % kStride == 0 && (m + 1) / kStride <= LOADS; };
+        // The step's memory instructions, spread evenly over the MFMAs behind the barrier, and the loads evenly among
+        // the reads. Two of either behind an MFMA for as long as they lasted took 8192 x 8192 x 16384 to 462 us (this:
+        // 435): an MFMA waited behind the LDS pipe in the first half of a step, and nothing used it in the second.
+        constexpr auto kSlotOf = [](int m) { return PRE + m * (N_MFMA - PRE) / N_MEM; };
+        constexpr auto kLoadsBefore = [](int m) { return m * LOADS / N_MEM; };
         const UnitOps& cur = ops[I % 2];
         UnitOps& nxt = ops[(I + 1) % 2];
         PairScales& cur_scales = scales[I / 2 % 2];
@@ -274,28 +271,24 @@ gemm_mx4_kernel(Mx4Args args, int tiles_n, int group_m) {
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 mfma_op(std::integral_constant<int, I % 2>{}, std::integral_constant<int, Q>{}, cur, cur_scales);
-                constexpr int S = Q < PRE ? 0 : (Q - PRE) * PER;
-                constexpr int lo = Q < PRE ? 0 : S < N_MEM ? S : N_MEM;
-                constexpr int hi = Q < PRE ? 0 : S + PER < N_MEM ? S + PER : N_MEM;
+                constexpr int here = Q;
                 [&]<int... R>(std::integer_sequence<int, R...>) {
                     ([&] {
-                        constexpr int m = lo + R;
-                        if constexpr (kIsLoad(m)) {
-                            constexpr int l = (m + 1) / kStride - 1, at = (I / 2) % 2 * SLOT;
-                            if constexpr (l >= DATA_LOADS) {
-                                issue_scales(chunk, std::integral_constant<int, l - DATA_LOADS>{});
-                            } else if constexpr (l < INSTR) {
-                                issue_x(pair, at, std::integral_constant<int, l>{});
+                        constexpr int m = R;
+                        if constexpr (kSlotOf(m) == here) {
+                            constexpr int l = kLoadsBefore(m), at = (I / 2) % 2 * SLOT;
+                            if constexpr (kLoadsBefore(m + 1) > l) {
+                                if constexpr (l >= DATA_LOADS)
+                                    issue_scales(chunk, std::integral_constant<int, l - DATA_LOADS>{});
+                                else if constexpr (l < INSTR) issue_x(pair, at, std::integral_constant<int, l>{});
+                                else issue_w(pair, at, std::integral_constant<int, l - INSTR>{});
                             } else {
-                                issue_w(pair, at, std::integral_constant<int, l - INSTR>{});
+                                read_op(std::integral_constant<int, I + 1>{}, std::integral_constant<int, m - l>{}, nxt,
+                                        nxt_scales);
                             }
-                        } else {
-                            constexpr int loads_before = m / kStride < LOADS ? m / kStride : LOADS;
-                            read_op(std::integral_constant<int, I + 1>{},
-                                    std::integral_constant<int, m - loads_before>{}, nxt, nxt_scales);
                         }
                     }(), ...);
-                }(std::make_integer_sequence<int, hi - lo>{});
+                }(std::make_integer_sequence<int, N_MEM>{});
                 __builtin_amdgcn_sched_barrier(0);
             }(), ...);
         }(std::make_integer_sequence<int, N_MFMA>{});
