@@ -35,7 +35,7 @@ bool is_config(int64_t v) { return v >= 0 && v <= 4; }
 bool is_splits(int64_t v) { return v >= 1 && v <= 512; }
 bool is_grouped_config(int64_t v) { return v >= 0 && v <= 3; }
 bool is_w4_config(int64_t v) { return v >= 0 && v < kW4ConfigCount; }
-bool is_mx4_config(int64_t v) { return v >= 0 && v <= 3; }
+bool is_mx4_config(int64_t v) { return v >= 0 && v <= 5; }
 bool is_mx4_splits(int64_t v) { return v >= 1 && v <= 16; }
 bool is_mfma(int64_t v) { return v == 16 || v == 32; }
 

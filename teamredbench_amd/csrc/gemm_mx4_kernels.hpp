@@ -11,6 +11,7 @@ namespace mb {
 struct Mx4Plan {
     int config;   // tiles of kMx4Tiles[config]; -1: gemm_mx4_any_kernel
     int splits;   // of K, over fp32 planes in the workspace
+    int cus;      // of the device
 };
 int gemm_mx4_tiled_bf16(const Mx4Call& c, const Mx4Plan& plan, void* workspace, hipStream_t stream);
 int gemm_mx4_tiled_f16(const Mx4Call& c, const Mx4Plan& plan, void* workspace, hipStream_t stream);
@@ -32,54 +33,114 @@ struct Mx4Args {
     bool out_16;                          // out's rows start on 16 bytes
 };
 
-// Ring slots: elements two slots of a pair of units (whole 128-byte lines of every row), scales two slots of 8
-// units (32 bytes of every row).
+// Ring slots: elements two or four slots of a pair of units (whole 128-byte lines of every row), scales two slots of
+// 8 units (32 bytes of every row).
 constexpr int kPairBytes = 128, kChunkUnits = 8, kChunkBytes = 32;
 
-// Loads of step j: pair (j - 1) / 2 + 2 of x and w on odd j, then scale chunk (j - 7) / 8 + 2 where j % 8 == 7,
-// `pair` and `chunk` instructions per wave; the prologue runs the same rule over the steps before 0. Step j reads
-// unit j + 1, so its wait leaves only the loads issued after that unit's. By j % 8, the least of all steps.
+// Loads of step j: pair (j - 1) / 2 + slots of x and w on odd j, then scale chunk (j - 7) / 8 + 2 where j % 8 == 7,
+// `pair` and `chunk` instructions per wave. Before step 0: chunk 0, pairs 0 .. slots - 1, chunk 1. Step j reads unit j + 1,
+// so its wait leaves only what was issued after that unit's loads (a wave's vector memory operations complete in the
+// order of their issue). By j % 8, the least of all steps.
+//
+// A tile whose block stored the one before with `groups` of `pieces` stores has them among its first loads: group g's
+// go out behind the loads of group g + 1, those of the first kLoadGroups. `behind_prologue` and `behind` are the waits
+// of the prologue and of the first three steps then.
+constexpr int kLoadGroups = 4;
 struct Mx4Waits {
-    int step[kChunkUnits], prologue;
+    int step[kChunkUnits], prologue, behind_prologue, behind[3];
 };
-constexpr Mx4Waits mx4_schedule(int pair, int chunk) {
-    constexpr int kSteps = 64, kFirst = -(kChunkUnits + 1);
+constexpr Mx4Waits mx4_schedule(int slots, int pair, int chunk, int groups, int pieces) {
+    constexpr int kSteps = 64;
     int pair_end[kSteps] = {}, chunk_end[kSteps] = {}, before[kSteps] = {};
-    int total = 0;
-    for (int v = kFirst; v < kSteps; ++v) {
-        if (v >= 0) before[v] = total;
-        if ((v & 1) != 0 && (v - 1) / 2 + 2 >= 0 && (v - 1) / 2 + 2 < kSteps) pair_end[(v - 1) / 2 + 2] = (total += pair);
-        if ((v & 7) == 7) chunk_end[(v + 1) / kChunkUnits + 1] = (total += chunk);
-    }
     Mx4Waits r{};
-    r.prologue = before[0] - (pair_end[0] > chunk_end[0] ? pair_end[0] : chunk_end[0]);
-    for (int i = 0; i < kChunkUnits; ++i) r.step[i] = 63;
-    for (int j = 0; j + 1 < kSteps; ++j) {
-        const int p = pair_end[(j + 1) / 2], c = chunk_end[(j + 1) / kChunkUnits];
-        const int wait = before[j] - (p > c ? p : c);
-        if (wait < r.step[j % kChunkUnits]) r.step[j % kChunkUnits] = wait;
+    for (int stores = 0; stores < 2; ++stores) {
+        int total = 0;
+        const int first = chunk + slots * pair;   // chunk 0, pair 0, pair 1 ...
+        chunk_end[0] = chunk;
+        for (int p = 0; p < slots; ++p) pair_end[p] = chunk + (p + 1) * pair;
+        if (stores) {
+            for (int g = 0; g < groups; ++g) {
+                for (int l = 0; g < kLoadGroups && l < first; ++l) {
+                    if (l * kLoadGroups / first != g) continue;
+                    ++total;
+                    for (int p = 0; p < slots; ++p)
+                        if (l + 1 == chunk + (p + 1) * pair) pair_end[p] = total;
+                }
+                if (g > 0) total += pieces;
+            }
+            total += pieces;
+        } else {
+            total = first;
+        }
+        chunk_end[1] = (total += chunk);
+        (stores ? r.behind_prologue : r.prologue) = total - pair_end[0];
+        for (int j = 0; j < kSteps; ++j) {
+            before[j] = total;
+            if ((j & 1) != 0) pair_end[(j - 1) / 2 + slots] = (total += pair);
+            if ((j & 7) == 7) chunk_end[(j + 1) / kChunkUnits + 1] = (total += chunk);
+        }
+        for (int i = 0; !stores && i < kChunkUnits; ++i) r.step[i] = 63;
+        for (int j = 0; j + 1 < kSteps; ++j) {
+            const int p = pair_end[(j + 1) / 2], c = chunk_end[(j + 1) / kChunkUnits];
+            const int wait = before[j] - (p > c ? p : c);
+            if (stores && j < 3) r.behind[j] = wait;   // these three need nothing that the steps loaded
+            if (!stores && wait < r.step[j % kChunkUnits]) r.step[j % kChunkUnits] = wait;
+        }
     }
     return r;
 }
 
+// Row tile and column of tile t: as in block_coords, in groups of kGroupM row tiles (without K splits, whose blocks
+// take block_coords), dividing by a multiplication: `magic` is 2^40 / (kGroupM tiles_n), rounded up.
+constexpr int kGroupM = 4;
+__device__ __forceinline__ void tile_coords(int b, int tiles, int tiles_m, int tiles_n, uint64_t magic, int* tm,
+                                            int* tn) {
+    const int t = (b & 7) * (tiles >> 3) + min(b & 7, tiles & 7) + (b >> 3);
+    const int per_group = kGroupM * tiles_n;
+    int g = (int)(((uint64_t)(unsigned)t * magic) >> 40);
+    if ((int64_t)g * per_group > t) --g;
+    const int first_m = g * kGroupM, rows = min(tiles_m - first_m, kGroupM), r = t - g * per_group;
+    const int column = rows == kGroupM ? r / kGroupM : rows == 3 ? r / 3 : r >> (rows - 1);
+    *tm = first_m + r - column * rows;
+    *tn = column;
+}
+
+// An accumulator's value, from where the matrix instructions keep it: left to itself the compiler copies all 256
+// into vector registers at once, and spills. The caller keeps the wait states behind the last matrix instruction.
+__device__ __forceinline__ float read_acc(float v) {
+    float f;
+    asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(f) : "a"(v));
+    return f;
+}
+
 template <int DT, int TILE>
 __global__ void __launch_bounds__(256)
-gemm_mx4_kernel(Mx4Args args, int tiles_n, int group_m) {
+gemm_mx4_kernel(Mx4Args all_args, int tiles_n, uint64_t magic) {
     constexpr int BM = TILE, BN = TILE;
     constexpr int WTM = BM / 2, WTN = BN / 2;
     constexpr int FM = WTM / 32, FN = WTN / 32;
     constexpr int SLOT = TILE * kPairBytes, SCALE_SLOT = TILE * kChunkBytes;   // one operand's
-    constexpr int W0 = 2 * SLOT;                          // x's elements, w's, x's scales, w's: two slots each
-    constexpr int XS0 = 4 * SLOT, WS0 = XS0 + 2 * SCALE_SLOT;
-    constexpr int LDS_BYTES = WS0 + 2 * SCALE_SLOT;
-    constexpr int INSTR = SLOT / 1024 / 4;                // DMA instructions per wave, operand and pair
+    // LDS: x's elements, w's (SLOTS slots each); slot 0 of x's scales and of w's, slot 1 of both.
+    constexpr int SLOTS = TILE == 64 ? 4 : 2;
+    constexpr int W0 = SLOTS * SLOT, XS0 = 2 * SLOTS * SLOT, WS0 = XS0 + SCALE_SLOT, NEXT_SCALES = 2 * SCALE_SLOT;
+    constexpr int LDS_BYTES = XS0 + 2 * NEXT_SCALES;
+    constexpr int INSTR = SLOT / 1024 / 4;                   // DMA instructions per wave, operand and pair
     constexpr int SCALE_INSTR = 2 * SCALE_SLOT / 1024 / 4;   // ... per wave and chunk, both operands
     static_assert(LDS_BYTES <= 160 * 1024 && SLOT % 4096 == 0 && SCALE_INSTR >= 1, "LDS rings");
-    constexpr Mx4Waits kWaits = mx4_schedule(2 * INSTR, SCALE_INSTR);
+    // Stores: groups of 32 rows and up to 64 columns of a wave's tile go through LDS and out as whole lines. A
+    // persistent block (one per CU) stages them in the second scale slot, while the next tile's loads fill the rest.
+    constexpr bool PERSISTENT = TILE == 256;
+    constexpr int GC = WTN < 64 ? WTN : 64, STAGE = 32 * GC * 2, PIECES = STAGE / 1024;
+    constexpr int STAGE0 = PERSISTENT ? XS0 + NEXT_SCALES : 0;
+    constexpr int GROUPS = FM * (WTN / GC);                  // of a wave's tile
+    static_assert(!PERSISTENT || 4 * STAGE <= NEXT_SCALES, "the staged groups fit the second scale slot");
+    constexpr Mx4Waits kWaits = mx4_schedule(SLOTS, 2 * INSTR, SCALE_INSTR, GROUPS, PIECES);
     static_assert([&] {
         for (int w : kWaits.step)
-            if (w < 0) return false;
-        return kWaits.prologue >= 0 && kWaits.prologue < 64;
+            if (w < 0 || w >= 64) return false;
+        for (int w : kWaits.behind)
+            if (PERSISTENT && (w < 0 || w >= 64)) return false;
+        return kWaits.prologue >= 0 && kWaits.prologue < 64 && (!PERSISTENT || kWaits.behind_prologue < 64);
     }(), "a needed unit is unissued, or vmcnt overflows");
     __shared__ __attribute__((aligned(1024))) unsigned char lds[LDS_BYTES];
 
@@ -89,88 +150,189 @@ gemm_mx4_kernel(Mx4Args args, int tiles_n, int group_m) {
     const int wm = wave >> 1, wn = wave & 1;
     const int half = lane >> 5, r32 = lane & 31;
 
-    ExpertRows ex{0, 0, args.total};
-    const int block = (int)block_number();
-    int tm, tn, split;
-    const bool by_expert = args.offsets != nullptr;
-    const int tiles_m = by_expert ? count_row_tiles(args.offsets, args.experts, args.total, BM)
-                                  : (args.total + BM - 1) / BM;
-    if (block >= tiles_m * tiles_n * args.splits) return;
-    block_coords(block, tiles_m, tiles_n, args.splits, group_m, &tm, &tn, &split);
-    if (by_expert && !find_row_tile(args.offsets, args.experts, args.total, tm, BM, &ex, &tm)) return;
-    const int M = ex.count, m0 = tm * BM, n0 = tn * BN;
-    // Units of K of this block, in whole pairs: the second unit of a last pair that has but one is zeros.
-    const int u0 = split * args.split_units, k_units = min(args.units - u0, args.split_units);
-    const int ksteps = (k_units + 1) & ~1, half_pair = k_units & 1 ? k_units / 2 : -1;
-
-    // Buffer resources over the tile's rows (gathered: all of x): rows and units past them read as zeros.
-    const bool gather = args.rows != nullptr;
-    const int64_t x_first = gather ? 0 : (int64_t)ex.first + m0;
-    const int64_t w_first = (int64_t)ex.expert * args.N + n0;
-    const int x_count = gather ? args.x_rows : min(M - m0, BM), w_count = min(args.N - n0, BN);
-    auto resource = [](const unsigned char* p, int64_t first, int ld, int count) {
-        return __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p) + first * ld, (short)0, count * ld,
-                                                 kBufferFlags);
+    // The arguments, read again for each tile: kept in registers they would crowd the K loop's out.
+    auto arguments = [&]() -> Mx4Args {
+#if defined(__HIP_DEVICE_COMPILE__)
+        if constexpr (PERSISTENT) {
+            auto p = (const __attribute__((address_space(4))) Mx4Args*)__builtin_amdgcn_kernarg_segment_ptr();
+            asm volatile("" : "+s"(p));
+            return *p;
+        }
+#endif
+        return all_args;
     };
-    const __amdgpu_buffer_rsrc_t rx = resource(args.x, x_first, args.ld, x_count);
-    const __amdgpu_buffer_rsrc_t rw = resource(args.w, w_first, args.ld, w_count);
 
-    auto x_row = [&](int r) {
-        if (m0 + r >= M) return -1;
-        if (!gather) return r;
-        const int listed = args.rows[ex.first + m0 + r];
-        return listed < args.x_rows ? listed : -1;
+    struct Tile {
+        ExpertRows ex;
+        int m0, n0, split;
     };
-    auto w_row = [&](int r) { return n0 + r < args.N ? r : -1; };
-
-    // This lane's byte offsets of its 16-byte pieces: an instruction fills 8 rows of a pair, or the scales of 32
-    // rows. Waves 0 and 1 load x's scales, 2 and 3 w's.
-    int x_off[INSTR], w_off[INSTR], s_off[SCALE_INSTR];
-    bool x_second[2];   // the piece lies in its pair's second unit (the swizzle repeats every 16 rows)
-#pragma unroll
-    for (int q = 0; q < INSTR; ++q) {
-        const int r = (wave * INSTR + q) * 8 + (lane >> 3);
-        const int byte = ((lane & 7) ^ swz_a2(r)) << 4;
-        const int xr = x_row(r), wr = w_row(r);
-        if (q < 2) x_second[q] = byte >= kMx4UnitBytes;
-        x_off[q] = xr < 0 ? kNowhere : xr * args.ld + byte;
-        w_off[q] = wr < 0 ? kNowhere : wr * args.ld + byte;
+    int tm, tn, tiles_before = 0;   // row tiles before the tile's expert
+    int t = (int)block_number(), tiles, tiles_m;
+    const int stride = (int)(gridDim.x * gridDim.y);   // tiles of this block: t, t + stride ...
+    Tile cur{{0, 0, 0}, 0, 0, 0};
+    {
+        const Mx4Args args = arguments();
+        const bool by_expert = args.offsets != nullptr;
+        tiles_m = by_expert ? count_row_tiles(args.offsets, args.experts, args.total, BM)
+                            : (args.total + BM - 1) / BM;
+        tiles = tiles_m * tiles_n * args.splits;
+        if (t >= tiles) return;
+        if (PERSISTENT) tile_coords(t, tiles, tiles_m, tiles_n, magic, &tm, &tn);
+        else block_coords(t, tiles_m, tiles_n, args.splits, kGroupM, &tm, &tn, &cur.split);
+        cur.ex.count = args.total;
+        if (by_expert) {
+            int in_expert;
+            if (!find_row_tile(args.offsets, args.experts, args.total, tm, BM, &cur.ex, &in_expert)) return;
+            tiles_before = tm - in_expert;
+        }
+        cur.m0 = (tm - tiles_before) * BM;
+        cur.n0 = tn * BN;
     }
+    // Another tile: its expert is near the last one's. Scalar loads, which the vmcnt waits do not see.
+    const bool by_expert = all_args.offsets != nullptr;
+    auto locate = [&](Tile& tile) {
+        tile_coords(t + stride, tiles, tiles_m, tiles_n, magic, &tm, &tn);
+        if (by_expert) {
+            const Mx4Args args = arguments();
+            typedef const __attribute__((address_space(4))) int32_t* ConstRows;
+            const ConstRows list = (ConstRows)(uintptr_t)args.offsets;
+            auto rows_of = [&](int i) {
+                const int lo = min(max(list[i], 0), args.total), hi = min(max(list[i + 1], 0), args.total);
+                return ExpertRows{i, lo, max(hi - lo, 0)};
+            };
+            int e = __builtin_amdgcn_readfirstlane(tile.ex.expert);
+            ExpertRows ex = rows_of(e);
+            while (tm < tiles_before && e > 0) {
+                ex = rows_of(--e);
+                tiles_before -= (ex.count + BM - 1) / BM;
+            }
+            while (tm >= tiles_before + (ex.count + BM - 1) / BM && e + 1 < args.experts) {
+                tiles_before += (ex.count + BM - 1) / BM;
+                ex = rows_of(++e);
+            }
+            tile.ex = ex;
+        }
+        tile.m0 = __builtin_amdgcn_readfirstlane((tm - tiles_before) * BM);
+        tile.n0 = __builtin_amdgcn_readfirstlane(tn * BN);
+    };
+
+    // The rows of x that this lane's loads go through (-1: none): of the wave's quarter of the tile, and of the half
+    // whose scales it loads (waves 0 and 1 load x's scales, 2 and 3 w's).
     const bool scales_of_x = wave < 2;
+    constexpr int WAVE_ROWS = BM / 4, SCALE_ROWS = BM / 2;
+    struct XRows {
+        int data, scales[2];
+    };
+    auto x_rows = [&](const Mx4Args& args, const Tile& tile) {
+        auto row = [&](int r) {
+            if (tile.m0 + r >= tile.ex.count) return -1;
+            return args.rows != nullptr ? args.rows[tile.ex.first + tile.m0 + r] : r;
+        };
+        XRows x{row(wave * WAVE_ROWS + lane % WAVE_ROWS), {-1, -1}};
+        if (scales_of_x) {
+            x.scales[0] = row(wave * SCALE_ROWS + lane % SCALE_ROWS);
+            if constexpr (SCALE_ROWS > 64) x.scales[1] = row(wave * SCALE_ROWS + 64 + lane);
+        }
+        return x;
+    };
+
+    // A tile's loads: buffer resources over its rows (gathered: all of x), past which rows and units read as zeros,
+    // and this lane's byte offsets of its 16-byte pieces. An instruction fills 8 rows of a pair, or the scales of 32.
+    struct Loads {
+        __amdgpu_buffer_rsrc_t x, w, scales;
+        int x_off[INSTR], w_off[2], s_off[SCALE_INSTR];
+        int ld16, at, scales_at;               // 16 rows of w; bytes to the first unit of K
+        int ksteps, k_bytes, half_pair;        // units of K, in whole pairs; the pair whose second unit is not there
+    };
+    int k_byte[2];   // of this lane's pieces within their pair (the swizzle repeats every 16 rows)
 #pragma unroll
-    for (int q = 0; q < SCALE_INSTR; ++q) {
-        const int r = ((wave & 1) * SCALE_INSTR + q) * 32 + (lane >> 1);
-        const int row = scales_of_x ? x_row(r) : w_row(r);
-        s_off[q] = row < 0 ? kNowhere : row * args.lds + (((lane & 1) ^ ((r >> 3) & 1)) << 4);
+    for (int q = 0; q < 2; ++q) k_byte[q] = ((lane & 7) ^ swz_a2(q * 8 + (lane >> 3))) << 4;
+    auto loads_of = [&](const Mx4Args& args, const Tile& tile, const XRows& rows) {
+        auto resource = [](const unsigned char* p, int64_t first, int ld, int count) {
+            const uint64_t at = (uint64_t)(uintptr_t)p + first * ld;   // the same in every lane, and held so
+            const uint64_t lo = (unsigned)__builtin_amdgcn_readfirstlane((int)at);
+            const uint64_t hi = (unsigned)__builtin_amdgcn_readfirstlane((int)(at >> 32));
+            return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(hi << 32 | lo), (short)0,
+                                                     __builtin_amdgcn_readfirstlane(count * ld), kBufferFlags);
+        };
+        const bool gather = args.rows != nullptr;
+        const int64_t x_first = gather ? 0 : (int64_t)tile.ex.first + tile.m0;
+        const int64_t w_first = (int64_t)tile.ex.expert * args.N + tile.n0;
+        const int x_count = gather ? args.x_rows : min(tile.ex.count - tile.m0, BM);
+        const int w_count = min(args.N - tile.n0, BN);
+        Loads l;
+        l.x = resource(args.x, x_first, args.ld, x_count);
+        l.w = resource(args.w, w_first, args.ld, w_count);
+        l.scales = resource(scales_of_x ? args.xs : args.ws, scales_of_x ? x_first : w_first, args.lds,
+                            scales_of_x ? x_count : w_count);
+#pragma unroll
+        for (int q = 0; q < INSTR; ++q) {
+            const int r = q * 8 + (lane >> 3), row = __shfl(rows.data, r);
+            l.x_off[q] = row < 0 || row >= x_count ? kNowhere : row * args.ld + k_byte[q & 1];
+            if (q < 2) l.w_off[q] = (wave * WAVE_ROWS + r) * args.ld + k_byte[q];
+        }
+#pragma unroll
+        for (int q = 0; q < SCALE_INSTR; ++q) {
+            const int r = q * 32 + (lane >> 1), byte = ((lane & 1) ^ ((r >> 3) & 1)) << 4;
+            const int listed = __shfl(rows.scales[q / 2], r % 64);
+            const int row = scales_of_x ? (listed < x_count ? listed : -1) : (wave & 1) * SCALE_ROWS + r;
+            l.s_off[q] = row < 0 ? kNowhere : row * args.lds + byte;
+        }
+        const int u0 = tile.split * args.split_units, units = min(args.units - u0, args.split_units);
+        l.ld16 = 16 * args.ld;
+        l.at = u0 * kMx4UnitBytes;
+        l.scales_at = u0 * kMx4UnitScales;
+        l.ksteps = (units + 1) & ~1;
+        l.k_bytes = units * kMx4UnitBytes;
+        l.half_pair = units & 1 ? units / 2 : -1;
+        return l;
+    };
+    XRows rows;
+    Loads from;
+    {
+        const Mx4Args args = arguments();
+        rows = x_rows(args, cur);
+        from = loads_of(args, cur, rows);
     }
-    const __amdgpu_buffer_rsrc_t rs = scales_of_x ? resource(args.xs, x_first, args.lds, x_count)
-                                                  : resource(args.ws, w_first, args.lds, w_count);
 
     const unsigned lds0 = (unsigned)(uintptr_t)(MB_LDS unsigned char*)lds;
+    // Pieces past the end of K are zeros, and not fetched.
     auto issue_x = [&](int pair, int at, auto idx) {
         constexpr int q = decltype(idx)::value;
-        const int off = pair == half_pair && x_second[q & 1] ? kNowhere : x_off[q];
-        lds_dma16(rx, lds0 + at + (wave * INSTR + q) * 1024, off, u0 * kMx4UnitBytes + pair * kPairBytes);
+        const int off = k_byte[q & 1] < from.k_bytes - pair * kPairBytes ? from.x_off[q] : kNowhere;
+        lds_dma16(from.x, lds0 + at + (wave * INSTR + q) * 1024, off, from.at + pair * kPairBytes);
     };
     auto issue_w = [&](int pair, int at, auto idx) {
         constexpr int q = decltype(idx)::value;
-        lds_dma16(rw, lds0 + W0 + at + (wave * INSTR + q) * 1024, w_off[q], u0 * kMx4UnitBytes + pair * kPairBytes);
+        const int off = k_byte[q & 1] < from.k_bytes - pair * kPairBytes ? from.w_off[q & 1] : kNowhere;
+        lds_dma16(from.w, lds0 + W0 + at + (wave * INSTR + q) * 1024, off,
+                  from.at + pair * kPairBytes + (q >> 1) * from.ld16);
     };
     auto issue_scales = [&](int chunk, auto idx) {
         constexpr int q = decltype(idx)::value;
-        const unsigned to = lds0 + (scales_of_x ? XS0 : WS0) + (chunk & 1) * SCALE_SLOT;
-        lds_dma16(rs, to + ((wave & 1) * SCALE_INSTR + q) * 1024, s_off[q],
-                  u0 * kMx4UnitScales + chunk * kChunkBytes);
+        const unsigned to = lds0 + (scales_of_x ? XS0 : WS0) + (chunk & 1) * NEXT_SCALES;
+        lds_dma16(from.scales, to + ((wave & 1) * SCALE_INSTR + q) * 1024, from.s_off[q],
+                  from.scales_at + chunk * kChunkBytes);
     };
+    auto all = [&](auto count, auto&& f) {
+        [&]<int... Q>(std::integer_sequence<int, Q...>) {
+            (f(std::integral_constant<int, Q>{}), ...);
+        }(std::make_integer_sequence<int, decltype(count)::value>{});
+    };
+    // Load l of a tile's first: scale chunk 0, a pair for every slot.
+    constexpr int FIRST_LOADS = SCALE_INSTR + 2 * SLOTS * INSTR;
+    auto first_load = [&](auto idx) {
+        constexpr int l = decltype(idx)::value, d = l - SCALE_INSTR;
+        if constexpr (d < 0) issue_scales(0, idx);
+        else if constexpr (d / INSTR % 2 == 0) issue_x(d / INSTR / 2, d / INSTR / 2 * SLOT, std::integral_constant<int, d % INSTR>{});
+        else issue_w(d / INSTR / 2, d / INSTR / 2 * SLOT, std::integral_constant<int, d % INSTR>{});
+    };
+    constexpr std::integral_constant<int, FIRST_LOADS> kFirstLoads{};
+    constexpr std::integral_constant<int, SCALE_INSTR> kScalePieces{};
+    // Chunk 1, where a persistent block's stores are staged. Past the row's end: zeros or other scales, unused.
+    auto second_chunk = [&] { all(kScalePieces, [&](auto q) { issue_scales(1, q); }); };
 
     f32x16 acc[FM][FN];
-#pragma unroll
-    for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-
     // Operands of a unit: two substeps of 64 k. Of the 8 blocks of a pair, lane half h takes 4h .. 4h + 3, two a
     // unit, so one dword brings its scales of a pair, a byte for each MFMA.
     struct UnitOps {
@@ -186,7 +348,7 @@ gemm_mx4_kernel(Mx4Args args, int tiles_n, int group_m) {
     auto scales_at = [&](int row, int unit) {   // 16 bytes hold 4 units; unit: the even one of the pair, modulo 8
         return row * kChunkBytes + (((unit >> 2) ^ ((row >> 3) & 1)) << 4) + 4 * (unit & 2) + 4 * half;
     };
-    int slot_flip = 0;   // SCALE_SLOT while the current chunk's number is odd
+    int slot_flip = 0;   // byte offset of the current chunk's slot
     // Read number r of unit u (its number modulo 8, 8 for the next chunk's first), in the order the MFMAs consume
     // operands: x fragment 0, w's, x's others; a pair's first unit brings the pair's scales too.
     auto read_op = [&](auto unit, auto idx, UnitOps& o, PairScales& s) {
@@ -195,12 +357,12 @@ gemm_mx4_kernel(Mx4Args args, int tiles_n, int group_m) {
         constexpr int t = r < FIRST ? 0 : 1;
         constexpr int f = t == 1 ? r - FIRST : u % 2 ? r : r / 2;
         constexpr bool scales = u % 2 == 0 && t == 0 && r % 2 == 1;
-        constexpr int at = (u / 2) % 2 * SLOT, chunk = 2 * (u % 2) + t;
+        constexpr int at = (u / 2) % SLOTS * SLOT, chunk = 2 * (u % 2) + t;
         constexpr bool is_w = f >= 1 && f <= FN;
         constexpr int frag = is_w ? f - 1 : f == 0 ? 0 : f - FN;
         const int row = (is_w ? w_lane : x_lane) + 32 * frag;
         if constexpr (scales) {
-            const int flip = u == kChunkUnits ? slot_flip ^ SCALE_SLOT : slot_flip;
+            const int flip = u == kChunkUnits ? slot_flip ^ NEXT_SCALES : slot_flip;
             const unsigned v =
                 *reinterpret_cast<const unsigned*>(lds + (is_w ? WS0 : XS0) + flip + scales_at(row, u % kChunkUnits));
             if constexpr (is_w) s.b[frag] = v;
@@ -219,27 +381,9 @@ gemm_mx4_kernel(Mx4Args args, int tiles_n, int group_m) {
         acc[i][j] = mfma_mx4<byte, byte>(o.b[t][j], s.b[j], o.a[t][i], s.a[i], acc[i][j]);
     };
 
-    const int last_pair = (ksteps - 1) / 2, last_chunk = (ksteps - 1) / kChunkUnits;
-    auto all = [&](auto count, auto&& f) {
-        [&]<int... Q>(std::integer_sequence<int, Q...>) {
-            (f(std::integral_constant<int, Q>{}), ...);
-        }(std::make_integer_sequence<int, decltype(count)::value>{});
-    };
-    constexpr std::integral_constant<int, INSTR> kPieces{};
-    constexpr std::integral_constant<int, SCALE_INSTR> kScalePieces{};
-    all(kScalePieces, [&](auto q) { issue_scales(0, q); });
-    all(kPieces, [&](auto q) { issue_x(0, 0, q); });
-    all(kPieces, [&](auto q) { issue_w(0, 0, q); });
-    all(kPieces, [&](auto q) { issue_x(min(1, last_pair), SLOT, q); });
-    all(kPieces, [&](auto q) { issue_w(min(1, last_pair), SLOT, q); });
-    all(kScalePieces, [&](auto q) { issue_scales(1, q); });   // past the row's end: zeros or other scales, unused
-
     UnitOps ops[2];
-    wait_vmcnt_and_barrier<kWaits.prologue>();
     PairScales scales[2];
-    all(std::integral_constant<int, 3 * (FM + FN)>{},
-        [&](auto r) { read_op(std::integral_constant<int, 0>{}, r, ops[0], scales[0]); });
-
+    bool behind_stores = false;   // the first loads went out among the stores of a whole tile
     auto step = [&](auto idx, int kt) {
         constexpr int I = decltype(idx)::value;               // kt % 8
         constexpr int DATA_LOADS = I % 2 ? 2 * INSTR : 0, LOADS = DATA_LOADS + (I == 7 ? SCALE_INSTR : 0);
@@ -250,14 +394,14 @@ gemm_mx4_kernel(Mx4Args args, int tiles_n, int group_m) {
         // 435): an MFMA waited behind the LDS pipe in the first half of a step, and nothing used it in the second.
         constexpr auto kSlotOf = [](int m) { return PRE + m * (N_MFMA - PRE) / N_MEM; };
         constexpr auto kLoadsBefore = [](int m) { return m * LOADS / N_MEM; };
-        const UnitOps& cur = ops[I % 2];
+        const UnitOps& cur_ops = ops[I % 2];
         UnitOps& nxt = ops[(I + 1) % 2];
         PairScales& cur_scales = scales[I / 2 % 2];
         PairScales& nxt_scales = scales[(I + 1) / 2 % 2];
-        const int pair = min((kt - 1) / 2 + 2, last_pair);    // into the slot of the pair that unit kt ends
-        const int chunk = min((kt - 7) / kChunkUnits + 2, last_chunk + 1);
+        const int pair = (kt - 1) / 2 + SLOTS;                // into the slot of the pair that unit kt ends
+        const int chunk = (kt - 7) / kChunkUnits + 2;         // past the row's end: zeros or other scales, unused
         if constexpr (I % 2 == 0) {
-            if (kt / 2 == half_pair) {   // no unit there: 2^-127 for whatever lies behind the row's scales
+            if (kt / 2 == from.half_pair) {   // no unit there: 2^-127 for whatever lies behind the row's scales
 #pragma unroll
                 for (int i = 0; i < FM; ++i) cur_scales.a[i] = half ? 0u : cur_scales.a[i];
 #pragma unroll
@@ -267,16 +411,21 @@ gemm_mx4_kernel(Mx4Args args, int tiles_n, int group_m) {
         [&]<int... Q>(std::integer_sequence<int, Q...>) {
             ([&] {
                 if constexpr (Q == PRE) {
-                    wait_vmcnt_and_barrier<kWaits.step[I]>();
+                    if constexpr (I < 3 && PERSISTENT) {
+                        if (behind_stores && kt == I) wait_vmcnt_and_barrier<kWaits.behind[I < 3 ? I : 0]>();
+                        else wait_vmcnt_and_barrier<kWaits.step[I]>();
+                    } else {
+                        wait_vmcnt_and_barrier<kWaits.step[I]>();
+                    }
                     __builtin_amdgcn_sched_barrier(0);
                 }
-                mfma_op(std::integral_constant<int, I % 2>{}, std::integral_constant<int, Q>{}, cur, cur_scales);
+                mfma_op(std::integral_constant<int, I % 2>{}, std::integral_constant<int, Q>{}, cur_ops, cur_scales);
                 constexpr int here = Q;
                 [&]<int... R>(std::integer_sequence<int, R...>) {
                     ([&] {
                         constexpr int m = R;
                         if constexpr (kSlotOf(m) == here) {
-                            constexpr int l = kLoadsBefore(m), at = (I / 2) % 2 * SLOT;
+                            constexpr int l = kLoadsBefore(m), at = (I / 2) % SLOTS * SLOT;
                             if constexpr (kLoadsBefore(m + 1) > l) {
                                 if constexpr (l >= DATA_LOADS)
                                     issue_scales(chunk, std::integral_constant<int, l - DATA_LOADS>{});
@@ -293,27 +442,51 @@ gemm_mx4_kernel(Mx4Args args, int tiles_n, int group_m) {
             }(), ...);
         }(std::make_integer_sequence<int, N_MFMA>{});
     };
-    for (int kt = 0; kt < ksteps; kt += kChunkUnits) {
-        [&]<int... I>(std::integer_sequence<int, I...>) {
-            ((kt + I < ksteps ? step(std::integral_constant<int, I>{}, kt + I) : void()), ...);
-        }(std::make_integer_sequence<int, kChunkUnits>{});
-        slot_flip ^= SCALE_SLOT;
-    }
-    wait_vmcnt_and_barrier<0>();
 
-    // Register 4g + q of lane l holds out(32i + l % 32, 32j + 8g + 4 (l / 32) + q).
-    if constexpr (BM < 256) {
-        if (args.planes != nullptr) {
-            float* part = args.planes + ((int64_t)split * args.total + ex.first) * args.ldp;
+    all(kFirstLoads, first_load);
+    second_chunk();
+    while (true) {
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+        if (PERSISTENT && behind_stores) wait_vmcnt_and_barrier<PERSISTENT ? kWaits.behind_prologue : 0>();
+        else wait_vmcnt_and_barrier<kWaits.prologue>();
+        all(std::integral_constant<int, 3 * (FM + FN)>{},
+            [&](auto r) { read_op(std::integral_constant<int, 0>{}, r, ops[0], scales[0]); });
+        Tile next = cur;
+        const bool more = PERSISTENT && t + stride < tiles;
+        for (int kt = 0; kt < from.ksteps; kt += kChunkUnits) {
+            if (more && kt + kChunkUnits >= from.ksteps) {   // the next tile's rows arrive during the last steps
+                locate(next);
+                rows = x_rows(arguments(), next);
+            }
+            [&]<int... I>(std::integer_sequence<int, I...>) {
+                ((kt + I < from.ksteps ? step(std::integral_constant<int, I>{}, kt + I) : void()), ...);
+            }(std::make_integer_sequence<int, kChunkUnits>{});
+            slot_flip ^= NEXT_SCALES;
+        }
+        wait_vmcnt_and_barrier<0>();
+        asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");   // what the last MFMAs wrote is read behind these
+        slot_flip = 0;
+        const Mx4Args args = arguments();
+        if (more) from = loads_of(args, next, rows);   // the next tile's first loads run while this one is stored
+
+        // Register 4g + q of lane l holds out(32i + l % 32, 32j + 8g + 4 (l / 32) + q).
+        const int M = cur.ex.count;
+        if (!PERSISTENT && args.planes != nullptr) {
+            float* part = args.planes + ((int64_t)cur.split * args.total + cur.ex.first) * args.ldp;
 #pragma unroll
             for (int i = 0; i < FM; ++i) {
-                const int m = m0 + wm * WTM + 32 * i + r32;
+                const int m = cur.m0 + wm * WTM + 32 * i + r32;
                 if (m >= M) continue;
 #pragma unroll
                 for (int j = 0; j < FN; ++j)
 #pragma unroll
                     for (int g = 0; g < 4; ++g) {
-                        const int n = n0 + wn * WTN + 32 * j + 8 * g + 4 * half;   // ldp is a multiple of 4
+                        const int n = cur.n0 + wn * WTN + 32 * j + 8 * g + 4 * half;   // ldp is a multiple of 4
                         const f32x16& v = acc[i][j];
                         if (n < args.ldp)
                             *reinterpret_cast<f32x4*>(part + m * (int64_t)args.ldp + n) =
@@ -322,59 +495,103 @@ gemm_mx4_kernel(Mx4Args args, int tiles_n, int group_m) {
             }
             return;
         }
-    }
-
-    // 16-bit rows through LDS, stored as whole row segments.
-    unsigned char* ob = args.out + (int64_t)ex.first * args.ldo;
-    constexpr int ROW_BYTES = WTN * 2, ROW_CHUNKS = ROW_BYTES / 16;
-    static_assert(4 * WTM * ROW_BYTES <= LDS_BYTES, "the waves' tiles must fit the LDS rings");
-    unsigned char* stage = lds + wave * WTM * ROW_BYTES;
-    constexpr int GROUP = WTM >= 128 ? 32 : WTM;   // rows per staged group
-    constexpr int ROWS_PER_STORE = 64 / ROW_CHUNKS;
-    constexpr int STORES = GROUP / ROWS_PER_STORE;
-    constexpr int BATCH = STORES < 8 ? STORES : 8;
-    const int oc = lane % ROW_CHUNKS, orow = lane / ROW_CHUNKS;
-    const int col = n0 + wn * WTN + 8 * oc, left = args.N - col;
+        // Group by group through LDS. A wave's LDS accesses take effect in their order, so a group's reads need no wait
+        // behind its writes, nor the next group's writes behind those reads.
+        const bool whole = args.out_16 && cur.m0 + BM <= M && cur.n0 + BN <= args.N;
+        constexpr int CHUNKS = GC / 8, ROWS = 64 / CHUNKS;   // rows per store
+        unsigned char* stage = lds + STAGE0 + wave * STAGE;
+        const int oc = lane % CHUNKS, orow = lane / CHUNKS;
+        const int m0 = cur.m0 + wm * WTM + orow, n0 = cur.n0 + wn * WTN + 8 * oc;
+        unsigned char* to = args.out + (int64_t)(cur.ex.first + m0) * args.ldo + (int64_t)n0 * 2;
+        const int64_t row_step = ROWS * args.ldo;
+        auto write_group = [&](auto idx) {
+            constexpr int i = decltype(idx)::value / (WTN / GC), j0 = decltype(idx)::value % (WTN / GC) * (GC / 32);
+            asm volatile("" ::: "memory");
 #pragma unroll
-    for (int grp = 0; grp < WTM / GROUP; ++grp) {
-#pragma unroll
-        for (int i = grp * (GROUP / 32); i < (grp + 1) * (GROUP / 32); ++i) {
-            const int r = 32 * i + r32;
-#pragma unroll
-            for (int j = 0; j < FN; ++j)
+            for (int j = j0; j < j0 + GC / 32; ++j)
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    const f32x16& v = acc[i][j];
-                    const int chunk = (4 * j + g) ^ (r % ROW_CHUNKS);
-                    *reinterpret_cast<u32x2*>(stage + r * ROW_BYTES + chunk * 16 + 8 * half) =
-                        pack4<DT>(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
+                    float v[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = read_acc(acc[i][j][4 * g + e]);
+                    const int chunk = (4 * (j - j0) + g) ^ (r32 % CHUNKS);
+                    *reinterpret_cast<u32x2*>(stage + r32 * GC * 2 + chunk * 16 + 8 * half) =
+                        pack4<DT>(v[0], v[1], v[2], v[3]);
                 }
-        }
-        const unsigned char* from = stage + grp * GROUP * ROW_BYTES;
+            asm volatile("" ::: "memory");
+        };
+        auto read_piece = [&](int p) {
+            const int r = p * ROWS + orow;
+            return *reinterpret_cast<const u32x4*>(stage + r * GC * 2 + ((oc ^ (r % CHUNKS)) << 4));
+        };
+        auto to_group = [&](auto idx) {
+            constexpr int i = decltype(idx)::value / (WTN / GC), j0 = decltype(idx)::value % (WTN / GC) * (GC / 32);
+            return to + i * (32 / ROWS) * row_step + j0 * 64;
+        };
+        if (whole) {
+            u32x4 v[2][PIECES];
+            auto store_group = [&](auto idx) {
+                constexpr int g = decltype(idx)::value;
+                unsigned char* at = to_group(idx);
 #pragma unroll
-        for (int p0 = 0; p0 < STORES; p0 += BATCH) {
-            u32x4 v[BATCH];
-#pragma unroll
-            for (int p = 0; p < BATCH; ++p) {
-                const int r = ROWS_PER_STORE * (p0 + p) + orow;
-                v[p] = *reinterpret_cast<const u32x4*>(from + r * ROW_BYTES + ((oc ^ (r % ROW_CHUNKS)) << 4));
-            }
-#pragma unroll
-            for (int p = 0; p < BATCH; ++p) {
-                const int m = m0 + wm * WTM + grp * GROUP + ROWS_PER_STORE * (p0 + p) + orow;
-                unsigned char* to = ob + m * args.ldo + (int64_t)col * 2;
-                if (m >= M) continue;
-                if (left >= 8) {
-                    // Rows off 16 bytes share cache lines with the neighbouring tiles: ordinary stores.
-                    if (args.out_16) __builtin_nontemporal_store(v[p], reinterpret_cast<u32x4*>(to));
-                    else *reinterpret_cast<u32x4_2*>(to) = v[p];
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 7; ++e)
-                        if (e < left) reinterpret_cast<uint16_t*>(to)[e] = (uint16_t)(v[p][e >> 1] >> 16 * (e & 1));
+                for (int p = 0; p < PIECES; ++p, at += row_step)
+                    __builtin_nontemporal_store(v[g % 2][p], reinterpret_cast<u32x4*>(at));
+            };
+            all(std::integral_constant<int, GROUPS>{}, [&](auto idx) {
+                constexpr int g = decltype(idx)::value;
+                if constexpr (PERSISTENT && g < kLoadGroups) {
+                    if (more) all(kFirstLoads, [&](auto l) {
+                        if constexpr (decltype(l)::value * kLoadGroups / FIRST_LOADS == g) first_load(l);
+                    });
                 }
-            }
+                write_group(idx);
+                if constexpr (g > 0) store_group(std::integral_constant<int, g - 1>{});
+                asm volatile("" ::: "memory");
+#pragma unroll
+                for (int p = 0; p < PIECES; ++p) v[g % 2][p] = read_piece(p);
+            });
+            store_group(std::integral_constant<int, GROUPS - 1>{});
+        } else {
+            if (more) all(kFirstLoads, first_load);
+            all(std::integral_constant<int, GROUPS>{}, [&](auto idx) {
+                constexpr int i = decltype(idx)::value / (WTN / GC), j0 = decltype(idx)::value % (WTN / GC) * (GC / 32);
+                write_group(idx);
+                unsigned char* at = to_group(idx);
+                const int left = args.N - (n0 + 32 * j0);
+#pragma unroll 1
+                for (int p = 0; p < PIECES; ++p, at += row_step) {
+                    if (m0 + 32 * i + p * ROWS >= M) continue;
+                    const u32x4 v = read_piece(p);
+                    if (left >= 8) {
+                        *reinterpret_cast<u32x4_2*>(at) = v;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 7; ++e)
+                            if (e < left) reinterpret_cast<uint16_t*>(at)[e] = (uint16_t)(v[e >> 1] >> 16 * (e & 1));
+                    }
+                }
+            });
         }
+        behind_stores = whole;
+        if (!more) return;
+        if (!behind_stores) __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): the waits count none of these stores
+        second_chunk();
+        cur = next;
+        t += stride;
+    }
+}
+
+// Four columns of a row, `left` of them in it.
+template <int DT>
+__device__ __forceinline__ void store4(unsigned char* to, const f32x4& v, int left) {
+    typedef u32x2 u32x2_2 __attribute__((aligned(2)));
+    const u32x2 p = pack4<DT>(v[0], v[1], v[2], v[3]);
+    if (left >= 4) {
+        *reinterpret_cast<u32x2_2*>(to) = p;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+            if (e < left) reinterpret_cast<uint16_t*>(to)[e] = (uint16_t)(p[e >> 1] >> 16 * (e & 1));
     }
 }
 
@@ -391,49 +608,51 @@ gemm_mx4_sum_kernel(Mx4Args a) {
     const float* from = a.planes + m * a.ldp + n;
     f32x4 v = *reinterpret_cast<const f32x4*>(from);
     for (int s = 1; s < a.splits; ++s) v += *reinterpret_cast<const f32x4*>(from + s * (int64_t)a.total * a.ldp);
-    const u32x2 p = pack4<DT>(v[0], v[1], v[2], v[3]);
-    unsigned char* to = a.out + m * a.ldo + (int64_t)n * 2;
-    typedef u32x2 u32x2_2 __attribute__((aligned(2)));
-    if (n + 4 <= a.N) {
-        *reinterpret_cast<u32x2_2*>(to) = p;
-    } else {
-#pragma unroll
-        for (int e = 0; e < 3; ++e)
-            if (n + e < a.N) reinterpret_cast<uint16_t*>(to)[e] = (uint16_t)(p[e >> 1] >> 16 * (e & 1));
-    }
+    store4<DT>(a.out + m * a.ldo + (int64_t)n * 2, v, a.N - n);
+}
+
+template <int DT>
+int mx4_sum(const Mx4Args& a, hipStream_t stream) {
+    hipLaunchKernelGGL((gemm_mx4_sum_kernel<DT>), launch_grid(((int64_t)a.total * (a.ldp / 4) + 255) / 256), dim3(256),
+                       0, stream, a);
+    MB_HIP_TRY(hipGetLastError());
+    return MB_OK;
+}
+
+// The kernels' arguments; `planes` where K is split.
+inline Mx4Args mx4_args(const Mx4Call& c, int splits, void* planes) {
+    const int split_units = (int)((c.units + 2 * splits - 1) / (2 * splits) * 2);   // whole pairs
+    const bool out_16 = ((reinterpret_cast<uintptr_t>(c.out) | (uintptr_t)(c.ldo * 2)) & 15) == 0;
+    return Mx4Args{static_cast<const unsigned char*>(c.x), static_cast<const unsigned char*>(c.x_scales),
+                   static_cast<const unsigned char*>(c.w), static_cast<const unsigned char*>(c.w_scales),
+                   static_cast<unsigned char*>(c.out), c.rows, c.offsets, c.ldo * 2, (int)c.units * kMx4UnitBytes,
+                   (int)c.units * kMx4UnitScales, (int)c.units, (int)c.x_rows, c.experts, (int)c.total_rows, (int)c.N,
+                   static_cast<float*>(planes), splits, split_units, (int)((c.N + 3) / 4 * 4), out_16};
 }
 
 template <int DT, int CFG>
-int launch_mx4(const Mx4Call& c, int splits, void* workspace, hipStream_t stream) {
+int launch_mx4(const Mx4Call& c, int splits, int cus, void* workspace, hipStream_t stream) {
     constexpr int TILE = kMx4Tiles[CFG];
     const int tiles_n = (int)((c.N + TILE - 1) / TILE);
     const int64_t tiles_m = c.offsets ? c.total_rows / TILE + std::min<int64_t>(c.experts, c.total_rows)
                                       : (c.total_rows + TILE - 1) / TILE;
-    const int split_units = (int)((c.units + 2 * splits - 1) / (2 * splits) * 2);   // whole pairs
-    splits = (int)((c.units + split_units - 1) / split_units);                      // none is empty
-    const bool out_16 = ((reinterpret_cast<uintptr_t>(c.out) | (uintptr_t)(c.ldo * 2)) & 15) == 0;
-    const Mx4Args a{static_cast<const unsigned char*>(c.x), static_cast<const unsigned char*>(c.x_scales),
-                    static_cast<const unsigned char*>(c.w), static_cast<const unsigned char*>(c.w_scales),
-                    static_cast<unsigned char*>(c.out), c.rows, c.offsets, c.ldo * 2, (int)c.units * kMx4UnitBytes,
-                    (int)c.units * kMx4UnitScales, (int)c.units, (int)c.x_rows, c.experts, (int)c.total_rows, (int)c.N,
-                    splits > 1 ? static_cast<float*>(workspace) : nullptr, splits, split_units,
-                    (int)((c.N + 3) / 4 * 4), out_16};
-    hipLaunchKernelGGL((gemm_mx4_kernel<DT, TILE>), launch_grid(tiles_m * tiles_n * splits), dim3(256), 0, stream, a,
-                       tiles_n, 4);
+    const int64_t pairs = (c.units + 1) / 2, split_pairs = (pairs + splits - 1) / splits;
+    splits = (int)((pairs + split_pairs - 1) / split_pairs);   // none is empty
+    const Mx4Args a = mx4_args(c, splits, splits > 1 ? workspace : nullptr);
+    // Tiles of 256: a block per CU, which loads its next tile while it stores one.
+    const int64_t blocks = tiles_m * tiles_n * splits;
+    const uint64_t per_group = (uint64_t)kGroupM * tiles_n, magic = ((1ull << 40) + per_group - 1) / per_group;
+    hipLaunchKernelGGL((gemm_mx4_kernel<DT, TILE>), launch_grid(TILE == 256 ? std::min<int64_t>(blocks, cus) : blocks),
+                       dim3(256), 0, stream, a, tiles_n, magic);
     MB_HIP_TRY(hipGetLastError());
-    if (splits > 1) {
-        hipLaunchKernelGGL((gemm_mx4_sum_kernel<DT>), launch_grid((c.total_rows * (a.ldp / 4) + 255) / 256), dim3(256),
-                           0, stream, a);
-        MB_HIP_TRY(hipGetLastError());
-    }
-    return MB_OK;
+    return splits > 1 ? mx4_sum<DT>(a, stream) : MB_OK;
 }
 
 template <int DT>
 int launch_mx4_config(const Mx4Call& c, const Mx4Plan& plan, void* workspace, hipStream_t stream) {
-    if (plan.config == 0) return launch_mx4<DT, 0>(c, plan.splits, workspace, stream);
-    if (plan.config == 1) return launch_mx4<DT, 1>(c, plan.splits, workspace, stream);
-    return launch_mx4<DT, 2>(c, plan.splits, workspace, stream);
+    if (plan.config == 0) return launch_mx4<DT, 0>(c, plan.splits, plan.cus, workspace, stream);
+    if (plan.config == 1) return launch_mx4<DT, 1>(c, plan.splits, plan.cus, workspace, stream);
+    return launch_mx4<DT, 2>(c, plan.splits, plan.cus, workspace, stream);
 }
 
 }  // namespace
