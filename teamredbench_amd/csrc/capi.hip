@@ -1,6 +1,7 @@
 // C ABI of libmi355bench.so (declared in include/mi355bench.h): argument
 // validation, per-device property cache, dispatch into the stream and GEMM
 // kernel families, event-timed loops and kernel metadata.
+#include "gemm_mx4_plan.hpp"
 #include "gemm_w4_plan.hpp"
 #include "mb_common.hpp"
 
@@ -35,8 +36,8 @@ bool is_config(int64_t v) { return v >= 0 && v <= 4; }
 bool is_splits(int64_t v) { return v >= 1 && v <= 512; }
 bool is_grouped_config(int64_t v) { return v >= 0 && v <= 3; }
 bool is_w4_config(int64_t v) { return v >= 0 && v < kW4ConfigCount; }
-bool is_mx4_config(int64_t v) { return v >= 0 && v <= 5; }
-bool is_mx4_splits(int64_t v) { return v >= 1 && v <= 16; }
+bool is_mx4_config(int64_t v) { return v >= 0 && v < kMx4ConfigCount; }
+bool is_mx4_splits(int64_t v) { return v >= 1 && v <= kMx4MostSplits; }
 bool is_mfma(int64_t v) { return v == 16 || v == 32; }
 
 const KnobSpec kKnobs[MB_TUNE_COUNT] = {

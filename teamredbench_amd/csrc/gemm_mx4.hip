@@ -228,7 +228,7 @@ int launch_rows(const Mx4Call& c, hipStream_t stream) {
 
 template <int DT>
 int launch_rows_config(const Mx4Call& c, const Mx4Plan& plan, hipStream_t stream) {
-    return plan.config == kMx4TileCount ? launch_rows<DT, 8>(c, stream) : launch_rows<DT, 32>(c, stream);
+    return plan.config == kMx4Rows8 ? launch_rows<DT, 8>(c, stream) : launch_rows<DT, 32>(c, stream);
 }
 
 int launch_any(const Mx4Call& c, hipStream_t stream) {
@@ -240,34 +240,22 @@ int launch_any(const Mx4Call& c, hipStream_t stream) {
     return MB_OK;
 }
 
-Mx4Plan mx4_plan(const Mx4Call& c, size_t workspace_bytes, const DeviceProps& props) {
-    // Rows read through a list lie within the 2^31 bytes that a buffer offset spans.
-    if (c.rows != nullptr && c.x_rows > ((1ll << 31) - 1) / (c.units * kMx4UnitBytes)) return {-1, 1, 0};
-    const int64_t forced = tuning(MB_TUNE_MX4_CONFIG);
-    int config = forced >= 0 ? (forced == 5 ? -1 : (int)forced) : c.total_rows <= 8 ? 3 : c.total_rows <= 32 ? 4 : c.total_rows > 512 ? 0 : 1;
-    int splits = 1;
-    if (config == 1 || config == 2) {
-        const int64_t want = tuning(MB_TUNE_MX4_SPLITS);
-        const size_t plane = (size_t)c.total_rows * ((c.N + 3) / 4 * 4) * 4;
-        splits = want > 0 ? (int)want : 1;
-        while (splits > 1 && plane * splits > workspace_bytes) --splits;
-    }
-    return {config, splits, props.cu_count};
-}
-
 }  // namespace
 
 int gemm_mx4_launch(const Mx4Call& c, void* workspace, size_t workspace_bytes, const DeviceProps& props,
                     hipStream_t stream) {
     // The workspace only makes small calls faster: one off 16 bytes is left alone.
     if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0) workspace_bytes = 0;
-    const Mx4Plan plan = mx4_plan(c, workspace_bytes, props);
-    if (plan.config < 0) return launch_any(c, stream);
+    const Mx4Shape shape{c.total_rows, c.N, c.units, c.x_rows, c.experts, c.offsets != nullptr, c.rows != nullptr};
+    const Mx4Plan plan = mx4_plan(shape, workspace_bytes, props.cu_count, tuning(MB_TUNE_MX4_CONFIG),
+                                  tuning(MB_TUNE_MX4_SPLITS));
+    const bool half = c.dtype == MB_DT_FLOAT16;
+    if (plan.config == kMx4Any) return launch_any(c, stream);
     if (plan.config >= kMx4TileCount)
-        return c.dtype == MB_DT_FLOAT16 ? launch_rows_config<MB_DT_FLOAT16>(c, plan, stream)
-                                        : launch_rows_config<MB_DT_BFLOAT16>(c, plan, stream);
-    return c.dtype == MB_DT_FLOAT16 ? gemm_mx4_tiled_f16(c, plan, workspace, stream)
-                                    : gemm_mx4_tiled_bf16(c, plan, workspace, stream);
+        return half ? launch_rows_config<MB_DT_FLOAT16>(c, plan, stream)
+                    : launch_rows_config<MB_DT_BFLOAT16>(c, plan, stream);
+    return half ? gemm_mx4_tiled_f16(c, plan, props.cu_count, workspace, stream)
+                : gemm_mx4_tiled_bf16(c, plan, props.cu_count, workspace, stream);
 }
 
 }  // namespace mb

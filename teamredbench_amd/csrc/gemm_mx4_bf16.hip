@@ -3,8 +3,8 @@
 
 namespace mb {
 
-int gemm_mx4_tiled_bf16(const Mx4Call& c, const Mx4Plan& plan, void* workspace, hipStream_t stream) {
-    return launch_mx4_config<MB_DT_BFLOAT16>(c, plan, workspace, stream);
+int gemm_mx4_tiled_bf16(const Mx4Call& c, const Mx4Plan& plan, int cus, void* workspace, hipStream_t stream) {
+    return launch_mx4_config<MB_DT_BFLOAT16>(c, plan, cus, workspace, stream);
 }
 
 }  // namespace mb

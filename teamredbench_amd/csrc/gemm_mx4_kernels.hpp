@@ -4,20 +4,15 @@
 #pragma once
 
 #include "gemm_grouped_kernels.hpp"
+#include "gemm_mx4_plan.hpp"
 #include "mx4_common.hpp"
 
 namespace mb {
 
-struct Mx4Plan {
-    int config;   // tiles of kMx4Tiles[config]; -1: gemm_mx4_any_kernel
-    int splits;   // of K, over fp32 planes in the workspace
-    int cus;      // of the device
-};
-int gemm_mx4_tiled_bf16(const Mx4Call& c, const Mx4Plan& plan, void* workspace, hipStream_t stream);
-int gemm_mx4_tiled_f16(const Mx4Call& c, const Mx4Plan& plan, void* workspace, hipStream_t stream);
-
-constexpr int kMx4TileCount = 3;
-constexpr int kMx4Tiles[kMx4TileCount] = {256, 128, 64};
+int gemm_mx4_tiled_bf16(const Mx4Call& c, const Mx4Plan& plan, int cus, void* workspace,
+                        hipStream_t stream);
+int gemm_mx4_tiled_f16(const Mx4Call& c, const Mx4Plan& plan, int cus, void* workspace,
+                        hipStream_t stream);
 
 namespace {
 
@@ -113,15 +108,14 @@ __device__ __forceinline__ float read_acc(float v) {
     return f;
 }
 
-template <int DT, int TILE>
+template <int DT, int CFG>
 __global__ void __launch_bounds__(256)
 gemm_mx4_kernel(Mx4Args all_args, int tiles_n, uint64_t magic) {
-    constexpr int BM = TILE, BN = TILE;
+    constexpr int TILE = kMx4Tiles[CFG].size, SLOTS = kMx4Tiles[CFG].slots, BM = TILE, BN = TILE;
     constexpr int WTM = BM / 2, WTN = BN / 2;
     constexpr int FM = WTM / 32, FN = WTN / 32;
     constexpr int SLOT = TILE * kPairBytes, SCALE_SLOT = TILE * kChunkBytes;   // one operand's
     // LDS: x's elements, w's (SLOTS slots each); slot 0 of x's scales and of w's, slot 1 of both.
-    constexpr int SLOTS = TILE == 64 ? 4 : 2;
     constexpr int W0 = SLOTS * SLOT, XS0 = 2 * SLOTS * SLOT, WS0 = XS0 + SCALE_SLOT, NEXT_SCALES = 2 * SCALE_SLOT;
     constexpr int LDS_BYTES = XS0 + 2 * NEXT_SCALES;
     constexpr int INSTR = SLOT / 1024 / 4;                   // DMA instructions per wave, operand and pair
@@ -632,7 +626,7 @@ inline Mx4Args mx4_args(const Mx4Call& c, int splits, void* planes) {
 
 template <int DT, int CFG>
 int launch_mx4(const Mx4Call& c, int splits, int cus, void* workspace, hipStream_t stream) {
-    constexpr int TILE = kMx4Tiles[CFG];
+    constexpr int TILE = kMx4Tiles[CFG].size;
     const int tiles_n = (int)((c.N + TILE - 1) / TILE);
     const int64_t tiles_m = c.offsets ? c.total_rows / TILE + std::min<int64_t>(c.experts, c.total_rows)
                                       : (c.total_rows + TILE - 1) / TILE;
@@ -642,17 +636,20 @@ int launch_mx4(const Mx4Call& c, int splits, int cus, void* workspace, hipStream
     // Tiles of 256: a block per CU, which loads its next tile while it stores one.
     const int64_t blocks = tiles_m * tiles_n * splits;
     const uint64_t per_group = (uint64_t)kGroupM * tiles_n, magic = ((1ull << 40) + per_group - 1) / per_group;
-    hipLaunchKernelGGL((gemm_mx4_kernel<DT, TILE>), launch_grid(TILE == 256 ? std::min<int64_t>(blocks, cus) : blocks),
+    hipLaunchKernelGGL((gemm_mx4_kernel<DT, CFG>), launch_grid(TILE == 256 ? std::min<int64_t>(blocks, cus) : blocks),
                        dim3(256), 0, stream, a, tiles_n, magic);
     MB_HIP_TRY(hipGetLastError());
     return splits > 1 ? mx4_sum<DT>(a, stream) : MB_OK;
 }
 
 template <int DT>
-int launch_mx4_config(const Mx4Call& c, const Mx4Plan& plan, void* workspace, hipStream_t stream) {
-    if (plan.config == 0) return launch_mx4<DT, 0>(c, plan.splits, plan.cus, workspace, stream);
-    if (plan.config == 1) return launch_mx4<DT, 1>(c, plan.splits, plan.cus, workspace, stream);
-    return launch_mx4<DT, 2>(c, plan.splits, plan.cus, workspace, stream);
+int launch_mx4_config(const Mx4Call& c, const Mx4Plan& plan, int cus, void* workspace, hipStream_t stream) {
+    switch (plan.config) {
+        case 0: return launch_mx4<DT, 0>(c, plan.splits, cus, workspace, stream);
+        case 1: return launch_mx4<DT, 1>(c, plan.splits, cus, workspace, stream);
+        case 2: return launch_mx4<DT, 2>(c, plan.splits, cus, workspace, stream);
+        default: return launch_mx4<DT, 3>(c, plan.splits, cus, workspace, stream);
+    }
 }
 
 }  // namespace

@@ -119,114 +119,245 @@ __device__ __forceinline__ unsigned max4(unsigned v) {   // over each four lanes
     return max(v, lane_xor2(v));
 }
 
-// Along rows: 16 lanes per unit of a row, 8 elements a lane, four lanes a block.
-template <int DT, bool FIT>
+// Along rows: 16 lanes per unit of a row, 8 elements a lane, four lanes a block; UNITS units a lane group, loaded before
+// any of them is used. The units of a matrix follow each other in q and in scales, whatever its rows.
+template <int DT, int UNITS>
 __global__ void __launch_bounds__(256)
 mx4_quantize_rows_kernel(const void* __restrict__ x, int64_t ldx, int64_t rows, int64_t columns, int64_t units,
-                         unsigned* __restrict__ q, unsigned char* __restrict__ scales) {
-    const int64_t i = (int64_t)block_number() * 256 + threadIdx.x;
-    const int64_t unit = i >> 4;
-    const int64_t row = unit / units;
-    if (row >= rows) return;
-    const int64_t column = (unit - row * units) * kMx4Unit + 8 * (i & 15);
-    unsigned v[Source<DT>::kWords];
-    load8<DT>(static_cast<const typename Source<DT>::Element*>(x) + row * ldx, column, columns, v);
-    const unsigned s = scale_byte(magnitude_bits<DT>(max4(largest8<DT>(v))), FIT);
-    q[i] = encode8<DT>(v, s);
-    if ((i & 3) == 0) scales[i >> 2] = (unsigned char)s;
-}
-
-// Along columns: a lane holds 32 rows of one column.
-template <int DT, bool FIT>
-__global__ void __launch_bounds__(256)
-mx4_quantize_columns_kernel(const void* __restrict__ x, int64_t ldx, int64_t rows, int64_t columns, int64_t units,
-                            u32x4* __restrict__ qt, unsigned char* __restrict__ scales_t) {
+                         bool fit, unsigned* __restrict__ q, unsigned char* __restrict__ scales) {
     typedef typename Source<DT>::Element Element;
-    const int64_t i = (int64_t)block_number() * 256 + threadIdx.x;
-    const int64_t blocks = 4 * units, block = i / columns, column = i - block * columns;
-    if (block >= blocks) return;
-    unsigned v[32], most = 0;
-    const Element* p = static_cast<const Element*>(x) + column;
+    const int64_t first = (int64_t)block_number() * (16 * UNITS) + threadIdx.x / 16;
+    const int lane16 = threadIdx.x % 16;
+    unsigned v[UNITS][Source<DT>::kWords];
+    const int64_t total = rows * units;
 #pragma unroll
-    for (int r = 0; r < 32; ++r) v[r] = block * 32 + r < rows ? p[(block * 32 + r) * ldx] : 0;
-#pragma unroll
-    for (int r = 0; r < 32; ++r) most = max(most, v[r] & (DT == MB_DT_FLOAT32 ? 0x7FFFFFFFu : 0x7FFFu));
-    const unsigned s = scale_byte(magnitude_bits<DT>(most), FIT);
-    u32x4 out;
-#pragma unroll
-    for (int d = 0; d < 4; ++d) {
-        unsigned w[Source<DT>::kWords];
-#pragma unroll
-        for (int j = 0; j < Source<DT>::kWords; ++j) {
-            if constexpr (DT == MB_DT_FLOAT32) w[j] = v[8 * d + j];
-            else w[j] = v[8 * d + 2 * j] | (v[8 * d + 2 * j + 1] << 16);
-        }
-        out[d] = encode8<DT>(w, s);
+    for (int k = 0; k < UNITS; ++k) {
+        const int64_t unit = min(first + 16 * k, total - 1);
+        const int64_t row = unit / units, column = (unit - row * units) * kMx4Unit + 8 * lane16;
+        load8<DT>(static_cast<const Element*>(x) + row * ldx, column, columns, v[k]);
     }
-    qt[column * blocks + block] = out;
-    scales_t[column * blocks + block] = (unsigned char)s;
+#pragma unroll
+    for (int k = 0; k < UNITS; ++k) {
+        const int64_t unit = first + 16 * k;
+        if (unit >= total) return;
+        const unsigned s = scale_byte(magnitude_bits<DT>(max4(largest8<DT>(v[k]))), fit);
+        q[unit * 16 + lane16] = encode8<DT>(v[k], s);
+        if (lane16 % 4 == 0) scales[unit * 4 + lane16 / 4] = (unsigned char)s;
+    }
 }
 
-// 8 elements a lane.
+// The largest of both 16-bit halves (fp32: of the whole).
 template <int DT>
+__device__ __forceinline__ unsigned max_bits(unsigned a, unsigned b) {
+    if constexpr (DT == MB_DT_FLOAT32) {
+        return max(a, b);
+    } else {
+        typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(unsigned,
+                                  __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+    }
+}
+
+// Along columns, or along both. A wave holds 128 rows x 128 columns (fp32: two halves of 64 columns, one after the
+// other) in registers: lane l has rows 32 (l / 16) .. + 31 of 8 (4) columns, 128 dwords, so the blocks of its columns
+// are its own, and those of a row span four (eight) neighbouring lanes. Whole lines are read, all 32 loads of a lane
+// before the first is used. The four waves of a block are a square of tiles, so that both forms' lines of 128 bytes are written by one CU.
+template <int DT, bool ROWS>
+__global__ void __launch_bounds__(256)
+mx4_quantize_tile_kernel(const void* __restrict__ x, int64_t ldx, int64_t rows, int64_t columns, bool fit,
+                         int64_t tiles_n, unsigned char* __restrict__ q, unsigned char* __restrict__ scales,
+                         unsigned char* __restrict__ qt, unsigned char* __restrict__ scales_t) {
+    typedef typename Source<DT>::Element Element;
+    constexpr bool WIDE = DT == MB_DT_FLOAT32;
+    constexpr int CPL = WIDE ? 4 : 8;                    // columns per lane
+    constexpr unsigned kMagnitude = WIDE ? 0x7FFFFFFFu : 0x7FFF7FFFu;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, group = lane >> 4;
+    const int64_t block = block_number(), bm = block / tiles_n, bn = block - bm * tiles_n;
+    const int64_t unit_r = 2 * bm + (wave >> 1), unit_c = 2 * bn + (wave & 1);   // of rows, of columns
+    const int64_t units = (columns + kMx4Unit - 1) / kMx4Unit, units_t = (rows + kMx4Unit - 1) / kMx4Unit;
+    if (unit_r >= units_t || unit_c >= units) return;
+    const int64_t r0 = unit_r * kMx4Unit + 32 * group;
+#pragma unroll 1
+    for (int part = 0; part < 8 / CPL; ++part) {
+        const int64_t c0 = unit_c * kMx4Unit + part * 64 + CPL * l16;
+        if (WIDE && unit_c * kMx4Unit + part * 64 >= columns && !ROWS) return;
+        unsigned v[32][4];
+        const Element* p = static_cast<const Element*>(x) + r0 * ldx + c0;
+        if (r0 + 32 <= rows && c0 + CPL <= columns) {
+#pragma unroll
+            for (int r = 0; r < 32; ++r) {
+                const u32x4 w = *reinterpret_cast<const u32x4_2*>(p + r * ldx);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[r][i] = w[i];
+            }
+        } else {   // an edge: element by element, zeros past it
+#pragma unroll
+            for (int r = 0; r < 32; ++r)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    v[r][i] = 0;
+                    if (r0 + r >= rows) continue;
+                    if constexpr (WIDE) {
+                        if (c0 + i < columns) v[r][i] = p[r * ldx + i];
+                    } else {
+                        if (c0 + 2 * i < columns) v[r][i] = p[r * ldx + 2 * i];
+                        if (c0 + 2 * i + 1 < columns) v[r][i] |= (unsigned)p[r * ldx + 2 * i + 1] << 16;
+                    }
+                }
+        }
+        // Along columns.
+        unsigned most[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int r = 0; r < 32; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) most[i] = max_bits<DT>(most[i], v[r][i] & kMagnitude);
+#pragma unroll
+        for (int j = 0; j < CPL; ++j) {
+            constexpr unsigned kPick[2] = {0x05040100u, 0x07060302u};   // low halves of two dwords, high halves
+            const unsigned m = WIDE ? most[j % 4] : most[j / 2] >> 16 * (j & 1) & 0xFFFFu;
+            const unsigned s = scale_byte(magnitude_bits<DT>(m), fit);
+            u32x4 out;
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                unsigned w[Source<DT>::kWords];
+#pragma unroll
+                for (int i = 0; i < Source<DT>::kWords; ++i) {
+                    if constexpr (WIDE) w[i] = v[8 * d + i][j];
+                    else w[i] = __builtin_amdgcn_perm(v[8 * d + 2 * i + 1][j / 2], v[8 * d + 2 * i][j / 2], kPick[j & 1]);
+                }
+                out[d] = encode8<DT>(w, s);
+            }
+            const int64_t c = c0 + j;
+            if (c < columns) {
+                *reinterpret_cast<u32x4*>(qt + (c * units_t + unit_r) * kMx4UnitBytes + 16 * group) = out;
+                scales_t[(c * units_t + unit_r) * kMx4UnitScales + group] = (unsigned char)s;
+            }
+        }
+        if constexpr (!ROWS) continue;
+        // Along rows. A lane keeps the scales of two of its group's rows, for whole dwords (fp32: halves) at the end.
+        unsigned kept[2] = {0, 0};
+#pragma unroll
+        for (int r = 0; r < 32; ++r) {
+            unsigned m = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m = max_bits<DT>(m, v[r][i] & kMagnitude);
+            if constexpr (!WIDE) m = max(m & 0xFFFFu, m >> 16);
+            m = max4(m);
+            if constexpr (WIDE) m = max(m, (unsigned)__builtin_amdgcn_mov_dpp((int)m, 0x141, 0xF, 0xF, true));   // l ^ 7
+            const unsigned s = scale_byte(magnitude_bits<DT>(m), fit);
+            unsigned code, bytes;
+            if constexpr (WIDE) {
+                const unsigned four[8] = {v[r][0], v[r][1], v[r][2], v[r][3], 0, 0, 0, 0};
+                const unsigned mine = encode8<DT>(four, s);
+                code = mine | lane_xor1(mine) << 16;       // even lanes: 8 elements
+                bytes = s << 8 * (l16 >> 3);
+            } else {
+                code = encode8<DT>(v[r], s);
+                bytes = s << 8 * (l16 >> 2);
+                bytes |= (unsigned)__builtin_amdgcn_mov_dpp((int)bytes, 0x124, 0xF, 0xF, true);   // four lanes round 16
+            }
+            bytes |= (unsigned)__builtin_amdgcn_mov_dpp((int)bytes, 0x128, 0xF, 0xF, true);       // eight
+            if (r0 + r < rows) {
+                unsigned char* to = q + ((r0 + r) * units + unit_c) * kMx4UnitBytes;
+                if constexpr (WIDE) {
+                    if (l16 % 2 == 0) *reinterpret_cast<unsigned*>(to + 32 * part + 2 * l16) = code;
+                } else {
+                    *reinterpret_cast<unsigned*>(to + 4 * l16) = code;
+                }
+            }
+            kept[r & 1] = l16 == r / 2 ? bytes : kept[r & 1];
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int64_t r = r0 + 2 * l16 + i;
+            if (r >= rows) continue;
+            unsigned char* to = scales + (r * units + unit_c) * kMx4UnitScales;
+            if constexpr (WIDE) *reinterpret_cast<uint16_t*>(to + 2 * part) = (uint16_t)kept[i];
+            else *reinterpret_cast<unsigned*>(to) = kept[i];
+        }
+    }
+}
+
+// 8 elements a lane, UNITS units a lane group.
+template <int DT, int UNITS>
 __global__ void __launch_bounds__(256)
 mx4_dequantize_kernel(const unsigned* __restrict__ q, const unsigned char* __restrict__ scales, int64_t rows,
                       int64_t columns, int64_t units, typename Source<DT>::Element* __restrict__ out, int64_t ldo) {
-    const int64_t i = (int64_t)block_number() * 256 + threadIdx.x;
-    const int64_t unit = i >> 4;
-    const int64_t row = unit / units;
-    if (row >= rows) return;
-    const int64_t column = (unit - row * units) * kMx4Unit + 8 * (i & 15);
-    if (column >= columns) return;
-    const unsigned codes = q[i];
-    const float scale = __builtin_bit_cast(float, (unsigned)scales[i >> 2] << 23);
-    unsigned v[Source<DT>::kWords];
-    auto two = [&](auto sel) {
-        constexpr int s = decltype(sel)::value;
-        if constexpr (DT == MB_DT_FLOAT32) {
-            const auto f = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, scale, s);
-            v[2 * s] = __builtin_bit_cast(unsigned, (float)f[0]);
-            v[2 * s + 1] = __builtin_bit_cast(unsigned, (float)f[1]);
-        } else if constexpr (DT == MB_DT_BFLOAT16) {
-            v[s] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, s));
-        } else {
-            v[s] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, s));
-        }
-    };
-    two(std::integral_constant<int, 0>{});
-    two(std::integral_constant<int, 1>{});
-    two(std::integral_constant<int, 2>{});
-    two(std::integral_constant<int, 3>{});
-    auto* p = out + row * ldo + column;
-    if (column + 8 <= columns) {
-        *reinterpret_cast<u32x4_2*>(p) = u32x4{v[0], v[1], v[2], v[3]};
-        if constexpr (DT == MB_DT_FLOAT32) *reinterpret_cast<u32x4_2*>(p + 4) = u32x4{v[4], v[5], v[6], v[7]};
-        return;
+    const int64_t first = (int64_t)block_number() * (16 * UNITS) + threadIdx.x / 16;
+    const int lane16 = threadIdx.x % 16;
+    const int64_t total = rows * units;
+    unsigned codes[UNITS], bytes[UNITS];
+#pragma unroll
+    for (int k = 0; k < UNITS; ++k) {
+        const int64_t unit = min(first + 16 * k, total - 1);
+        codes[k] = q[unit * 16 + lane16];
+        bytes[k] = scales[unit * 4 + lane16 / 4];
     }
 #pragma unroll
-    for (int e = 0; e < 7; ++e)
-        if (column + e < columns) {
-            if constexpr (DT == MB_DT_FLOAT32) p[e] = v[e];
-            else p[e] = (uint16_t)(v[e / 2] >> (16 * (e & 1)));
+    for (int k = 0; k < UNITS; ++k) {
+        const int64_t unit = first + 16 * k;
+        if (unit >= total) return;
+        const int64_t row = unit / units, column = (unit - row * units) * kMx4Unit + 8 * lane16;
+        if (column >= columns) continue;
+        const float scale = __builtin_bit_cast(float, bytes[k] << 23);
+        unsigned v[Source<DT>::kWords];
+        auto two = [&](auto sel) {
+            constexpr int s = decltype(sel)::value;
+            if constexpr (DT == MB_DT_FLOAT32) {
+                const auto f = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[k], scale, s);
+                v[2 * s] = __builtin_bit_cast(unsigned, (float)f[0]);
+                v[2 * s + 1] = __builtin_bit_cast(unsigned, (float)f[1]);
+            } else if constexpr (DT == MB_DT_BFLOAT16) {
+                v[s] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes[k], scale, s));
+            } else {
+                v[s] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes[k], scale, s));
+            }
+        };
+        two(std::integral_constant<int, 0>{});
+        two(std::integral_constant<int, 1>{});
+        two(std::integral_constant<int, 2>{});
+        two(std::integral_constant<int, 3>{});
+        auto* p = out + row * ldo + column;
+        if (column + 8 <= columns) {
+            *reinterpret_cast<u32x4_2*>(p) = u32x4{v[0], v[1], v[2], v[3]};
+            if constexpr (DT == MB_DT_FLOAT32) *reinterpret_cast<u32x4_2*>(p + 4) = u32x4{v[4], v[5], v[6], v[7]};
+            continue;
         }
+#pragma unroll
+        for (int e = 0; e < 7; ++e)
+            if (column + e < columns) {
+                if constexpr (DT == MB_DT_FLOAT32) p[e] = v[e];
+                else p[e] = (uint16_t)(v[e / 2] >> (16 * (e & 1)));
+            }
+    }
 }
 
-template <int DT, bool FIT>
+// Units a lane group takes: several in flight, while that leaves a block for every CU.
+constexpr int64_t kManyUnits = 4 * 16 * 256;
+
+template <int DT>
 int quantize(const Mx4Quantize& c, hipStream_t stream) {
-    if (c.q != nullptr) {
-        const int64_t units = mx4_units(c.columns);
-        hipLaunchKernelGGL((mx4_quantize_rows_kernel<DT, FIT>), launch_grid((c.rows * units + 15) / 16), dim3(256), 0,
-                           stream, c.x, c.ldx, c.rows, c.columns, units, static_cast<unsigned*>(c.q),
-                           static_cast<unsigned char*>(c.scales));
-        MB_HIP_TRY(hipGetLastError());
-    }
-    if (c.qt != nullptr) {
-        const int64_t units = mx4_units(c.rows);
-        hipLaunchKernelGGL((mx4_quantize_columns_kernel<DT, FIT>), launch_grid((c.columns * units * 4 + 255) / 256),
-                           dim3(256), 0, stream, c.x, c.ldx, c.rows, c.columns, units, static_cast<u32x4*>(c.qt),
+    const int64_t units = mx4_units(c.columns);
+    auto* q = static_cast<unsigned char*>(c.q);
+    auto* scales = static_cast<unsigned char*>(c.scales);
+    if (c.qt == nullptr) {
+        const int64_t total = c.rows * units;
+        auto launch = [&](auto many) {
+            constexpr int N = decltype(many)::value;
+            hipLaunchKernelGGL((mx4_quantize_rows_kernel<DT, N>), launch_grid((total + 16 * N - 1) / (16 * N)),
+                               dim3(256), 0, stream, c.x, c.ldx, c.rows, c.columns, units, c.fit,
+                               reinterpret_cast<unsigned*>(q), scales);
+        };
+        if (total >= kManyUnits) launch(std::integral_constant<int, 4>{});
+        else launch(std::integral_constant<int, 1>{});
+    } else {
+        const int64_t tiles_m = (mx4_units(c.rows) + 1) / 2, tiles_n = (units + 1) / 2;
+        auto kernel = q != nullptr ? mx4_quantize_tile_kernel<DT, true> : mx4_quantize_tile_kernel<DT, false>;
+        hipLaunchKernelGGL(kernel, launch_grid(tiles_m * tiles_n), dim3(256), 0, stream, c.x, c.ldx, c.rows, c.columns,
+                           c.fit, tiles_n, q, scales, static_cast<unsigned char*>(c.qt),
                            static_cast<unsigned char*>(c.scales_t));
-        MB_HIP_TRY(hipGetLastError());
     }
+    MB_HIP_TRY(hipGetLastError());
     return MB_OK;
 }
 
@@ -234,10 +365,15 @@ template <int DT>
 int dequantize(const void* q, const void* scales, int64_t rows, int64_t columns, void* out, int64_t ldo,
                hipStream_t stream) {
     typedef typename Source<DT>::Element Element;
-    const int64_t units = mx4_units(columns);
-    hipLaunchKernelGGL((mx4_dequantize_kernel<DT>), launch_grid((rows * units + 15) / 16), dim3(256), 0, stream,
-                       static_cast<const unsigned*>(q), static_cast<const unsigned char*>(scales), rows, columns, units,
-                       static_cast<Element*>(out), ldo);
+    const int64_t units = mx4_units(columns), total = rows * units;
+    auto launch = [&](auto many) {
+        constexpr int N = decltype(many)::value;
+        hipLaunchKernelGGL((mx4_dequantize_kernel<DT, N>), launch_grid((total + 16 * N - 1) / (16 * N)), dim3(256), 0,
+                           stream, static_cast<const unsigned*>(q), static_cast<const unsigned char*>(scales), rows,
+                           columns, units, static_cast<Element*>(out), ldo);
+    };
+    if (total >= kManyUnits) launch(std::integral_constant<int, 4>{});
+    else launch(std::integral_constant<int, 1>{});
     MB_HIP_TRY(hipGetLastError());
     return MB_OK;
 }
@@ -245,11 +381,9 @@ int dequantize(const void* q, const void* scales, int64_t rows, int64_t columns,
 }  // namespace
 
 int mx4_quantize_launch(const Mx4Quantize& c, hipStream_t stream) {
-    if (c.dtype == MB_DT_FLOAT32)
-        return c.fit ? quantize<MB_DT_FLOAT32, true>(c, stream) : quantize<MB_DT_FLOAT32, false>(c, stream);
-    if (c.dtype == MB_DT_BFLOAT16)
-        return c.fit ? quantize<MB_DT_BFLOAT16, true>(c, stream) : quantize<MB_DT_BFLOAT16, false>(c, stream);
-    return c.fit ? quantize<MB_DT_FLOAT16, true>(c, stream) : quantize<MB_DT_FLOAT16, false>(c, stream);
+    if (c.dtype == MB_DT_FLOAT32) return quantize<MB_DT_FLOAT32>(c, stream);
+    if (c.dtype == MB_DT_BFLOAT16) return quantize<MB_DT_BFLOAT16>(c, stream);
+    return quantize<MB_DT_FLOAT16>(c, stream);
 }
 
 int mx4_dequantize_launch(int dtype, const void* q, const void* scales, int64_t rows, int64_t columns, void* out,
