@@ -100,6 +100,27 @@ __device__ __forceinline__ unsigned encode8(const unsigned* v, unsigned s) {
     return s == 255 ? 0u : q;
 }
 
+// The first 4 of them, 16 bits.
+template <int DT>
+__device__ __forceinline__ unsigned encode4(const unsigned* v, unsigned s) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    const float scale = __builtin_bit_cast(float, s << 23);
+    unsigned q = 0;
+    if constexpr (DT == MB_DT_FLOAT32) {
+        auto f = [&](int i) { return __builtin_bit_cast(float, v[i]); };
+        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f(0), f(1), scale, 0);
+        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f(2), f(3), scale, 1);
+    } else if constexpr (DT == MB_DT_BFLOAT16) {
+        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(q, __builtin_bit_cast(bf16x2, v[0]), scale, 0);
+        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(q, __builtin_bit_cast(bf16x2, v[1]), scale, 1);
+    } else {
+        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(q, __builtin_bit_cast(f16x2, v[0]), scale, 0);
+        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(q, __builtin_bit_cast(f16x2, v[1]), scale, 1);
+    }
+    return s == 255 ? 0u : q;
+}
+
 // The largest magnitude of 8 elements, as their own type's bits.
 template <int DT>
 __device__ __forceinline__ unsigned largest8(const unsigned (&v)[Source<DT>::kWords]) {
@@ -158,10 +179,11 @@ __device__ __forceinline__ unsigned max_bits(unsigned a, unsigned b) {
     }
 }
 
-// Along columns, or along both. A wave holds 128 rows x 128 columns (fp32: two halves of 64 columns, one after the
-// other) in registers: lane l has rows 32 (l / 16) .. + 31 of 8 (4) columns, 128 dwords, so the blocks of its columns
-// are its own, and those of a row span four (eight) neighbouring lanes. Whole lines are read, all 32 loads of a lane
-// before the first is used. The four waves of a block are a square of tiles, so that both forms' lines of 128 bytes are written by one CU.
+// Along columns, or along both: 128 rows x 256 bytes of each a block, through LDS. Lanes take 16 bytes of a row (16 lanes
+// a row), so a row's blocks span four lanes (fp32: eight); then a lane takes 32 rows of one dword's columns. Four
+// neighbouring lanes take the four blocks of 128 rows, and store 64 bytes; 16-byte chunk c of row r lies at chunk
+// c ^ 4 (r / 32), which spreads their reads over the banks. (Both forms from registers, a lane holding 32 rows x 4 or 8
+// columns, took 72 us for bf16 8192 x 8192: two waves a SIMD, and long chains of lane exchanges.)
 template <int DT, bool ROWS>
 __global__ void __launch_bounds__(256)
 mx4_quantize_tile_kernel(const void* __restrict__ x, int64_t ldx, int64_t rows, int64_t columns, bool fit,
@@ -169,144 +191,144 @@ mx4_quantize_tile_kernel(const void* __restrict__ x, int64_t ldx, int64_t rows, 
                          unsigned char* __restrict__ qt, unsigned char* __restrict__ scales_t) {
     typedef typename Source<DT>::Element Element;
     constexpr bool WIDE = DT == MB_DT_FLOAT32;
-    constexpr int CPL = WIDE ? 4 : 8;                    // columns per lane
+    constexpr int EACH = WIDE ? 4 : 8, COLUMNS = 16 * EACH;   // columns of a lane's 16 bytes, of a tile
     constexpr unsigned kMagnitude = WIDE ? 0x7FFFFFFFu : 0x7FFF7FFFu;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, group = lane >> 4;
-    const int64_t block = block_number(), bm = block / tiles_n, bn = block - bm * tiles_n;
-    const int64_t unit_r = 2 * bm + (wave >> 1), unit_c = 2 * bn + (wave & 1);   // of rows, of columns
+    __shared__ u32x4 tile[128 * 16];
+    const int tid = threadIdx.x, l16 = tid % 16;
+    const int64_t block = block_number(), unit_r = block / tiles_n, tile_c = block - unit_r * tiles_n;
     const int64_t units = (columns + kMx4Unit - 1) / kMx4Unit, units_t = (rows + kMx4Unit - 1) / kMx4Unit;
-    if (unit_r >= units_t || unit_c >= units) return;
-    const int64_t r0 = unit_r * kMx4Unit + 32 * group;
-#pragma unroll 1
-    for (int part = 0; part < 8 / CPL; ++part) {
-        const int64_t c0 = unit_c * kMx4Unit + part * 64 + CPL * l16;
-        if (WIDE && unit_c * kMx4Unit + part * 64 >= columns && !ROWS) return;
-        unsigned v[32][4];
-        const Element* p = static_cast<const Element*>(x) + r0 * ldx + c0;
-        if (r0 + 32 <= rows && c0 + CPL <= columns) {
+    const int64_t r0 = unit_r * kMx4Unit, c0 = tile_c * COLUMNS;
+    const int row_count = (int)min(rows - r0, (int64_t)kMx4Unit);
+    auto piece = [&](int k) -> u32x4& {   // this lane's of row tid / 16 + 16 k
+        const int r = tid / 16 + 16 * k;
+        return tile[r * 16 + (l16 ^ 4 * (r / 32))];
+    };
+    {
+        const Element* p = static_cast<const Element*>(x) + (r0 + tid / 16) * ldx + c0 + EACH * l16;
+        if (row_count == kMx4Unit && c0 + COLUMNS <= columns) {
+            u32x4 v[8];
 #pragma unroll
-            for (int r = 0; r < 32; ++r) {
-                const u32x4 w = *reinterpret_cast<const u32x4_2*>(p + r * ldx);
+            for (int k = 0; k < 8; ++k) v[k] = *reinterpret_cast<const u32x4_2*>(p + 16 * k * ldx);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[r][i] = w[i];
-            }
-        } else {   // an edge: element by element, zeros past it
-#pragma unroll
-            for (int r = 0; r < 32; ++r)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    v[r][i] = 0;
-                    if (r0 + r >= rows) continue;
-                    if constexpr (WIDE) {
-                        if (c0 + i < columns) v[r][i] = p[r * ldx + i];
+            for (int k = 0; k < 8; ++k) piece(k) = v[k];
+        } else {   // an edge: zeros past it, none of which is read
+            const int64_t left = columns - (c0 + EACH * l16);
+#pragma unroll 2
+            for (int k = 0; k < 8; ++k) {
+                u32x4 v = {0, 0, 0, 0};
+                if (tid / 16 + 16 * k < row_count) {
+                    if (left >= EACH) {
+                        v = *reinterpret_cast<const u32x4_2*>(p + 16 * k * ldx);
                     } else {
-                        if (c0 + 2 * i < columns) v[r][i] = p[r * ldx + 2 * i];
-                        if (c0 + 2 * i + 1 < columns) v[r][i] |= (unsigned)p[r * ldx + 2 * i + 1] << 16;
+#pragma unroll
+                        for (int i = 0; i < EACH - 1; ++i)
+                            if (i < left) {
+                                if constexpr (WIDE) v[i] = p[16 * k * ldx + i];
+                                else v[i / 2] |= (unsigned)p[16 * k * ldx + i] << 16 * (i & 1);
+                            }
                     }
                 }
-        }
-        // Along columns.
-        unsigned most[4] = {0, 0, 0, 0};
-#pragma unroll
-        for (int r = 0; r < 32; ++r)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) most[i] = max_bits<DT>(most[i], v[r][i] & kMagnitude);
-#pragma unroll
-        for (int j = 0; j < CPL; ++j) {
-            constexpr unsigned kPick[2] = {0x05040100u, 0x07060302u};   // low halves of two dwords, high halves
-            const unsigned m = WIDE ? most[j % 4] : most[j / 2] >> 16 * (j & 1) & 0xFFFFu;
-            const unsigned s = scale_byte(magnitude_bits<DT>(m), fit);
-            u32x4 out;
-#pragma unroll
-            for (int d = 0; d < 4; ++d) {
-                unsigned w[Source<DT>::kWords];
-#pragma unroll
-                for (int i = 0; i < Source<DT>::kWords; ++i) {
-                    if constexpr (WIDE) w[i] = v[8 * d + i][j];
-                    else w[i] = __builtin_amdgcn_perm(v[8 * d + 2 * i + 1][j / 2], v[8 * d + 2 * i][j / 2], kPick[j & 1]);
-                }
-                out[d] = encode8<DT>(w, s);
-            }
-            const int64_t c = c0 + j;
-            if (c < columns) {
-                *reinterpret_cast<u32x4*>(qt + (c * units_t + unit_r) * kMx4UnitBytes + 16 * group) = out;
-                scales_t[(c * units_t + unit_r) * kMx4UnitScales + group] = (unsigned char)s;
+                piece(k) = v;
             }
         }
-        if constexpr (!ROWS) continue;
-        // Along rows. A lane keeps the scales of two of its group's rows, for whole dwords (fp32: halves) at the end.
-        unsigned kept[2] = {0, 0};
+        if constexpr (ROWS) {
+            // fp32: a tile is half a unit wide, and past the last column's unit there is nothing to write.
+            const int64_t unit_c = WIDE ? tile_c / 2 : tile_c;
+            const int part = WIDE ? (int)(tile_c % 2) : 0;
 #pragma unroll
-        for (int r = 0; r < 32; ++r) {
-            unsigned m = 0;
+            for (int k = 0; k < 8; ++k) {
+                const u32x4 v = piece(k);
+                unsigned m = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) m = max_bits<DT>(m, v[r][i] & kMagnitude);
-            if constexpr (!WIDE) m = max(m & 0xFFFFu, m >> 16);
-            m = max4(m);
-            if constexpr (WIDE) m = max(m, (unsigned)__builtin_amdgcn_mov_dpp((int)m, 0x141, 0xF, 0xF, true));   // l ^ 7
-            const unsigned s = scale_byte(magnitude_bits<DT>(m), fit);
-            unsigned code, bytes;
-            if constexpr (WIDE) {
-                const unsigned four[8] = {v[r][0], v[r][1], v[r][2], v[r][3], 0, 0, 0, 0};
-                const unsigned mine = encode8<DT>(four, s);
-                code = mine | lane_xor1(mine) << 16;       // even lanes: 8 elements
-                bytes = s << 8 * (l16 >> 3);
-            } else {
-                code = encode8<DT>(v[r], s);
-                bytes = s << 8 * (l16 >> 2);
-                bytes |= (unsigned)__builtin_amdgcn_mov_dpp((int)bytes, 0x124, 0xF, 0xF, true);   // four lanes round 16
-            }
-            bytes |= (unsigned)__builtin_amdgcn_mov_dpp((int)bytes, 0x128, 0xF, 0xF, true);       // eight
-            if (r0 + r < rows) {
-                unsigned char* to = q + ((r0 + r) * units + unit_c) * kMx4UnitBytes;
-                if constexpr (WIDE) {
-                    if (l16 % 2 == 0) *reinterpret_cast<unsigned*>(to + 32 * part + 2 * l16) = code;
-                } else {
-                    *reinterpret_cast<unsigned*>(to + 4 * l16) = code;
+                for (int i = 0; i < 4; ++i) m = max_bits<DT>(m, v[i] & kMagnitude);
+                if constexpr (!WIDE) m = max(m & 0xFFFFu, m >> 16);
+                m = max4(m);
+                if constexpr (WIDE) m = max(m, (unsigned)__builtin_amdgcn_mov_dpp((int)m, 0x141, 0xF, 0xF, true));   // 7 - l
+                const unsigned s = scale_byte(magnitude_bits<DT>(m), fit);
+                unsigned w[Source<DT>::kWords] = {};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = v[i];
+                const int r = tid / 16 + 16 * k;
+                if (r < row_count) {
+                    const int64_t unit = (r0 + r) * units + unit_c;
+                    if constexpr (WIDE) {
+                        *reinterpret_cast<uint16_t*>(q + unit * kMx4UnitBytes + 32 * part + 2 * l16) =
+                            (uint16_t)encode4<DT>(w, s);
+                        if (l16 % 8 == 0) scales[unit * kMx4UnitScales + 2 * part + l16 / 8] = (unsigned char)s;
+                    } else {
+                        *reinterpret_cast<unsigned*>(q + unit * kMx4UnitBytes + 4 * l16) = encode8<DT>(w, s);
+                        if (l16 % 4 == 0) scales[unit * kMx4UnitScales + l16 / 4] = (unsigned char)s;
+                    }
                 }
             }
-            kept[r & 1] = l16 == r / 2 ? bytes : kept[r & 1];
         }
+    }
+    __syncthreads();
+    const int group = tid % 4, at = tid / 4;   // 32 rows, dword of a row
+    const int64_t c = c0 + (WIDE ? at : 2 * at);
+    const unsigned* from = reinterpret_cast<const unsigned*>(tile) + 32 * group * 64 + (at ^ 16 * group);
+    unsigned v[32], most = 0;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int64_t r = r0 + 2 * l16 + i;
-            if (r >= rows) continue;
-            unsigned char* to = scales + (r * units + unit_c) * kMx4UnitScales;
-            if constexpr (WIDE) *reinterpret_cast<uint16_t*>(to + 2 * part) = (uint16_t)kept[i];
-            else *reinterpret_cast<unsigned*>(to) = kept[i];
+    for (int r = 0; r < 32; ++r) v[r] = from[r * 64];
+#pragma unroll
+    for (int r = 0; r < 32; ++r) most = max_bits<DT>(most, v[r] & kMagnitude);
+#pragma unroll
+    for (int j = 0; j < (WIDE ? 1 : 2); ++j) {
+        constexpr unsigned kPick[2] = {0x05040100u, 0x07060302u};   // low halves of two dwords, high halves
+        const unsigned s = scale_byte(magnitude_bits<DT>(WIDE ? most : most >> 16 * j & 0xFFFFu), fit);
+        u32x4 out;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            unsigned w[Source<DT>::kWords];
+#pragma unroll
+            for (int i = 0; i < Source<DT>::kWords; ++i) {
+                if constexpr (WIDE) w[i] = v[8 * d + i];
+                else w[i] = __builtin_amdgcn_perm(v[8 * d + 2 * i + 1], v[8 * d + 2 * i], kPick[j]);
+            }
+            out[d] = encode8<DT>(w, s);
+        }
+        unsigned four = s << 8 * group;   // the scales of a column's four blocks
+        four |= lane_xor1(four);
+        four |= lane_xor2(four);
+        if (c + j < columns) {
+            *reinterpret_cast<u32x4*>(qt + ((c + j) * units_t + unit_r) * kMx4UnitBytes + 16 * group) = out;
+            if (group == 0) *reinterpret_cast<unsigned*>(scales_t + ((c + j) * units_t + unit_r) * kMx4UnitScales) = four;
         }
     }
 }
 
-// 8 elements a lane, UNITS units a lane group.
-template <int DT, int UNITS>
+// 16 bytes of values a lane (8 elements, fp32: 4), RUNS of them, whose codes and scales are loaded before any is used.
+template <int DT, int RUNS>
 __global__ void __launch_bounds__(256)
-mx4_dequantize_kernel(const unsigned* __restrict__ q, const unsigned char* __restrict__ scales, int64_t rows,
+mx4_dequantize_kernel(const unsigned char* __restrict__ q, const unsigned char* __restrict__ scales, int64_t rows,
                       int64_t columns, int64_t units, typename Source<DT>::Element* __restrict__ out, int64_t ldo) {
-    const int64_t first = (int64_t)block_number() * (16 * UNITS) + threadIdx.x / 16;
-    const int lane16 = threadIdx.x % 16;
-    const int64_t total = rows * units;
-    unsigned codes[UNITS], bytes[UNITS];
+    constexpr bool WIDE = DT == MB_DT_FLOAT32;
+    constexpr int EACH = WIDE ? 4 : 8, LANES = kMx4Unit / EACH;   // elements per lane, lanes per unit
+    const int64_t first = (int64_t)block_number() * (256 * RUNS) + threadIdx.x, total = rows * units * LANES;
+    unsigned codes[RUNS], bytes[RUNS];
 #pragma unroll
-    for (int k = 0; k < UNITS; ++k) {
-        const int64_t unit = min(first + 16 * k, total - 1);
-        codes[k] = q[unit * 16 + lane16];
-        bytes[k] = scales[unit * 4 + lane16 / 4];
+    for (int k = 0; k < RUNS; ++k) {
+        const int64_t i = min(first + 256 * k, total - 1);
+        codes[k] = WIDE ? reinterpret_cast<const uint16_t*>(q)[i] : reinterpret_cast<const unsigned*>(q)[i];
+        bytes[k] = scales[i / (LANES / 4)];
     }
 #pragma unroll
-    for (int k = 0; k < UNITS; ++k) {
-        const int64_t unit = first + 16 * k;
-        if (unit >= total) return;
-        const int64_t row = unit / units, column = (unit - row * units) * kMx4Unit + 8 * lane16;
+    for (int k = 0; k < RUNS; ++k) {
+        const int64_t i = first + 256 * k;
+        if (i >= total) return;
+        const int64_t unit = i / LANES, row = unit / units;
+        const int64_t column = (unit - row * units) * kMx4Unit + EACH * (i % LANES);
         if (column >= columns) continue;
         const float scale = __builtin_bit_cast(float, bytes[k] << 23);
-        unsigned v[Source<DT>::kWords];
+        u32x4 v;
         auto two = [&](auto sel) {
             constexpr int s = decltype(sel)::value;
-            if constexpr (DT == MB_DT_FLOAT32) {
-                const auto f = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[k], scale, s);
-                v[2 * s] = __builtin_bit_cast(unsigned, (float)f[0]);
-                v[2 * s + 1] = __builtin_bit_cast(unsigned, (float)f[1]);
+            if constexpr (WIDE) {
+                if constexpr (s < 2) {
+                    const auto f = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[k], scale, s);
+                    v[2 * s] = __builtin_bit_cast(unsigned, (float)f[0]);
+                    v[2 * s + 1] = __builtin_bit_cast(unsigned, (float)f[1]);
+                }
             } else if constexpr (DT == MB_DT_BFLOAT16) {
                 v[s] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes[k], scale, s));
             } else {
@@ -318,15 +340,14 @@ mx4_dequantize_kernel(const unsigned* __restrict__ q, const unsigned char* __res
         two(std::integral_constant<int, 2>{});
         two(std::integral_constant<int, 3>{});
         auto* p = out + row * ldo + column;
-        if (column + 8 <= columns) {
-            *reinterpret_cast<u32x4_2*>(p) = u32x4{v[0], v[1], v[2], v[3]};
-            if constexpr (DT == MB_DT_FLOAT32) *reinterpret_cast<u32x4_2*>(p + 4) = u32x4{v[4], v[5], v[6], v[7]};
+        if (column + EACH <= columns) {
+            *reinterpret_cast<u32x4_2*>(p) = v;
             continue;
         }
 #pragma unroll
-        for (int e = 0; e < 7; ++e)
+        for (int e = 0; e < EACH - 1; ++e)
             if (column + e < columns) {
-                if constexpr (DT == MB_DT_FLOAT32) p[e] = v[e];
+                if constexpr (WIDE) p[e] = v[e];
                 else p[e] = (uint16_t)(v[e / 2] >> (16 * (e & 1)));
             }
     }
@@ -351,7 +372,7 @@ int quantize(const Mx4Quantize& c, hipStream_t stream) {
         if (total >= kManyUnits) launch(std::integral_constant<int, 4>{});
         else launch(std::integral_constant<int, 1>{});
     } else {
-        const int64_t tiles_m = (mx4_units(c.rows) + 1) / 2, tiles_n = (units + 1) / 2;
+        const int64_t tiles_m = mx4_units(c.rows), tiles_n = DT == MB_DT_FLOAT32 ? 2 * units : units;   // whole units
         auto kernel = q != nullptr ? mx4_quantize_tile_kernel<DT, true> : mx4_quantize_tile_kernel<DT, false>;
         hipLaunchKernelGGL(kernel, launch_grid(tiles_m * tiles_n), dim3(256), 0, stream, c.x, c.ldx, c.rows, c.columns,
                            c.fit, tiles_n, q, scales, static_cast<unsigned char*>(c.qt),
@@ -366,10 +387,11 @@ int dequantize(const void* q, const void* scales, int64_t rows, int64_t columns,
                hipStream_t stream) {
     typedef typename Source<DT>::Element Element;
     const int64_t units = mx4_units(columns), total = rows * units;
+    const int64_t lanes = total * (DT == MB_DT_FLOAT32 ? 32 : 16);
     auto launch = [&](auto many) {
         constexpr int N = decltype(many)::value;
-        hipLaunchKernelGGL((mx4_dequantize_kernel<DT, N>), launch_grid((total + 16 * N - 1) / (16 * N)), dim3(256), 0,
-                           stream, static_cast<const unsigned*>(q), static_cast<const unsigned char*>(scales), rows,
+        hipLaunchKernelGGL((mx4_dequantize_kernel<DT, N>), launch_grid((lanes + 256 * N - 1) / (256 * N)), dim3(256), 0,
+                           stream, static_cast<const unsigned char*>(q), static_cast<const unsigned char*>(scales), rows,
                            columns, units, static_cast<Element*>(out), ldo);
     };
     if (total >= kManyUnits) launch(std::integral_constant<int, 4>{});
