@@ -195,9 +195,17 @@ mx4_quantize_tile_kernel(const void* __restrict__ x, int64_t ldx, int64_t rows, 
     constexpr unsigned kMagnitude = WIDE ? 0x7FFFFFFFu : 0x7FFF7FFFu;
     __shared__ u32x4 tile[128 * 16];
     const int tid = threadIdx.x, l16 = tid % 16;
-    const int64_t block = block_number(), unit_r = block / tiles_n, tile_c = block - unit_r * tiles_n;
+    // Tiles in squares of 256 x 256: those of one XCD (block b runs on XCD b % 8), one after the other, so that its L2
+    // joins their halves (fp32: quarters) of both forms' lines of 128 bytes.
+    constexpr int WIDTH = 256 / COLUMNS, SQUARE = 2 * WIDTH;
+    const int64_t block = block_number(), local = block / 8, square = local / SQUARE * 8 + block % 8;
+    const int64_t squares_n = (tiles_n + WIDTH - 1) / WIDTH, square_r = square / squares_n;
+    const int within = (int)(local % SQUARE);
+    const int64_t unit_r = 2 * square_r + within / WIDTH;
+    const int64_t tile_c = (square - square_r * squares_n) * WIDTH + within % WIDTH;
     const int64_t units = (columns + kMx4Unit - 1) / kMx4Unit, units_t = (rows + kMx4Unit - 1) / kMx4Unit;
     const int64_t r0 = unit_r * kMx4Unit, c0 = tile_c * COLUMNS;
+    if (unit_r >= units_t || tile_c >= tiles_n) return;
     const int row_count = (int)min(rows - r0, (int64_t)kMx4Unit);
     auto piece = [&](int k) -> u32x4& {   // this lane's of row tid / 16 + 16 k
         const int r = tid / 16 + 16 * k;
@@ -372,10 +380,12 @@ int quantize(const Mx4Quantize& c, hipStream_t stream) {
         if (total >= kManyUnits) launch(std::integral_constant<int, 4>{});
         else launch(std::integral_constant<int, 1>{});
     } else {
-        const int64_t tiles_m = mx4_units(c.rows), tiles_n = DT == MB_DT_FLOAT32 ? 2 * units : units;   // whole units
+        const int64_t tiles_n = DT == MB_DT_FLOAT32 ? 2 * units : units;   // whole units
+        const int64_t squares = ((mx4_units(c.rows) + 1) / 2) * ((units + 1) / 2);
+        const int64_t blocks = (squares + 7) / 8 * 8 * (DT == MB_DT_FLOAT32 ? 8 : 4);
         auto kernel = q != nullptr ? mx4_quantize_tile_kernel<DT, true> : mx4_quantize_tile_kernel<DT, false>;
-        hipLaunchKernelGGL(kernel, launch_grid(tiles_m * tiles_n), dim3(256), 0, stream, c.x, c.ldx, c.rows, c.columns,
-                           c.fit, tiles_n, q, scales, static_cast<unsigned char*>(c.qt),
+        hipLaunchKernelGGL(kernel, launch_grid(blocks), dim3(256), 0, stream, c.x, c.ldx, c.rows, c.columns, c.fit,
+                           tiles_n, q, scales, static_cast<unsigned char*>(c.qt),
                            static_cast<unsigned char*>(c.scales_t));
     }
     MB_HIP_TRY(hipGetLastError());
