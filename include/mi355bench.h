@@ -352,8 +352,8 @@ int mb_mx4_dequantize(int dtype, const void* q, const void* scales, int64_t rows
  *
  * x: x_rows rows, w: experts x N rows, both along K and MX4; out: BFLOAT16 or FLOAT16.
  * Sums are fp32, rounded once. NaN blocks make their rows' (columns') outputs NaN. Output rows
- * at and past offsets[experts] are left alone; rows that are not there give zeros.
- * 1 <= K <= MB_MX4_MAX_K, 1 <= N < 2^30. x, w and out must not overlap.
+ * before offsets[0] and from offsets[experts] on are left alone; rows that are not there count as zeros.
+ * 1 <= K <= MB_MX4_MAX_K, 1 <= N < 2^30, total_rows <= 2^31 - 256. x, w and out must not overlap.
  * workspace: any size, NULL included; calls of few tiles run faster with one on
  * 16 bytes that holds 2 to 16 fp32 copies of out (they split K).
  */

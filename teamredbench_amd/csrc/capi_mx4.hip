@@ -88,7 +88,8 @@ int mb_gemm_mx4(int dtype, const void* x, const void* x_scales, int64_t x_rows, 
     if (!leading(&ldo, N, total_rows))
         return refuse(MB_ERR_INVALID_ARG, "mb_gemm_mx4: leading dimension %lld is below N = %lld", (long long)ldo,
                       (long long)N);
-    if (total_rows / 32 + experts >= kMostBlocks / ((N + 31) / 32))
+    // Ends of tiles of up to 256 rows are int32 too.
+    if (total_rows > kMostRows - 256 || total_rows / 32 + experts >= kMostBlocks / ((N + 31) / 32))
         return refuse(MB_ERR_SHAPE, "mb_gemm_mx4: too many tiles for one launch");
     const DeviceProps* props = nullptr;
     if (total_rows == 0) return device_for_launch(&props);

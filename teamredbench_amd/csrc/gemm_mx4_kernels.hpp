@@ -88,7 +88,7 @@ constexpr Mx4Waits mx4_schedule(int slots, int pair, int chunk, int groups, int 
 // Row tile and column of tile t: as in block_coords, in groups of kGroupM row tiles (without K splits, whose blocks
 // take block_coords), dividing by a multiplication: `magic` is 2^40 / (kGroupM tiles_n), rounded up.
 constexpr int kGroupM = 4;
-__device__ __forceinline__ void tile_coords(int b, int tiles, int tiles_m, int tiles_n, uint64_t magic, int* tm,
+__host__ __device__ __forceinline__ void tile_coords(int b, int tiles, int tiles_m, int tiles_n, uint64_t magic, int* tm,
                                             int* tn) {
     const int t = (b & 7) * (tiles >> 3) + min(b & 7, tiles & 7) + (b >> 3);
     const int per_group = kGroupM * tiles_n;
@@ -127,7 +127,8 @@ gemm_mx4_kernel(Mx4Args all_args, int tiles_n, uint64_t magic) {
     constexpr int GC = WTN < 64 ? WTN : 64, STAGE = 32 * GC * 2, PIECES = STAGE / 1024;
     constexpr int STAGE0 = PERSISTENT ? XS0 + NEXT_SCALES : 0;
     constexpr int GROUPS = FM * (WTN / GC);                  // of a wave's tile
-    static_assert(!PERSISTENT || 4 * STAGE <= NEXT_SCALES, "the staged groups fit the second scale slot");
+    static_assert(!PERSISTENT || (4 * STAGE == NEXT_SCALES && STAGE == SCALE_INSTR * 1024),
+                  "a wave stages its stores in what its own loads of the second scale slot fill");
     constexpr Mx4Waits kWaits = mx4_schedule(SLOTS, 2 * INSTR, SCALE_INSTR, GROUPS, PIECES);
     static_assert([&] {
         for (int w : kWaits.step)
@@ -167,7 +168,9 @@ gemm_mx4_kernel(Mx4Args all_args, int tiles_n, uint64_t magic) {
     {
         const Mx4Args args = arguments();
         const bool by_expert = args.offsets != nullptr;
-        tiles_m = by_expert ? count_row_tiles(args.offsets, args.experts, args.total, BM)
+        // Offsets out of order may count any number of tiles.
+        tiles_m = by_expert ? min(count_row_tiles(args.offsets, args.experts, args.total, BM),
+                                  args.total / BM + min(args.experts, args.total))
                             : (args.total + BM - 1) / BM;
         tiles = tiles_m * tiles_n * args.splits;
         if (t >= tiles) return;
@@ -252,7 +255,7 @@ gemm_mx4_kernel(Mx4Args all_args, int tiles_n, uint64_t magic) {
         const bool gather = args.rows != nullptr;
         const int64_t x_first = gather ? 0 : (int64_t)tile.ex.first + tile.m0;
         const int64_t w_first = (int64_t)tile.ex.expert * args.N + tile.n0;
-        const int x_count = gather ? args.x_rows : min(tile.ex.count - tile.m0, BM);
+        const int x_count = gather ? args.x_rows : max(min(tile.ex.count - tile.m0, BM), 0);
         const int w_count = min(args.N - tile.n0, BN);
         Loads l;
         l.x = resource(args.x, x_first, args.ld, x_count);
@@ -323,7 +326,7 @@ gemm_mx4_kernel(Mx4Args all_args, int tiles_n, uint64_t magic) {
     };
     constexpr std::integral_constant<int, FIRST_LOADS> kFirstLoads{};
     constexpr std::integral_constant<int, SCALE_INSTR> kScalePieces{};
-    // Chunk 1, where a persistent block's stores are staged. Past the row's end: zeros or other scales, unused.
+    // Chunk 1, where a persistent block's stores are staged: a wave's loads fill what the wave itself staged. Past the row's end: zeros or other scales, unused.
     auto second_chunk = [&] { all(kScalePieces, [&](auto q) { issue_scales(1, q); }); };
 
     f32x16 acc[FM][FN];

@@ -62,7 +62,10 @@ inline Mx4Plan mx4_plan(const Mx4Shape& s, size_t workspace_bytes, int cus, int6
         if (rows <= 8) return {kMx4Rows8, 1};
         if (!s.by_expert && (rows <= 32 || (rows <= 64 && 2 * columns <= cus))) return {kMx4Rows32, 1};
     }
-    if (config >= kMx4TileCount) return {(int)config, 1};
+    if (config >= kMx4TileCount) {
+        const double rows8 = std::ceil((double)s.total_rows / 8) + s.experts, columns = (double)(s.N / 32 + 8);
+        return {config == kMx4Rows8 && rows8 * columns >= (double)(1 << 30) ? kMx4Rows32 : (int)config, 1};   // int32
+    }
 
     // The tile and split count whose predicted time is least. Splits cost a second launch and their planes, written
     // and read, and none has less than 16 units; each smaller tile or further split has to gain 3%.

@@ -1,0 +1,52 @@
+// Host code, compiled from the MX4 products' own headers by tests/test_mx4_plan.py.
+//   plan   "config splits" for each line "total_rows experts N units by_expert listed x_rows workspace cus config splits"
+//   waits  "slots pair chunk groups pieces persistent step[8] prologue behind_prologue behind[3]" of every tile
+//   tiles  "tm tn" of every tile of tiles_m x tiles_n, for each line "tiles_m tiles_n", then an empty line
+#include <cstdio>
+#include <cstring>
+
+#include "../teamredbench_amd/csrc/gemm_mx4_kernels.hpp"
+
+using namespace mb;
+
+template <int CFG>
+void print_waits() {   // the constants of gemm_mx4_kernel<DT, CFG>
+    const int size = kMx4Tiles[CFG].size, slots = kMx4Tiles[CFG].slots, wave = size / 2, wide = wave < 64 ? wave : 64;
+    const int pair = 2 * (size * kPairBytes / 1024 / 4), chunk = 2 * size * kChunkBytes / 1024 / 4;
+    const int groups = wave / 32 * (wave / wide), pieces = 32 * wide * 2 / 1024;
+    const Mx4Waits w = mx4_schedule(slots, pair, chunk, groups, pieces);
+    std::printf("%d %d %d %d %d %d", slots, pair, chunk, groups, pieces, size == 256);
+    for (int s : w.step) std::printf(" %d", s);
+    std::printf(" %d %d %d %d %d\n", w.prologue, w.behind_prologue, w.behind[0], w.behind[1], w.behind[2]);
+}
+
+int main(int, char** argv) {
+    if (!std::strcmp(argv[1], "plan")) {
+        Mx4Shape s;
+        int by_expert, listed, cus;
+        long long total, n, units, x_rows, workspace, config, splits;
+        while (std::scanf("%lld %d %lld %lld %d %d %lld %lld %d %lld %lld", &total, &s.experts, &n, &units, &by_expert,
+                          &listed, &x_rows, &workspace, &cus, &config, &splits) == 11) {
+            s = {total, n, units, x_rows, s.experts, by_expert != 0, listed != 0};
+            const Mx4Plan p = mx4_plan(s, (size_t)workspace, cus, config, splits);
+            std::printf("%d %d\n", p.config, p.splits);
+        }
+    } else if (!std::strcmp(argv[1], "waits")) {
+        print_waits<0>();
+        print_waits<1>();
+        print_waits<2>();
+        print_waits<3>();
+    } else {
+        int tiles_m, tiles_n;
+        while (std::scanf("%d %d", &tiles_m, &tiles_n) == 2) {
+            const uint64_t per_group = (uint64_t)kGroupM * tiles_n, magic = ((1ull << 40) + per_group - 1) / per_group;
+            for (int t = 0; t < tiles_m * tiles_n; ++t) {
+                int tm, tn;
+                tile_coords(t, tiles_m * tiles_n, tiles_m, tiles_n, magic, &tm, &tn);
+                std::printf("%d %d\n", tm, tn);
+            }
+            std::printf("\n");
+        }
+    }
+    return 0;
+}

@@ -1,0 +1,172 @@
+"""Which kernel an MX4 product runs on, its tiles' order, and its loads' order and waits (CPU): the kernels' own
+host code, compiled and replayed."""
+from __future__ import annotations
+
+from pathlib import Path
+import shutil
+import subprocess
+
+import pytest
+
+from teamredbench_amd.native import capi
+
+TESTS = Path(__file__).resolve().parent
+WORKSPACE = 64 << 20
+T256, T128, T128_DEEP, T64, ROWS8, ROWS32, ANY = range(7)
+
+# (rows, N, K) -> configuration at 256 CUs: both sides of the bounds on rows, and the calls whose times are quoted
+DENSE = [
+    ((1, 14336, 4096), ROWS8), ((8, 50257, 4096), ROWS8), ((9, 50257, 4096), ROWS32), ((32, 14336, 4096), ROWS32),
+    ((33, 4096, 4096), ROWS32), ((64, 4096, 4096), ROWS32), ((64, 4097, 4096), T64), ((65, 4096, 4096), T64),
+    ((64, 14336, 4096), T64), ((64, 50257, 4096), T128), ((256, 4096, 4096), T64), ((1024, 4096, 4096), T128_DEEP),
+    ((2048, 4096, 4096), T128), ((8192, 8192, 8192), T256), ((4096, 14336, 4096), T256), ((300, 264, 1000), T64),
+]
+# (rows, experts, N, K) by expert
+EXPERTS = [((256, 64, 2048, 4096), ROWS8), ((512, 64, 2048, 4096), ROWS8), ((16384, 8, 14336, 4096), T256)]
+
+
+@pytest.fixture(autouse=True)
+def _no_error_left():
+    yield
+    capi.load_library().set_tuning("mx4_config", None)   # a call that succeeds clears the thread's last error
+
+
+@pytest.fixture(scope="module")
+def host(tmp_path_factory):
+    hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
+    exe = tmp_path_factory.mktemp("mx4") / "mx4_plan_host"
+    subprocess.run([hipcc, "--offload-host-only", "-O1", "-std=c++20", "-w", str(TESTS / "mx4_plan_host.cpp"),
+                    "-o", str(exe)], check=True)
+
+    def run(what: str, lines=()) -> list[tuple[int, ...]]:
+        text = "".join(" ".join(map(str, line)) + "\n" for line in lines)
+        out = subprocess.run([str(exe), what], input=text, capture_output=True, text=True, check=True).stdout
+        return [tuple(int(v) for v in line.split()) for line in out.splitlines()]
+
+    return run
+
+
+def _call(rows, n, k, *, experts=1, by_expert=False, listed=False, x_rows=None, workspace=WORKSPACE, cus=256, config=-1,
+          splits=-1):
+    return (rows, experts, n, -(-k // 128), int(by_expert), int(listed), rows if x_rows is None else x_rows, workspace,
+            cus, config, splits)
+
+
+def test_picks(host):
+    picked = host("plan", [_call(*shape) for shape, _ in DENSE])
+    assert [config for config, _ in picked] == [config for _, config in DENSE]
+    calls = [_call(rows, n, k, experts=e, by_expert=True, listed=True) for (rows, e, n, k), _ in EXPERTS]
+    assert [config for config, _ in host("plan", calls)] == [config for _, config in EXPERTS]
+
+
+def test_k_is_split_only_over_a_workspace_that_holds_the_sums(host):
+    rows, n, k = 128, 512, 8192
+    plane = 4 * rows * n
+    with_one, = host("plan", [_call(rows, n, k)])
+    assert with_one == (T64, 4)
+    assert host("plan", [_call(rows, n, k, workspace=0), _call(rows, n, k, workspace=4 * plane - 1)]) == [(T64, 1), (T64, 2)]
+    assert host("plan", [_call(rows, n, k, config=T128, splits=5), _call(rows, n, k, config=T256, splits=5),
+                         _call(rows, n, k, config=ROWS32, splits=5)]) == [(T128, 5), (T256, 1), (ROWS32, 1)]
+
+
+def test_lists_over_more_than_2_to_31_bytes_take_the_kernel_for_any_size(host):
+    row = 64 * 32   # bytes at K = 4096
+    fits = ((1 << 31) - 1) // row
+    for rows in (1, 100, 8192):
+        calls = [_call(rows, 4096, 4096, listed=True, x_rows=x_rows, config=c) for x_rows in (fits, fits + 1)
+                 for c in (-1, T256)]
+        picked = [config for config, _ in host("plan", calls)]
+        assert ANY not in picked[:2] and picked[2:] == [ANY, ANY]
+    assert host("plan", [_call(fits + 1, 4096, 4096, config=T64)])[0][0] == T64   # without a list: tile by tile
+
+
+def test_tiles_of_8_rows_past_2_to_30_blocks_give_way(host):
+    rows = (1 << 31) - 256
+    assert [c for c, _ in host("plan", [_call(rows, 1, 1, config=ROWS8), _call(1 << 20, 32, 1, config=ROWS8)])] == \
+        [ROWS32, ROWS8]
+
+
+def test_every_tile_once(host):
+    """Each tile of a launch is one of the matrix's, and none comes twice."""
+    shapes = [(1, 1), (1, 300), (300, 1), (4, 4), (5, 7), (16, 56), (31, 33), (32, 32), (63, 196), (129, 11), (2, 4093)]
+    out = iter(host("tiles", shapes))
+    for tiles_m, tiles_n in shapes:
+        tiles = []
+        while (line := next(out)):
+            tiles.append(line)
+        assert len(tiles) == tiles_m * tiles_n == len(set(tiles))
+        assert all(0 <= m < tiles_m and 0 <= n < tiles_n for m, n in tiles)
+
+
+# ---- the loads' order and the waits -------------------------------------------
+
+
+def _loads(first: int, groups: int, pieces: int) -> list[str]:
+    """What a persistent block issues for its next tile while it stores one: "L" loads, "S" stores."""
+    order = []
+    for g in range(groups):
+        order += ["L"] * sum(l * 4 // first == g for l in range(first) if g < 4)
+        order += ["S"] * (pieces if g > 0 else 0)
+    return order + ["S"] * pieces
+
+
+def _replay(slots, pair, chunk, groups, pieces, behind, step, prologue, first_waits) -> str | None:
+    """What goes wrong, or None. A wave's memory operations complete in the order of their issue; a wait for n leaves the
+    n newest in flight."""
+    queue = [("chunk", 0)] * chunk + [("pair", p) for p in range(slots) for _ in range(pair)]
+    if behind:
+        first, at = len(queue), iter(queue)
+        queue = [next(at) if what == "L" else ("store", 0) for what in _loads(first, groups, pieces)]
+        assert next(at, None) is None
+    queue += [("chunk", 1)] * chunk
+
+    def landed(unit: int, wait: int) -> bool:
+        done = queue[:len(queue) - wait]
+        return done.count(("pair", unit // 2)) == pair and done.count(("chunk", unit // 8)) == chunk
+
+    if not 0 <= prologue < 64 or not landed(0, prologue):
+        return "unit 0 has not landed"
+    for j in range(60):
+        wait = first_waits[j] if behind and j < 3 else step[j % 8]
+        if not 0 <= wait < 64 or not landed(j + 1, wait):
+            return f"unit {j + 1} has not landed at step {j}"
+        if j % 2:   # over the pair of units j - 1 and j, the last of which step j - 1 has read
+            new = (j - 1) // 2 + slots
+            if 2 * (new - slots) + 1 > j:
+                return f"pair {new} overwrites a pair that is not read"
+            queue += [("pair", new)] * pair
+        if j % 8 == 7:
+            new = (j - 7) // 8 + 2
+            if 8 * (new - 2) + 7 > j:
+                return f"chunk {new} overwrites a chunk that is not read"
+            queue += [("chunk", new)] * chunk
+    return None
+
+
+def test_no_step_reads_before_its_loads_land(host):
+    tiles = host("waits")
+    assert len(tiles) == 4 and [t[5] for t in tiles] == [1, 0, 0, 0]
+    for slots, pair, chunk, groups, pieces, persistent, *waits in tiles:
+        step, (prologue, behind_prologue), behind = waits[:8], waits[8:10], waits[10:]
+        assert _replay(slots, pair, chunk, groups, pieces, False, step, prologue, []) is None
+        if persistent:
+            assert _replay(slots, pair, chunk, groups, pieces, True, step, behind_prologue, behind) is None
+        # a wait that leaves one more in flight is noticed
+        for j in range(8):
+            longer = [w + (i == j) for i, w in enumerate(step)]
+            assert _replay(slots, pair, chunk, groups, pieces, False, longer, prologue, []) is not None
+        assert _replay(slots, pair, chunk, groups, pieces, False, step, prologue + 1, []) is not None
+        for j in range(3 if persistent else 0):
+            longer = [w + (i == j) for i, w in enumerate(behind)]
+            assert _replay(slots, pair, chunk, groups, pieces, True, step, behind_prologue, longer) is not None
+
+
+def test_the_knobs_take_every_configuration_and_no_other():
+    lib = capi.load_library()
+    for knob, good, bad in (("mx4_config", range(7), (7, -2)), ("mx4_splits", (1, 2, 5, 16), (0, 17))):
+        for value in good:
+            with lib.tuned(**{knob: value}):
+                assert lib.get_tuning(knob) == value
+        for value in bad:
+            with pytest.raises(capi.NativeLibraryError, match="cannot take"):
+                lib.set_tuning(knob, value)

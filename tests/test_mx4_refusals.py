@@ -43,6 +43,7 @@ REFUSED = [
     ("gemm_mx4", GEMM, dict(n=1 << 30), INVALID), ("gemm_mx4", GEMM, dict(k=0), INVALID),
     ("gemm_mx4", GEMM, dict(k=capi.MX4_MAX_K + 1), SHAPE), ("gemm_mx4", GEMM, dict(ldo=15), INVALID),
     ("gemm_mx4", GEMM, dict(total_rows=(1 << 31) - 1, x_rows=(1 << 31) - 1, n=1 << 20), SHAPE),
+    ("gemm_mx4", GEMM, dict(total_rows=(1 << 31) - 255, x_rows=(1 << 31) - 255, n=1, k=1), SHAPE),
     ("gemm_mx4", GEMM, dict(x=None), INVALID), ("gemm_mx4", GEMM, dict(x_scales=None), INVALID),
     ("gemm_mx4", GEMM, dict(w=None), INVALID), ("gemm_mx4", GEMM, dict(w_scales=None), INVALID),
     ("gemm_mx4", GEMM, dict(out=None), INVALID), ("gemm_mx4", GEMM, dict(out=P + 1), SHAPE),
