@@ -30,23 +30,17 @@ mb_combine and their gradients) on torch's current stream; torch owns the memory
 """
 from __future__ import annotations
 
-import copy
-import itertools
 from typing import Any
 
-from teamredbench_amd.benchmarks.base import Benchmark, BenchmarkRecord
-from teamredbench_amd.benchmarks.mfu import INFINITY_CACHE_BYTES, MAX_OPERAND_SETS, OPERAND_FOOTPRINT_TARGET
-from teamredbench_amd.device import rocm_device_available
+from teamredbench_amd.benchmarks.layers import Layer, LayerBenchmark, moved_or_product_bytes, parity_of  # noqa: F401
 from teamredbench_amd.native import capi
-from teamredbench_amd.parity import gemm_parity
 from teamredbench_amd.registry import register_benchmark
-from teamredbench_amd.utils import tensor_nbytes, timed_iterations
 
 GRADIENTS = ("combine_grad", "rows_grad", "up_grad", "route_grad")
 DEFAULT_LAYERS = [{"tokens": 4096, "experts": 16, "top_k": 4, "k": 4096, "n": 2048}]
 
 
-class ExpertLayer:
+class ExpertLayer(Layer):
     """The buffers of one layer and its operators' calls, forward and backward."""
 
     def __init__(self, torch: Any, lib: capi.NativeLibrary, dtype: str, layer: dict[str, int], device: Any, seed: int):
@@ -55,6 +49,8 @@ class ExpertLayer:
             int(layer[name]) for name in ("tokens", "experts", "top_k", "k", "n"))
         self.group = int(layer.get("group", 0))
         self.total = self.tokens * self.top_k
+        self.suffix = f"t{self.tokens}e{self.experts}k{self.top_k}_{self.k}x{self.n}"
+        self.differentiable = not self.group
         self.stream = torch.cuda.current_stream(device).cuda_stream
         generator = torch.Generator(device=device).manual_seed(seed)
         half = getattr(torch, dtype)
@@ -88,18 +84,6 @@ class ExpertLayer:
         self.grad_y, self.grad_weights = torch.empty_like(self.y), torch.empty_like(self.weights)
         self.grad_hidden, self.grad_up = torch.empty_like(self.hidden), torch.empty_like(self.up)
         self.grad_logits = torch.empty_like(self.logits)
-
-    def buffers(self) -> dict[str, Any]:
-        """Every tensor of the layer but the workspace, by attribute."""
-        return {name: value for name, value in vars(self).items()
-                if isinstance(value, self.torch.Tensor) and name != "workspace"}
-
-    def clone(self) -> "ExpertLayer":
-        """The same layer on buffers of its own. The workspace, which no call leaves anything in, is shared."""
-        other = copy.copy(self)
-        for name, value in self.buffers().items():
-            setattr(other, name, value.clone())
-        return other
 
     def backward(self) -> None:
         for name in GRADIENTS:
@@ -220,28 +204,12 @@ class ExpertLayer:
         return {"grad_logits": ("float32", self.grad_logits[:tokens], wanted)}
 
 
-def _bytes(work: dict[str, int]) -> int:
-    return work.get("gemm_bytes", 0) or work.get("moved_bytes", 0)
-
-
-def parity_of(torch: Any, checked: dict[str, tuple[str, Any, Any]]) -> dict[str, Any]:
-    """The parity of the output that is nearest to its bound, or furthest over it, and every output's distance."""
-    each = {name: gemm_parity(torch, dtype, got, want) if torch.count_nonzero(want) else
-            {"rel_frobenius": 0.0, "bound": 0.0, "passed": not torch.count_nonzero(got)}
-            for name, (dtype, got, want) in checked.items()}
-    worst = max(each.values(), key=lambda p: (not p["passed"], p["rel_frobenius"] / p["bound"] if p["bound"] else 0.0))
-    return {"vs": "torch", **{key: worst[key] for key in ("rel_frobenius", "bound")},
-            "passed": all(p["passed"] for p in each.values()),
-            "outputs": {name: p["rel_frobenius"] for name, p in each.items()}}
-
-
 @register_benchmark("experts")
-class ExpertsBenchmark(Benchmark):
-    default_metrics = ["latency_us", "achieved_tops", "mfu_pct", "hbm_bandwidth_gbps", "gemm_bandwidth_gbps"]
+class ExpertsBenchmark(LayerBenchmark):
+    layer_type, default_layers, what = ExpertLayer, DEFAULT_LAYERS, "the expert layer"
+    checks = gradients = GRADIENTS
 
     def _operators(self, layer: ExpertLayer, size: int, backward: bool) -> list[tuple[str, str, dict]]:
-        """(name, the layer's method, what it computes and moves) of each operator, inputs read once and outputs
-        written once."""
         tokens, experts, total, k, n = layer.tokens, layer.experts, layer.total, layer.k, layer.n
         hit = min(experts, total)
         product = {"achieved_ops": 2 * total * k * n}
@@ -254,7 +222,7 @@ class ExpertsBenchmark(Benchmark):
             ("down", "down_product", {**product, "gemm_bytes": down + total * (n + k) * size}),
             ("combine", "combine", {"moved_bytes": (total + tokens) * k * size + total * 8}),
         ]
-        moved = sum(_bytes(work) for _, _, work in operators)
+        moved = sum(moved_or_product_bytes(work) for _, _, work in operators)
         operators.append(("layer", "forward", {"achieved_ops": 4 * total * k * n, "gemm_bytes": moved}))
         if backward:
             operators += [
@@ -265,99 +233,3 @@ class ExpertsBenchmark(Benchmark):
                 ("route_grad", "route_grad", {"moved_bytes": 2 * tokens * experts * 4 + total * 8}),
             ]
         return operators
-
-    def _operand_sets(self, operators: list[tuple[str, str, dict]], peak_tops: float | None, set_bytes: int,
-                      free_bytes: int) -> int:
-        """Copies of the layer to cycle through (see the module's operand_sets)."""
-        requested = self.params.get("operand_sets", "auto")
-        if requested != "auto":
-            return max(1, int(requested))
-        hbm = self.context.hardware_profile.peak_hbm_bandwidth_gbps
-        if not peak_tops or not hbm:
-            return 1
-        ridge = peak_tops * 1e12 / (hbm * 1e9)
-        bound = [work["gemm_bytes"] for name, _, work in operators
-                 if name != "layer" and "gemm_bytes" in work and work["achieved_ops"] < ridge * work["gemm_bytes"]]
-        if not bound:
-            return 1
-        sets = -(-OPERAND_FOOTPRINT_TARGET // min(bound))
-        return max(1, min(sets, MAX_OPERAND_SETS, free_bytes // 2 // set_bytes))
-
-    def _cases(self, lib, torch, spec, shape: dict[str, int], peak_tops) -> list[BenchmarkRecord]:
-        peak_hbm = self.context.hardware_profile.peak_hbm_bandwidth_gbps
-        warmup, iterations = int(self.params.get("warmup", 10)), int(self.params.get("iterations", 50))
-        layer = ExpertLayer(torch, lib, spec.name, shape, self.device, int(self.params.get("seed", 0)))
-        backward = bool(self.params.get("backward", True)) and not layer.group
-        layer.forward()
-        if backward:
-            layer.prepare_backward()
-            layer.backward()
-        suffix = f"t{layer.tokens}e{layer.experts}k{layer.top_k}_{layer.k}x{layer.n}"
-        operators = self._operators(layer, spec.bytes_per_element, backward)
-        set_bytes = sum(tensor_nbytes(value) for value in layer.buffers().values())
-        sets = self._operand_sets(operators, peak_tops, set_bytes, torch.cuda.mem_get_info(self.device)[0])
-        layers = [layer, *(layer.clone() for _ in range(sets - 1))]
-        times = {}
-        for name, method, _ in operators:
-            calls = itertools.cycle([getattr(one, method) for one in layers])
-            times[name] = timed_iterations(lambda: next(calls)(), torch_module=torch, warmup=warmup,
-                                           iterations=iterations)
-        del layers, calls
-        rows = min(layer.tokens, int(self.params.get("verify_max_tokens", 64)))
-        parity: dict[str, dict[str, Any]] = {}
-        if bool(self.params.get("verify", True)):
-            for name in ("forward", *(GRADIENTS if backward else ())):
-                checked = getattr(layer, f"check_{name}")(rows)
-                parity[name] = {**parity_of(torch, checked), "rows_checked": rows}
-        records = []
-        for name, _, work in operators:
-            metadata = {"backend": "native", "kernel": "experts_gfx950", "operator": name, "timing": "wall_clock",
-                        "operand_sets": sets, "operand_footprint_bytes": sets * _bytes(work),
-                        "cache_resident": sets * _bytes(work) <= INFINITY_CACHE_BYTES,
-                        **{key: int(value) for key, value in shape.items()}}
-            check = name if name in GRADIENTS else "forward"
-            if check in parity:
-                metadata["parity"] = parity[check]
-            raw = {"elapsed_s": times[name], **work}
-            if "achieved_ops" in work:
-                raw["peak_tops"] = peak_tops
-            if "moved_bytes" in work:
-                raw["peak_bandwidth_gbps"] = peak_hbm
-            records.append(self.measured(case=f"experts_{name}_{suffix}", dtype=spec.name, raw_metrics=raw,
-                                         metadata=metadata))
-        return records
-
-    def run(self) -> list[BenchmarkRecord]:
-        backend = str(self.params.get("backend", "native")).lower()
-        if backend != "native":
-            raise KeyError(f"Unknown experts backend: {backend}")
-        layers = [dict(layer) for layer in self.params.get("layers", DEFAULT_LAYERS)]
-        specs = self.selected_dtype_specs()
-        torch = self.context.torch_module
-        why, lib = None, None
-        try:
-            lib = capi.load_library()
-        except capi.NativeLibraryError as exc:
-            why = str(exc)
-        if why is None and not rocm_device_available(torch):
-            why = "No ROCm device visible to PyTorch."
-        if why is None:
-            self.set_device()
-        records: list[BenchmarkRecord] = []
-        for spec in specs:
-            peak_tops = self.context.hardware_profile.peak_compute_tops.get(spec.name)
-            for shape in layers:
-                case = "experts_" + "_".join(f"{key}{value}" for key, value in shape.items())
-                unsupported = spec.name not in capi.EXPERT_DTYPES
-                if why is not None or unsupported:
-                    error = why or f"unsupported dtype for the expert layer: {spec.name}"
-                    records.append(self.skip(case=case, dtype=spec.name, error=error, metadata={"backend": "native"}))
-                    continue
-                try:
-                    records += self._cases(lib, torch, spec, shape, peak_tops)
-                except (capi.NativeLibraryError, RuntimeError) as exc:
-                    records.append(self.skip(case=case, dtype=spec.name, error=str(exc),
-                                             metadata={"backend": "native"}))
-                finally:
-                    torch.cuda.empty_cache()
-        return records

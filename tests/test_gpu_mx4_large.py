@@ -1,0 +1,163 @@
+"""MX4 calls past 2^31 bytes, 2^31 outputs, 2^32 threads, and at the largest K; workspaces and streams (-m gpu).
+Sums are exact in fp32 in any order, so every result has to match bit for bit."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import mx4_inputs as mx4
+from teamredbench_amd.benchmarks.mx4 import values_of
+from teamredbench_amd.native import capi
+
+pytestmark = pytest.mark.gpu
+BF = capi.DT_BFLOAT16
+
+
+def _stream() -> int:
+    return torch.cuda.current_stream().cuda_stream
+
+
+def _random(rows: int, columns: int, seed: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """tests/mx4_inputs.py's random matrix, made on the GPU; columns: whole units."""
+    assert columns % 128 == 0
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    q = torch.empty(rows, columns // 2, dtype=torch.uint8, device="cuda").random_(0, 256, generator=g)
+    return q, torch.empty(rows, columns // 32, dtype=torch.uint8, device="cuda").random_(126, 129, generator=g)
+
+
+def _gemm(lib, x, w, out, k, *, rows=None, workspace=None, stream=None):
+    lib.gemm_mx4(BF, x[0].data_ptr(), x[1].data_ptr(), x[0].shape[0], None if rows is None else rows.data_ptr(),
+                 w[0].data_ptr(), w[1].data_ptr(), out.data_ptr(), 0, None, 1, out.shape[0], out.shape[1], k,
+                 None if workspace is None else workspace.data_ptr(), 0 if workspace is None else workspace.numel(),
+                 stream or _stream())
+
+
+def test_a_list_over_more_than_2_to_31_bytes(lib):
+    k, n = 4096, 200
+    x, w = _random((1 << 20) + 50, k, 1), _random(n, k, 2)
+    assert x[0].numel() > 1 << 31
+    g = torch.Generator().manual_seed(3)
+    rows = torch.randint(0, x[0].shape[0], (300,), generator=g).to(torch.int32)
+    rows[:3] = torch.tensor([x[0].shape[0] - 1, 1 << 20, (1 << 20) - 1])
+    out = torch.empty(300, n, dtype=torch.bfloat16, device="cuda")
+    _gemm(lib, x, w, out, k, rows=rows.cuda())
+    at = rows.long().cuda()
+    exact = values_of(torch, x[0][at], x[1][at], k).double() @ values_of(torch, w[0], w[1], k).double().t()
+    assert torch.equal(out, exact.float().bfloat16())
+
+
+@pytest.mark.parametrize("config", [None, 0, 1, 3, 5, 6])
+def test_outputs_past_2_to_31(lib, tune, config):
+    tune(mx4_config=config)
+    n, k = 2050, 128
+    rows = (1 << 31) // n + 300
+    x, w = _random(rows, k, 4), _random(n, k, 5)
+    out = torch.full((rows, n), 7.0, dtype=torch.bfloat16, device="cuda")
+    _gemm(lib, x, w, out, k)
+    wv = values_of(torch, w[0], w[1], k).t().contiguous()
+    for lo in range(0, rows, 1 << 17):
+        hi = min(lo + (1 << 17), rows)
+        wanted = values_of(torch, x[0][lo:hi], x[1][lo:hi], k) @ wv   # exact: any order
+        assert torch.equal(out[lo:hi], wanted.bfloat16()), lo
+
+
+@pytest.mark.parametrize("config", [None, 0, 2, 5, 6])
+def test_launches_past_2_to_21_blocks(lib, tune, config):
+    tune(mx4_config=config)
+    rows = (1 << 28) + 70
+    x = torch.zeros(rows, 64, dtype=torch.uint8, device="cuda")
+    x[:, 0] = (torch.arange(rows, dtype=torch.int32, device="cuda") % 13).to(torch.uint8)
+    scales = torch.full((rows, 4), 128, dtype=torch.uint8, device="cuda")
+    w = mx4.on_gpu(*mx4.random(1, 1, 3, (127, 127)))
+    w[0][0, 0] = 3   # 1.5
+    out = torch.full((rows, 1), 7.0, dtype=torch.bfloat16, device="cuda")
+    _gemm(lib, (x, scales), w, out, 1)
+    table = torch.tensor(mx4.VALUES * 3.0, dtype=torch.bfloat16, device="cuda")
+    assert torch.equal(out[:, 0], table[x[:, 0].int()])
+
+
+@pytest.mark.parametrize("transposed", [False, True])
+def test_quantisation_of_many_rows_and_of_many_columns(lib, transposed):
+    long = (1 << 28) + 5
+    x = torch.randint(-3, 4, (8, long) if transposed else (long, 8), dtype=torch.int8, device="cuda").bfloat16()
+    q = torch.empty(long, 64, dtype=torch.uint8, device="cuda")
+    scales = torch.empty(long, 4, dtype=torch.uint8, device="cuda")
+    forms = (None, None, q.data_ptr(), scales.data_ptr()) if transposed else (q.data_ptr(), scales.data_ptr(), None, None)
+    lib.mx4_quantize(BF, x.data_ptr(), 0, *x.shape, 0, *forms, _stream())
+    back = torch.full((long, 8), 7.0, dtype=torch.bfloat16, device="cuda")
+    lib.mx4_dequantize(BF, q.data_ptr(), scales.data_ptr(), long, 8, back.data_ptr(), 0, _stream())
+    for lo in range(0, long, 1 << 26):   # -3 .. 3 are held exactly
+        piece = slice(lo, lo + (1 << 26))
+        assert torch.equal(back[piece], x[:, piece].t() if transposed else x[piece])
+    assert int(scales[:, 1:].max()) == 0 and not q[:, 4:].any()
+
+
+@pytest.mark.parametrize("config, splits", [(None, None), (0, None), (1, None), (2, 16), (3, 7), (5, None), (6, None)])
+def test_the_largest_k(lib, tune, config, splits):
+    tune(mx4_config=config, mx4_splits=splits)
+    k = capi.MX4_MAX_K
+    m, n = 5, 37
+    a, b = mx4.random(m, k, 1), mx4.random(n, k, 2)
+    kept = np.random.default_rng(3).random(k) < mx4.EXACT_COLUMNS / 2 / k   # the others multiply zeros
+    kept[-1] = True
+    assert kept.sum() < mx4.EXACT_COLUMNS
+    a[0][:, ~kept] = 0
+    blocks = np.unique(np.nonzero(kept)[0] // 32)
+    columns = (blocks[:, None] * 32 + np.arange(32)).ravel()
+    exact = mx4.values(a[0][:, columns], a[1][:, blocks]) @ mx4.values(b[0][:, columns], b[1][:, blocks]).T
+    out = torch.empty(m, n, dtype=torch.bfloat16, device="cuda")
+    workspace = torch.full((1 << 20,), 255, dtype=torch.uint8, device="cuda")
+    _gemm(lib, mx4.on_gpu(*a), mx4.on_gpu(*b), out, k, workspace=workspace)
+    assert torch.equal(out.cpu(), torch.from_numpy(exact).float().bfloat16())
+
+
+def test_a_workspace_off_16_bytes_is_left_alone(lib, tune):
+    tune(mx4_config=3, mx4_splits=4)
+    m, n, k = 128, 512, 6144
+    a, b = _random(m, k, 1), _random(n, k, 2)
+    outs = []
+    for shift in (0, 4):
+        workspace = torch.full((64 << 20,), 255, dtype=torch.uint8, device="cuda")
+        out = torch.empty(m, n, dtype=torch.bfloat16, device="cuda")
+        _gemm(lib, a, b, out, k, workspace=workspace[shift:])
+        outs.append(out)
+        assert bool((workspace == 255).all()) == (shift == 4)   # K is split over the aligned one
+    assert torch.equal(*outs)
+
+
+def test_two_streams_at_once_and_a_graph_of_split_sums(lib, tune):
+    """Calls that overlap, each with a workspace of its own; the same calls captured together and replayed."""
+    tune(mx4_config=3, mx4_splits=4)
+    m, n, k = 128, 512, 6144
+    inputs = [(_random(m, k, i), _random(n, k, 10 + i)) for i in range(2)]
+    wanted = [(values_of(torch, *a, k).double() @ values_of(torch, *b, k).double().t()).float().bfloat16()
+              for a, b in inputs]
+    outs = [torch.empty(m, n, dtype=torch.bfloat16, device="cuda") for _ in inputs]
+    workspaces = [torch.empty(8 << 20, dtype=torch.uint8, device="cuda") for _ in inputs]
+    sides = [torch.cuda.Stream() for _ in inputs]
+
+    def both() -> None:
+        here = torch.cuda.current_stream()
+        for side, (a, b), out, workspace in zip(sides, inputs, outs, workspaces):
+            side.wait_stream(here)
+            with torch.cuda.stream(side):
+                for _ in range(5):
+                    _gemm(lib, a, b, out, k, workspace=workspace, stream=side.cuda_stream)
+        for side in sides:
+            here.wait_stream(side)
+
+    def check() -> None:
+        torch.cuda.synchronize()
+        for out, want in zip(outs, wanted):
+            assert torch.equal(out, want)
+            out.fill_(7.0)
+
+    both()
+    check()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        both()
+    for _ in range(3):
+        graph.replay()
+        check()
