@@ -419,9 +419,10 @@ int mb_kernel_info(int kind, int a, int b, int64_t m, int64_t n, int64_t k,
 #define MB_TUNE_W4_CONFIG 11            /* mb_gemm_w4, tiles of rows x columns: 0 and 1: 16 x 16 and 16 x 32, 8 waves
                                            split K; 2: 16 x 32, 4 waves do; 3: 16 x 256; 4: 32 x 128; 5: 32 x 64;
                                            6: 64 x 256; 7: 64 x 128; 8: 64 x 64 */
-#define MB_TUNE_MX4_CONFIG 12           /* mb_gemm_mx4: 0: 256x256, 1 and 2: 128x128 (two and four slots), 3: 64x64 tiles;
-                                           4 and 5: few rows, by 8 and by 32; 6: the kernel for any size */
-#define MB_TUNE_MX4_SPLITS 13           /* mb_gemm_mx4: K splits of the 128x128 and 64x64 tiles, 1..16, if the workspace
+#define MB_TUNE_MX4_CONFIG 12           /* mb_gemm_mx4: tiles of rows x columns: 0: 256x256, 1 and 2: 128x128
+                                           (two and four slots), 3: 64x128, 4: 64x64; 5 and 6: few rows, by 8 and
+                                           by 32; 7: the kernel for any size */
+#define MB_TUNE_MX4_SPLITS 13           /* mb_gemm_mx4: K splits of the tiles without 256x256, 1..16, if the workspace
                                            holds their sums */
 #define MB_TUNE_COUNT 14
 

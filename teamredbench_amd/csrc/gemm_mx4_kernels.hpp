@@ -111,25 +111,28 @@ __device__ __forceinline__ float read_acc(float v) {
 template <int DT, int CFG>
 __global__ void __launch_bounds__(256)
 gemm_mx4_kernel(Mx4Args all_args, int tiles_n, uint64_t magic) {
-    constexpr int TILE = kMx4Tiles[CFG].size, SLOTS = kMx4Tiles[CFG].slots, BM = TILE, BN = TILE;
+    constexpr int BM = kMx4Tiles[CFG].rows, BN = kMx4Tiles[CFG].columns, SLOTS = kMx4Tiles[CFG].slots;
     constexpr int WTM = BM / 2, WTN = BN / 2;
     constexpr int FM = WTM / 32, FN = WTN / 32;
-    constexpr int SLOT = TILE * kPairBytes, SCALE_SLOT = TILE * kChunkBytes;   // one operand's
+    // A wave loads as many scales as any other: of both operands those of the longer side's rows.
+    constexpr int SIDE = BM > BN ? BM : BN;
+    constexpr int X_SLOT = BM * kPairBytes, W_SLOT = BN * kPairBytes, SCALE_SLOT = SIDE * kChunkBytes;
     // LDS: x's elements, w's (SLOTS slots each); slot 0 of x's scales and of w's, slot 1 of both.
-    constexpr int W0 = SLOTS * SLOT, XS0 = 2 * SLOTS * SLOT, WS0 = XS0 + SCALE_SLOT, NEXT_SCALES = 2 * SCALE_SLOT;
+    constexpr int W0 = SLOTS * X_SLOT, XS0 = W0 + SLOTS * W_SLOT, WS0 = XS0 + SCALE_SLOT, NEXT_SCALES = 2 * SCALE_SLOT;
     constexpr int LDS_BYTES = XS0 + 2 * NEXT_SCALES;
-    constexpr int INSTR = SLOT / 1024 / 4;                   // DMA instructions per wave, operand and pair
-    constexpr int SCALE_INSTR = 2 * SCALE_SLOT / 1024 / 4;   // ... per wave and chunk, both operands
-    static_assert(LDS_BYTES <= 160 * 1024 && SLOT % 4096 == 0 && SCALE_INSTR >= 1, "LDS rings");
+    // DMA instructions per wave: of x and of w a pair, of both operands' scales a chunk.
+    constexpr int X_INSTR = X_SLOT / 1024 / 4, W_INSTR = W_SLOT / 1024 / 4, PAIR_INSTR = X_INSTR + W_INSTR;
+    constexpr int SCALE_INSTR = 2 * SCALE_SLOT / 1024 / 4;
+    static_assert(LDS_BYTES <= 160 * 1024 && X_SLOT % 8192 == 0 && W_SLOT % 8192 == 0 && SCALE_INSTR >= 1, "LDS rings");
     // Stores: groups of 32 rows and up to 64 columns of a wave's tile go through LDS and out as whole lines. A
     // persistent block (one per CU) stages them in the second scale slot, while the next tile's loads fill the rest.
-    constexpr bool PERSISTENT = TILE == 256;
+    constexpr bool PERSISTENT = BM == 256;
     constexpr int GC = WTN < 64 ? WTN : 64, STAGE = 32 * GC * 2, PIECES = STAGE / 1024;
     constexpr int STAGE0 = PERSISTENT ? XS0 + NEXT_SCALES : 0;
     constexpr int GROUPS = FM * (WTN / GC);                  // of a wave's tile
     static_assert(!PERSISTENT || (4 * STAGE == NEXT_SCALES && STAGE == SCALE_INSTR * 1024),
                   "a wave stages its stores in what its own loads of the second scale slot fill");
-    constexpr Mx4Waits kWaits = mx4_schedule(SLOTS, 2 * INSTR, SCALE_INSTR, GROUPS, PIECES);
+    constexpr Mx4Waits kWaits = mx4_schedule(SLOTS, PAIR_INSTR, SCALE_INSTR, GROUPS, PIECES);
     static_assert([&] {
         for (int w : kWaits.step)
             if (w < 0 || w >= 64) return false;
@@ -216,7 +219,7 @@ gemm_mx4_kernel(Mx4Args all_args, int tiles_n, uint64_t magic) {
     // The rows of x that this lane's loads go through (-1: none): of the wave's quarter of the tile, and of the half
     // whose scales it loads (waves 0 and 1 load x's scales, 2 and 3 w's).
     const bool scales_of_x = wave < 2;
-    constexpr int WAVE_ROWS = BM / 4, SCALE_ROWS = BM / 2;
+    constexpr int X_ROWS = BM / 4, W_ROWS = BN / 4, SCALE_ROWS = SIDE / 2;
     struct XRows {
         int data, scales[2];
     };
@@ -225,7 +228,7 @@ gemm_mx4_kernel(Mx4Args all_args, int tiles_n, uint64_t magic) {
             if (tile.m0 + r >= tile.ex.count) return -1;
             return args.rows != nullptr ? args.rows[tile.ex.first + tile.m0 + r] : r;
         };
-        XRows x{row(wave * WAVE_ROWS + lane % WAVE_ROWS), {-1, -1}};
+        XRows x{row(wave * X_ROWS + lane % X_ROWS), {-1, -1}};
         if (scales_of_x) {
             x.scales[0] = row(wave * SCALE_ROWS + lane % SCALE_ROWS);
             if constexpr (SCALE_ROWS > 64) x.scales[1] = row(wave * SCALE_ROWS + 64 + lane);
@@ -237,7 +240,7 @@ gemm_mx4_kernel(Mx4Args all_args, int tiles_n, uint64_t magic) {
     // and this lane's byte offsets of its 16-byte pieces. An instruction fills 8 rows of a pair, or the scales of 32.
     struct Loads {
         __amdgpu_buffer_rsrc_t x, w, scales;
-        int x_off[INSTR], w_off[2], s_off[SCALE_INSTR];
+        int x_off[X_INSTR], w_off[2], s_off[SCALE_INSTR];
         int ld16, at, scales_at;               // 16 rows of w; bytes to the first unit of K
         int ksteps, k_bytes, half_pair;        // units of K, in whole pairs; the pair whose second unit is not there
     };
@@ -263,11 +266,12 @@ gemm_mx4_kernel(Mx4Args all_args, int tiles_n, uint64_t magic) {
         l.scales = resource(scales_of_x ? args.xs : args.ws, scales_of_x ? x_first : w_first, args.lds,
                             scales_of_x ? x_count : w_count);
 #pragma unroll
-        for (int q = 0; q < INSTR; ++q) {
+        for (int q = 0; q < X_INSTR; ++q) {
             const int r = q * 8 + (lane >> 3), row = __shfl(rows.data, r);
             l.x_off[q] = row < 0 || row >= x_count ? kNowhere : row * args.ld + k_byte[q & 1];
-            if (q < 2) l.w_off[q] = (wave * WAVE_ROWS + r) * args.ld + k_byte[q];
         }
+#pragma unroll
+        for (int q = 0; q < 2; ++q) l.w_off[q] = (wave * W_ROWS + q * 8 + (lane >> 3)) * args.ld + k_byte[q];
 #pragma unroll
         for (int q = 0; q < SCALE_INSTR; ++q) {
             const int r = q * 32 + (lane >> 1), byte = ((lane & 1) ^ ((r >> 3) & 1)) << 4;
@@ -297,12 +301,12 @@ gemm_mx4_kernel(Mx4Args all_args, int tiles_n, uint64_t magic) {
     auto issue_x = [&](int pair, int at, auto idx) {
         constexpr int q = decltype(idx)::value;
         const int off = k_byte[q & 1] < from.k_bytes - pair * kPairBytes ? from.x_off[q] : kNowhere;
-        lds_dma16(from.x, lds0 + at + (wave * INSTR + q) * 1024, off, from.at + pair * kPairBytes);
+        lds_dma16(from.x, lds0 + at + (wave * X_INSTR + q) * 1024, off, from.at + pair * kPairBytes);
     };
     auto issue_w = [&](int pair, int at, auto idx) {
         constexpr int q = decltype(idx)::value;
         const int off = k_byte[q & 1] < from.k_bytes - pair * kPairBytes ? from.w_off[q & 1] : kNowhere;
-        lds_dma16(from.w, lds0 + W0 + at + (wave * INSTR + q) * 1024, off,
+        lds_dma16(from.w, lds0 + W0 + at + (wave * W_INSTR + q) * 1024, off,
                   from.at + pair * kPairBytes + (q >> 1) * from.ld16);
     };
     auto issue_scales = [&](int chunk, auto idx) {
@@ -317,12 +321,12 @@ gemm_mx4_kernel(Mx4Args all_args, int tiles_n, uint64_t magic) {
         }(std::make_integer_sequence<int, decltype(count)::value>{});
     };
     // Load l of a tile's first: scale chunk 0, a pair for every slot.
-    constexpr int FIRST_LOADS = SCALE_INSTR + 2 * SLOTS * INSTR;
+    constexpr int FIRST_LOADS = SCALE_INSTR + SLOTS * PAIR_INSTR;
     auto first_load = [&](auto idx) {
-        constexpr int l = decltype(idx)::value, d = l - SCALE_INSTR;
+        constexpr int l = decltype(idx)::value, d = l - SCALE_INSTR, pair = d / PAIR_INSTR, q = d % PAIR_INSTR;
         if constexpr (d < 0) issue_scales(0, idx);
-        else if constexpr (d / INSTR % 2 == 0) issue_x(d / INSTR / 2, d / INSTR / 2 * SLOT, std::integral_constant<int, d % INSTR>{});
-        else issue_w(d / INSTR / 2, d / INSTR / 2 * SLOT, std::integral_constant<int, d % INSTR>{});
+        else if constexpr (q < X_INSTR) issue_x(pair, pair * X_SLOT, std::integral_constant<int, q>{});
+        else issue_w(pair, pair * W_SLOT, std::integral_constant<int, q - X_INSTR>{});
     };
     constexpr std::integral_constant<int, FIRST_LOADS> kFirstLoads{};
     constexpr std::integral_constant<int, SCALE_INSTR> kScalePieces{};
@@ -354,7 +358,7 @@ gemm_mx4_kernel(Mx4Args all_args, int tiles_n, uint64_t magic) {
         constexpr int t = r < FIRST ? 0 : 1;
         constexpr int f = t == 1 ? r - FIRST : u % 2 ? r : r / 2;
         constexpr bool scales = u % 2 == 0 && t == 0 && r % 2 == 1;
-        constexpr int at = (u / 2) % SLOTS * SLOT, chunk = 2 * (u % 2) + t;
+        constexpr int slot = (u / 2) % SLOTS, chunk = 2 * (u % 2) + t;
         constexpr bool is_w = f >= 1 && f <= FN;
         constexpr int frag = is_w ? f - 1 : f == 0 ? 0 : f - FN;
         const int row = (is_w ? w_lane : x_lane) + 32 * frag;
@@ -366,7 +370,7 @@ gemm_mx4_kernel(Mx4Args all_args, int tiles_n, uint64_t magic) {
             else s.a[frag] = v;
         } else {
             const u32x4 v =
-                *reinterpret_cast<const u32x4*>(lds + (is_w ? W0 : 0) + at + piece_at(row, chunk + 4 * half));
+                *reinterpret_cast<const u32x4*>(lds + (is_w ? W0 + slot * W_SLOT : slot * X_SLOT) + piece_at(row, chunk + 4 * half));
             if constexpr (is_w) o.b[t][frag] = v;
             else o.a[t][frag] = v;
         }
@@ -383,7 +387,7 @@ gemm_mx4_kernel(Mx4Args all_args, int tiles_n, uint64_t magic) {
     bool behind_stores = false;   // the first loads went out among the stores of a whole tile
     auto step = [&](auto idx, int kt) {
         constexpr int I = decltype(idx)::value;               // kt % 8
-        constexpr int DATA_LOADS = I % 2 ? 2 * INSTR : 0, LOADS = DATA_LOADS + (I == 7 ? SCALE_INSTR : 0);
+        constexpr int DATA_LOADS = I % 2 ? PAIR_INSTR : 0, LOADS = DATA_LOADS + (I == 7 ? SCALE_INSTR : 0);
         constexpr int N_READS = (I % 2 ? 3 : 2) * (FM + FN), N_MEM = N_READS + LOADS;
         constexpr int PRE = N_MFMA >= 16 ? kPreBarrierMfma : 0;
         // The step's memory instructions, spread evenly over the MFMAs behind the barrier, and the loads evenly among
@@ -422,12 +426,14 @@ gemm_mx4_kernel(Mx4Args all_args, int tiles_n, uint64_t magic) {
                     ([&] {
                         constexpr int m = R;
                         if constexpr (kSlotOf(m) == here) {
-                            constexpr int l = kLoadsBefore(m), at = (I / 2) % SLOTS * SLOT;
+                            constexpr int l = kLoadsBefore(m), slot = (I / 2) % SLOTS;
                             if constexpr (kLoadsBefore(m + 1) > l) {
                                 if constexpr (l >= DATA_LOADS)
                                     issue_scales(chunk, std::integral_constant<int, l - DATA_LOADS>{});
-                                else if constexpr (l < INSTR) issue_x(pair, at, std::integral_constant<int, l>{});
-                                else issue_w(pair, at, std::integral_constant<int, l - INSTR>{});
+                                else if constexpr (l < X_INSTR)
+                                    issue_x(pair, slot * X_SLOT, std::integral_constant<int, l>{});
+                                else
+                                    issue_w(pair, slot * W_SLOT, std::integral_constant<int, l - X_INSTR>{});
                             } else {
                                 read_op(std::integral_constant<int, I + 1>{}, std::integral_constant<int, m - l>{}, nxt,
                                         nxt_scales);
@@ -629,17 +635,17 @@ inline Mx4Args mx4_args(const Mx4Call& c, int splits, void* planes) {
 
 template <int DT, int CFG>
 int launch_mx4(const Mx4Call& c, int splits, int cus, void* workspace, hipStream_t stream) {
-    constexpr int TILE = kMx4Tiles[CFG].size;
-    const int tiles_n = (int)((c.N + TILE - 1) / TILE);
-    const int64_t tiles_m = c.offsets ? c.total_rows / TILE + std::min<int64_t>(c.experts, c.total_rows)
-                                      : (c.total_rows + TILE - 1) / TILE;
+    constexpr int BM = kMx4Tiles[CFG].rows, BN = kMx4Tiles[CFG].columns;
+    const int tiles_n = (int)((c.N + BN - 1) / BN);
+    const int64_t tiles_m = c.offsets ? c.total_rows / BM + std::min<int64_t>(c.experts, c.total_rows)
+                                      : (c.total_rows + BM - 1) / BM;
     const int64_t pairs = (c.units + 1) / 2, split_pairs = (pairs + splits - 1) / splits;
     splits = (int)((pairs + split_pairs - 1) / split_pairs);   // none is empty
     const Mx4Args a = mx4_args(c, splits, splits > 1 ? workspace : nullptr);
     // Tiles of 256: a block per CU, which loads its next tile while it stores one.
     const int64_t blocks = tiles_m * tiles_n * splits;
     const uint64_t per_group = (uint64_t)kGroupM * tiles_n, magic = ((1ull << 40) + per_group - 1) / per_group;
-    hipLaunchKernelGGL((gemm_mx4_kernel<DT, CFG>), launch_grid(TILE == 256 ? std::min<int64_t>(blocks, cus) : blocks),
+    hipLaunchKernelGGL((gemm_mx4_kernel<DT, CFG>), launch_grid(BM == 256 ? std::min<int64_t>(blocks, cus) : blocks),
                        dim3(256), 0, stream, a, tiles_n, magic);
     MB_HIP_TRY(hipGetLastError());
     return splits > 1 ? mx4_sum<DT>(a, stream) : MB_OK;
@@ -651,7 +657,8 @@ int launch_mx4_config(const Mx4Call& c, const Mx4Plan& plan, int cus, void* work
         case 0: return launch_mx4<DT, 0>(c, plan.splits, cus, workspace, stream);
         case 1: return launch_mx4<DT, 1>(c, plan.splits, cus, workspace, stream);
         case 2: return launch_mx4<DT, 2>(c, plan.splits, cus, workspace, stream);
-        default: return launch_mx4<DT, 3>(c, plan.splits, cus, workspace, stream);
+        case 3: return launch_mx4<DT, 3>(c, plan.splits, cus, workspace, stream);
+        default: return launch_mx4<DT, 4>(c, plan.splits, cus, workspace, stream);
     }
 }
 

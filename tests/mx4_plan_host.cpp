@@ -11,11 +11,11 @@ using namespace mb;
 
 template <int CFG>
 void print_waits() {   // the constants of gemm_mx4_kernel<DT, CFG>
-    const int size = kMx4Tiles[CFG].size, slots = kMx4Tiles[CFG].slots, wave = size / 2, wide = wave < 64 ? wave : 64;
-    const int pair = 2 * (size * kPairBytes / 1024 / 4), chunk = 2 * size * kChunkBytes / 1024 / 4;
-    const int groups = wave / 32 * (wave / wide), pieces = 32 * wide * 2 / 1024;
+    const int rows = kMx4Tiles[CFG].rows, columns = kMx4Tiles[CFG].columns, slots = kMx4Tiles[CFG].slots;
+    const int pair = (rows + columns) * kPairBytes / 1024 / 4, chunk = 2 * (rows > columns ? rows : columns) * kChunkBytes / 1024 / 4;
+    const int wide = columns / 2 < 64 ? columns / 2 : 64, groups = rows / 64 * (columns / 2 / wide), pieces = 32 * wide * 2 / 1024;
     const Mx4Waits w = mx4_schedule(slots, pair, chunk, groups, pieces);
-    std::printf("%d %d %d %d %d %d", slots, pair, chunk, groups, pieces, size == 256);
+    std::printf("%d %d %d %d %d %d", slots, pair, chunk, groups, pieces, rows == 256);
     for (int s : w.step) std::printf(" %d", s);
     std::printf(" %d %d %d %d %d\n", w.prologue, w.behind_prologue, w.behind[0], w.behind[1], w.behind[2]);
 }
@@ -36,6 +36,7 @@ int main(int, char** argv) {
         print_waits<1>();
         print_waits<2>();
         print_waits<3>();
+        print_waits<4>();
     } else {
         int tiles_m, tiles_n;
         while (std::scanf("%d %d", &tiles_m, &tiles_n) == 2) {

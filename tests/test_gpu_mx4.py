@@ -325,7 +325,8 @@ def test_results_repeat_bit_for_bit(lib):
         assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
 
 
-CONFIGS = [(0, None), (1, 1), (1, 2), (1, 5), (2, 1), (2, 3), (3, 1), (3, 3), (3, 16), (4, None), (5, None), (6, None)]
+CONFIGS = [(0, None), (1, 1), (1, 2), (1, 5), (2, 1), (2, 3), (3, 1), (3, 4), (4, 1), (4, 3), (4, 16),
+           (5, None), (6, None), (7, None)]
 
 
 @pytest.mark.parametrize("config, splits", CONFIGS)

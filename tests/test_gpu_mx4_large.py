@@ -47,7 +47,7 @@ def test_a_list_over_more_than_2_to_31_bytes(lib):
     assert torch.equal(out, exact.float().bfloat16())
 
 
-@pytest.mark.parametrize("config", [None, 0, 1, 3, 5, 6])
+@pytest.mark.parametrize("config", [None, 0, 1, 3, 4, 6, 7])
 def test_outputs_past_2_to_31(lib, tune, config):
     tune(mx4_config=config)
     n, k = 2050, 128
@@ -62,7 +62,7 @@ def test_outputs_past_2_to_31(lib, tune, config):
         assert torch.equal(out[lo:hi], wanted.bfloat16()), lo
 
 
-@pytest.mark.parametrize("config", [None, 0, 2, 5, 6])
+@pytest.mark.parametrize("config", [None, 0, 2, 3, 6, 7])
 def test_launches_past_2_to_21_blocks(lib, tune, config):
     tune(mx4_config=config)
     rows = (1 << 28) + 70
@@ -93,7 +93,7 @@ def test_quantisation_of_many_rows_and_of_many_columns(lib, transposed):
     assert int(scales[:, 1:].max()) == 0 and not q[:, 4:].any()
 
 
-@pytest.mark.parametrize("config, splits", [(None, None), (0, None), (1, None), (2, 16), (3, 7), (5, None), (6, None)])
+@pytest.mark.parametrize("config, splits", [(None, None), (0, None), (1, None), (2, 16), (3, 7), (4, 9), (5, None), (6, None), (7, None)])
 def test_the_largest_k(lib, tune, config, splits):
     tune(mx4_config=config, mx4_splits=splits)
     k = capi.MX4_MAX_K
@@ -113,7 +113,7 @@ def test_the_largest_k(lib, tune, config, splits):
 
 
 def test_a_workspace_off_16_bytes_is_left_alone(lib, tune):
-    tune(mx4_config=3, mx4_splits=4)
+    tune(mx4_config=4, mx4_splits=4)
     m, n, k = 128, 512, 6144
     a, b = _random(m, k, 1), _random(n, k, 2)
     outs = []
@@ -128,7 +128,7 @@ def test_a_workspace_off_16_bytes_is_left_alone(lib, tune):
 
 def test_two_streams_at_once_and_a_graph_of_split_sums(lib, tune):
     """Calls that overlap, each with a workspace of its own; the same calls captured together and replayed."""
-    tune(mx4_config=3, mx4_splits=4)
+    tune(mx4_config=4, mx4_splits=4)
     m, n, k = 128, 512, 6144
     inputs = [(_random(m, k, i), _random(n, k, 10 + i)) for i in range(2)]
     wanted = [(values_of(torch, *a, k).double() @ values_of(torch, *b, k).double().t()).float().bfloat16()

@@ -12,17 +12,19 @@ from teamredbench_amd.native import capi
 
 TESTS = Path(__file__).resolve().parent
 WORKSPACE = 64 << 20
-T256, T128, T128_DEEP, T64, ROWS8, ROWS32, ANY = range(7)
+T256, T128, T128_DEEP, T64_128, T64, ROWS8, ROWS32, ANY = range(8)
 
-# (rows, N, K) -> configuration at 256 CUs: both sides of the bounds on rows, and the calls whose times are quoted
+# (rows, N, K) -> configuration at 256 CUs: calls whose times under every kernel were compared
 DENSE = [
-    ((1, 14336, 4096), ROWS8), ((8, 50257, 4096), ROWS8), ((9, 50257, 4096), ROWS32), ((32, 14336, 4096), ROWS32),
-    ((33, 4096, 4096), ROWS32), ((64, 4096, 4096), ROWS32), ((64, 4097, 4096), T64), ((65, 4096, 4096), T64),
-    ((64, 14336, 4096), T64), ((64, 50257, 4096), T128), ((256, 4096, 4096), T64), ((1024, 4096, 4096), T128_DEEP),
-    ((2048, 4096, 4096), T128), ((8192, 8192, 8192), T256), ((4096, 14336, 4096), T256), ((300, 264, 1000), T64),
+    ((1, 14336, 4096), ROWS8), ((16, 4096, 14336), ROWS8), ((16, 50257, 4096), T64_128), ((32, 14336, 4096), ROWS32),
+    ((32, 8192, 8192), ROWS32), ((64, 4096, 4096), ROWS32), ((64, 14336, 4096), T64), ((64, 50257, 4096), T64_128),
+    ((64, 32768, 8192), T64), ((128, 14336, 4096), T64), ((128, 50257, 4096), T128), ((256, 4096, 4096), T64),
+    ((512, 4096, 4096), T64), ((1024, 4096, 4096), T128_DEEP), ((2048, 4096, 4096), T128), ((8192, 8192, 8192), T256),
+    ((4096, 14336, 4096), T256), ((300, 264, 1000), T64),
 ]
 # (rows, experts, N, K) by expert
-EXPERTS = [((256, 64, 2048, 4096), ROWS8), ((512, 64, 2048, 4096), ROWS8), ((16384, 8, 14336, 4096), T256)]
+EXPERTS = [((256, 64, 2048, 4096), ROWS8), ((512, 64, 2048, 4096), T64_128), ((1024, 64, 2048, 4096), T64_128),
+           ((2048, 64, 2048, 4096), T128), ((128, 8, 14336, 4096), T64_128), ((16384, 8, 14336, 4096), T256)]
 
 
 @pytest.fixture(autouse=True)
@@ -60,11 +62,12 @@ def test_picks(host):
 
 
 def test_k_is_split_only_over_a_workspace_that_holds_the_sums(host):
-    rows, n, k = 128, 512, 8192
+    rows, n, k = 792, 200, 14464
     plane = 4 * rows * n
     with_one, = host("plan", [_call(rows, n, k)])
     assert with_one == (T64, 4)
-    assert host("plan", [_call(rows, n, k, workspace=0), _call(rows, n, k, workspace=4 * plane - 1)]) == [(T64, 1), (T64, 2)]
+    assert host("plan", [_call(rows, n, k, workspace=0)])[0][1] == 1
+    assert host("plan", [_call(rows, n, k, workspace=4 * plane - i, config=T64) for i in (0, 1)]) == [(T64, 4), (T64, 2)]
     assert host("plan", [_call(rows, n, k, config=T128, splits=5), _call(rows, n, k, config=T256, splits=5),
                          _call(rows, n, k, config=ROWS32, splits=5)]) == [(T128, 5), (T256, 1), (ROWS32, 1)]
 
@@ -145,7 +148,7 @@ def _replay(slots, pair, chunk, groups, pieces, behind, step, prologue, first_wa
 
 def test_no_step_reads_before_its_loads_land(host):
     tiles = host("waits")
-    assert len(tiles) == 4 and [t[5] for t in tiles] == [1, 0, 0, 0]
+    assert len(tiles) == 5 and [t[5] for t in tiles] == [1, 0, 0, 0, 0]
     for slots, pair, chunk, groups, pieces, persistent, *waits in tiles:
         step, (prologue, behind_prologue), behind = waits[:8], waits[8:10], waits[10:]
         assert _replay(slots, pair, chunk, groups, pieces, False, step, prologue, []) is None
@@ -163,7 +166,7 @@ def test_no_step_reads_before_its_loads_land(host):
 
 def test_the_knobs_take_every_configuration_and_no_other():
     lib = capi.load_library()
-    for knob, good, bad in (("mx4_config", range(7), (7, -2)), ("mx4_splits", (1, 2, 5, 16), (0, 17))):
+    for knob, good, bad in (("mx4_config", range(8), (8, -2)), ("mx4_splits", (1, 2, 5, 16), (0, 17))):
         for value in good:
             with lib.tuned(**{knob: value}):
                 assert lib.get_tuning(knob) == value
