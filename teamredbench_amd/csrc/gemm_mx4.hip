@@ -2,7 +2,14 @@
 // both operands in rows along k (layout: mx4_common.hpp), dense or by expert.
 //
 // gemm_mx4_any_kernel: a wave makes 32 rows x 32 columns from operands that go
-// from global memory straight into the matrix cores' registers. 64-bit addresses, any size.
+// from global memory straight into the matrix cores' registers. 64-bit addresses, any size; for lists of rows over more
+// than 2^31 bytes, which buffer offsets do not span. 8192^3 takes it 2.9 ms (tiles: 0.24), each load bringing 32 of
+// a line's 128 bytes.
+//
+// gemm_mx4_rows_kernel: few rows, bound by the bytes of w. 1 x 14336 x 4096 7.3 us (31 MB: 6.2 at the rate of a copy,
+// launch included in neither), 64 tokens x 4 of 64 experts, 4096 -> 2048, 50 us (5.6 TB/s of w's, x's and out's bytes).
+//
+// gemm_mx4_launch: which kernel (gemm_mx4_plan.hpp).
 #include "gemm_mx4_kernels.hpp"
 
 namespace mb {
@@ -157,7 +164,9 @@ gemm_mx4_rows_kernel(Mx4Args args, int tiles_m, int tiles_n) {
 #pragma unroll
     for (int s = 0; s < kRowsDepth; ++s) issue(s, s);
     const int xr = XR == 8 ? r32 & 7 : r32;   // 8 rows: the others repeat them, and are not stored
-    auto scales_at = [&](int row, int pair) { return row * kChunkBytes + ((((pair >> 1) & 1) ^ ((row >> 3) & 1)) << 4) + 8 * (pair & 1) + 4 * half; };
+    auto scales_at = [&](int row, int pair) {   // as in gemm_mx4_kernel
+        return row * kChunkBytes + ((((pair >> 1) & 1) ^ ((row >> 3) & 1)) << 4) + 8 * (pair & 1) + 4 * half;
+    };
     for (int p0 = 0; p0 < count; p0 += kRowsDepth) {
         [&]<int... S>(std::integer_sequence<int, S...>) {
             ([&] {
@@ -176,9 +185,9 @@ gemm_mx4_rows_kernel(Mx4Args args, int tiles_m, int tiles_n) {
                 u32x4 a[4], b[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    b[i] = *reinterpret_cast<const u32x4*>(slot + r32 * kPairBytes + (((4 * half + i) ^ swz_a2(r32)) << 4));
-                    a[i] = *reinterpret_cast<const u32x4*>(slot + R::kW + xr * kPairBytes +
-                                                           (((4 * half + i) ^ swz_a2(xr)) << 4));
+                    const int bk = ((4 * half + i) ^ swz_a2(r32)) << 4, ak = ((4 * half + i) ^ swz_a2(xr)) << 4;
+                    b[i] = *reinterpret_cast<const u32x4*>(slot + r32 * kPairBytes + bk);
+                    a[i] = *reinterpret_cast<const u32x4*>(slot + R::kW + xr * kPairBytes + ak);
                 }
                 if (p == half_pair) {   // no unit there: 2^-127 for whatever lies behind the row's scales
                     sa = half ? 0u : sa;

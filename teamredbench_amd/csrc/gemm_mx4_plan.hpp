@@ -17,8 +17,8 @@ struct Mx4Tile {
     // us of a round of blocks, one at most on every CU or per_cu: fixed, and per unit of K (128). Measured, less a
     // launch, at K = 4096 and other K: 256 x 256 36.5 us (4096^3); 128 x 128 15.9 (1024 x 4096 x 4096, a block a CU)
     // and 23.4 (2048 x 4096 x 4096, two), four slots 14.3; 64 x 128 16.2 (64 x 14336 x 4096) and 16.3 (1024 x 4096 x
-    // 4096, two); 64 x 64 7.2 (256 x 4096 x 4096), 14.8 (128 x 8192 x 8192) and 23.1 (256 x ..., two); 8 x 32 8.5 (16 x 4096 x 14336); 32 x 32
-    // 5.2 (64 x 4096 x 4096), 12.2 (64 x 4096 x 14336) and 13.4 (64 x 8192 x 8192, two).
+    // 4096, two); 64 x 64 7.2 (256 x 4096 x 4096), 14.8 (128 x 8192 x 8192) and 23.1 (256 x ..., two); 8 x 32 8.5 (16 x
+    // 4096 x 14336); 32 x 32 5.2 (64 x 4096 x 4096), 12.2 (64 x 4096 x 14336) and 13.4 (64 x 8192 x 8192, two).
     double one_us, one_unit_us, round_us, round_unit_us;
     double w_us, w_rate;   // a round that w's bytes bound: fixed us, bytes a us
 };
@@ -46,7 +46,8 @@ struct Mx4Shape {
 // Row tiles of `size` in all experts, were their rows spread evenly but for where they end.
 inline double mx4_row_tiles(const Mx4Shape& s, int size) {
     if (!s.by_expert) return (double)((s.total_rows + size - 1) / size);
-    const double hit = (double)std::min<int64_t>(s.experts, s.total_rows), tiles = (double)s.total_rows / s.experts / size;
+    const double hit = (double)std::min<int64_t>(s.experts, s.total_rows);
+    const double tiles = (double)s.total_rows / s.experts / size;
     return hit * std::max(1.0 + 0.55 * std::max(0.0, tiles - 0.35), tiles + 0.45);
 }
 
@@ -76,7 +77,8 @@ inline Mx4Plan mx4_plan(const Mx4Shape& s, size_t workspace_bytes, int cus, int6
         const double w_once = row_tiles / (s.by_expert ? (double)std::min<int64_t>(s.experts, s.total_rows) : 1.0);
         for (int n = 1; n <= kMx4MostSplits; ++n) {
             if (splits >= 0 ? n != splits && n != 1 : (n & (n - 1)) != 0) continue;
-            if (n > 1 && (tile.rows == 256 || i >= kMx4TileCount || !fits(n) || (splits < 0 && s.units < 16 * n))) continue;
+            if (n > 1 && (tile.rows == 256 || i >= kMx4TileCount)) continue;
+            if (n > 1 && (!fits(n) || (splits < 0 && s.units < 16 * n))) continue;
             const double blocks = tiles * n, units = (double)s.units / n, whole = cus * tile.per_cu;
             // Matrix cores and LDS, or w's bytes: a round of 64 x 128 tiles takes 28 us at K = 4096 where each tile has
             // columns of its own (128 tokens x 4 of 64 experts, 4096 -> 2048), 16 where 16 share them.

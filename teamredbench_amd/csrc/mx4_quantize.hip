@@ -9,7 +9,9 @@
 // value under 15 scales, and for fp32 at and next to every border. A block that holds an infinity or a
 // NaN has no scale: it becomes NaN as a whole (scale 255, elements 0).
 //
-// Bytes bound all of it: x is read once, whichever forms are written.
+// Bytes bound all of it: x is read once, whichever forms are written. bf16 8192 x 8192, inputs and outputs not in the
+// caches: rows 31 us (5.4 TB/s), columns 37 (4.6), both 49 (4.2), values back 32 (5.4); fp32 57, 61, 76 and 57. From the
+// Infinity Cache rows take 25 us and both 38.
 #include "mx4_common.hpp"
 
 namespace mb {
@@ -179,11 +181,24 @@ __device__ __forceinline__ unsigned max_bits(unsigned a, unsigned b) {
     }
 }
 
+// 16 bytes of elements without the first n of them, zeros behind; n < 4 (fp32) or 8.
+template <int DT>
+__device__ __forceinline__ u32x4 drop_first(u32x4 v, int n) {
+    if constexpr (DT != MB_DT_FLOAT32) {
+        if (n & 1) v = {v[0] >> 16 | v[1] << 16, v[1] >> 16 | v[2] << 16, v[2] >> 16 | v[3] << 16, v[3] >> 16};
+        n >>= 1;
+    }
+    if (n & 1) v = {v[1], v[2], v[3], 0};
+    if (n & 2) v = {v[2], v[3], 0, 0};
+    return v;
+}
+
 // Along columns, or along both: 128 rows x 256 bytes of each a block, through LDS. Lanes take 16 bytes of a row (16 lanes
 // a row), so a row's blocks span four lanes (fp32: eight); then a lane takes 32 rows of one dword's columns. Four
 // neighbouring lanes take the four blocks of 128 rows, and store 64 bytes; 16-byte chunk c of row r lies at chunk
 // c ^ 4 (r / 32), which spreads their reads over the banks. (Both forms from registers, a lane holding 32 rows x 4 or 8
-// columns, took 72 us for bf16 8192 x 8192: two waves a SIMD, and long chains of lane exchanges.)
+// columns, took 72 us for bf16 8192 x 8192: two waves a SIMD, and long chains of lane exchanges. Tiles of 256 rows, which
+// store whole lines of the columns' form, took 50: what binds is the memory's turning between reads and writes.)
 template <int DT, bool ROWS>
 __global__ void __launch_bounds__(256)
 mx4_quantize_tile_kernel(const void* __restrict__ x, int64_t ldx, int64_t rows, int64_t columns, bool fit,
@@ -196,7 +211,8 @@ mx4_quantize_tile_kernel(const void* __restrict__ x, int64_t ldx, int64_t rows, 
     __shared__ u32x4 tile[128 * 16];
     const int tid = threadIdx.x, l16 = tid % 16;
     // Tiles in squares of 256 x 256: those of one XCD (block b runs on XCD b % 8), one after the other, so that its L2
-    // joins their halves (fp32: quarters) of both forms' lines of 128 bytes.
+    // joins their halves (fp32: quarters) of both forms' lines of 128 bytes: fp32 8192 x 8192 90 -> 76 us. Squares along x's
+    // rows: in panels of 2 to 16 squares' width down x both forms took 52 to 62 us for 49.
     constexpr int WIDTH = 256 / COLUMNS, SQUARE = 2 * WIDTH;
     const int64_t block = block_number(), local = block / 8, square = local / SQUARE * 8 + block % 8;
     const int64_t squares_n = (tiles_n + WIDTH - 1) / WIDTH, square_r = square / squares_n;
@@ -219,22 +235,28 @@ mx4_quantize_tile_kernel(const void* __restrict__ x, int64_t ldx, int64_t rows, 
             for (int k = 0; k < 8; ++k) v[k] = *reinterpret_cast<const u32x4_2*>(p + 16 * k * ldx);
 #pragma unroll
             for (int k = 0; k < 8; ++k) piece(k) = v[k];
-        } else {   // an edge: zeros past it, none of which is read
+        } else if (columns >= EACH) {   // an edge: pieces of the last rows and columns, less what lies before
+            // them, so that eight loads are in flight here too (guarded one by one: fp32 3001 x 2057 11.9 us, this 10.8)
+            const int64_t past = max(c0 + EACH * l16 - (columns - EACH), (int64_t)0);
+            u32x4 v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                v[k] = *reinterpret_cast<const u32x4_2*>(p + min(16 * k, row_count - 1 - tid / 16) * ldx - past);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                piece(k) = past < EACH && tid / 16 + 16 * k < row_count ? drop_first<DT>(v[k], (int)past)
+                                                                        : u32x4{0, 0, 0, 0};
+        } else {
             const int64_t left = columns - (c0 + EACH * l16);
-#pragma unroll 2
             for (int k = 0; k < 8; ++k) {
                 u32x4 v = {0, 0, 0, 0};
                 if (tid / 16 + 16 * k < row_count) {
-                    if (left >= EACH) {
-                        v = *reinterpret_cast<const u32x4_2*>(p + 16 * k * ldx);
-                    } else {
 #pragma unroll
-                        for (int i = 0; i < EACH - 1; ++i)
-                            if (i < left) {
-                                if constexpr (WIDE) v[i] = p[16 * k * ldx + i];
-                                else v[i / 2] |= (unsigned)p[16 * k * ldx + i] << 16 * (i & 1);
-                            }
-                    }
+                    for (int i = 0; i < EACH - 1; ++i)
+                        if (i < left) {
+                            if constexpr (WIDE) v[i] = p[16 * k * ldx + i];
+                            else v[i / 2] |= (unsigned)p[16 * k * ldx + i] << 16 * (i & 1);
+                        }
                 }
                 piece(k) = v;
             }

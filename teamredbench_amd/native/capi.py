@@ -77,8 +77,6 @@ GROUPED_FORWARD, GROUPED_GRAD_ROWS, GROUPED_GRAD_WEIGHTS = 0, 1, 2
 # Microscaled 4-bit floating point (mb_mx4_*, mb_gemm_mx4)
 MX4_SCALE_FLOOR, MX4_SCALE_FIT = 0, 1   # MB_MX4_SCALE_*
 MX4_MAX_K = 8388608                     # MB_MX4_MAX_K
-MX4_VALUE_DTYPES = ("float32", "bfloat16", "float16")
-MX4_OUTPUT_DTYPES = ("bfloat16", "float16")
 
 
 def mx4_row_bytes(columns: int) -> int:
