@@ -90,8 +90,10 @@ def detect_device(torch_module: Any, device_id: int = 0) -> DeviceInfo | None:
 
 # Peak engine clock (MHz) -> SKU, for gfx950 parts whose marketing name the platform does not report
 # (the device name comes from libdrm's amdgpu.ids table, which a container may lack). MI355X and MI350X
-# are both gfx950 with 256 CUs; their published peak engine clocks differ.
+# are both gfx950 with 256 CUs; their published peak engine clocks differ. The one reported is now and then the clock
+# of the moment, a few MHz over (2402 and 2403 have been read).
 _GFX950_SKU_BY_MAX_CLOCK = {2400: "AMD Instinct MI355X", 2200: "AMD Instinct MI350X"}
+_MAX_CLOCK_TOLERANCE_MHZ = 20
 
 
 def _amdsmi_names(torch_module: Any, device_id: int) -> list[str]:
@@ -129,8 +131,9 @@ def _amdsmi_names(torch_module: Any, device_id: int) -> list[str]:
                 top = int(amdsmi.amdsmi_get_clock_info(handle, amdsmi.AmdSmiClkType.GFX)["max_clk"])
             except Exception:  # noqa: BLE001
                 top = None
-            if top in _GFX950_SKU_BY_MAX_CLOCK:
-                names.append(f"{_GFX950_SKU_BY_MAX_CLOCK[top]} (gfx950, peak engine clock {top} MHz)")
+            for clock, sku in _GFX950_SKU_BY_MAX_CLOCK.items():
+                if top is not None and abs(top - clock) <= _MAX_CLOCK_TOLERANCE_MHZ:
+                    names.append(f"{sku} (gfx950, peak engine clock {clock} MHz)")
     except Exception:  # noqa: BLE001
         return names
     finally:
