@@ -40,7 +40,7 @@ struct Mx4Args {
     int x_rows, experts, total, N;
     float* planes;                        // K splits: [split][total][ldp]
     int splits, split_units, ldp;
-    bool out_16;                          // out's rows start on 16 bytes
+    bool out_lines;                       // out's rows start on lines of 128 bytes
 };
 
 // Ring slots: elements two or four slots of a pair of units (whole 128-byte lines of every row), scales two slots of
@@ -516,7 +516,7 @@ gemm_mx4_kernel(Mx4Args all_args, int tiles_n, uint64_t magic) {
         }
         // Group by group through LDS. A wave's LDS accesses take effect in their order, so a group's reads need no wait
         // behind its writes, nor the next group's writes behind those reads.
-        const bool whole = args.out_16 && cur.m0 + BM <= M && cur.n0 + BN <= args.N;
+        const bool whole = cur.m0 + BM <= M && cur.n0 + BN <= args.N, out_lines = args.out_lines;
         constexpr int CHUNKS = GC / 8, ROWS = 64 / CHUNKS;   // rows per store
         unsigned char* stage = lds + STAGE0 + wave * STAGE;
         const int oc = lane % CHUNKS, orow = lane / CHUNKS;
@@ -552,9 +552,14 @@ gemm_mx4_kernel(Mx4Args all_args, int tiles_n, uint64_t magic) {
             auto store_group = [&](auto idx) {
                 constexpr int g = decltype(idx)::value;
                 unsigned char* at = to_group(idx);
+                if (out_lines) {
 #pragma unroll
-                for (int p = 0; p < PIECES; ++p, at += row_step)
-                    __builtin_nontemporal_store(v[g % 2][p], reinterpret_cast<u32x4*>(at));
+                    for (int p = 0; p < PIECES; ++p, at += row_step)
+                        __builtin_nontemporal_store(v[g % 2][p], reinterpret_cast<u32x4*>(at));
+                } else {   // parts of lines, which L2 joins: 8192 x 8200 x 4096 153 us, past it 181
+#pragma unroll
+                    for (int p = 0; p < PIECES; ++p, at += row_step) *reinterpret_cast<u32x4_2*>(at) = v[g % 2][p];
+                }
             };
             all(std::integral_constant<int, GROUPS>{}, [&](auto idx) {
                 constexpr int g = decltype(idx)::value;
@@ -576,18 +581,21 @@ gemm_mx4_kernel(Mx4Args all_args, int tiles_n, uint64_t magic) {
                 constexpr int i = decltype(idx)::value / (WTN / GC), j0 = decltype(idx)::value % (WTN / GC) * (GC / 32);
                 write_group(idx);
                 unsigned char* at = to_group(idx);
-                const int left = args.N - (n0 + 32 * j0);
-#pragma unroll 1
-                for (int p = 0; p < PIECES; ++p, at += row_step) {
-                    if (m0 + 32 * i + p * ROWS >= M) continue;
-                    const u32x4 v = read_piece(p);
-                    if (left >= 8) {
-                        *reinterpret_cast<u32x4_2*>(at) = v;
-                    } else {
+                const int left = args.N - (n0 + 32 * j0), rows_left = M - (m0 + 32 * i);
+                u32x4 v[PIECES];
+#pragma unroll
+                for (int p = 0; p < PIECES; ++p) v[p] = read_piece(p);
+                if (left >= 8) {
+#pragma unroll
+                    for (int p = 0; p < PIECES; ++p, at += row_step)
+                        if (p * ROWS < rows_left) *reinterpret_cast<u32x4_2*>(at) = v[p];
+                } else if (left > 0) {   // the last columns
+#pragma unroll
+                    for (int p = 0; p < PIECES; ++p, at += row_step)
 #pragma unroll
                         for (int e = 0; e < 7; ++e)
-                            if (e < left) reinterpret_cast<uint16_t*>(at)[e] = (uint16_t)(v[e >> 1] >> 16 * (e & 1));
-                    }
+                            if (p * ROWS < rows_left && e < left)
+                                reinterpret_cast<uint16_t*>(at)[e] = (uint16_t)(v[p][e >> 1] >> 16 * (e & 1));
                 }
             });
         }
@@ -641,12 +649,12 @@ int mx4_sum(const Mx4Args& a, hipStream_t stream) {
 // The kernels' arguments; `planes` where K is split.
 inline Mx4Args mx4_args(const Mx4Call& c, int splits, void* planes) {
     const int split_units = (int)((c.units + 2 * splits - 1) / (2 * splits) * 2);   // whole pairs
-    const bool out_16 = ((reinterpret_cast<uintptr_t>(c.out) | (uintptr_t)(c.ldo * 2)) & 15) == 0;
+    const bool out_lines = ((reinterpret_cast<uintptr_t>(c.out) | (uintptr_t)(c.ldo * 2)) & 127) == 0;
     return Mx4Args{static_cast<const unsigned char*>(c.x), static_cast<const unsigned char*>(c.x_scales),
                    static_cast<const unsigned char*>(c.w), static_cast<const unsigned char*>(c.w_scales),
                    static_cast<unsigned char*>(c.out), c.rows, c.offsets, c.ldo * 2, (int)c.units * kMx4UnitBytes,
                    (int)c.units * kMx4UnitScales, (int)c.units, (int)c.x_rows, c.experts, (int)c.total_rows, (int)c.N,
-                   static_cast<float*>(planes), splits, split_units, (int)((c.N + 3) / 4 * 4), out_16};
+                   static_cast<float*>(planes), splits, split_units, (int)((c.N + 3) / 4 * 4), out_lines};
 }
 
 template <int DT, int CFG>
