@@ -100,12 +100,16 @@ constexpr Mx4Waits mx4_schedule(int slots, int pair, int chunk, int groups, int 
     return r;
 }
 
-// Row tile and column of tile t: as in block_coords, in groups of kGroupM row tiles (without K splits, whose blocks
-// take block_coords), dividing by a multiplication: `magic` is 2^40 / (kGroupM tiles_n), rounded up.
+// Row tile and column of tile b of a persistent launch of `stride` blocks: in groups of kGroupM row tiles, as in
+// block_coords, and round by round, each XCD (block b runs on XCD b % 8) taking an eighth of a round's tiles, one patch of
+// them. So the XCDs share a group's rows, and one expert's w at a time (each XCD its own eighth of all tiles: 16384 rows
+// over 8 experts, 4096 -> 14336, 519 us for 502; 2048 x 50257 x 4096 244 for 229). Divides by a multiplication:
+// `magic` is 2^40 / (kGroupM tiles_n), rounded up.
 constexpr int kGroupM = 4;
-__host__ __device__ __forceinline__ void tile_coords(int b, int tiles, int tiles_m, int tiles_n, uint64_t magic,
-                                                     int* tm, int* tn) {
-    const int t = (b & 7) * (tiles >> 3) + min(b & 7, tiles & 7) + (b >> 3);
+__host__ __device__ __forceinline__ void tile_coords(int b, int stride, int tiles, int tiles_m, int tiles_n,
+                                                     uint64_t magic, int* tm, int* tn) {
+    const int c = (int)((unsigned)b % (unsigned)stride), n = min(tiles - (b - c), stride);
+    const int t = b - c + (c & 7) * (n >> 3) + min(c & 7, n & 7) + (c >> 3);
     const int per_group = kGroupM * tiles_n;
     int g = (int)(((uint64_t)(unsigned)t * magic) >> 40);
     if ((int64_t)g * per_group > t) --g;
@@ -192,7 +196,7 @@ gemm_mx4_kernel(Mx4Args all_args, int tiles_n, uint64_t magic) {
                             : (args.total + BM - 1) / BM;
         tiles = tiles_m * tiles_n * args.splits;
         if (t >= tiles) return;
-        if (PERSISTENT) tile_coords(t, tiles, tiles_m, tiles_n, magic, &tm, &tn);
+        if (PERSISTENT) tile_coords(t, stride, tiles, tiles_m, tiles_n, magic, &tm, &tn);
         else block_coords(t, tiles_m, tiles_n, args.splits, kGroupM, &tm, &tn, &cur.split);
         cur.ex.count = args.total;
         if (by_expert) {
@@ -206,7 +210,7 @@ gemm_mx4_kernel(Mx4Args all_args, int tiles_n, uint64_t magic) {
     // Another tile: its expert is near the last one's. Scalar loads, which the vmcnt waits do not see.
     const bool by_expert = all_args.offsets != nullptr;
     auto locate = [&](Tile& tile) {
-        tile_coords(t + stride, tiles, tiles_m, tiles_n, magic, &tm, &tn);
+        tile_coords(t + stride, stride, tiles, tiles_m, tiles_n, magic, &tm, &tn);
         if (by_expert) {
             const Mx4Args args = arguments();
             typedef const __attribute__((address_space(4))) int32_t* ConstRows;

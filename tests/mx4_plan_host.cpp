@@ -1,7 +1,7 @@
 // Host code, compiled from the MX4 products' own headers by tests/test_mx4_plan.py.
 //   plan   "config splits" for each line "total_rows experts N units by_expert listed x_rows workspace cus config splits"
 //   waits  "slots pair chunk groups pieces persistent step[8] prologue behind_prologue behind[3]" of every tile
-//   tiles  "tm tn" of every tile of tiles_m x tiles_n, for each line "tiles_m tiles_n", then an empty line
+//   tiles  "tm tn" of every tile of tiles_m x tiles_n, for each line "tiles_m tiles_n blocks", then an empty line
 #include <cstdio>
 #include <cstring>
 
@@ -38,12 +38,12 @@ int main(int, char** argv) {
         print_waits<3>();
         print_waits<4>();
     } else {
-        int tiles_m, tiles_n;
-        while (std::scanf("%d %d", &tiles_m, &tiles_n) == 2) {
+        int tiles_m, tiles_n, blocks;
+        while (std::scanf("%d %d %d", &tiles_m, &tiles_n, &blocks) == 3) {
             const uint64_t per_group = (uint64_t)kGroupM * tiles_n, magic = ((1ull << 40) + per_group - 1) / per_group;
             for (int t = 0; t < tiles_m * tiles_n; ++t) {
                 int tm, tn;
-                tile_coords(t, tiles_m * tiles_n, tiles_m, tiles_n, magic, &tm, &tn);
+                tile_coords(t, blocks, tiles_m * tiles_n, tiles_m, tiles_n, magic, &tm, &tn);
                 std::printf("%d %d\n", tm, tn);
             }
             std::printf("\n");

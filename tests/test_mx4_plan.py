@@ -91,9 +91,10 @@ def test_tiles_of_8_rows_past_2_to_30_blocks_give_way(host):
 
 def test_every_tile_once(host):
     """Each tile of a launch is one of the matrix's, and none comes twice."""
-    shapes = [(1, 1), (1, 300), (300, 1), (4, 4), (5, 7), (16, 56), (31, 33), (32, 32), (63, 196), (129, 11), (2, 4093)]
+    sizes = [(1, 1), (1, 300), (300, 1), (4, 4), (5, 7), (16, 56), (31, 33), (32, 32), (63, 196), (129, 11), (2, 4093)]
+    shapes = [(m, n, min(blocks, m * n)) for m, n in sizes for blocks in (256, 250, 8, 5)]
     out = iter(host("tiles", shapes))
-    for tiles_m, tiles_n in shapes:
+    for tiles_m, tiles_n, _ in shapes:
         tiles = []
         while (line := next(out)):
             tiles.append(line)
