@@ -11,7 +11,7 @@
 // slot, so that the 64 lanes of a read meet every bank evenly. Lane half h takes blocks 4h .. 4h + 3 of a pair: K may
 // come in any order that both operands share, and so one dword brings a lane its four scales.
 //
-// 256 x 256 tiles, persistent blocks of one a CU: 8192^3 232-240 us, 4.6-4.7 PFLOP/s, 70% of what these MFMAs sustain
+// 256 x 256 tiles, persistent blocks of one a CU: 8192^3 232-242 us, 4.5-4.7 PFLOP/s, 70% of what these MFMAs sustain
 // alone (6.66). Of a tile's 49000 cycles at K = 4096, 33000 are MFMAs, 5000 to 7000 waits for LDS and barriers in the
 // K loop, and 10000 lie around it (first loads, stores; the next tile's first loads run among the stores). The
 // clock is what the power limit leaves, 1.55 to 1.75 GHz, and rises where matrix cores idle: the last half round of
