@@ -62,6 +62,54 @@ def test_outputs_past_2_to_31(lib, tune, config):
         assert torch.equal(out[lo:hi], wanted.bfloat16()), lo
 
 
+@pytest.mark.parametrize("listed", [False, True])
+@pytest.mark.parametrize("config", [None, 0])
+def test_blocks_that_make_several_tiles_by_expert(lib, tune, config, listed):
+    """Tiles of 256 are made by one block a CU: here three to four each, over experts with and without rows."""
+    tune(mx4_config=config)
+    n, k = 2050, 384
+    g = torch.Generator().manual_seed(8)
+    counts = torch.randint(0, 900, (60,), generator=g)
+    counts[torch.rand(60, generator=g) < 0.3] = 0
+    counts[10:14] = torch.tensor([256, 512, 1, 257])
+    total = int(counts.sum()) + 9
+    offsets = torch.cat([torch.tensor([4]), counts.cumsum(0) + 4]).int()
+    x, w = _random(total, k, 1), _random(60 * n, k, 2)
+    rows = torch.randint(-1, total + 1, (total,), generator=g).int()
+    out = torch.full((total, n), 7.0, dtype=torch.bfloat16, device="cuda")
+    d_rows, d_offsets = rows.cuda(), offsets.cuda()
+    lib.gemm_mx4(BF, x[0].data_ptr(), x[1].data_ptr(), total, d_rows.data_ptr() if listed else None, w[0].data_ptr(),
+                 w[1].data_ptr(), out.data_ptr(), 0, d_offsets.data_ptr(), 60, total, n, k, None, 0, _stream())
+    values = values_of(torch, *x, k)
+    if listed:
+        there = ((rows >= 0) & (rows < total)).cuda()
+        values = values[rows.clamp(0, total - 1).long().cuda()] * there[:, None]
+    for e in range(60):
+        lo, hi = int(offsets[e]), int(offsets[e + 1])
+        wv = values_of(torch, w[0][e * n:(e + 1) * n], w[1][e * n:(e + 1) * n], k)
+        assert torch.equal(out[lo:hi], (values[lo:hi].contiguous() @ wv.t().contiguous()).bfloat16()), e
+    assert (out[:4] == 7).all() and (out[int(offsets[-1]):] == 7).all()
+
+
+@pytest.mark.parametrize("config", [0, 1, 3, 4, 5, 6, 7])
+def test_offsets_out_of_order_stay_in_bounds(lib, tune, config):
+    """They count many times the tiles that the launch has blocks for."""
+    tune(mx4_config=config)
+    n, k, total, experts = 520, 256, 3000, 50
+    x, w = _random(total, k, 1), _random(experts * n, k, 2)
+    for offsets in ([0, total] * 25 + [0], [total, 0] * 25 + [total], [1 << 30, -5] * 25 + [7],
+                    [0] * 25 + [total] * 10 + [600] * 16):
+        d = torch.tensor(offsets, dtype=torch.int32, device="cuda")
+        whole = torch.full((total + 2, n), 7.0, dtype=torch.bfloat16, device="cuda")
+        out = whole[1:-1]
+        workspace = torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
+        lib.gemm_mx4(BF, x[0].data_ptr(), x[1].data_ptr(), total, None, w[0].data_ptr(), w[1].data_ptr(),
+                     out.data_ptr(), 0, d.data_ptr(), experts, total, n, k, workspace.data_ptr(), workspace.numel(),
+                     _stream())
+        torch.cuda.synchronize()
+        assert (whole[0] == 7).all() and (whole[-1] == 7).all()
+
+
 @pytest.mark.parametrize("config", [None, 0, 2, 3, 6, 7])
 def test_launches_past_2_to_21_blocks(lib, tune, config):
     tune(mx4_config=config)
