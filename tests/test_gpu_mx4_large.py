@@ -141,6 +141,19 @@ def test_quantisation_of_many_rows_and_of_many_columns(lib, transposed):
     assert int(scales[:, 1:].max()) == 0 and not q[:, 4:].any()
 
 
+@pytest.mark.parametrize("dtype, rows", [(torch.bfloat16, 16385), (torch.float16, 16384), (torch.float32, 8193)])
+@pytest.mark.parametrize("columns, ld, shift", [(4096, 4096, 0), (4090, 4160, 0), (4096, 4100, 0), (4096, 4096, 1)])
+def test_values_past_the_caches(lib, dtype, rows, columns, ld, shift):
+    """128 MB of values and more are stored past the caches where their rows are whole lines."""
+    q, scales = _random(rows, 4096, 6)
+    whole = torch.full((shift + rows * ld + 1,), 7.0, dtype=dtype, device="cuda")
+    lib.mx4_dequantize(capi.DTYPES[str(dtype).split(".")[1]], q.data_ptr(), scales.data_ptr(), rows, columns,
+                       whole[shift:].data_ptr(), ld, _stream())
+    out = whole[shift:-1].view(rows, ld)
+    assert torch.equal(out[:, :columns], values_of(torch, q, scales, columns).to(dtype))   # all held exactly
+    assert (out[:, columns:] == 7).all() and (whole[:shift] == 7).all() and whole[-1] == 7
+
+
 @pytest.mark.parametrize("config, splits", [(None, None), (0, None), (1, None), (2, 16), (3, 7), (4, 9), (5, None), (6, None), (7, None)])
 def test_the_largest_k(lib, tune, config, splits):
     tune(mx4_config=config, mx4_splits=splits)
