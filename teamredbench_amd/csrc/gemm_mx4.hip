@@ -7,7 +7,7 @@
 // a line's 128 bytes.
 //
 // gemm_mx4_rows_kernel: few rows, bound by the bytes of w. 1 x 14336 x 4096 7.3 us (31 MB: 6.2 at the rate of a copy,
-// launch included in neither), 64 tokens x 4 of 64 experts, 4096 -> 2048, 50 us (5.6 TB/s of w's, x's and out's bytes).
+// launch included in neither), 64 tokens x 4 of 64 experts, 4096 -> 2048, 47.5 us (6.0 TB/s of w's, x's and out's bytes).
 //
 // gemm_mx4_launch: which kernel (gemm_mx4_plan.hpp).
 #include "gemm_mx4_kernels.hpp"
@@ -76,7 +76,7 @@ struct RowsRing {
     static constexpr int kBytes = kRowsDepth * kSlot + 2 * kScales;
 };
 
-template <int DT, int XR>
+template <int DT, int XR, bool STREAM>
 __global__ void __launch_bounds__(64 * kRowsWaves)
 gemm_mx4_rows_kernel(Mx4Args args, int tiles_m, int tiles_n) {
     typedef RowsRing<XR> R;
@@ -143,6 +143,7 @@ gemm_mx4_rows_kernel(Mx4Args args, int tiles_m, int tiles_n) {
     const unsigned ring = (unsigned)(uintptr_t)(MB_LDS unsigned char*)lds + wave * R::kBytes;
     unsigned char* mine = lds + wave * R::kBytes;
     constexpr int SCALES0 = kRowsDepth * R::kSlot;
+    constexpr auto load_w = STREAM ? lds_dma16_once : lds_dma16;
     auto issue = [&](int pair, int slot) {   // pairs past the wave's: nothing is fetched
         const int left = pair < count ? k_bytes - pair * kPairBytes : 0, at = (first + pair) * kPairBytes;
         if (slot == 0) {
@@ -153,7 +154,7 @@ gemm_mx4_rows_kernel(Mx4Args args, int tiles_m, int tiles_n) {
         }
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-            lds_dma16(rw, ring + slot * R::kSlot + q * 1024, k_byte[q & 1] < left ? w_off[q] : kNowhere, at);
+            load_w(rw, ring + slot * R::kSlot + q * 1024, k_byte[q & 1] < left ? w_off[q] : kNowhere, at);
 #pragma unroll
         for (int q = 0; q < XR / 8; ++q)
             lds_dma16(rx, ring + slot * R::kSlot + R::kW + q * 1024, k_byte[q & 1] < left ? x_off[q] : kNowhere, at);
@@ -225,11 +226,12 @@ gemm_mx4_rows_kernel(Mx4Args args, int tiles_m, int tiles_n) {
 }
 
 template <int DT, int XR>
-int launch_rows(const Mx4Call& c, hipStream_t stream) {
+int launch_rows(const Mx4Call& c, bool stream_w, hipStream_t stream) {
     const int64_t tiles_m = c.offsets ? c.total_rows / XR + std::min<int64_t>(c.experts, c.total_rows)
                                       : (c.total_rows + XR - 1) / XR;
     const int64_t tiles_n = (c.N + 31) / 32, columns = c.offsets ? tiles_n : (tiles_n + 7) / 8 * 8;
-    hipLaunchKernelGGL((gemm_mx4_rows_kernel<DT, XR>), launch_grid(tiles_m * columns), dim3(64 * kRowsWaves), 0, stream,
+    auto kernel = stream_w ? gemm_mx4_rows_kernel<DT, XR, true> : gemm_mx4_rows_kernel<DT, XR, false>;
+    hipLaunchKernelGGL(kernel, launch_grid(tiles_m * columns), dim3(64 * kRowsWaves), 0, stream,
                        mx4_args(c, 1, nullptr), (int)tiles_m, (int)tiles_n);
     MB_HIP_TRY(hipGetLastError());
     return MB_OK;
@@ -237,7 +239,8 @@ int launch_rows(const Mx4Call& c, hipStream_t stream) {
 
 template <int DT>
 int launch_rows_config(const Mx4Call& c, const Mx4Plan& plan, hipStream_t stream) {
-    return plan.config == kMx4Rows8 ? launch_rows<DT, 8>(c, stream) : launch_rows<DT, 32>(c, stream);
+    return plan.config == kMx4Rows8 ? launch_rows<DT, 8>(c, plan.stream, stream)
+                                    : launch_rows<DT, 32>(c, plan.stream, stream);
 }
 
 int launch_any(const Mx4Call& c, hipStream_t stream) {

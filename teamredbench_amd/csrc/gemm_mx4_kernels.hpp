@@ -119,6 +119,17 @@ __host__ __device__ __forceinline__ void tile_coords(int b, int stride, int tile
     *tn = column;
 }
 
+// lds_dma16 of what is read once.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void lds_dma16_once(__amdgpu_buffer_rsrc_t rsrc, unsigned lds_addr, int voff, int soff) {
+    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen nt lds"
+                 :
+                 : "s"(lds_addr), "v"(voff), "s"(rsrc), "s"(soff)
+                 : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
 // An accumulator's value, from where the matrix instructions keep it: left to itself the compiler copies all 256
 // into vector registers at once, and spills. The caller keeps the wait states behind the last matrix instruction.
 __device__ __forceinline__ float read_acc(float v) {
@@ -127,7 +138,7 @@ __device__ __forceinline__ float read_acc(float v) {
     return f;
 }
 
-template <int DT, int CFG>
+template <int DT, int CFG, bool STREAM>
 __global__ void __launch_bounds__(256)
 gemm_mx4_kernel(Mx4Args all_args, int tiles_n, uint64_t magic) {
     constexpr int BM = kMx4Tiles[CFG].rows, BN = kMx4Tiles[CFG].columns, SLOTS = kMx4Tiles[CFG].slots;
@@ -325,8 +336,9 @@ gemm_mx4_kernel(Mx4Args all_args, int tiles_n, uint64_t magic) {
     auto issue_w = [&](int pair, int at, auto idx) {
         constexpr int q = decltype(idx)::value;
         const int off = k_byte[q & 1] < from.k_bytes - pair * kPairBytes ? from.w_off[q & 1] : kNowhere;
-        lds_dma16(from.w, lds0 + W0 + at + (wave * W_INSTR + q) * 1024, off,
-                  from.at + pair * kPairBytes + (q >> 1) * from.ld16);
+        constexpr auto load = STREAM ? lds_dma16_once : lds_dma16;
+        load(from.w, lds0 + W0 + at + (wave * W_INSTR + q) * 1024, off,
+             from.at + pair * kPairBytes + (q >> 1) * from.ld16);
     };
     auto issue_scales = [&](int chunk, auto idx) {
         constexpr int q = decltype(idx)::value;
@@ -662,7 +674,7 @@ inline Mx4Args mx4_args(const Mx4Call& c, int splits, void* planes) {
 }
 
 template <int DT, int CFG>
-int launch_mx4(const Mx4Call& c, int splits, int cus, void* workspace, hipStream_t stream) {
+int launch_mx4(const Mx4Call& c, int splits, bool stream_w, int cus, void* workspace, hipStream_t stream) {
     constexpr int BM = kMx4Tiles[CFG].rows, BN = kMx4Tiles[CFG].columns;
     const int tiles_n = (int)((c.N + BN - 1) / BN);
     const int64_t tiles_m = c.offsets ? c.total_rows / BM + std::min<int64_t>(c.experts, c.total_rows)
@@ -673,7 +685,8 @@ int launch_mx4(const Mx4Call& c, int splits, int cus, void* workspace, hipStream
     // Tiles of 256: a block per CU, which loads its next tile while it stores one.
     const int64_t blocks = tiles_m * tiles_n * splits;
     const uint64_t per_group = (uint64_t)kGroupM * tiles_n, magic = ((1ull << 40) + per_group - 1) / per_group;
-    hipLaunchKernelGGL((gemm_mx4_kernel<DT, CFG>), launch_grid(BM == 256 ? std::min<int64_t>(blocks, cus) : blocks),
+    auto kernel = stream_w ? gemm_mx4_kernel<DT, CFG, true> : gemm_mx4_kernel<DT, CFG, false>;
+    hipLaunchKernelGGL(kernel, launch_grid(BM == 256 ? std::min<int64_t>(blocks, cus) : blocks),
                        dim3(256), 0, stream, a, tiles_n, magic);
     MB_HIP_TRY(hipGetLastError());
     return splits > 1 ? mx4_sum<DT>(a, stream) : MB_OK;
@@ -682,11 +695,11 @@ int launch_mx4(const Mx4Call& c, int splits, int cus, void* workspace, hipStream
 template <int DT>
 int launch_mx4_config(const Mx4Call& c, const Mx4Plan& plan, int cus, void* workspace, hipStream_t stream) {
     switch (plan.config) {
-        case 0: return launch_mx4<DT, 0>(c, plan.splits, cus, workspace, stream);
-        case 1: return launch_mx4<DT, 1>(c, plan.splits, cus, workspace, stream);
-        case 2: return launch_mx4<DT, 2>(c, plan.splits, cus, workspace, stream);
-        case 3: return launch_mx4<DT, 3>(c, plan.splits, cus, workspace, stream);
-        default: return launch_mx4<DT, 4>(c, plan.splits, cus, workspace, stream);
+        case 0: return launch_mx4<DT, 0>(c, plan.splits, plan.stream, cus, workspace, stream);
+        case 1: return launch_mx4<DT, 1>(c, plan.splits, plan.stream, cus, workspace, stream);
+        case 2: return launch_mx4<DT, 2>(c, plan.splits, plan.stream, cus, workspace, stream);
+        case 3: return launch_mx4<DT, 3>(c, plan.splits, plan.stream, cus, workspace, stream);
+        default: return launch_mx4<DT, 4>(c, plan.splits, plan.stream, cus, workspace, stream);
     }
 }
 

@@ -35,6 +35,7 @@ constexpr int kMx4MostSplits = 16;
 struct Mx4Plan {
     int config;
     int splits;   // of K, over fp32 planes in the workspace (tiles without 256)
+    bool stream;  // w is loaded nontemporal
 };
 
 struct Mx4Shape {
@@ -51,30 +52,46 @@ inline double mx4_row_tiles(const Mx4Shape& s, int size) {
     return hit * std::max(1.0 + 0.55 * std::max(0.0, tiles - 0.35), tiles + 0.45);
 }
 
+// Row tiles of `size` that read one part of w, on average.
+inline double mx4_w_reads(const Mx4Shape& s, int size) {
+    return mx4_row_tiles(s, size) / (s.by_expert ? (double)std::min<int64_t>(s.experts, s.total_rows) : 1.0);
+}
+
+// w read once, and too much of it for the 256 MB Infinity Cache to hold from one call to the next beside what else
+// runs: 64 x 50257 x 4096 (109 MB) 29.3 -> 25.1 us, 512 rows over 64 experts, 4096 -> 2048 57 -> 51.5. Where it lies there
+// still or is read again it costs: 64 x 14336 x 4096 (31 MB) 10.0 -> 10.6, 512 rows over 16 experts (71 MB) 16.1 -> 18.9,
+// 8192^3 236 -> 258.
+inline bool mx4_stream(const Mx4Shape& s, int size) {
+    const double hit = s.by_expert ? (double)std::min<int64_t>(s.experts, s.total_rows) : 1.0;
+    return mx4_w_reads(s, size) <= 1.2 && hit * (double)s.N * (double)s.units * 68 >= (double)(96 << 20);
+}
+
 // `config`, `splits`: forced, or negative.
 inline Mx4Plan mx4_plan(const Mx4Shape& s, size_t workspace_bytes, int cus, int64_t config, int64_t splits) {
     // Rows read through a list lie within the 2^31 bytes that a buffer offset spans.
-    if (s.listed && s.x_rows > ((1ll << 31) - 1) / (s.units * 64)) return {kMx4Any, 1};
+    if (s.listed && s.x_rows > ((1ll << 31) - 1) / (s.units * 64)) return {kMx4Any, 1, false};
     const double plane = 4.0 * (double)s.total_rows * (double)((s.N + 3) / 4 * 4);
     auto fits = [&](int n) { return plane * n <= (double)workspace_bytes; };
     if (config >= kMx4TileCount) {
         const double rows8 = std::ceil((double)s.total_rows / 8) + s.experts, columns = (double)(s.N / 32 + 8);
-        return {config == kMx4Rows8 && rows8 * columns >= (double)(1 << 30) ? kMx4Rows32 : (int)config, 1};   // int32
+        if (config == kMx4Rows8 && rows8 * columns >= (double)(1 << 30)) config = kMx4Rows32;   // int32
+        return {(int)config, 1, config != kMx4Any && mx4_stream(s, kMx4Tiles[config].rows)};
     }
 
     // The tile and split count whose predicted time is least. Splits cost a second launch and their planes, written
     // and read, and none has less than 16 units; each smaller tile or further split has to gain 3%. Few rows by 8 or
-    // 32, whose waves stream w with no barriers: 64 tokens x 4 of 64 experts, 4096 -> 2048: 51 us, on 64 x 128
-    // tiles 53; with 128 tokens 63 and 57. 32 x 8192 x 8192: 8.4 us, 10.1; 32 x 50257 x 4096: 34 us, 27.
+    // 32, whose waves stream w with no barriers: 64 tokens x 4 of 64 experts, 4096 -> 2048: 49 us, on 64 x 128
+    // tiles 49.5; with 128 tokens 63 and 52. 32 x 8192 x 8192: 8.4 us, 10.1 on 64 x 64; 16 x 50257 x 4096: 29 us, 23 on
+    // 64 x 128.
     constexpr double kSumUs = 3.5, kBytesPerUs = 5e6;
-    Mx4Plan best{-1, 1};
+    Mx4Plan best{-1, 1, false};
     double best_us = 0;
     for (int i = 0; i < kMx4Any; ++i) {
         if (config >= 0 && config != i) continue;
         const Mx4Tile& tile = kMx4Tiles[i];
         const double row_tiles = mx4_row_tiles(s, tile.rows);
         const double tiles = row_tiles * (double)((s.N + tile.columns - 1) / tile.columns);
-        const double w_once = row_tiles / (s.by_expert ? (double)std::min<int64_t>(s.experts, s.total_rows) : 1.0);
+        const double w_reads = mx4_w_reads(s, tile.rows);
         for (int n = 1; n <= kMx4MostSplits; ++n) {
             if (splits >= 0 ? n != splits && n != 1 : (n & (n - 1)) != 0) continue;
             if (n > 1 && (tile.rows == 256 || i >= kMx4TileCount)) continue;
@@ -86,13 +103,13 @@ inline Mx4Plan mx4_plan(const Mx4Shape& s, size_t workspace_bytes, int cus, int6
                 const double one = tile.one_us + units * tile.one_unit_us;
                 const double more = tile.round_us + units * tile.round_unit_us - one, on_cu = std::ceil(b / cus);
                 const double busy = on_cu <= 1 ? one : one + more * (on_cu - 1) / (tile.per_cu - 1);
-                return std::max(busy, tile.w_us + b / w_once * tile.columns * units * 68 / tile.w_rate);
+                return std::max(busy, tile.w_us + b / w_reads * tile.columns * units * 68 / tile.w_rate);
             };
             const double rounds = std::floor(blocks / whole), rest = blocks - rounds * whole;
             double us = rounds * (rounds > 0 ? round(whole) : 0) + (rest > 0 ? round(rest) : 0);
             if (n > 1) us += kSumUs + 2 * n * plane / kBytesPerUs;
             if (best.config < 0 || us < 0.97 * best_us || (n > 1 && n == splits && best.config == i)) {
-                best = {i, n};
+                best = {i, n, mx4_stream(s, tile.rows)};
                 best_us = us;
             }
         }

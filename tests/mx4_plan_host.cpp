@@ -1,5 +1,5 @@
 // Host code, compiled from the MX4 products' own headers by tests/test_mx4_plan.py.
-//   plan   "config splits" for each line "total_rows experts N units by_expert listed x_rows workspace cus config splits"
+//   plan   "config splits stream" for each line "total_rows experts N units by_expert listed x_rows workspace cus config splits"
 //   waits  "slots pair chunk groups pieces persistent step[8] prologue behind_prologue behind[3]" of every tile
 //   tiles  "tm tn" of every tile of tiles_m x tiles_n, for each line "tiles_m tiles_n blocks", then an empty line
 #include <cstdio>
@@ -29,7 +29,7 @@ int main(int, char** argv) {
                           &listed, &x_rows, &workspace, &cus, &config, &splits) == 11) {
             s = {total, n, units, x_rows, s.experts, by_expert != 0, listed != 0};
             const Mx4Plan p = mx4_plan(s, (size_t)workspace, cus, config, splits);
-            std::printf("%d %d\n", p.config, p.splits);
+            std::printf("%d %d %d\n", p.config, p.splits, p.stream);
         }
     } else if (!std::strcmp(argv[1], "waits")) {
         print_waits<0>();

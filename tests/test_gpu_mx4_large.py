@@ -62,6 +62,36 @@ def test_outputs_past_2_to_31(lib, tune, config):
         assert torch.equal(out[lo:hi], wanted.bfloat16()), lo
 
 
+@pytest.mark.parametrize("config, splits", [(None, None), (0, None), (1, 1), (2, 3), (3, 2), (4, 1), (5, None), (6, None)])
+def test_w_past_the_caches(lib, tune, config, splits):
+    """96 MB of w and more, read once, are loaded past the caches; 300 rows read it again on most tiles."""
+    tune(mx4_config=config, mx4_splits=splits)
+    k = 6016
+    w = _random(31003, k, 2)
+    wv = values_of(torch, *w, k).t().contiguous()
+    workspace = torch.empty(64 << 20, dtype=torch.uint8, device="cuda")
+    for m in (1, 8, 30, 64, 100, 250, 300):
+        x, out = _random(m, k, m), torch.full((m + 1, 31003), 7.0, dtype=torch.bfloat16, device="cuda")
+        _gemm(lib, x, w, out[:m], k, workspace=workspace)
+        assert torch.equal(out[:m], (values_of(torch, *x, k) @ wv).bfloat16()), m
+        assert (out[m] == 7).all()
+    experts, n, k = 40, 1200, 4096
+    w = _random(experts * n, k, 3)
+    for each in (3, 50):
+        counts = torch.arange(experts) % (2 * each + 1)
+        offsets = torch.cat([torch.zeros(1, dtype=torch.int64), counts.cumsum(0)]).int()
+        total = int(offsets[-1])
+        x, d = _random(total, k, each), offsets.cuda()
+        out = torch.full((total, n), 7.0, dtype=torch.bfloat16, device="cuda")
+        lib.gemm_mx4(BF, x[0].data_ptr(), x[1].data_ptr(), total, None, w[0].data_ptr(), w[1].data_ptr(), out.data_ptr(),
+                     0, d.data_ptr(), experts, total, n, k, workspace.data_ptr(), workspace.numel(), _stream())
+        xv = values_of(torch, *x, k)
+        for e in range(experts):
+            lo, hi = int(offsets[e]), int(offsets[e + 1])
+            we = values_of(torch, w[0][e * n:(e + 1) * n], w[1][e * n:(e + 1) * n], k).t().contiguous()
+            assert torch.equal(out[lo:hi], (xv[lo:hi] @ we).bfloat16()), e
+
+
 @pytest.mark.parametrize("listed", [False, True])
 @pytest.mark.parametrize("config", [None, 0])
 def test_blocks_that_make_several_tiles_by_expert(lib, tune, config, listed):

@@ -56,20 +56,29 @@ def _call(rows, n, k, *, experts=1, by_expert=False, listed=False, x_rows=None, 
 
 def test_picks(host):
     picked = host("plan", [_call(*shape) for shape, _ in DENSE])
-    assert [config for config, _ in picked] == [config for _, config in DENSE]
+    assert [config for config, *_ in picked] == [config for _, config in DENSE]
     calls = [_call(rows, n, k, experts=e, by_expert=True, listed=True) for (rows, e, n, k), _ in EXPERTS]
-    assert [config for config, _ in host("plan", calls)] == [config for _, config in EXPERTS]
+    assert [config for config, *_ in host("plan", calls)] == [config for _, config in EXPERTS]
+
+
+def test_w_is_streamed_where_it_is_large_and_read_once(host):
+    streamed = [(1, 50257, 4096), (64, 50257, 4096), (128, 50257, 4096), (8, 32768, 8192)]
+    kept = [(1, 14336, 4096), (64, 14336, 4096), (129, 50257, 4096, T128), (8192, 8192, 8192), (4096, 50257, 4096)]
+    calls = [_call(*shape[:3], config=shape[3] if len(shape) > 3 else -1) for shape in streamed + kept]
+    assert [stream for *_, stream in host("plan", calls)] == [1] * len(streamed) + [0] * len(kept)
+    experts = [_call(rows, 2048, 4096, experts=64, by_expert=True, listed=True) for rows in (256, 512, 2048, 16384)]
+    assert [stream for *_, stream in host("plan", experts)] == [1, 1, 1, 0]
 
 
 def test_k_is_split_only_over_a_workspace_that_holds_the_sums(host):
     rows, n, k = 792, 200, 14464
     plane = 4 * rows * n
-    with_one, = host("plan", [_call(rows, n, k)])
-    assert with_one == (T64, 4)
-    assert host("plan", [_call(rows, n, k, workspace=0)])[0][1] == 1
-    assert host("plan", [_call(rows, n, k, workspace=4 * plane - i, config=T64) for i in (0, 1)]) == [(T64, 4), (T64, 2)]
-    assert host("plan", [_call(rows, n, k, config=T128, splits=5), _call(rows, n, k, config=T256, splits=5),
-                         _call(rows, n, k, config=ROWS32, splits=5)]) == [(T128, 5), (T256, 1), (ROWS32, 1)]
+    picked = lambda *calls: [(config, splits) for config, splits, _ in host("plan", calls)]   # noqa: E731
+    assert picked(_call(rows, n, k)) == [(T64, 4)]
+    assert picked(_call(rows, n, k, workspace=0))[0][1] == 1
+    assert picked(*(_call(rows, n, k, workspace=4 * plane - i, config=T64) for i in (0, 1))) == [(T64, 4), (T64, 2)]
+    assert picked(_call(rows, n, k, config=T128, splits=5), _call(rows, n, k, config=T256, splits=5),
+                  _call(rows, n, k, config=ROWS32, splits=5)) == [(T128, 5), (T256, 1), (ROWS32, 1)]
 
 
 def test_lists_over_more_than_2_to_31_bytes_take_the_kernel_for_any_size(host):
@@ -78,14 +87,14 @@ def test_lists_over_more_than_2_to_31_bytes_take_the_kernel_for_any_size(host):
     for rows in (1, 100, 8192):
         calls = [_call(rows, 4096, 4096, listed=True, x_rows=x_rows, config=c) for x_rows in (fits, fits + 1)
                  for c in (-1, T256)]
-        picked = [config for config, _ in host("plan", calls)]
+        picked = [config for config, *_ in host("plan", calls)]
         assert ANY not in picked[:2] and picked[2:] == [ANY, ANY]
     assert host("plan", [_call(fits + 1, 4096, 4096, config=T64)])[0][0] == T64   # without a list: tile by tile
 
 
 def test_tiles_of_8_rows_past_2_to_30_blocks_give_way(host):
     rows = (1 << 31) - 256
-    assert [c for c, _ in host("plan", [_call(rows, 1, 1, config=ROWS8), _call(1 << 20, 32, 1, config=ROWS8)])] == \
+    assert [c for c, *_ in host("plan", [_call(rows, 1, 1, config=ROWS8), _call(1 << 20, 32, 1, config=ROWS8)])] == \
         [ROWS32, ROWS8]
 
 
