@@ -90,10 +90,10 @@ def detect_device(torch_module: Any, device_id: int = 0) -> DeviceInfo | None:
 
 # Peak engine clock (MHz) -> SKU, for gfx950 parts whose marketing name the platform does not report
 # (the device name comes from libdrm's amdgpu.ids table, which a container may lack). MI355X and MI350X
-# are both gfx950 with 256 CUs; their published peak engine clocks differ. The one reported is now and then the clock
-# of the moment, a few MHz over (2402 and 2403 have been read).
+# are both gfx950 with 256 CUs; their published peak engine clocks differ. The one reported may be a few MHz off: 1539
+# readings of an MI355X, idle and under load, were 2400 (1072), 2402 (463) and 2403 (4), none lower.
 _GFX950_SKU_BY_MAX_CLOCK = {2400: "AMD Instinct MI355X", 2200: "AMD Instinct MI350X"}
-_MAX_CLOCK_TOLERANCE_MHZ = 20
+_MAX_CLOCK_UNDER_MHZ, _MAX_CLOCK_OVER_MHZ = 10, 5
 
 
 def _amdsmi_names(torch_module: Any, device_id: int) -> list[str]:
@@ -132,8 +132,8 @@ def _amdsmi_names(torch_module: Any, device_id: int) -> list[str]:
             except Exception:  # noqa: BLE001
                 top = None
             for clock, sku in _GFX950_SKU_BY_MAX_CLOCK.items():
-                if top is not None and abs(top - clock) <= _MAX_CLOCK_TOLERANCE_MHZ:
-                    names.append(f"{sku} (gfx950, peak engine clock {clock} MHz)")
+                if top is not None and clock - _MAX_CLOCK_UNDER_MHZ <= top <= clock + _MAX_CLOCK_OVER_MHZ:
+                    names.append(f"{sku} (gfx950, peak engine clock {clock} MHz, read as {top})")
     except Exception:  # noqa: BLE001
         return names
     finally:
