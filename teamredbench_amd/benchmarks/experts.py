@@ -13,7 +13,8 @@ metrics are the ones of its GEMM benchmark (src/teamredbench/benchmarks/mfu.py:3
           verify_max_tokens (default 64), operand_sets ("auto", or a count: the timed calls cycle through that
           many copies of the layer's buffers; "auto" takes enough that the smallest product bound by memory, by
           its arithmetic intensity, spans three times the 256 MB Infinity Cache, at most 1024 and half of the
-          free memory)
+          free memory; an operator that only moves bytes takes as many as it needs to span that itself, if
+          its calls are enough to pass the cache)
   records, one per operator of a layer: case "experts_<operator>_t<tokens>e<experts>k<top_k>_<k>x<n>"
           with raw_metrics elapsed_s, achieved_ops / peak_tops and gemm_bytes for the products,
           moved_bytes / peak_bandwidth_gbps for the rest; operator "layer" is the whole forward pass. The

@@ -84,6 +84,22 @@ class LayerBenchmark(Benchmark):
         sets = -(-OPERAND_FOOTPRINT_TARGET // min(bound))
         return max(1, min(sets, MAX_OPERAND_SETS, free_bytes // 2 // set_bytes))
 
+    def _sets_by_operator(self, operators: list[tuple[str, str, dict]], peak_tops: float | None, set_bytes: int,
+                          free_bytes: int, calls: int) -> dict[str, int]:
+        """Copies that each operator's calls cycle through: `_operand_sets` for the products and the whole layer. What only
+        moves bytes takes more where that is short of the footprint of its own, since its rate is reported as
+        HBM's: up to the number of its calls, where those pass the cache at all."""
+        sets = self._operand_sets(operators, peak_tops, set_bytes, free_bytes)
+        by_operator = {name: sets for name, _, _ in operators}
+        if self.params.get("operand_sets", "auto") == "auto":
+            for name, _, work in operators:
+                if "gemm_bytes" not in work:
+                    own = min(-(-OPERAND_FOOTPRINT_TARGET // work["moved_bytes"]), MAX_OPERAND_SETS, calls,
+                              free_bytes // 2 // set_bytes)
+                    if own * work["moved_bytes"] > INFINITY_CACHE_BYTES:
+                        by_operator[name] = max(sets, own)
+        return by_operator
+
     def _cases(self, lib, torch, spec, shape: dict[str, int], peak_tops) -> list[BenchmarkRecord]:
         peak_hbm = self.context.hardware_profile.peak_hbm_bandwidth_gbps
         warmup, iterations = int(self.params.get("warmup", 10)), int(self.params.get("iterations", 50))
@@ -95,11 +111,12 @@ class LayerBenchmark(Benchmark):
             layer.backward()
         operators = self._operators(layer, spec.bytes_per_element, backward)
         set_bytes = sum(tensor_nbytes(value) for value in layer.buffers().values())
-        sets = self._operand_sets(operators, peak_tops, set_bytes, torch.cuda.mem_get_info(self.device)[0])
-        layers = [layer, *(layer.clone() for _ in range(sets - 1))]
+        sets = self._sets_by_operator(operators, peak_tops, set_bytes, torch.cuda.mem_get_info(self.device)[0],
+                                      max(warmup, 0) + max(iterations, 1))
+        layers = [layer, *(layer.clone() for _ in range(max(sets.values()) - 1))]
         times = {}
         for name, method, _ in operators:
-            calls = itertools.cycle([getattr(one, method) for one in layers])
+            calls = itertools.cycle([getattr(one, method) for one in layers[:sets[name]]])
             times[name] = timed_iterations(lambda: next(calls)(), torch_module=torch, warmup=warmup,
                                            iterations=iterations)
         del layers, calls
@@ -111,9 +128,10 @@ class LayerBenchmark(Benchmark):
                 parity[name] = {**parity_of(torch, checked), "rows_checked": rows}
         records = []
         for name, _, work in operators:
+            footprint = sets[name] * moved_or_product_bytes(work)
             metadata = {"backend": "native", "kernel": f"{self.name}_gfx950", "operator": name, "timing": "wall_clock",
-                        "operand_sets": sets, "operand_footprint_bytes": sets * moved_or_product_bytes(work),
-                        "cache_resident": sets * moved_or_product_bytes(work) <= INFINITY_CACHE_BYTES,
+                        "operand_sets": sets[name], "operand_footprint_bytes": footprint,
+                        "cache_resident": footprint <= INFINITY_CACHE_BYTES,
                         **{key: int(value) for key, value in shape.items()}}
             check = name if name in self.checks else "forward"
             if check in parity:
