@@ -5,9 +5,9 @@
 //   FIT    2^(e - 1) where m > 1.5, so that nothing saturates
 // not below 2^-127. a's exponent is read off its fp32 bits (subnormal a: 2^-127
 // either way). Elements are x / scale, rounded to the nearest e2m1 value, ties to the even code,
-// by v_cvt_scalef32_pk_fp4_*: checked against the definition for every bf16
-// value under 15 scales, and for fp32 at and next to every border. A block that holds an infinity or a
-// NaN has no scale: it becomes NaN as a whole (scale 255, elements 0).
+// by v_cvt_scalef32_pk_fp4_*, which the tests compare with the definition for every 16-bit
+// value under scales from its own to 5 binades above, and for the fp32 values next to them. A block that holds an
+// infinity or a NaN has no scale: it becomes NaN as a whole (scale 255, elements 0).
 //
 // Bytes bound all of it: x is read once, whichever forms are written. bf16 8192 x 8192, inputs and outputs not in the
 // caches: rows 31 us (5.4 TB/s), columns 37 (4.6), both 49 (4.2), values back 25 (6.7); fp32 57, 61, 76 and 44. From the
