@@ -354,6 +354,8 @@ int mb_mx4_dequantize(int dtype, const void* q, const void* scales, int64_t rows
  * Sums are fp32, rounded once. NaN blocks make their rows' (columns') outputs NaN. Output rows
  * before offsets[0] and from offsets[experts] on are left alone; rows that are not there count as zeros.
  * 1 <= K <= MB_MX4_MAX_K, 1 <= N < 2^30, total_rows <= 2^31 - 256. x, w and out must not overlap.
+ * By expert, dx is this call on every expert's w along its columns (an mb_mx4_quantize for each, the forms one after
+ * another); dw, a sum over an expert's own rows, is not offered (mb_gemm_grouped has it for 16-bit operands).
  * workspace: any size, NULL included; calls of few tiles run faster with one on
  * 16 bytes that holds 2 to 16 fp32 copies of out (they split K).
  */
