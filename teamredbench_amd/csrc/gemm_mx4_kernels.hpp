@@ -8,14 +8,18 @@
 // of L1 as the elements did). A step is one unit: the MFMAs of unit j, the LDS reads of unit j + 1 spread evenly among
 // them, and the loads of a pair or of scales some slots ahead; one barrier and one vmcnt wait a step, derived from the
 // order of the loads at compile time (mx4_schedule). 16-byte chunk c of a row lies at chunk c ^ swz_a2(row) of its
-// slot, so that the 64 lanes of a read meet every bank evenly. Lane half h takes blocks 4h .. 4h + 3 of a pair: K may
-// come in any order that both operands share, and so one dword brings a lane its four scales.
+// slot, so that the 64 lanes of a read of elements meet every bank evenly (4 LDS cycles, no conflicts). Lane half h takes
+// blocks 4h .. 4h + 3 of a pair: K may come in any order that both operands share, and so one dword brings a lane its
+// four scales. Those dwords, of rows 32 bytes apart, take 8 LDS cycles where 2 would do, and are most of the 26% of its LDS
+// cycles that 8192^3 spends in bank conflicts; LDS is busy for 29% of that product's cycles.
 //
-// 256 x 256 tiles, persistent blocks of one a CU: 8192^3 232-242 us, 4.5-4.7 PFLOP/s, 70% of what these MFMAs sustain
-// alone (6.66). Of a tile's 49000 cycles at K = 4096, 33000 are MFMAs, 5000 to 7000 waits for LDS and barriers in the
-// K loop, and 10000 lie around it (first loads, stores; the next tile's first loads run among the stores). The
-// clock is what the power limit leaves, 1.55 to 1.75 GHz, and rises where matrix cores idle: the last half round of
-// tiles of 4096 x 14336 x 4096 costs 23 us, a whole one 34.
+// 256 x 256 tiles, persistent blocks of one a CU: 8192^3 232-245 us on the GPUs seen, 4.5-4.7 PFLOP/s, 69-71% of what
+// these MFMAs sustain alone there (6.5-6.7). 8192 x 8192 x K, four tiles a block, on one GPU: K = 2048 88.2 us at 1.69
+// GHz, 4096 139 (1.67), 8192 245 (1.55), 16384 457 (1.51). So a tile takes 37200, 58000, 95100 and 172600 cycles: about
+// 1190 for a unit of K, 1024 of them MFMAs, and 18000 to 20000 around the K loop (first loads, stores, its part of the
+// launch; the next tile's first loads run among the stores). The clock is what the power limit leaves; the MFMAs
+// alone run at 1.56 GHz there, no slower than 8192^3 with its idle cycles. The last half round of tiles of 4096 x 14336 x
+// 4096 costs 23 us, a whole one 34.
 #pragma once
 
 #include "gemm_grouped_kernels.hpp"

@@ -45,7 +45,8 @@ namespace {
 
 // acc += b a^T over 64 elements of K (32 columns of b, 32 rows of a). Lane l holds 32 elements of row l % 32 of
 // each; A and B may spread K over l / 32 and the calls in any order they share. Byte SEL of the scale dwords is used.
-// 32 x 32 x 64 sustains 6.66 PFLOP/s on random operands, 16 x 16 x 128 5.48.
+// Alone on random operands, under the power limit, 32 x 32 x 64 sustains 6.5 to 6.7 PFLOP/s on the GPUs seen, 16 x 16 x 128
+// 5.3 to 5.5.
 template <int SEL_B, int SEL_A>
 __device__ __forceinline__ f32x16 mfma_mx4(const u32x4& b, unsigned scale_b, const u32x4& a, unsigned scale_a,
                                            f32x16 acc) {
