@@ -57,10 +57,15 @@ inline double mx4_w_reads(const Mx4Shape& s, int size) {
     return mx4_row_tiles(s, size) / (s.by_expert ? (double)std::min<int64_t>(s.experts, s.total_rows) : 1.0);
 }
 
-// w read once, and too much of it for the 256 MB Infinity Cache to hold from one call to the next beside what else
-// runs: 64 x 50257 x 4096 (109 MB) 29.3 -> 25.1 us, 512 rows over 64 experts, 4096 -> 2048 57 -> 51.5. Where it lies there
-// still or is read again it costs: 64 x 14336 x 4096 (31 MB) 10.0 -> 10.6, 512 rows over 16 experts (71 MB) 16.1 -> 18.9,
-// 8192^3 236 -> 258.
+// w read once, and too much of it for the 256 MB Infinity Cache to hold from one call to the next beside what else runs.
+// What it gains where w comes from HBM (several matrices in turn), and costs where the same w still lies in the cache, us
+// (8 and 64 rows by 4096, then 512 rows by expert, 4096 -> 2048):
+//   w, MiB    64                    72                    80                    96                    104
+//   8 rows    16.8->15.6 13.1->14.2 18.8->17.6 15.0->15.9 19.6->18.3 16.0->17.2 21.6->19.4 18.0->18.0 24.1->22.3 18.5->21.0
+//   64 rows   19.9->17.5 14.1->17.0 24.2->23.6 16.5->23.1 24.7->23.8 17.2->23.5 25.8->24.2 18.7->23.7 29.2->25.3 20.3->24.5
+//   experts   68: 20.9->18.7 16.3->16.7; 85: 25.5->23.9 18.0->22.4; 102: 26.3->24.2 20.3->23.6; 272: 56.8->51.0 50.3->51.3
+// From HBM it gains at every size, by the most from about 96 MiB on; below, w more often lies in the cache still, and there
+// it costs up to 7 us. Read more than once: 8192^3 236 -> 258.
 inline bool mx4_stream(const Mx4Shape& s, int size) {
     const double hit = s.by_expert ? (double)std::min<int64_t>(s.experts, s.total_rows) : 1.0;
     return mx4_w_reads(s, size) <= 1.2 && hit * (double)s.N * (double)s.units * 68 >= (double)(96 << 20);

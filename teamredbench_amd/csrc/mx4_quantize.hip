@@ -10,8 +10,8 @@
 // infinity or a NaN has no scale: it becomes NaN as a whole (scale 255, elements 0).
 //
 // Bytes bound all of it: x is read once, whichever forms are written. bf16 8192 x 8192, inputs and outputs not in the
-// caches: rows 31 us (5.4 TB/s), columns 37 (4.6), both 49 (4.2), values back 25 (6.7); fp32 57, 61, 76 and 44. From the
-// Infinity Cache rows take 25 us and both 38.
+// caches: rows 31 us (5.4 TB/s), columns 37 (4.6), both 49 (4.2), values back 25 (6.7; 30 over nine and more outputs in
+// turn); fp32 57, 61, 75 and 44 (54). From the Infinity Cache rows take 25 us and both 37.
 #include "mx4_common.hpp"
 
 namespace mb {
@@ -211,7 +211,8 @@ mx4_quantize_tile_kernel(const void* __restrict__ x, int64_t ldx, int64_t rows, 
     __shared__ u32x4 tile[128 * 16];
     const int tid = threadIdx.x, l16 = tid % 16;
     // Tiles in squares of 256 x 256: those of one XCD (block b runs on XCD b % 8), one after the other, so that its L2
-    // joins their halves (fp32: quarters) of both forms' lines of 128 bytes: fp32 8192 x 8192 90 -> 76 us. Squares along x's
+    // joins their halves (fp32: quarters) of both forms' lines of 128 bytes: fp32 8192 x 8192 90 -> 76 us, 1.54 million
+    // write requests where tile by tile makes 2.11 (whole ones of 64 bytes: 1.11). Squares along x's
     // rows: in panels of 2 to 16 squares' width down x both forms took 52 to 62 us for 49.
     constexpr int WIDTH = 256 / COLUMNS, SQUARE = 2 * WIDTH;
     const int64_t block = block_number(), local = block / 8, square = local / SQUARE * 8 + block % 8;
@@ -329,8 +330,15 @@ mx4_quantize_tile_kernel(const void* __restrict__ x, int64_t ldx, int64_t rows, 
 
 // 16 bytes of values a lane (8 elements, fp32: 4), RUNS of them, whose codes and scales are loaded before any is used.
 // Whole lines are stored nontemporal where the values take half of the 256 MB Infinity Cache or more, which keeps little
-// of them for who reads them next: bf16 8192 x 8192 31.8 -> 25.4 us, with a product of 64 rows behind it 67 -> 62; 4096 x
-// 4096 10.4 -> 9.2, but 23 -> 25 with the product.
+// of them for who reads them next. bf16, us over three to six outputs in turn (over nine and more), and with a product of
+// 1, 64 and 1024 rows behind it:
+//    32 MiB ( 4096 x  4096)   8.0 ->  6.5 ( 9.9 ->  7.7), 22.4 -> 23.1, 22.7 -> 23.2, 48.5 -> 51.0
+//   112 MiB (14336 x  4096)  28.6 -> 22.4 (28.6 -> 26.7), 51.7 -> 54.5, 55.5 -> 53.8, 116.5 -> 121.4
+//   112 MiB ( 4096 x 14336)  28.6 -> 22.3 (28.6 -> 26.6), 51.0 -> 51.7, 65.5 -> 66.2, 160.8 -> 156.4
+//   128 MiB ( 8192 x  8192)  31.8 -> 25.3 (31.8 -> 30.1), 62.5 -> 58.7, 67.0 -> 62.3, 146.5 -> 145.2
+//   160 MiB (10240 x  8192)  38.5 -> 33.4 (38.5 -> 36.7), 71.7 -> 70.6, 85.4 -> 77.8, 174.2 -> 175.3
+//   448 MiB (28672 x  8192)  99.9 -> 97.4 (99.9 -> 97.5), 222.2 -> 204.4, 214.4 -> 191.2, 472.4 -> 489.3
+// Alone it always gains; with a reader behind it from 128 MiB on, at 112 as often as not.
 template <int DT, int RUNS>
 __global__ void __launch_bounds__(256)
 mx4_dequantize_kernel(const unsigned char* __restrict__ q, const unsigned char* __restrict__ scales, int64_t rows,
