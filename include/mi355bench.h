@@ -332,6 +332,7 @@ int mb_combine_grad(int dtype, const void* grad_out, int64_t ldg, const void* y,
  * NaN as a whole (scale 255, codes 0). A linear layer's gradients are products of such forms:
  * with y = x w^T, dx = dy w contracts over y's columns (dy along its rows, w along its columns), dw = dy^T x over
  * its rows (dy and x along their columns). The gradient of the quantisation itself is passed straight through.
+ * x and the forms must not overlap.
  */
 #define MB_MX4_SCALE_FLOOR 0
 #define MB_MX4_SCALE_FIT 1
@@ -341,6 +342,7 @@ int mb_mx4_quantize(int dtype, const void* x, int64_t ldx, int64_t rows, int64_t
 /*
  * mb_mx4_dequantize -- the values of an MX4 matrix, out (rows x columns,
  * FLOAT32 / BFLOAT16 / FLOAT16), rounded once (BFLOAT16 holds every value below 2^128 exactly).
+ * The matrix and out must not overlap.
  */
 int mb_mx4_dequantize(int dtype, const void* q, const void* scales, int64_t rows, int64_t columns, void* out,
                       int64_t ldo, void* stream);
@@ -357,7 +359,7 @@ int mb_mx4_dequantize(int dtype, const void* q, const void* scales, int64_t rows
  * By expert, dx is this call on every expert's w along its columns (an mb_mx4_quantize for each, the forms one after
  * another); dw, a sum over an expert's own rows, is not offered (mb_gemm_grouped has it for 16-bit operands).
  * workspace: any size, NULL included; calls of few tiles run faster with one on
- * 16 bytes that holds 2 to 16 fp32 copies of out (they split K).
+ * 16 bytes that holds 2 to 16 fp32 copies of out (they split K). Calls that may run at once need one each.
  */
 #define MB_MX4_MAX_K 8388608
 int mb_gemm_mx4(int dtype, const void* x, const void* x_scales, int64_t x_rows, const int32_t* rows, const void* w,
